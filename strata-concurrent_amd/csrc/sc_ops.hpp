@@ -1,0 +1,138 @@
+// sc_ops.hpp - the arguments of the operators' kernels (include/sc_ops.h), shared by their host layer (sc_ops_capi.cpp)
+// and the kernels (sc_rope.hip, sc_attn.hip, sc_gdn.hip).  Everything travels in the kernel arguments.
+#pragma once
+
+#include <hip/hip_runtime.h>
+
+#include <cstdint>
+
+#include "sc_internal.hpp"
+
+namespace sc {
+
+// A paged cache (sc_kv_cache) as the kernels see it.
+struct CacheArgs {
+    uint8_t *k, *v;
+    uint16_t *k_scale, *v_scale;
+    const int32_t* table;
+    int64_t table_ld;
+    uint32_t cells;       // table_ld * page_size: cells of a sequence
+    uint32_t n_pages;
+    uint32_t H;
+    FastDiv ps;
+};
+
+struct RopeArgs {
+    CacheArgs c;
+    const uint8_t *k, *v, *q;
+    uint8_t* q_out;
+    int64_t k_ld, v_ld, q_ld, q_out_ld;   // bytes from token to token
+    const int64_t *cu, *pos0;
+    const float* inv_freq;
+    uint32_t tokens, n_seqs, n_head, rot, neighbours;
+};
+
+struct AttnArgs {
+    CacheArgs c;
+    const int64_t* lens;
+    const uint8_t* q;
+    uint8_t* out;
+    float* lse;
+    int64_t q_ld, out_ld;                 // bytes from sequence to sequence
+    uint32_t n_seqs, n_head, max_len, window;
+    float scale;
+    uint32_t chunk, parts;                // cells of a part, parts of a sequence
+    float* ws;
+};
+
+struct GdnArgs {
+    const uint8_t *q, *k, *v;
+    uint8_t* out;
+    int64_t q_ld, k_ld, v_ld, out_ld;     // bytes from token to token
+    const float *g, *beta;
+    int64_t gate_ld;
+    float* const* state;
+    int64_t state_offset, head_ld, key_ld;
+    const int64_t* cu;
+    uint32_t n_seqs, tokens, v_heads, l2norm;
+    FastDiv share;                        // value heads of a key head
+    float scale, eps;
+};
+
+hipError_t launch_rope(const RopeArgs& a, int head_dim, int format, bool f16, hipStream_t stream);
+hipError_t launch_attn(const AttnArgs& a, int head_dim, int format, bool f16, hipStream_t stream);
+hipError_t launch_gdn_step(const GdnArgs& a, int size, bool f16, hipStream_t stream);
+hipError_t launch_gdn_chunk(const GdnArgs& a, int size, bool f16, void* workspace, hipStream_t stream);
+
+#if defined(__HIPCC__)
+using f32x4 = __attribute__((ext_vector_type(4))) float;
+using ops_u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
+using ops_u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+using f16x2 = __attribute__((ext_vector_type(2))) _Float16;
+using f16x4 = __attribute__((ext_vector_type(4))) _Float16;
+using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
+
+__device__ __forceinline__ uint32_t ops_div(uint32_t n, const FastDiv& f) {
+    return uint32_t((uint64_t(__umulhi(n, f.m)) + uint64_t(n)) >> f.s);
+}
+
+// Global memory said to be such, so that accesses are not flat ones.
+template <class T>
+__device__ __forceinline__ T ld_global(const void* p) {
+    return *(const __attribute__((address_space(1))) T*) (p);
+}
+template <class T>
+__device__ __forceinline__ void st_global(void* p, T v) {
+    *(__attribute__((address_space(1))) T*) (p) = v;
+}
+
+// Four consecutive values of an activation row, in f32.
+template <bool kF16>
+__device__ __forceinline__ f32x4 ld_act4(const uint8_t* row, uint32_t at) {
+    if constexpr (kF16) {
+        const f16x4 h = __builtin_bit_cast(f16x4, ld_global<ops_u32x2>(row + uint64_t(at) * 2));
+        return f32x4{float(h.x), float(h.y), float(h.z), float(h.w)};
+    } else {
+        return __builtin_bit_cast(f32x4, ld_global<ops_u32x4>(row + uint64_t(at) * 4));
+    }
+}
+template <bool kF16>
+__device__ __forceinline__ void st_act4(uint8_t* row, uint32_t at, f32x4 v) {
+    if constexpr (kF16) {
+        // round to nearest even: the results' type holds 11 bits
+        const f16x4 h{_Float16(v.x), _Float16(v.y), _Float16(v.z), _Float16(v.w)};
+        st_global<ops_u32x2>(row + uint64_t(at) * 2, __builtin_bit_cast(ops_u32x2, h));
+    } else {
+        st_global<ops_u32x4>(row + uint64_t(at) * 4, __builtin_bit_cast(ops_u32x4, v));
+    }
+}
+
+// The physical page of a sequence's cell, or -1 where it is not resident.  `cell` is below c.cells.
+__device__ __forceinline__ int32_t cache_page(const CacheArgs& c, uint32_t seq, uint32_t page) {
+    const int64_t at = int64_t(seq) * c.table_ld + page;
+    const int64_t p = c.table ? int64_t(ld_global<int32_t>(c.table + at)) : at;
+    return p >= 0 && p < int64_t(c.n_pages) ? int32_t(p) : -1;
+}
+
+// The sequence of row t of a packed batch by its first rows cu[0 .. n], or n when it is past them all; every lane of the
+// wave gives the same t.  One load a lane and a vote for 64 sequences.
+__device__ __forceinline__ uint32_t seq_of_row(const int64_t* cu, uint32_t n, int64_t t, uint32_t lane) {
+    uint32_t s = 0;
+    for (uint32_t base = 0; base < n; base += 64) {
+        const int64_t end = base + lane < n ? ld_global<int64_t>(cu + base + lane + 1) : INT64_MAX;
+        const uint64_t before = __ballot(end <= t);
+        s += uint32_t(__popcll(before));
+        if (before != ~0ull) break;
+    }
+    return s;
+}
+
+// Sum over a wave, the same in every lane and in the same order every time.
+__device__ __forceinline__ float wave_sum(float x) {
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) x += __shfl_xor(x, m);
+    return x;
+}
+#endif
+
+}  // namespace sc
