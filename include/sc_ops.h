@@ -36,7 +36,7 @@ typedef struct sc_kv_cache {
     int64_t n_head_kv;        /* 1 .. 256 */
     int64_t head_dim;         /* 64, 128 or 256 */
     int64_t page_size;        /* cells in a page, 1 .. 65536 */
-    int64_t n_pages;          /* physical pages of each pool, at most 2^31 - 1 */
+    int64_t n_pages;          /* physical pages of each pool; n_pages * n_head_kv * page_size < 2^31 rows */
     void* k;                  /* [n_pages][n_head_kv][page_size][head_dim], 16-byte aligned */
     void* v;
     uint16_t* k_scale;        /* [n_pages][n_head_kv][page_size][head_dim / 64], 8-byte aligned; NULL for f16 */

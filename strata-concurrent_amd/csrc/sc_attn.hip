@@ -1,8 +1,24 @@
 // sc_attn.hip - attention of one new token a sequence over its paged cache (sc_attn_decode_async).
 //
-// With scores s_j = scale * q . k_j over the cells left by the length, the window and the page table, a part of them gives
-// m = max s_j, l = sum exp(s_j - m) and acc = sum exp(s_j - m) v_j; two parts join by bringing both to the larger m.  A wave
-// takes a part of one query head's cells, a few lanes a cell, and a second kernel joins the parts of a head.
+// With scores x_j = scale * q . k_j * log2(e) over the cells left by the length, the window and the page table, a part of
+// them gives l = sum 2^(x_j - m) and o = sum 2^(x_j - m) v_j for a reference m near its largest score; parts join by
+// bringing them to one m, and out = o / l.  A kv head's query heads share its cells, so both products are matrix products:
+// scores [cells] x [16 heads], outputs [values] x [16 heads].  What bounds a call is reading the cache once.
+//
+// A wave takes 32 cells a turn, its rows straight from memory into the matrix instructions' operands, nothing through LDS:
+//   scores   A = keys (row = cell, 8 consecutive values a lane), B = queries; a lane ends with the scores of one head
+//            (lane % 16) for cells 4 g + i and 16 + 4 g + i, g = lane / 16, i < 4;
+//   outputs  A = values transposed (row = value index, 8 cells a lane), B = probabilities.  The products' cells may come
+//            in any order that both agree on, so the lane's eight cells are the ones whose scores it already holds, and its
+//            A operand is an 8 x 8 block of the cache that it loads as 16-byte rows and transposes in its registers.
+// The head is the lane's column in both results, so the running statistics are the lane's own: only the largest score of a
+// turn crosses lanes (two swaps), and bringing o to a new m is a product by the lane's own factor.
+//
+// Accuracy: probabilities and f32 queries enter the matrix instructions as two f16 parts (high part truncated, the rest
+// rounded likewise: 22 bits), keys, values and f16 queries are exact, int8 codes are exact in f16 and their scales are
+// applied in f32; sums are in 32 bits.  m leaves the largest probability at 2^10, so that small ones stay in f16's normal
+// range; an f32 query head is first scaled by a power of two.  The low part of a probability is at least 2^-24, so that an
+// infinite value in the cache meets no zero: it would make a NaN where the formula has an infinity.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -13,99 +29,544 @@ namespace sc {
 namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
+constexpr float kInf = __builtin_inff();
+constexpr int kAttnWaves = 4, kAttnThreads = kAttnWaves * 64;
+constexpr int kTurn = 32;                       // cells of a wave's turn
+constexpr uint32_t kUnit = kTurn * kAttnWaves;  // cells of a workgroup's turn
+constexpr float kTop = 10.0f, kMost = 15.0f;    // log2 of the largest probability after a new m, and before one is needed
 
-// Four values of a pool row.
+// 2^x by the hardware's instruction (1 unit in the last place; results below the normal range are 0).
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
+// 2^(a - b) for a <= b or -inf: nothing weighs nothing.
+__device__ __forceinline__ float weight(float a, float b) { return a == -kInf ? 0.0f : exp2_fast(a - b); }
+
+// The maximum and the sum over the four lanes that share lane % 16 (the 16-lane rows of the wave), in every one of them.
+template <class F>
+__device__ __forceinline__ float over_rows(float x, F f) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
+// ---- which cells a workgroup takes ------------------------------------------------------------------------------------
+
+struct Span {
+    uint32_t first, len, begin, units;   // cells [first, len), counted in units from `begin`, a multiple of a turn
+};
+__device__ __forceinline__ Span span_of(const AttnArgs& a, uint32_t s) {
+    const int64_t n = ld_global<int64_t>(a.lens + s);
+    Span p;
+    p.len = n < 0 ? 0u : n > int64_t(a.max_len) ? a.max_len : uint32_t(n);
+    p.first = a.window && p.len > a.window ? p.len - a.window : 0u;
+    p.begin = p.first & ~uint32_t(kTurn - 1);
+    p.units = (p.len - p.begin + kUnit - 1) / kUnit;
+    return p;
+}
+
+struct Place {
+    uint32_t s, ht, part, parts;   // sequence, kv head and tile of query heads, part of its units, how many parts
+    uint32_t id;                   // this part's place in the workspace (parts > 1)
+};
+// The units of all sequences are shared out among about `slots` workgroups: a part takes `per` units at most, `per` being
+// what one of them would get, so long and short sequences of a ragged batch give parts of like size.  Every workgroup (and
+// the joining kernel) finds its place from the lengths alone: one load a lane and a scan for 64 sequences.  `find` says
+// whether the workgroup with sequence-wise index range [lo, hi) is the one that is looked for.
+template <class Find>
+__device__ __forceinline__ bool place_of(const AttnArgs& a, uint32_t lane, Find find, Place& p) {
+    uint64_t total = 0;
+    for (uint32_t base = 0; base < a.n_seqs; base += 64)
+        if (base + lane < a.n_seqs) total += span_of(a, base + lane).units;
+#pragma unroll
+    for (int m = 1; m < 64; m <<= 1) total += __shfl_xor(total, m);
+    uint64_t per = (total * a.tiles + a.slots - 1) / a.slots;
+    per = per < a.least ? a.least : per;
+    uint32_t wgs = 0, ids = 0;
+    for (uint32_t base = 0; base < a.n_seqs; base += 64) {
+        const uint32_t units = base + lane < a.n_seqs ? span_of(a, base + lane).units : 0u;
+        const uint32_t parts = base + lane >= a.n_seqs ? 0u : units <= per ? 1u : uint32_t((units + per - 1) / per);
+        uint32_t w = parts, d = parts > 1 ? parts : 0u;   // inclusive sums over the lanes
+#pragma unroll
+        for (int m = 1; m < 64; m <<= 1) {
+            const uint32_t ow = __shfl_up(w, m), od = __shfl_up(d, m);
+            if (lane >= uint32_t(m)) w += ow, d += od;
+        }
+        const uint32_t lo = wgs + (w - parts) * a.tiles, hi = wgs + w * a.tiles;
+        const uint64_t here = __ballot(base + lane < a.n_seqs && find(base + lane, lo, hi));
+        if (here) {
+            const int at = __builtin_ctzll(here);
+            p.s = base + at;
+            p.parts = __shfl(parts, at);
+            p.part = __shfl(lo, at);   // the sequence's first workgroup: the caller makes it the part
+            p.id = ids + (__shfl(d, at) - (p.parts > 1 ? p.parts : 0u)) * a.tiles;
+            return true;
+        }
+        wgs += __shfl(w, 63) * a.tiles;
+        ids += __shfl(d, 63) * a.tiles;
+    }
+    return false;
+}
+
+// ---- a wave's turn ------------------------------------------------------------------------------------------------------
+
+__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+__device__ __forceinline__ f16x2 two(uint32_t w) { return __builtin_bit_cast(f16x2, w); }
+__device__ __forceinline__ uint32_t bits(f16x2 h) { return __builtin_bit_cast(uint32_t, h); }
+__device__ __forceinline__ f16x8 eight(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    return __builtin_bit_cast(f16x8, ops_u32x4{a, b, c, d});
+}
+__device__ __forceinline__ uint32_t pack_rtz(float a, float b) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
+}
+// Two f16 parts of eight values that are not negative: the truncated value, and what it left out, at least 2^-24.
+__device__ __forceinline__ void split8(const float (&p)[8], f16x8& hi, f16x8& lo) {
+    uint32_t h[4], r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        h[i] = pack_rtz(p[2 * i], p[2 * i + 1]);
+        const f16x2 t = two(h[i]);
+        r[i] = bits(__builtin_elementwise_max(two(pack_rtz(p[2 * i] - float(t.x), p[2 * i + 1] - float(t.y))), two(0x00010001u)));
+    }
+    hi = eight(h[0], h[1], h[2], h[3]);
+    lo = eight(r[0], r[1], r[2], r[3]);
+}
+
+// Four int8 codes with 128 added (one exclusive or) as f16: 0x64 above a byte is 1024 + the byte, exactly.
+__device__ __forceinline__ void codes4(uint32_t w, uint32_t& a, uint32_t& b) {
+    const f16x2 off = two(0xE480E480u);   // -1152
+    a = bits(two(__builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) + off);
+    b = bits(two(__builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) + off);
+}
+
 template <int D, bool kInt8>
-__device__ __forceinline__ f32x4 ld_cache4(const uint8_t* pool, const uint16_t* scales, uint64_t row, uint32_t d) {
-    if constexpr (kInt8) {
-        const uint32_t c = ld_global<uint32_t>(pool + row * D + d);
-        const float s = float(__builtin_bit_cast(_Float16, ld_global<uint16_t>(scales + row * (D / 64) + d / 64)));
-        return f32x4{float(int8_t(c)) * s, float(int8_t(c >> 8)) * s, float(int8_t(c >> 16)) * s, float(int8_t(c >> 24)) * s};
+struct Rows {
+    // f16: 16 bytes of 32 values a step; int8: 16 bytes of 64 values a step
+    static constexpr int kKeySteps = kInt8 ? D / 64 : D / 32;
+    // f16: D / 16 consecutive values a lane in pieces of 16 bytes; int8: 4 values of every block of 64
+    static constexpr int kValWords = kInt8 ? 1 : D >= 128 ? 4 : 2, kValPieces = kInt8 ? D / 64 : D >= 128 ? D / 128 : 1;
+    ops_u32x4 k[2][kKeySteps];
+    uint32_t v[8][kValPieces][kValWords];
+    uint32_t ks[kInt8 ? 8 : 1][2], vs[kInt8 ? 8 : 1][2];   // f16 scales of the lane's eight cells, a block each
+};
+
+// The value index of row r of output product j: what lane r loaded at its place j.
+template <int D, bool kInt8>
+__device__ __forceinline__ uint32_t value_of(uint32_t j, uint32_t r) {
+    if constexpr (kInt8) return j / 4 * 64 + r * 4 + j % 4;
+    constexpr uint32_t each = D >= 128 ? 8 : 4;
+    return j / each * 128 + r * each + j % each;
+}
+
+template <int D>
+__device__ __forceinline__ void ld_scales(uint32_t (&s)[2], const uint16_t* scales, uint64_t row) {
+    if constexpr (D == 256) {
+        const ops_u32x2 w = ld_global<ops_u32x2>(scales + row * 4);
+        s[0] = w.x, s[1] = w.y;
+    } else if constexpr (D == 128) {
+        s[0] = ld_global<uint32_t>(scales + row * 2);
     } else {
-        return ld_act4<true>(pool + row * (D * 2), d);
+        s[0] = ld_global<uint16_t>(scales + row);
+    }
+}
+__device__ __forceinline__ float scale_of(const uint32_t (&s)[2], int block) {
+    const f16x2 t = two(s[block / 2]);
+    return float(block & 1 ? t.y : t.x);
+}
+
+// Pool rows of the turn's 32 cells, cell l % 32 in lane l: the row (0 where there is none) and which cells there are.
+__device__ __forceinline__ int32_t row_of(const AttnArgs& a, const Span& p, uint32_t s, uint32_t h, uint32_t base, uint32_t lane) {
+    const uint32_t cell = base + (lane & 31);
+    if (cell < p.first || cell >= p.len) return -1;
+    const uint32_t page = ops_div(cell, a.c.ps);
+    const int32_t phys = cache_page(a.c, s, page);
+    return phys < 0 ? -1 : int32_t((uint32_t(phys) * a.c.H + h) * a.c.ps.d + (cell - page * a.c.ps.d));
+}
+
+template <int D, bool kInt8>
+__device__ __forceinline__ void load_keys(Rows<D, kInt8>& r, const AttnArgs& a, int32_t row, uint32_t lane) {
+    using R = Rows<D, kInt8>;
+    constexpr uint64_t bytes = kInt8 ? D : D * 2;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        const uint32_t at = uint32_t(__shfl(row, int(t * 16 + (lane & 15))));
+        const uint8_t* p = a.c.k + at * bytes + (lane >> 4) * 16;
+#pragma unroll
+        for (int i = 0; i < R::kKeySteps; ++i) r.k[t][i] = ld_global<ops_u32x4>(p + i * 64);
     }
 }
 
-// exp2(a - b) where either may be -inf: nothing weighs nothing.
-__device__ __forceinline__ float weight(float a, float b) { return a == -__builtin_inff() ? 0.0f : __builtin_exp2f(a - b); }
+template <int D, bool kInt8>
+__device__ __forceinline__ void load_values(Rows<D, kInt8>& r, const AttnArgs& a, int32_t row, uint32_t lane) {
+    using R = Rows<D, kInt8>;
+    constexpr uint64_t bytes = kInt8 ? D : D * 2;
+    const uint32_t g4 = (lane >> 4) * 4;
+#pragma unroll
+    for (int n = 0; n < 8; ++n) {
+        const uint32_t at = uint32_t(__shfl(row, int((n & 3) + g4 + (n >> 2) * 16)));
+        const uint8_t* p = a.c.v + at * bytes + (lane & 15) * (R::kValWords * 4);
+#pragma unroll
+        for (int i = 0; i < R::kValPieces; ++i) {
+            if constexpr (R::kValWords == 4) {
+                const ops_u32x4 w = ld_global<ops_u32x4>(p + i * 256);
+                r.v[n][i][0] = w.x, r.v[n][i][1] = w.y, r.v[n][i][2] = w.z, r.v[n][i][3] = w.w;
+            } else if constexpr (R::kValWords == 2) {
+                const ops_u32x2 w = ld_global<ops_u32x2>(p);
+                r.v[n][i][0] = w.x, r.v[n][i][1] = w.y;
+            } else {
+                r.v[n][i][0] = ld_global<uint32_t>(p + i * 64);
+            }
+        }
+        if constexpr (kInt8) {
+            ld_scales<D>(r.ks[n], a.c.k_scale, at);
+            ld_scales<D>(r.vs[n], a.c.v_scale, at);
+        }
+    }
+}
+
+// A query part's operand for value step i (lane = head % 16 + 16 * group).
+template <int D, int kParts>
+struct Queries {
+    ops_u32x4 q[kParts][D / 32][64];
+};
+
+// ---- the kernel -----------------------------------------------------------------------------------------------------------
 
 template <int D, bool kInt8, bool kF16>
-__global__ void __launch_bounds__(64) attn_part_kernel(AttnArgs a) {
-    constexpr uint32_t kLanes = D / 4, kRows = 64 / kLanes;
-    const uint32_t lane = threadIdx.x, s = blockIdx.x / a.n_head, head = blockIdx.x % a.n_head;
-    const uint32_t h = head / (a.n_head / a.c.H), d = (lane % kLanes) * 4;
-    int64_t len = ld_global<int64_t>(a.lens + s);
-    len = len < 0 ? 0 : len > int64_t(a.max_len) ? int64_t(a.max_len) : len;
-    const int64_t first = a.window && len > int64_t(a.window) ? len - a.window : 0;
-    const int64_t lo = first > int64_t(blockIdx.y) * a.chunk ? first : int64_t(blockIdx.y) * a.chunk;
-    const int64_t hi = len < int64_t(blockIdx.y + 1) * a.chunk ? len : int64_t(blockIdx.y + 1) * a.chunk;
-    f32x4 q = ld_act4<kF16>(a.q + s * a.q_ld, head * D + d) * (a.scale * kLog2e), acc{};
-    float m = -__builtin_inff(), l = 0;
-    for (int64_t j = lo + lane / kLanes; j < hi; j += kRows) {
-        const uint32_t page = ops_div(uint32_t(j), a.c.ps);
-        const int32_t phys = cache_page(a.c, s, page);
-        if (phys < 0) continue;
-        const uint64_t row = (uint64_t(phys) * a.c.H + h) * a.c.ps.d + (uint32_t(j) - page * a.c.ps.d);
-        const f32x4 k = ld_cache4<D, kInt8>(a.c.k, a.c.k_scale, row, d), v = ld_cache4<D, kInt8>(a.c.v, a.c.v_scale, row, d);
-        float x = q.x * k.x + q.y * k.y + q.z * k.z + q.w * k.w;
-        for (uint32_t i = 1; i < kLanes; i <<= 1) x += __shfl_xor(x, int(i));
-        if (x == -__builtin_inff()) continue;
-        const float top = x > m || x != x ? x : m, w = weight(m, top), p = __builtin_exp2f(x - top);
-        l = l * w + p;
-        acc = acc * w + p * v;
-        m = top;
+__global__ void __launch_bounds__(kAttnThreads, 1) attn_part_kernel(AttnArgs a) {
+    using R = Rows<D, kInt8>;
+    constexpr int kParts = kF16 ? 1 : 2;        // f16 queries are exact
+    constexpr int kSteps = D / 32, kOut = D / 16, kBlocks = D / 64;
+    constexpr int kRowF = D + 4;                // floats of a head's row in LDS
+    __shared__ Queries<D, kParts> s_q;
+    __shared__ float s_c[16], s_m[kAttnWaves][16], s_l[kAttnWaves][16];
+    __shared__ __align__(16) float s_o[kAttnWaves][16 * kRowF];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t g = lane >> 4, col = lane & 15;
+
+    Place p;
+    if (!place_of(a, lane, [&](uint32_t, uint32_t lo, uint32_t hi) { return blockIdx.x >= lo && blockIdx.x < hi; }, p)) return;
+    p.s = __builtin_amdgcn_readfirstlane(p.s);
+    p.parts = __builtin_amdgcn_readfirstlane(p.parts);
+    const uint32_t within = blockIdx.x - __builtin_amdgcn_readfirstlane(p.part);
+    p.ht = within / p.parts;
+    p.part = within - p.ht * p.parts;
+    p.id = __builtin_amdgcn_readfirstlane(p.id) + within;
+    const uint32_t per_head = a.tiles / a.c.H, h = p.ht / per_head, G = a.n_head / a.c.H;
+    const uint32_t head0 = h * G + (p.ht - h * per_head) * 16;
+    const uint32_t heads = (h + 1) * G - head0 < 16 ? (h + 1) * G - head0 : 16;
+    Span span = span_of(a, p.s);
+    const uint32_t each = (span.units + p.parts - 1) / p.parts;
+    const uint32_t u0 = p.part * each, u1 = u0 + each < span.units ? u0 + each : span.units;
+    const uint32_t base0 = span.begin + wave * kTurn;
+
+    // the first turn's rows are on their way while the queries are laid out
+    R r;
+    int32_t row = u0 < u1 ? row_of(a, span, p.s, h, base0 + u0 * kUnit, lane) : -1;
+    uint32_t there = uint32_t(__ballot(row >= 0));
+    row = row < 0 ? 0 : row;
+    if (u0 < u1) {
+        load_keys<D, kInt8>(r, a, row, lane);
+        load_values<D, kInt8>(r, a, row, lane);
     }
-    for (uint32_t i = kLanes; i < 64; i <<= 1) {
-        const float om = __shfl_xor(m, int(i)), ol = __shfl_xor(l, int(i));
-        f32x4 oa;
-        for (int j = 0; j < 4; ++j) oa[j] = __shfl_xor(acc[j], int(i));
-        const float top = m > om || m != m ? m : om, w = weight(m, top), ow = weight(om, top);
-        l = l * w + ol * ow;
-        acc = acc * w + oa * ow;
-        m = top;
+    for (uint32_t i = wave; i < 16; i += kAttnWaves) {
+        // head i: values lane, lane + 64, ...; an f32 head is scaled by a power of two to a largest value of 1 .. 2
+        float x[D / 64], top = 0;
+        const uint8_t* q = a.q + int64_t(p.s) * a.q_ld;
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k) {
+            const uint32_t at = (head0 + i) * D + k * 64 + lane;
+            if constexpr (kF16) x[k] = i < heads ? float(__builtin_bit_cast(_Float16, ld_global<uint16_t>(q + at * 2))) : 0.0f;
+            else x[k] = i < heads ? ld_global<float>(q + at * 4) : 0.0f;
+            top = fmaxf(top, fabsf(x[k]));
+        }
+        float by = 1.0f, back = 1.0f;
+        if constexpr (!kF16) {
+#pragma unroll
+            for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
+            if (top > 0 && top < kInf) {
+                const int e = int(__float_as_uint(top) >> 23) - 127;   // -127 for a subnormal: it stays below 1
+                const int f = e > 126 ? 126 : e < -126 ? -126 : e;
+                by = __uint_as_float(uint32_t(127 - f) << 23);
+                back = __uint_as_float(uint32_t(127 + f) << 23);
+            }
+        }
+        if (lane == 0) s_c[i] = a.scale * kLog2e * back;
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k) {
+            const uint32_t d = k * 64 + lane;
+            // f16 rows: step d / 32, group (d % 32) / 8.  int8 rows: half u of 64-value step, group (d % 64) / 16
+            const uint32_t step = kInt8 ? d / 64 * 2 + (d % 16) / 8 : d / 32, grp = kInt8 ? (d % 64) / 16 : (d % 32) / 8;
+            const _Float16 hi = _Float16(x[k] * by);
+            reinterpret_cast<_Float16*>(&s_q.q[0][step][grp * 16 + i])[d % 8] = hi;
+            if constexpr (!kF16)
+                reinterpret_cast<_Float16*>(&s_q.q[kParts - 1][step][grp * 16 + i])[d % 8] = _Float16(x[k] * by - float(hi));
+        }
     }
-    float* part = a.ws + (uint64_t(blockIdx.x) * a.parts + blockIdx.y) * (D + 4);
-    if (lane < kLanes) *reinterpret_cast<f32x4*>(part + 4 + d) = acc;
-    if (lane == 0) part[0] = m, part[1] = l;
+    __syncthreads();
+    const float c = s_c[col];
+
+    f32x4 o[kOut];
+#pragma unroll
+    for (int j = 0; j < kOut; ++j) o[j] = f32x4{};
+    float m = -kInf, l = 0;
+    // a table entry is read two turns ahead of its rows: loads return in order, so one that was asked for after a turn's
+    // rows could only be used once they all have come
+    int32_t next = u0 + 1 < u1 ? row_of(a, span, p.s, h, base0 + (u0 + 1) * kUnit, lane) : -1;
+    for (uint32_t u = u0; u < u1; ++u) {
+        // scores: x[t * 4 + i] of cell 16 t + 4 g + i
+        float x[8], ks_top[8];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            f32x4 hi{}, lo{};
+            if constexpr (kInt8) {
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) {
+                    f32x4 bh{}, bl{};
+                    uint32_t w[8];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) codes4(r.k[t][b][k] ^ 0x80808080u, w[2 * k], w[2 * k + 1]);
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const f16x8 key = eight(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                        bh = mfma(key, __builtin_bit_cast(f16x8, s_q.q[0][2 * b + k][lane]), bh);
+                        if constexpr (!kF16) bl = mfma(key, __builtin_bit_cast(f16x8, s_q.q[kParts - 1][2 * b + k][lane]), bl);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float ks = scale_of(r.ks[t * 4 + i], b);
+                        hi[i] += ks * bh[i];
+                        if constexpr (!kF16) lo[i] += ks * bl[i];
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) {
+                    const f16x8 key = __builtin_bit_cast(f16x8, r.k[t][k]);
+                    hi = mfma(key, __builtin_bit_cast(f16x8, s_q.q[0][k][lane]), hi);
+                    if constexpr (!kF16) lo = mfma(key, __builtin_bit_cast(f16x8, s_q.q[kParts - 1][k][lane]), lo);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                // an infinite key makes the low part's product NaN: the high part has the score
+                const float s = kF16 ? hi[i] : fabsf(hi[i]) < kInf ? hi[i] + lo[i] : hi[i];
+                x[t * 4 + i] = s * c;
+            }
+        }
+        // the next turn's keys take the place of this one's
+        const uint32_t seen = there;
+        int32_t after = -1, next_row = next < 0 ? 0 : next;
+        if (u + 1 < u1) {
+            there = uint32_t(__ballot(next >= 0));
+            if (u + 2 < u1) after = row_of(a, span, p.s, h, base0 + (u + 2) * kUnit, lane);
+            load_keys<D, kInt8>(r, a, next_row, lane);
+        }
+        uint32_t gone[8];   // all ones where a cell is not there
+        const bool whole = seen == 0xFFFFFFFFu;
+        if (!whole) {
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                gone[n] = (seen >> ((n & 3) + g * 4 + (n >> 2) * 16)) & 1u ? 0u : ~0u;
+                if (gone[n]) x[n] = -kInf;
+#pragma unroll
+                for (int i = 0; i < R::kValPieces; ++i)
+#pragma unroll
+                    for (int k = 0; k < R::kValWords; ++k) r.v[n][i][k] = gone[n] ? 0u : r.v[n][i][k];
+                if constexpr (kInt8) r.vs[n][0] = gone[n] ? 0u : r.vs[n][0], r.vs[n][1] = gone[n] ? 0u : r.vs[n][1];
+            }
+        }
+        // what a probability is multiplied with before it becomes f16: int8 values' scales, by their exponent
+        float top = -kInf;
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            ks_top[n] = 0;
+            if constexpr (kInt8) {
+                uint32_t e = 0;   // exponents of the scales, which are not negative
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) {
+                    const uint32_t s = (r.vs[n][b / 2] >> (b & 1 ? 16 : 0)) & 0x7FFFu;
+                    e = e > s ? e : s;
+                }
+                ks_top[n] = float(int(e >> 10) - 14);
+            }
+            top = fmaxf(top, x[n] + ks_top[n]);
+        }
+        top = over_rows(top, [](float p, float q) { return fmaxf(p, q); });
+        if (__any(top > m + kMost)) {
+            const float to = top > m + kMost ? top - kTop : m, w = weight(m, to);
+            m = to;
+            l *= w;
+#pragma unroll
+            for (int j = 0; j < kOut; ++j) o[j] *= w;
+        }
+        const float ref = m == -kInf ? 0.0f : m;
+        float pr[8];
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            pr[n] = exp2_fast(x[n] - ref);
+            l += pr[n];
+        }
+        if constexpr (kInt8) {
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b) {
+                float pb[8];
+#pragma unroll
+                for (int n = 0; n < 8; ++n) pb[n] = pr[n] * scale_of(r.vs[n], b);
+                f16x8 hi, lo;
+                split8(pb, hi, lo);
+                uint32_t w[8];
+#pragma unroll
+                for (int n = 0; n < 8; ++n) w[n] = r.v[n][b][0] ^ 0x80808080u;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    uint32_t e0[4], e1[4];   // the pair of places 2 k, 2 k + 1 of cells 2 i, 2 i + 1
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        codes4(__builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], k ? 0x07030602u : 0x05010400u), e0[i], e1[i]);
+                    const f16x8 v0 = eight(e0[0], e0[1], e0[2], e0[3]), v1 = eight(e1[0], e1[1], e1[2], e1[3]);
+                    o[b * 4 + 2 * k] = mfma(v0, hi, o[b * 4 + 2 * k]);
+                    o[b * 4 + 2 * k] = mfma(v0, lo, o[b * 4 + 2 * k]);
+                    o[b * 4 + 2 * k + 1] = mfma(v1, hi, o[b * 4 + 2 * k + 1]);
+                    o[b * 4 + 2 * k + 1] = mfma(v1, lo, o[b * 4 + 2 * k + 1]);
+                }
+            }
+        } else {
+            f16x8 hi, lo;
+            split8(pr, hi, lo);
+#pragma unroll
+            for (int i = 0; i < R::kValPieces; ++i)
+#pragma unroll
+                for (int k = 0; k < R::kValWords; ++k) {
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t sel = e ? 0x07060302u : 0x05040100u;
+                        uint32_t w[4];
+#pragma unroll
+                        for (int n = 0; n < 4; ++n) w[n] = __builtin_amdgcn_perm(r.v[2 * n + 1][i][k], r.v[2 * n][i][k], sel);
+                        const f16x8 v = eight(w[0], w[1], w[2], w[3]);
+                        const int j = (i * R::kValWords + k) * 2 + e;
+                        o[j] = mfma(v, hi, o[j]);
+                        o[j] = mfma(v, lo, o[j]);
+                    }
+                }
+        }
+        if (u + 1 < u1) load_values<D, kInt8>(r, a, next_row, lane);
+        next = after;
+    }
+
+    // the waves' results to one m, summed through LDS
+    l = over_rows(l, [](float p, float q) { return p + q; });
+    if (g == 0) s_m[wave][col] = m, s_l[wave][col] = l;
+    __syncthreads();
+    float M = s_m[0][col];
+#pragma unroll
+    for (int w = 1; w < kAttnWaves; ++w) M = fmaxf(M, s_m[w][col]);
+    const float w = weight(m, M);
+#pragma unroll
+    for (int j = 0; j < kOut; j += 4)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const f32x4 four{o[j][i] * w, o[j + 1][i] * w, o[j + 2][i] * w, o[j + 3][i] * w};
+            *reinterpret_cast<f32x4*>(&s_o[wave][col * kRowF + value_of<D, kInt8>(j, g * 4 + i)]) = four;
+        }
+    __syncthreads();
+    constexpr uint32_t kQuads = D / 4;
+    for (uint32_t at = threadIdx.x; at < heads * kQuads; at += kAttnThreads) {
+        const uint32_t i = at / kQuads, d = at % kQuads * 4;
+        float top = s_m[0][i], sum = 0;
+#pragma unroll
+        for (int k = 1; k < kAttnWaves; ++k) top = fmaxf(top, s_m[k][i]);
+        f32x4 acc{};
+#pragma unroll
+        for (int k = 0; k < kAttnWaves; ++k) {
+            acc += *reinterpret_cast<const f32x4*>(&s_o[k][i * kRowF + d]);
+            sum += s_l[k][i] * weight(s_m[k][i], top);
+        }
+        if (p.parts == 1) {
+            st_act4<kF16>(a.out + int64_t(p.s) * a.out_ld, (head0 + i) * D + d, sum == 0 ? f32x4{} : acc / sum);
+            if (d == 0 && a.lse) a.lse[uint64_t(p.s) * a.n_head + head0 + i] = sum == 0 ? -kInf : (top + __builtin_log2f(sum)) * kLn2;
+        } else {
+            float* part = a.ws + uint64_t(p.id) * (16 * kRowF) + i * kRowF;
+            if (d == 0) *reinterpret_cast<f32x4*>(part) = f32x4{top, sum, 0, 0};
+            *reinterpret_cast<f32x4*>(part + 4 + d) = acc;
+        }
+    }
 }
 
+// Joins the parts of one query head: the waves share the parts, then add up through LDS.
 template <int D, bool kF16>
-__global__ void __launch_bounds__(64) attn_join_kernel(AttnArgs a) {
-    const uint32_t lane = threadIdx.x, s = blockIdx.x / a.n_head, head = blockIdx.x % a.n_head;
-    const float* part = a.ws + uint64_t(blockIdx.x) * a.parts * (D + 4);
-    float m = -__builtin_inff(), l = 0;
+__global__ void __launch_bounds__(kAttnThreads) attn_join_kernel(AttnArgs a) {
+    constexpr uint32_t kRowF = D + 4, kLanes = D / 4, kSets = kAttnThreads / kLanes;   // sets of lanes, a part each
+    __shared__ f32x4 s_acc[kSets][kLanes];
+    __shared__ float s_m[kAttnWaves], s_l[kAttnWaves];
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t s = blockIdx.x / a.n_head, head = blockIdx.x - s * a.n_head;
+    Place p;
+    if (!place_of(a, lane, [&](uint32_t at, uint32_t, uint32_t) { return at == s; }, p)) return;
+    if (p.parts <= 1) return;
+    const uint32_t G = a.n_head / a.c.H, h = head / G, tile = (head - h * G) / 16;
+    const uint32_t ht = h * (a.tiles / a.c.H) + tile, i = head - h * G - tile * 16;
+    const float* first = a.ws + (uint64_t(p.id) + uint64_t(ht) * p.parts) * (16 * kRowF) + i * kRowF;
+    const uint64_t step = 16 * kRowF;
+    float m = -kInf;
+    for (uint32_t k = threadIdx.x; k < p.parts; k += kAttnThreads) m = fmaxf(m, first[k * step]);
+#pragma unroll
+    for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+    if (lane == 0) s_m[wave] = m;
+    __syncthreads();
+    m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
+    float l = 0;
+    for (uint32_t k = threadIdx.x; k < p.parts; k += kAttnThreads) l += first[k * step + 1] * weight(first[k * step], m);
+    l = wave_sum(l);
+    if (lane == 0) s_l[wave] = l;
+    const uint32_t set = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
     f32x4 acc{};
-    for (uint32_t i = 0; i < a.parts; ++i, part += D + 4) {
-        const float om = part[0], ol = part[1], top = m > om || m != m ? m : om, w = weight(m, top), ow = weight(om, top);
-        l = l * w + ol * ow;
-        if (lane < D / 4) acc = acc * w + *reinterpret_cast<const f32x4*>(part + 4 + lane * 4) * ow;
-        m = top;
-    }
-    const bool none = m == -__builtin_inff();
-    if (lane < D / 4) st_act4<kF16>(a.out + s * a.out_ld, head * D + lane * 4, none ? f32x4{} : acc / l);
-    if (lane == 0 && a.lse) a.lse[uint64_t(s) * a.n_head + head] = none ? m : (m + __builtin_log2f(l)) * kLn2;
+#pragma unroll 4
+    for (uint32_t k = set; k < p.parts; k += kSets)
+        acc += *reinterpret_cast<const f32x4*>(first + k * step + 4 + d) * weight(first[k * step], m);
+    s_acc[set][d / 4] = acc;
+    __syncthreads();
+    if (set) return;
+#pragma unroll
+    for (uint32_t k = 1; k < kSets; ++k) acc += s_acc[k][d / 4];
+    l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
+    st_act4<kF16>(a.out + int64_t(s) * a.out_ld, head * D + d, l == 0 ? f32x4{} : acc / l);
+    if (d == 0 && a.lse) a.lse[uint64_t(s) * a.n_head + head] = l == 0 ? -kInf : (m + __builtin_log2f(l)) * kLn2;
 }
 
-template <int D, bool kInt8>
-hipError_t launch_of(const AttnArgs& a, bool f16, hipStream_t stream) {
-    const dim3 grid(a.n_seqs * a.n_head, a.parts), join(a.n_seqs * a.n_head);
-    if (f16) {
-        hipLaunchKernelGGL((attn_part_kernel<D, kInt8, true>), grid, dim3(64), 0, stream, a);
-        hipLaunchKernelGGL((attn_join_kernel<D, true>), join, dim3(64), 0, stream, a);
-    } else {
-        hipLaunchKernelGGL((attn_part_kernel<D, kInt8, false>), grid, dim3(64), 0, stream, a);
-        hipLaunchKernelGGL((attn_join_kernel<D, false>), join, dim3(64), 0, stream, a);
-    }
+template <int D, bool kInt8, bool kF16>
+hipError_t launch_of(const AttnArgs& a, hipStream_t stream) {
+    hipLaunchKernelGGL((attn_part_kernel<D, kInt8, kF16>), dim3(a.grid), dim3(kAttnThreads), 0, stream, a);
+    if (a.join) hipLaunchKernelGGL((attn_join_kernel<D, kF16>), dim3(a.n_seqs * a.n_head), dim3(kAttnThreads), 0, stream, a);
     return hipGetLastError();
+}
+template <int D>
+hipError_t launch_of(const AttnArgs& a, int format, bool f16, hipStream_t stream) {
+    if (format == 1) return f16 ? launch_of<D, true, true>(a, stream) : launch_of<D, true, false>(a, stream);
+    return f16 ? launch_of<D, false, true>(a, stream) : launch_of<D, false, false>(a, stream);
 }
 
 }  // namespace
 
+uint64_t plan_attn(AttnArgs& a, int head_dim) {
+    a.tiles = a.c.H * ((a.n_head / a.c.H + 15) / 16);
+    const uint64_t rows = uint64_t(a.n_seqs) * a.tiles;
+    // a window may begin anywhere in a turn, so it can touch a unit more
+    const uint64_t most = ((a.window ? a.window + kTurn : a.max_len) + kUnit - 1) / kUnit;
+    a.slots = 512;
+    a.least = 1;
+    a.join = most > a.least;
+    // parts of all sequences: at most a slot's share each, and one more a sequence
+    const uint64_t shares = a.slots < rows * most ? a.slots : rows * most;
+    a.grid = uint32_t(rows + (a.join ? shares : 0));
+    return a.join ? 2 * shares * 16 * uint64_t(head_dim + 4) * 4 : 16;
+}
+
 hipError_t launch_attn(const AttnArgs& a, int head_dim, int format, bool f16, hipStream_t stream) {
-    const bool q8 = format == 1;
-    if (head_dim == 64) return q8 ? launch_of<64, true>(a, f16, stream) : launch_of<64, false>(a, f16, stream);
-    if (head_dim == 128) return q8 ? launch_of<128, true>(a, f16, stream) : launch_of<128, false>(a, f16, stream);
-    if (head_dim == 256) return q8 ? launch_of<256, true>(a, f16, stream) : launch_of<256, false>(a, f16, stream);
+    if (head_dim == 64) return launch_of<64>(a, format, f16, stream);
+    if (head_dim == 128) return launch_of<128>(a, format, f16, stream);
+    if (head_dim == 256) return launch_of<256>(a, format, f16, stream);
     return hipErrorInvalidValue;
 }
 

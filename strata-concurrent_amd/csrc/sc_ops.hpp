@@ -41,7 +41,10 @@ struct AttnArgs {
     int64_t q_ld, out_ld;                 // bytes from sequence to sequence
     uint32_t n_seqs, n_head, max_len, window;
     float scale;
-    uint32_t chunk, parts;                // cells of a part, parts of a sequence
+    // how the length is split, by plan_attn
+    uint32_t tiles;                       // kv heads times the tiles of 16 query heads of each
+    uint32_t slots, least;                // workgroups the units are shared out among, units of a part at least
+    uint32_t grid, join;                  // workgroups of the launch, whether a sequence can have more than one part
     float* ws;
 };
 
@@ -60,6 +63,8 @@ struct GdnArgs {
 };
 
 hipError_t launch_rope(const RopeArgs& a, int head_dim, int format, bool f16, hipStream_t stream);
+// Fills the split of a call and returns the bytes of its workspace.
+uint64_t plan_attn(AttnArgs& a, int head_dim);
 hipError_t launch_attn(const AttnArgs& a, int head_dim, int format, bool f16, hipStream_t stream);
 hipError_t launch_gdn_step(const GdnArgs& a, int size, bool f16, hipStream_t stream);
 hipError_t launch_gdn_chunk(const GdnArgs& a, int size, bool f16, void* workspace, hipStream_t stream);

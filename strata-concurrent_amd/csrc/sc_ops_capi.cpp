@@ -47,6 +47,7 @@ int cache_args(const char* op, const sc_kv_cache* c, int64_t n_seqs, sc::CacheAr
     if (c->page_size < 1 || c->page_size > 65536) return bad(op, "page_size must be 1 .. 65536");
     if (c->n_pages < 1 || c->n_pages > INT32_MAX) return bad(op, "n_pages must be 1 .. 2^31 - 1");
     if (c->table_ld < 1 || c->table_ld > INT32_MAX / c->page_size) return bad(op, "table_ld * page_size must be 1 .. 2^31 - 1");
+    if (c->n_pages > INT32_MAX / (c->n_head_kv * c->page_size)) return beyond(op, "a pool of 2^31 rows or more");
     if (!c->table && n_seqs > INT32_MAX / c->table_ld) return beyond(op, "an identity table past 2^31 pages");
     if (!c->k || !c->v || off(c->k, 16) || off(c->v, 16)) return bad(op, "the cache's pools must be given, 16-byte aligned");
     if (c->format == SC_KV_INT8 && (!c->k_scale || !c->v_scale || off(c->k_scale, 8) || off(c->v_scale, 8)))
@@ -65,13 +66,7 @@ int cache_args(const char* op, const sc_kv_cache* c, int64_t n_seqs, sc::CacheAr
     return SC_OK;
 }
 
-// Cells of a part of a sequence's length: about 2048 waves of parts, and at least 64 cells each.
-int64_t attn_chunk(int64_t rows, int64_t max_len) {
-    const int64_t want = (rows * max_len + 2047) / 2048;
-    return want < 64 ? 64 : (want + 63) / 64 * 64;
-}
-
-int attn_args(const sc_kv_cache* cache, const sc_attn_decode* d, sc::AttnArgs& a) {
+int attn_args(const sc_kv_cache* cache, const sc_attn_decode* d, sc::AttnArgs& a, uint64_t& ws_bytes) {
     const char* op = "attn_decode";
     if (!d) return bad(op, "missing request");
     if (d->n_seqs < 1 || d->n_seqs > SC_ATTN_MAX_SEQS) return bad(op, "n_seqs must be 1 .. SC_ATTN_MAX_SEQS");
@@ -98,15 +93,9 @@ int attn_args(const sc_kv_cache* cache, const sc_attn_decode* d, sc::AttnArgs& a
     a.max_len = uint32_t(d->max_len);
     a.window = d->window >= d->max_len ? 0 : uint32_t(d->window);
     a.scale = d->scale;
-    a.chunk = uint32_t(attn_chunk(int64_t(d->n_seqs) * d->n_head, d->max_len));
-    a.parts = uint32_t((d->max_len + a.chunk - 1) / a.chunk);
-    if (!a.parts) a.parts = 1;
     a.ws = nullptr;
+    ws_bytes = sc::plan_attn(a, int(cache->head_dim));
     return SC_OK;
-}
-
-uint64_t attn_bytes(const sc_kv_cache* cache, const sc::AttnArgs& a) {
-    return uint64_t(a.n_seqs) * a.n_head * a.parts * uint64_t(cache->head_dim + 4) * 4;
 }
 
 int gdn_args(const char* op, const sc_gdn* d, bool step, sc::GdnArgs& a) {
@@ -215,8 +204,8 @@ int sc_rope_append_async(const sc_kv_cache* cache, const sc_rope_append* d, void
 
 uint64_t sc_attn_decode_workspace_bytes(const sc_kv_cache* cache, const sc_attn_decode* d) {
     sc::AttnArgs a{};
-    if (guarded([&] { return attn_args(cache, d, a); }) != SC_OK) return 0;
-    return attn_bytes(cache, a);
+    uint64_t need = 0;
+    return guarded([&] { return attn_args(cache, d, a, need); }) == SC_OK ? need : 0;
 }
 
 int sc_attn_decode_async(const sc_kv_cache* cache, const sc_attn_decode* d, void* workspace, uint64_t workspace_bytes,
@@ -224,8 +213,9 @@ int sc_attn_decode_async(const sc_kv_cache* cache, const sc_attn_decode* d, void
     return guarded([&] {
         const char* op = "attn_decode";
         sc::AttnArgs a{};
-        if (const int e = attn_args(cache, d, a)) return e;
-        if (!workspace || off(workspace, 16) || workspace_bytes < attn_bytes(cache, a))
+        uint64_t need = 0;
+        if (const int e = attn_args(cache, d, a, need)) return e;
+        if (!workspace || off(workspace, 16) || workspace_bytes < need)
             return bad(op, "workspace missing, not 16-byte aligned or below sc_attn_decode_workspace_bytes");
         a.ws = static_cast<float*>(workspace);
         return launched(sc::launch_attn(a, int(cache->head_dim), cache->format, d->dtype == SC_DTYPE_F16,
