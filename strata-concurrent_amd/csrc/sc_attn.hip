@@ -33,6 +33,7 @@ constexpr float kInf = __builtin_inff();
 constexpr int kAttnWaves = 4, kAttnThreads = kAttnWaves * 64;
 constexpr int kTurn = 32;                       // cells of a wave's turn
 constexpr uint32_t kUnit = kTurn * kAttnWaves;  // cells of a workgroup's turn
+constexpr uint32_t kAttnSlots = 512;            // workgroups that the units are shared out among
 constexpr float kTop = 10.0f, kMost = 15.0f;    // log2 of the largest probability after a new m, and before one is needed
 
 // 2^x by the hardware's instruction (1 unit in the last place; results below the normal range are 0).
@@ -54,8 +55,7 @@ __device__ __forceinline__ float over_rows(float x, F f) {
 struct Span {
     uint32_t first, len, begin, units;   // cells [first, len), counted in units from `begin`, a multiple of a turn
 };
-__device__ __forceinline__ Span span_of(const AttnArgs& a, uint32_t s) {
-    const int64_t n = ld_global<int64_t>(a.lens + s);
+__device__ __forceinline__ Span span_of(const AttnArgs& a, int64_t n) {
     Span p;
     p.len = n < 0 ? 0u : n > int64_t(a.max_len) ? a.max_len : uint32_t(n);
     p.first = a.window && p.len > a.window ? p.len - a.window : 0u;
@@ -64,45 +64,51 @@ __device__ __forceinline__ Span span_of(const AttnArgs& a, uint32_t s) {
     return p;
 }
 
+// The workgroups of a sequence are its parts times its tiles (kv heads and tiles of query heads), the tiles of a part next
+// to each other: they read the same pages.
 struct Place {
-    uint32_t s, ht, part, parts;   // sequence, kv head and tile of query heads, part of its units, how many parts
-    uint32_t id;                   // this part's place in the workspace (parts > 1)
+    uint32_t s, parts;    // sequence, how many parts its units are in
+    uint32_t wg0, ws0;    // its first workgroup, and the first one's place in the workspace (parts > 1)
+    Span span;
 };
 // The units of all sequences are shared out among about `slots` workgroups: a part takes `per` units at most, `per` being
 // what one of them would get, so long and short sequences of a ragged batch give parts of like size.  Every workgroup (and
 // the joining kernel) finds its place from the lengths alone: one load a lane and a scan for 64 sequences.  `find` says
-// whether the workgroup with sequence-wise index range [lo, hi) is the one that is looked for.
+// whether the sequence whose workgroups are [lo, hi) is the one that is looked for.
 template <class Find>
 __device__ __forceinline__ bool place_of(const AttnArgs& a, uint32_t lane, Find find, Place& p) {
-    uint64_t total = 0;
-    for (uint32_t base = 0; base < a.n_seqs; base += 64)
-        if (base + lane < a.n_seqs) total += span_of(a, base + lane).units;
-#pragma unroll
-    for (int m = 1; m < 64; m <<= 1) total += __shfl_xor(total, m);
+    auto length = [&](uint32_t s) { return s < a.n_seqs ? ld_global<int64_t>(a.lens + s) : int64_t(0); };
+    const uint32_t lanes = a.n_seqs < 64 ? a.n_seqs : 64;
+    const int64_t mine = length(lane);   // kept for batches of 64
+    uint64_t total = span_of(a, mine).units;
+    for (uint32_t base = 64; base < a.n_seqs; base += 64) total += span_of(a, length(base + lane)).units;
+    for (uint32_t m = 1; m < lanes; m <<= 1) total += __shfl_xor(total, int(m));   // lanes past the batch add nothing
     uint64_t per = (total * a.tiles + a.slots - 1) / a.slots;
     per = per < a.least ? a.least : per;
     uint32_t wgs = 0, ids = 0;
     for (uint32_t base = 0; base < a.n_seqs; base += 64) {
-        const uint32_t units = base + lane < a.n_seqs ? span_of(a, base + lane).units : 0u;
+        const int64_t n = base ? length(base + lane) : mine;
+        const uint32_t units = span_of(a, n).units;
         const uint32_t parts = base + lane >= a.n_seqs ? 0u : units <= per ? 1u : uint32_t((units + per - 1) / per);
         uint32_t w = parts, d = parts > 1 ? parts : 0u;   // inclusive sums over the lanes
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
+        for (uint32_t m = 1; m < lanes; m <<= 1) {
             const uint32_t ow = __shfl_up(w, m), od = __shfl_up(d, m);
-            if (lane >= uint32_t(m)) w += ow, d += od;
+            if (lane >= m) w += ow, d += od;
         }
         const uint32_t lo = wgs + (w - parts) * a.tiles, hi = wgs + w * a.tiles;
         const uint64_t here = __ballot(base + lane < a.n_seqs && find(base + lane, lo, hi));
         if (here) {
             const int at = __builtin_ctzll(here);
-            p.s = base + at;
-            p.parts = __shfl(parts, at);
-            p.part = __shfl(lo, at);   // the sequence's first workgroup: the caller makes it the part
-            p.id = ids + (__shfl(d, at) - (p.parts > 1 ? p.parts : 0u)) * a.tiles;
+            p.s = __builtin_amdgcn_readfirstlane(base + at);
+            p.parts = __builtin_amdgcn_readlane(parts, at);
+            p.wg0 = __builtin_amdgcn_readlane(lo, at);
+            p.ws0 = ids + (__builtin_amdgcn_readlane(d, at) - (p.parts > 1 ? p.parts : 0u)) * a.tiles;
+            p.span = span_of(a, int64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(n)), at)) |
+                                        uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(uint64_t(n) >> 32)), at))) << 32));
             return true;
         }
-        wgs += __shfl(w, 63) * a.tiles;
-        ids += __shfl(d, 63) * a.tiles;
+        wgs += __builtin_amdgcn_readlane(w, int(lanes - 1)) * a.tiles;   // a whole block of 64: the last one ends the loop
+        ids += __builtin_amdgcn_readlane(d, int(lanes - 1)) * a.tiles;
     }
     return false;
 }
@@ -174,13 +180,18 @@ __device__ __forceinline__ float scale_of(const uint32_t (&s)[2], int block) {
     return float(block & 1 ? t.y : t.x);
 }
 
-// Pool rows of the turn's 32 cells, cell l % 32 in lane l: the row (0 where there is none) and which cells there are.
-__device__ __forceinline__ int32_t row_of(const AttnArgs& a, const Span& p, uint32_t s, uint32_t h, uint32_t base, uint32_t lane) {
-    const uint32_t cell = base + (lane & 31);
-    if (cell < p.first || cell >= p.len) return -1;
-    const uint32_t page = ops_div(cell, a.c.ps);
-    const int32_t phys = cache_page(a.c, s, page);
-    return phys < 0 ? -1 : int32_t((uint32_t(phys) * a.c.H + h) * a.c.ps.d + (cell - page * a.c.ps.d));
+// The page table's entry for cell base + l % 32 of a sequence in lane l; a cell past the table reads the last entry.  The
+// load is only waited for where the entry becomes a row.
+__device__ __forceinline__ int32_t entry_of(const AttnArgs& a, uint32_t s, uint32_t base, uint32_t lane) {
+    const uint32_t cell = base + (lane & 31), page = ops_div(cell < a.c.cells ? cell : a.c.cells - 1, a.c.ps);
+    const int64_t at = int64_t(s) * a.c.table_ld + page;
+    return a.c.table ? ld_global<int32_t>(a.c.table + at) : int32_t(at);
+}
+// The pool row of that cell, or -1 where it is outside the span or not resident.
+__device__ __forceinline__ int32_t row_of(const AttnArgs& a, const Span& p, int32_t entry, uint32_t h, uint32_t base, uint32_t lane) {
+    const uint32_t cell = base + (lane & 31), page = ops_div(cell, a.c.ps);
+    const bool in = cell >= p.first && cell < p.len && uint32_t(entry) < a.c.n_pages;
+    return in ? int32_t((uint32_t(entry) * a.c.H + h) * a.c.ps.d + (cell - page * a.c.ps.d)) : -1;
 }
 
 template <int D, bool kInt8>
@@ -233,51 +244,84 @@ struct Queries {
 // ---- the kernel -----------------------------------------------------------------------------------------------------------
 
 template <int D, bool kInt8, bool kF16>
-__global__ void __launch_bounds__(kAttnThreads, 1) attn_part_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(kAttnThreads, 2) attn_part_kernel(AttnArgs a) {
     using R = Rows<D, kInt8>;
     constexpr int kParts = kF16 ? 1 : 2;        // f16 queries are exact
-    constexpr int kSteps = D / 32, kOut = D / 16, kBlocks = D / 64;
+    constexpr int kOut = D / 16, kBlocks = D / 64;
     constexpr int kRowF = D + 4;                // floats of a head's row in LDS
-    __shared__ Queries<D, kParts> s_q;
+    // the queries' place is taken by the waves' outputs at the end
+    __shared__ union {
+        Queries<D, kParts> q;
+        float o[kAttnWaves][16 * kRowF];
+    } s;
     __shared__ float s_c[16], s_m[kAttnWaves][16], s_l[kAttnWaves][16];
-    __shared__ __align__(16) float s_o[kAttnWaves][16 * kRowF];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t g = lane >> 4, col = lane & 15;
 
+    // In the direct form a workgroup takes one unit, and which one does not depend on the lengths: the first loads need
+    // not wait for them
     Place p;
-    if (!place_of(a, lane, [&](uint32_t, uint32_t lo, uint32_t hi) { return blockIdx.x >= lo && blockIdx.x < hi; }, p)) return;
-    p.s = __builtin_amdgcn_readfirstlane(p.s);
-    p.parts = __builtin_amdgcn_readfirstlane(p.parts);
-    const uint32_t within = blockIdx.x - __builtin_amdgcn_readfirstlane(p.part);
-    p.ht = within / p.parts;
-    p.part = within - p.ht * p.parts;
-    p.id = __builtin_amdgcn_readfirstlane(p.id) + within;
-    const uint32_t per_head = a.tiles / a.c.H, h = p.ht / per_head, G = a.n_head / a.c.H;
-    const uint32_t head0 = h * G + (p.ht - h * per_head) * 16;
+    uint32_t within;
+    int64_t n = 0;
+    if (a.direct) {
+        const uint32_t wgs = a.direct * a.tiles;
+        p.s = blockIdx.x / wgs;
+        within = blockIdx.x - p.s * wgs;
+        n = ld_global<int64_t>(a.lens + p.s);
+        p.ws0 = p.s * wgs;
+    } else {
+        if (!place_of(a, lane, [&](uint32_t, uint32_t lo, uint32_t hi) { return blockIdx.x >= lo && blockIdx.x < hi; }, p)) return;
+        within = blockIdx.x - p.wg0;
+    }
+    const uint32_t part = within / a.tiles, ht = within - part * a.tiles;
+    const uint32_t per_head = a.tiles / a.c.H, h = ht / per_head, G = a.n_head / a.c.H;
+    const uint32_t head0 = h * G + (ht - h * per_head) * 16;
     const uint32_t heads = (h + 1) * G - head0 < 16 ? (h + 1) * G - head0 : 16;
-    Span span = span_of(a, p.s);
-    const uint32_t each = (span.units + p.parts - 1) / p.parts;
-    const uint32_t u0 = p.part * each, u1 = u0 + each < span.units ? u0 + each : span.units;
-    const uint32_t base0 = span.begin + wave * kTurn;
+    uint32_t u0 = part, u1 = part + 1;
+    if (!a.direct) {
+        const uint32_t each = (p.span.units + p.parts - 1) / p.parts;
+        u0 = part * each;
+        u1 = u0 + each < p.span.units ? u0 + each : p.span.units;
+    }
+    uint32_t base0 = (a.direct ? 0u : p.span.begin) + wave * kTurn;
+    // loads return in the order they are asked for: the first turn's table entries, the queries, then that turn's rows
+    int32_t entry = entry_of(a, p.s, base0 + u0 * kUnit, lane);
+    float xq[4][D / 64];   // heads wave, wave + 4, ...: values lane, lane + 64, ...
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < D / 64; ++k) {
+            const uint32_t at = (head0 + (i * 4 + wave < heads ? i * 4 + wave : 0)) * D + k * 64 + lane;
+            const uint8_t* q = a.q + int64_t(p.s) * a.q_ld;
+            if constexpr (kF16) xq[i][k] = float(__builtin_bit_cast(_Float16, ld_global<uint16_t>(q + at * 2)));
+            else xq[i][k] = ld_global<float>(q + at * 4);
+        }
+    if (a.direct) {
+        p.span = span_of(a, n);
+        p.parts = p.span.units ? p.span.units : 1;
+        if (part >= p.parts) return;
+        u1 = u1 < p.span.units ? u1 : p.span.units;
+    }
+    const Span& span = p.span;
 
     // the first turn's rows are on their way while the queries are laid out
     R r;
-    int32_t row = u0 < u1 ? row_of(a, span, p.s, h, base0 + u0 * kUnit, lane) : -1;
+    int32_t row = row_of(a, span, entry, h, base0 + u0 * kUnit, lane);
     uint32_t there = uint32_t(__ballot(row >= 0));
     row = row < 0 ? 0 : row;
     if (u0 < u1) {
+        entry = entry_of(a, p.s, base0 + (u0 + 1) * kUnit, lane);
         load_keys<D, kInt8>(r, a, row, lane);
         load_values<D, kInt8>(r, a, row, lane);
     }
-    for (uint32_t i = wave; i < 16; i += kAttnWaves) {
-        // head i: values lane, lane + 64, ...; an f32 head is scaled by a power of two to a largest value of 1 .. 2
+#pragma unroll
+    for (uint32_t i4 = 0; i4 < 4; ++i4) {
+        // an f32 head is scaled by a power of two to a largest value of 1 .. 2
+        const uint32_t i = i4 * 4 + wave;
         float x[D / 64], top = 0;
-        const uint8_t* q = a.q + int64_t(p.s) * a.q_ld;
 #pragma unroll
         for (int k = 0; k < D / 64; ++k) {
-            const uint32_t at = (head0 + i) * D + k * 64 + lane;
-            if constexpr (kF16) x[k] = i < heads ? float(__builtin_bit_cast(_Float16, ld_global<uint16_t>(q + at * 2))) : 0.0f;
-            else x[k] = i < heads ? ld_global<float>(q + at * 4) : 0.0f;
+            x[k] = i < heads ? xq[i4][k] : 0.0f;
             top = fmaxf(top, fabsf(x[k]));
         }
         float by = 1.0f, back = 1.0f;
@@ -298,9 +342,9 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_part_kernel(AttnArgs a) 
             // f16 rows: step d / 32, group (d % 32) / 8.  int8 rows: half u of 64-value step, group (d % 64) / 16
             const uint32_t step = kInt8 ? d / 64 * 2 + (d % 16) / 8 : d / 32, grp = kInt8 ? (d % 64) / 16 : (d % 32) / 8;
             const _Float16 hi = _Float16(x[k] * by);
-            reinterpret_cast<_Float16*>(&s_q.q[0][step][grp * 16 + i])[d % 8] = hi;
+            reinterpret_cast<_Float16*>(&s.q.q[0][step][grp * 16 + i])[d % 8] = hi;
             if constexpr (!kF16)
-                reinterpret_cast<_Float16*>(&s_q.q[kParts - 1][step][grp * 16 + i])[d % 8] = _Float16(x[k] * by - float(hi));
+                reinterpret_cast<_Float16*>(&s.q.q[kParts - 1][step][grp * 16 + i])[d % 8] = _Float16(x[k] * by - float(hi));
         }
     }
     __syncthreads();
@@ -310,18 +354,24 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_part_kernel(AttnArgs a) 
 #pragma unroll
     for (int j = 0; j < kOut; ++j) o[j] = f32x4{};
     float m = -kInf, l = 0;
-    // a table entry is read two turns ahead of its rows: loads return in order, so one that was asked for after a turn's
-    // rows could only be used once they all have come
-    int32_t next = u0 + 1 < u1 ? row_of(a, span, p.s, h, base0 + (u0 + 1) * kUnit, lane) : -1;
+    // a turn's table entries are asked for before the rows of the turn before it: asked for after them, they would only
+    // come when all of those have
     for (uint32_t u = u0; u < u1; ++u) {
-        // scores: x[t * 4 + i] of cell 16 t + 4 g + i
+        // scores: x[t * 4 + i] of cell 16 t + 4 g + i.  The queries are read from LDS every turn, two steps at a time (the
+        // barriers to the compiler): kept in registers they would take the place of rows in flight
         float x[8], ks_top[8];
+        f32x4 hi[2]{}, lo[2]{};
 #pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            f32x4 hi{}, lo{};
-            if constexpr (kInt8) {
+        for (int b = 0; b < kBlocks; ++b) {
+            asm volatile("" ::: "memory");
+            f16x8 q[kParts][2];
 #pragma unroll
-                for (int b = 0; b < kBlocks; ++b) {
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < kParts; ++i) q[i][k] = __builtin_bit_cast(f16x8, s.q.q[i][2 * b + k][lane]);
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                if constexpr (kInt8) {
                     f32x4 bh{}, bl{};
                     uint32_t w[8];
 #pragma unroll
@@ -329,38 +379,40 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_part_kernel(AttnArgs a) 
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         const f16x8 key = eight(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-                        bh = mfma(key, __builtin_bit_cast(f16x8, s_q.q[0][2 * b + k][lane]), bh);
-                        if constexpr (!kF16) bl = mfma(key, __builtin_bit_cast(f16x8, s_q.q[kParts - 1][2 * b + k][lane]), bl);
+                        bh = mfma(key, q[0][k], bh);
+                        if constexpr (!kF16) bl = mfma(key, q[kParts - 1][k], bl);
                     }
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         const float ks = scale_of(r.ks[t * 4 + i], b);
-                        hi[i] += ks * bh[i];
-                        if constexpr (!kF16) lo[i] += ks * bl[i];
+                        hi[t][i] += ks * bh[i];
+                        if constexpr (!kF16) lo[t][i] += ks * bl[i];
+                    }
+                } else {
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const f16x8 key = __builtin_bit_cast(f16x8, r.k[t][2 * b + k]);
+                        hi[t] = mfma(key, q[0][k], hi[t]);
+                        if constexpr (!kF16) lo[t] = mfma(key, q[kParts - 1][k], lo[t]);
                     }
                 }
-            } else {
-#pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
-                    const f16x8 key = __builtin_bit_cast(f16x8, r.k[t][k]);
-                    hi = mfma(key, __builtin_bit_cast(f16x8, s_q.q[0][k][lane]), hi);
-                    if constexpr (!kF16) lo = mfma(key, __builtin_bit_cast(f16x8, s_q.q[kParts - 1][k][lane]), lo);
-                }
             }
+        }
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                // an infinite key makes the low part's product NaN: the high part has the score
-                const float s = kF16 ? hi[i] : fabsf(hi[i]) < kInf ? hi[i] + lo[i] : hi[i];
-                x[t * 4 + i] = s * c;
-            }
+        for (int n = 0; n < 8; ++n) {
+            // an infinite key makes the low part's product NaN: the high part has the score
+            const float high = hi[n / 4][n % 4], sum = kF16 || !(fabsf(high) < kInf) ? high : high + lo[n / 4][n % 4];
+            x[n] = sum * c;
         }
         // the next turn's keys take the place of this one's
         const uint32_t seen = there;
-        int32_t after = -1, next_row = next < 0 ? 0 : next;
-        if (u + 1 < u1) {
-            there = uint32_t(__ballot(next >= 0));
-            if (u + 2 < u1) after = row_of(a, span, p.s, h, base0 + (u + 2) * kUnit, lane);
-            load_keys<D, kInt8>(r, a, next_row, lane);
+        const bool more = u + 1 < u1;
+        if (more) {
+            row = row_of(a, span, entry, h, base0 + (u + 1) * kUnit, lane);
+            there = uint32_t(__ballot(row >= 0));
+            row = row < 0 ? 0 : row;
+            entry = entry_of(a, p.s, base0 + (u + 2) * kUnit, lane);
+            load_keys<D, kInt8>(r, a, row, lane);
         }
         uint32_t gone[8];   // all ones where a cell is not there
         const bool whole = seen == 0xFFFFFFFFu;
@@ -451,8 +503,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_part_kernel(AttnArgs a) 
                     }
                 }
         }
-        if (u + 1 < u1) load_values<D, kInt8>(r, a, next_row, lane);
-        next = after;
+        if (more) load_values<D, kInt8>(r, a, row, lane);
     }
 
     // the waves' results to one m, summed through LDS
@@ -468,7 +519,7 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_part_kernel(AttnArgs a) 
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const f32x4 four{o[j][i] * w, o[j + 1][i] * w, o[j + 2][i] * w, o[j + 3][i] * w};
-            *reinterpret_cast<f32x4*>(&s_o[wave][col * kRowF + value_of<D, kInt8>(j, g * 4 + i)]) = four;
+            *reinterpret_cast<f32x4*>(&s.o[wave][col * kRowF + value_of<D, kInt8>(j, g * 4 + i)]) = four;
         }
     __syncthreads();
     constexpr uint32_t kQuads = D / 4;
@@ -480,56 +531,73 @@ __global__ void __launch_bounds__(kAttnThreads, 1) attn_part_kernel(AttnArgs a) 
         f32x4 acc{};
 #pragma unroll
         for (int k = 0; k < kAttnWaves; ++k) {
-            acc += *reinterpret_cast<const f32x4*>(&s_o[k][i * kRowF + d]);
+            acc += *reinterpret_cast<const f32x4*>(&s.o[k][i * kRowF + d]);
             sum += s_l[k][i] * weight(s_m[k][i], top);
         }
         if (p.parts == 1) {
             st_act4<kF16>(a.out + int64_t(p.s) * a.out_ld, (head0 + i) * D + d, sum == 0 ? f32x4{} : acc / sum);
             if (d == 0 && a.lse) a.lse[uint64_t(p.s) * a.n_head + head0 + i] = sum == 0 ? -kInf : (top + __builtin_log2f(sum)) * kLn2;
         } else {
-            float* part = a.ws + uint64_t(p.id) * (16 * kRowF) + i * kRowF;
+            float* part = a.ws + uint64_t(p.ws0 + within) * (16 * kRowF) + i * kRowF;
             if (d == 0) *reinterpret_cast<f32x4*>(part) = f32x4{top, sum, 0, 0};
             *reinterpret_cast<f32x4*>(part + 4 + d) = acc;
         }
     }
 }
 
-// Joins the parts of one query head: the waves share the parts, then add up through LDS.
-template <int D, bool kF16>
+// Joins the parts of kCols values of one query head: sets of lanes share the parts, then add up through LDS.
+template <int D, int kCols, bool kF16>
 __global__ void __launch_bounds__(kAttnThreads) attn_join_kernel(AttnArgs a) {
-    constexpr uint32_t kRowF = D + 4, kLanes = D / 4, kSets = kAttnThreads / kLanes;   // sets of lanes, a part each
+    constexpr uint32_t kRowF = D + 4, kLanes = kCols / 4, kSets = kAttnThreads / kLanes;
     __shared__ f32x4 s_acc[kSets][kLanes];
-    __shared__ float s_m[kAttnWaves], s_l[kAttnWaves];
+    __shared__ float s_w[kAttnSlots + 1], s_m[kAttnWaves], s_l[kAttnWaves];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t s = blockIdx.x / a.n_head, head = blockIdx.x - s * a.n_head;
     Place p;
-    if (!place_of(a, lane, [&](uint32_t at, uint32_t, uint32_t) { return at == s; }, p)) return;
+    if (a.direct) {
+        p.parts = span_of(a, ld_global<int64_t>(a.lens + s)).units;
+        p.ws0 = s * a.direct * a.tiles;
+    } else if (!place_of(a, lane, [&](uint32_t at, uint32_t, uint32_t) { return at == s; }, p)) {
+        return;
+    }
     if (p.parts <= 1) return;
     const uint32_t G = a.n_head / a.c.H, h = head / G, tile = (head - h * G) / 16;
     const uint32_t ht = h * (a.tiles / a.c.H) + tile, i = head - h * G - tile * 16;
-    const float* first = a.ws + (uint64_t(p.id) + uint64_t(ht) * p.parts) * (16 * kRowF) + i * kRowF;
-    const uint64_t step = 16 * kRowF;
-    float m = -kInf;
-    for (uint32_t k = threadIdx.x; k < p.parts; k += kAttnThreads) m = fmaxf(m, first[k * step]);
+    const uint64_t step = uint64_t(a.tiles) * (16 * kRowF);   // from part to part
+    const float* first = a.ws + (uint64_t(p.ws0) + ht) * (16 * kRowF) + i * kRowF;
+    constexpr uint32_t kMine = (kAttnSlots + 1 + kAttnThreads - 1) / kAttnThreads;   // parts whose statistics a thread reads
+    float pm[kMine], pl[kMine], m = -kInf, l = 0;
+#pragma unroll
+    for (uint32_t k = 0; k < kMine; ++k) {
+        const uint32_t at = threadIdx.x + k * kAttnThreads;
+        pm[k] = at < p.parts ? first[at * step] : -kInf;
+        pl[k] = at < p.parts ? first[at * step + 1] : 0.0f;
+        m = fmaxf(m, pm[k]);
+    }
 #pragma unroll
     for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
     if (lane == 0) s_m[wave] = m;
     __syncthreads();
     m = fmaxf(fmaxf(s_m[0], s_m[1]), fmaxf(s_m[2], s_m[3]));
-    float l = 0;
-    for (uint32_t k = threadIdx.x; k < p.parts; k += kAttnThreads) l += first[k * step + 1] * weight(first[k * step], m);
+#pragma unroll
+    for (uint32_t k = 0; k < kMine; ++k) {
+        const uint32_t at = threadIdx.x + k * kAttnThreads;
+        const float w = weight(pm[k], m);
+        l += pl[k] * w;
+        if (at < p.parts) s_w[at] = w;
+    }
     l = wave_sum(l);
     if (lane == 0) s_l[wave] = l;
-    const uint32_t set = threadIdx.x / kLanes, d = threadIdx.x % kLanes * 4;
+    __syncthreads();
+    const uint32_t set = threadIdx.x / kLanes, d = blockIdx.y * kCols + threadIdx.x % kLanes * 4;
     f32x4 acc{};
-#pragma unroll 4
-    for (uint32_t k = set; k < p.parts; k += kSets)
-        acc += *reinterpret_cast<const f32x4*>(first + k * step + 4 + d) * weight(first[k * step], m);
-    s_acc[set][d / 4] = acc;
+#pragma unroll 8
+    for (uint32_t k = set; k < p.parts; k += kSets) acc += *reinterpret_cast<const f32x4*>(first + k * step + 4 + d) * s_w[k];
+    s_acc[set][threadIdx.x % kLanes] = acc;
     __syncthreads();
     if (set) return;
 #pragma unroll
-    for (uint32_t k = 1; k < kSets; ++k) acc += s_acc[k][d / 4];
+    for (uint32_t k = 1; k < kSets; ++k) acc += s_acc[k][threadIdx.x];
     l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
     st_act4<kF16>(a.out + int64_t(s) * a.out_ld, head * D + d, l == 0 ? f32x4{} : acc / l);
     if (d == 0 && a.lse) a.lse[uint64_t(s) * a.n_head + head] = l == 0 ? -kInf : (m + __builtin_log2f(l)) * kLn2;
@@ -538,7 +606,10 @@ __global__ void __launch_bounds__(kAttnThreads) attn_join_kernel(AttnArgs a) {
 template <int D, bool kInt8, bool kF16>
 hipError_t launch_of(const AttnArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL((attn_part_kernel<D, kInt8, kF16>), dim3(a.grid), dim3(kAttnThreads), 0, stream, a);
-    if (a.join) hipLaunchKernelGGL((attn_join_kernel<D, kF16>), dim3(a.n_seqs * a.n_head), dim3(kAttnThreads), 0, stream, a);
+    // a head's parts by one workgroup where the heads fill the chip, by one for 64 values each where they do not
+    const uint32_t rows = a.n_seqs * a.n_head;
+    if (a.join && rows >= 128) hipLaunchKernelGGL((attn_join_kernel<D, D, kF16>), dim3(rows), dim3(kAttnThreads), 0, stream, a);
+    else if (a.join) hipLaunchKernelGGL((attn_join_kernel<D, 64, kF16>), dim3(rows, D / 64), dim3(kAttnThreads), 0, stream, a);
     return hipGetLastError();
 }
 template <int D>
@@ -554,12 +625,13 @@ uint64_t plan_attn(AttnArgs& a, int head_dim) {
     const uint64_t rows = uint64_t(a.n_seqs) * a.tiles;
     // a window may begin anywhere in a turn, so it can touch a unit more
     const uint64_t most = ((a.window ? a.window + kTurn : a.max_len) + kUnit - 1) / kUnit;
-    a.slots = 512;
+    a.slots = kAttnSlots;
     a.least = 1;
     a.join = most > a.least;
+    a.direct = a.join && !a.window && rows * most <= a.slots ? uint32_t(most) : 0;
     // parts of all sequences: at most a slot's share each, and one more a sequence
     const uint64_t shares = a.slots < rows * most ? a.slots : rows * most;
-    a.grid = uint32_t(rows + (a.join ? shares : 0));
+    a.grid = uint32_t(a.direct ? rows * most : rows + (a.join ? shares : 0));
     return a.join ? 2 * shares * 16 * uint64_t(head_dim + 4) * 4 : 16;
 }
 

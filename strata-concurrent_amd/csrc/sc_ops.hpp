@@ -45,6 +45,7 @@ struct AttnArgs {
     uint32_t tiles;                       // kv heads times the tiles of 16 query heads of each
     uint32_t slots, least;                // workgroups the units are shared out among, units of a part at least
     uint32_t grid, join;                  // workgroups of the launch, whether a sequence can have more than one part
+    uint32_t direct;                      // units a sequence can have, where each is a workgroup of its own; else 0
     float* ws;
 };
 
