@@ -50,6 +50,18 @@ __device__ __forceinline__ float over_rows(float x, F f) {
     return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// Inclusive sums over the wave's lanes, by row shifts and row broadcasts (no trip through LDS).
+__device__ __forceinline__ uint32_t scan_add(uint32_t x) {
+    x += uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x111, 0xF, 0xF, false));   // row_shr 1, 2, 4, 8
+    x += uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x112, 0xF, 0xF, false));
+    x += uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x114, 0xF, 0xF, false));
+    x += uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x118, 0xF, 0xF, false));
+    x += uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x142, 0xA, 0xF, false));   // lane 15 of a row to the next one
+    x += uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x143, 0xC, 0xF, false));   // lane 31 to the upper half
+    return x;
+}
+__device__ __forceinline__ uint32_t last_lane(uint32_t x) { return uint32_t(__builtin_amdgcn_readlane(int(x), 63)); }
+
 // ---- which cells a workgroup takes ------------------------------------------------------------------------------------
 
 struct Span {
@@ -72,43 +84,40 @@ struct Place {
     Span span;
 };
 // The units of all sequences are shared out among about `slots` workgroups: a part takes `per` units at most, `per` being
-// what one of them would get, so long and short sequences of a ragged batch give parts of like size.  Every workgroup (and
-// the joining kernel) finds its place from the lengths alone: one load a lane and a scan for 64 sequences.  `find` says
-// whether the sequence whose workgroups are [lo, hi) is the one that is looked for.
-template <class Find>
-__device__ __forceinline__ bool place_of(const AttnArgs& a, uint32_t lane, Find find, Place& p) {
+// what one of them would get, so long and short sequences of a ragged batch give parts of like size.  Every workgroup
+// finds its place from the lengths alone: one load a lane and a few scans for 64 sequences.
+__device__ __forceinline__ bool place_of(const AttnArgs& a, uint32_t lane, uint32_t wg, Place& p) {
     auto length = [&](uint32_t s) { return s < a.n_seqs ? ld_global<int64_t>(a.lens + s) : int64_t(0); };
-    const uint32_t lanes = a.n_seqs < 64 ? a.n_seqs : 64;
     const int64_t mine = length(lane);   // kept for batches of 64
-    uint64_t total = span_of(a, mine).units;
-    for (uint32_t base = 64; base < a.n_seqs; base += 64) total += span_of(a, length(base + lane)).units;
-    for (uint32_t m = 1; m < lanes; m <<= 1) total += __shfl_xor(total, int(m));   // lanes past the batch add nothing
-    uint64_t per = (total * a.tiles + a.slots - 1) / a.slots;
-    per = per < a.least ? a.least : per;
+    const uint32_t my_units = span_of(a, mine).units;
+    uint32_t sum = my_units;             // at most 2^24 units a sequence and 16 sequences a lane
+    for (uint32_t base = 64; base < a.n_seqs; base += 64) sum += span_of(a, length(base + lane)).units;
+    const uint64_t total = uint64_t(last_lane(scan_add(sum & 0xFFFFFFu))) + (uint64_t(last_lane(scan_add(sum >> 24))) << 24);
+    uint64_t share = (total * a.tiles + a.slots - 1) / a.slots;
+    uint32_t per = share < a.least ? a.least : uint32_t(share);   // below 2^31: a sequence has at most 2^24 units
+    auto parts_of = [&](uint32_t s, uint32_t units) { return s >= a.n_seqs ? 0u : units <= per ? 1u : (units + per - 1) / per; };
+    // a few workgroups more than run at once would run alone at the end; twice the share is always enough here
+    if (a.n_seqs <= 64 && a.n_seqs * a.tiles * 2 <= a.slots)
+        while (last_lane(scan_add(parts_of(lane, my_units))) * a.tiles > a.slots) per += per / 32 + 1;
     uint32_t wgs = 0, ids = 0;
     for (uint32_t base = 0; base < a.n_seqs; base += 64) {
         const int64_t n = base ? length(base + lane) : mine;
-        const uint32_t units = span_of(a, n).units;
-        const uint32_t parts = base + lane >= a.n_seqs ? 0u : units <= per ? 1u : uint32_t((units + per - 1) / per);
-        uint32_t w = parts, d = parts > 1 ? parts : 0u;   // inclusive sums over the lanes
-        for (uint32_t m = 1; m < lanes; m <<= 1) {
-            const uint32_t ow = __shfl_up(w, m), od = __shfl_up(d, m);
-            if (lane >= m) w += ow, d += od;
-        }
+        const uint32_t parts = parts_of(base + lane, base ? span_of(a, n).units : my_units), more = parts > 1 ? parts : 0u;
+        const uint32_t w = scan_add(parts), d = scan_add(more);
         const uint32_t lo = wgs + (w - parts) * a.tiles, hi = wgs + w * a.tiles;
-        const uint64_t here = __ballot(base + lane < a.n_seqs && find(base + lane, lo, hi));
+        const uint64_t here = __ballot(wg >= lo && wg < hi);
         if (here) {
             const int at = __builtin_ctzll(here);
             p.s = __builtin_amdgcn_readfirstlane(base + at);
             p.parts = __builtin_amdgcn_readlane(parts, at);
             p.wg0 = __builtin_amdgcn_readlane(lo, at);
-            p.ws0 = ids + (__builtin_amdgcn_readlane(d, at) - (p.parts > 1 ? p.parts : 0u)) * a.tiles;
+            p.ws0 = ids + __builtin_amdgcn_readlane(d - more, at) * a.tiles;
             p.span = span_of(a, int64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(n)), at)) |
                                         uint64_t(uint32_t(__builtin_amdgcn_readlane(int(uint32_t(uint64_t(n) >> 32)), at))) << 32));
             return true;
         }
-        wgs += __builtin_amdgcn_readlane(w, int(lanes - 1)) * a.tiles;   // a whole block of 64: the last one ends the loop
-        ids += __builtin_amdgcn_readlane(d, int(lanes - 1)) * a.tiles;
+        wgs += last_lane(w) * a.tiles;
+        ids += last_lane(d) * a.tiles;
     }
     return false;
 }
@@ -194,6 +203,12 @@ __device__ __forceinline__ int32_t row_of(const AttnArgs& a, const Span& p, int3
     return in ? int32_t((uint32_t(entry) * a.c.H + h) * a.c.ps.d + (cell - page * a.c.ps.d)) : -1;
 }
 
+// A load of what is read once, past the caches' keeping.
+template <class T>
+__device__ __forceinline__ T ld_once(const void* p) {
+    return __builtin_nontemporal_load((const __attribute__((address_space(1))) T*) (p));
+}
+
 template <int D, bool kInt8>
 __device__ __forceinline__ void load_keys(Rows<D, kInt8>& r, const AttnArgs& a, int32_t row, uint32_t lane) {
     using R = Rows<D, kInt8>;
@@ -203,7 +218,7 @@ __device__ __forceinline__ void load_keys(Rows<D, kInt8>& r, const AttnArgs& a, 
         const uint32_t at = uint32_t(__shfl(row, int(t * 16 + (lane & 15))));
         const uint8_t* p = a.c.k + at * bytes + (lane >> 4) * 16;
 #pragma unroll
-        for (int i = 0; i < R::kKeySteps; ++i) r.k[t][i] = ld_global<ops_u32x4>(p + i * 64);
+        for (int i = 0; i < R::kKeySteps; ++i) r.k[t][i] = kInt8 ? ld_once<ops_u32x4>(p + i * 64) : ld_global<ops_u32x4>(p + i * 64);
     }
 }
 
@@ -219,7 +234,7 @@ __device__ __forceinline__ void load_values(Rows<D, kInt8>& r, const AttnArgs& a
 #pragma unroll
         for (int i = 0; i < R::kValPieces; ++i) {
             if constexpr (R::kValWords == 4) {
-                const ops_u32x4 w = ld_global<ops_u32x4>(p + i * 256);
+                const ops_u32x4 w = ld_once<ops_u32x4>(p + i * 256);
                 r.v[n][i][0] = w.x, r.v[n][i][1] = w.y, r.v[n][i][2] = w.z, r.v[n][i][3] = w.w;
             } else if constexpr (R::kValWords == 2) {
                 const ops_u32x2 w = ld_global<ops_u32x2>(p);
@@ -270,7 +285,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_part_kernel(AttnArgs a) 
         n = ld_global<int64_t>(a.lens + p.s);
         p.ws0 = p.s * wgs;
     } else {
-        if (!place_of(a, lane, [&](uint32_t, uint32_t lo, uint32_t hi) { return blockIdx.x >= lo && blockIdx.x < hi; }, p)) return;
+        if (!place_of(a, lane, blockIdx.x, p)) return;
         within = blockIdx.x - p.wg0;
     }
     const uint32_t part = within / a.tiles, ht = within - part * a.tiles;
@@ -303,6 +318,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_part_kernel(AttnArgs a) 
         u1 = u1 < p.span.units ? u1 : p.span.units;
     }
     const Span& span = p.span;
+    // where the joining kernel finds the sequence's parts
+    if (a.join && within == 0 && threadIdx.x == 0) a.where[p.s] = ops_u32x2{p.parts, p.ws0};
 
     // the first turn's rows are on their way while the queries are laid out
     R r;
@@ -553,27 +570,29 @@ __global__ void __launch_bounds__(kAttnThreads) attn_join_kernel(AttnArgs a) {
     __shared__ float s_w[kAttnSlots + 1], s_m[kAttnWaves], s_l[kAttnWaves];
     const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint32_t s = blockIdx.x / a.n_head, head = blockIdx.x - s * a.n_head;
-    Place p;
-    if (a.direct) {
-        p.parts = span_of(a, ld_global<int64_t>(a.lens + s)).units;
-        p.ws0 = s * a.direct * a.tiles;
-    } else if (!place_of(a, lane, [&](uint32_t at, uint32_t, uint32_t) { return at == s; }, p)) {
-        return;
-    }
-    if (p.parts <= 1) return;
+    const ops_u32x2 where = a.where[s];
+    const uint32_t parts = where.x;
+    if (parts <= 1) return;
     const uint32_t G = a.n_head / a.c.H, h = head / G, tile = (head - h * G) / 16;
     const uint32_t ht = h * (a.tiles / a.c.H) + tile, i = head - h * G - tile * 16;
     const uint64_t step = uint64_t(a.tiles) * (16 * kRowF);   // from part to part
-    const float* first = a.ws + (uint64_t(p.ws0) + ht) * (16 * kRowF) + i * kRowF;
+    const float* first = a.ws + (uint64_t(where.y) + ht) * (16 * kRowF) + i * kRowF;
     constexpr uint32_t kMine = (kAttnSlots + 1 + kAttnThreads - 1) / kAttnThreads;   // parts whose statistics a thread reads
+    constexpr uint32_t kAhead = 8;                                                   // its parts that are read meanwhile
+    const uint32_t set = threadIdx.x / kLanes, d = blockIdx.y * kCols + threadIdx.x % kLanes * 4;
     float pm[kMine], pl[kMine], m = -kInf, l = 0;
 #pragma unroll
     for (uint32_t k = 0; k < kMine; ++k) {
         const uint32_t at = threadIdx.x + k * kAttnThreads;
-        pm[k] = at < p.parts ? first[at * step] : -kInf;
-        pl[k] = at < p.parts ? first[at * step + 1] : 0.0f;
-        m = fmaxf(m, pm[k]);
+        const ops_u32x2 ml = ld_global<ops_u32x2>(first + (at < parts ? at : 0) * step);
+        pm[k] = at < parts ? __uint_as_float(ml.x) : -kInf;
+        pl[k] = at < parts ? __uint_as_float(ml.y) : 0.0f;
     }
+    f32x4 ahead[kAhead];
+#pragma unroll
+    for (uint32_t k = 0; k < kAhead; ++k) ahead[k] = ld_global<f32x4>(first + (set + k * kSets < parts ? set + k * kSets : 0) * step + 4 + d);
+#pragma unroll
+    for (uint32_t k = 0; k < kMine; ++k) m = fmaxf(m, pm[k]);
 #pragma unroll
     for (int x = 1; x < 64; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
     if (lane == 0) s_m[wave] = m;
@@ -584,15 +603,17 @@ __global__ void __launch_bounds__(kAttnThreads) attn_join_kernel(AttnArgs a) {
         const uint32_t at = threadIdx.x + k * kAttnThreads;
         const float w = weight(pm[k], m);
         l += pl[k] * w;
-        if (at < p.parts) s_w[at] = w;
+        if (at < parts) s_w[at] = w;
     }
     l = wave_sum(l);
     if (lane == 0) s_l[wave] = l;
     __syncthreads();
-    const uint32_t set = threadIdx.x / kLanes, d = blockIdx.y * kCols + threadIdx.x % kLanes * 4;
     f32x4 acc{};
+#pragma unroll
+    for (uint32_t k = 0; k < kAhead; ++k)
+        if (set + k * kSets < parts) acc += ahead[k] * s_w[set + k * kSets];
 #pragma unroll 8
-    for (uint32_t k = set; k < p.parts; k += kSets) acc += *reinterpret_cast<const f32x4*>(first + k * step + 4 + d) * s_w[k];
+    for (uint32_t k = set + kAhead * kSets; k < parts; k += kSets) acc += ld_global<f32x4>(first + k * step + 4 + d) * s_w[k];
     s_acc[set][threadIdx.x % kLanes] = acc;
     __syncthreads();
     if (set) return;
@@ -632,7 +653,12 @@ uint64_t plan_attn(AttnArgs& a, int head_dim) {
     // parts of all sequences: at most a slot's share each, and one more a sequence
     const uint64_t shares = a.slots < rows * most ? a.slots : rows * most;
     a.grid = uint32_t(a.direct ? rows * most : rows + (a.join ? shares : 0));
-    return a.join ? 2 * shares * 16 * uint64_t(head_dim + 4) * 4 : 16;
+    return a.join ? 2 * shares * 16 * uint64_t(head_dim + 4) * 4 + (uint64_t(a.n_seqs) * 8 + 15) / 16 * 16 : 16;
+}
+
+void place_attn(AttnArgs& a, void* workspace, uint64_t bytes) {
+    a.ws = static_cast<float*>(workspace);
+    if (a.join) a.where = reinterpret_cast<ops_u32x2*>(static_cast<uint8_t*>(workspace) + bytes - (uint64_t(a.n_seqs) * 8 + 15) / 16 * 16);
 }
 
 hipError_t launch_attn(const AttnArgs& a, int head_dim, int format, bool f16, hipStream_t stream) {

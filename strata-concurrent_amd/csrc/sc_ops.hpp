@@ -10,6 +10,8 @@
 
 namespace sc {
 
+using ops_u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
+
 // A paged cache (sc_kv_cache) as the kernels see it.
 struct CacheArgs {
     uint8_t *k, *v;
@@ -46,7 +48,8 @@ struct AttnArgs {
     uint32_t slots, least;                // workgroups the units are shared out among, units of a part at least
     uint32_t grid, join;                  // workgroups of the launch, whether a sequence can have more than one part
     uint32_t direct;                      // units a sequence can have, where each is a workgroup of its own; else 0
-    float* ws;
+    float* ws;                            // the parts' results
+    ops_u32x2* where;                     // [n_seqs] parts of a sequence and its first one's place
 };
 
 struct GdnArgs {
@@ -66,13 +69,14 @@ struct GdnArgs {
 hipError_t launch_rope(const RopeArgs& a, int head_dim, int format, bool f16, hipStream_t stream);
 // Fills the split of a call and returns the bytes of its workspace.
 uint64_t plan_attn(AttnArgs& a, int head_dim);
+// Places its parts in a workspace of those bytes.
+void place_attn(AttnArgs& a, void* workspace, uint64_t bytes);
 hipError_t launch_attn(const AttnArgs& a, int head_dim, int format, bool f16, hipStream_t stream);
 hipError_t launch_gdn_step(const GdnArgs& a, int size, bool f16, hipStream_t stream);
 hipError_t launch_gdn_chunk(const GdnArgs& a, int size, bool f16, void* workspace, hipStream_t stream);
 
 #if defined(__HIPCC__)
 using f32x4 = __attribute__((ext_vector_type(4))) float;
-using ops_u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
 using ops_u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 using f16x2 = __attribute__((ext_vector_type(2))) _Float16;
 using f16x4 = __attribute__((ext_vector_type(4))) _Float16;

@@ -217,7 +217,7 @@ int sc_attn_decode_async(const sc_kv_cache* cache, const sc_attn_decode* d, void
         if (const int e = attn_args(cache, d, a, need)) return e;
         if (!workspace || off(workspace, 16) || workspace_bytes < need)
             return bad(op, "workspace missing, not 16-byte aligned or below sc_attn_decode_workspace_bytes");
-        a.ws = static_cast<float*>(workspace);
+        sc::place_attn(a, workspace, need);
         return launched(sc::launch_attn(a, int(cache->head_dim), cache->format, d->dtype == SC_DTYPE_F16,
                                         static_cast<hipStream_t>(stream)), op);
     });
