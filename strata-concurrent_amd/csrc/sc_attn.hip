@@ -50,18 +50,6 @@ __device__ __forceinline__ float over_rows(float x, F f) {
     return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
-// Inclusive sums over the wave's lanes, by row shifts and row broadcasts (no trip through LDS).
-__device__ __forceinline__ uint32_t scan_add(uint32_t x) {
-    x += uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x111, 0xF, 0xF, false));   // row_shr 1, 2, 4, 8
-    x += uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x112, 0xF, 0xF, false));
-    x += uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x114, 0xF, 0xF, false));
-    x += uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x118, 0xF, 0xF, false));
-    x += uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x142, 0xA, 0xF, false));   // lane 15 of a row to the next one
-    x += uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x143, 0xC, 0xF, false));   // lane 31 to the upper half
-    return x;
-}
-__device__ __forceinline__ uint32_t last_lane(uint32_t x) { return uint32_t(__builtin_amdgcn_readlane(int(x), 63)); }
-
 // ---- which cells a workgroup takes ------------------------------------------------------------------------------------
 
 struct Span {

@@ -122,8 +122,4 @@ hipError_t launch_gdn_step(const GdnArgs& a, int size, bool f16, hipStream_t str
     return hipErrorInvalidValue;
 }
 
-hipError_t launch_gdn_chunk(const GdnArgs& a, int size, bool f16, void*, hipStream_t stream) {
-    return launch_gdn_step(a, size, f16, stream);
-}
-
 }  // namespace sc

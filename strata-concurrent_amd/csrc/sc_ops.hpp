@@ -11,6 +11,7 @@
 namespace sc {
 
 using ops_u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
+using ops_u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 
 // A paged cache (sc_kv_cache) as the kernels see it.
 struct CacheArgs {
@@ -66,6 +67,14 @@ struct GdnArgs {
     float scale, eps;
 };
 
+// The chunks of one pair of launches of the chunk form.
+struct ChunkArgs {
+    uint32_t first, count, total;         // chunks [first, first + count) of at most `total`, of all sequences in order
+    uint32_t k_heads;
+    uint64_t rows_at;                     // 16-byte words before `rows`
+    ops_u32x4 *chunks, *rows;             // the workspace: operands and factors of each chunk and value head; f32 rows' parts
+};
+
 hipError_t launch_rope(const RopeArgs& a, int head_dim, int format, bool f16, hipStream_t stream);
 // Fills the split of a call and returns the bytes of its workspace.
 uint64_t plan_attn(AttnArgs& a, int head_dim);
@@ -73,11 +82,12 @@ uint64_t plan_attn(AttnArgs& a, int head_dim);
 void place_attn(AttnArgs& a, void* workspace, uint64_t bytes);
 hipError_t launch_attn(const AttnArgs& a, int head_dim, int format, bool f16, hipStream_t stream);
 hipError_t launch_gdn_step(const GdnArgs& a, int size, bool f16, hipStream_t stream);
+// Fills the pieces that a call goes in and returns the bytes of its workspace.
+uint64_t plan_gdn_chunks(const GdnArgs& a, int size, bool f16, ChunkArgs& c);
 hipError_t launch_gdn_chunk(const GdnArgs& a, int size, bool f16, void* workspace, hipStream_t stream);
 
 #if defined(__HIPCC__)
 using f32x4 = __attribute__((ext_vector_type(4))) float;
-using ops_u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
 using f16x2 = __attribute__((ext_vector_type(2))) _Float16;
 using f16x4 = __attribute__((ext_vector_type(4))) _Float16;
 using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
@@ -136,6 +146,18 @@ __device__ __forceinline__ uint32_t seq_of_row(const int64_t* cu, uint32_t n, in
     }
     return s;
 }
+
+// Inclusive sums over the wave's lanes, by row shifts and row broadcasts (no trip through LDS).
+__device__ __forceinline__ uint32_t scan_add(uint32_t x) {
+    x += uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x111, 0xF, 0xF, false));   // row_shr 1, 2, 4, 8
+    x += uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x112, 0xF, 0xF, false));
+    x += uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x114, 0xF, 0xF, false));
+    x += uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x118, 0xF, 0xF, false));
+    x += uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x142, 0xA, 0xF, false));   // lane 15 of a row to the next one
+    x += uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x143, 0xC, 0xF, false));   // lane 31 to the upper half
+    return x;
+}
+__device__ __forceinline__ uint32_t last_lane(uint32_t x) { return uint32_t(__builtin_amdgcn_readlane(int(x), 63)); }
 
 // Sum over a wave, the same in every lane and in the same order every time.
 __device__ __forceinline__ float wave_sum(float x) {

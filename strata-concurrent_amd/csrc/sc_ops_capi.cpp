@@ -235,7 +235,8 @@ int sc_gdn_step_async(const sc_gdn* d, void* stream) {
 uint64_t sc_gdn_chunk_workspace_bytes(const sc_gdn* d) {
     sc::GdnArgs a{};
     if (guarded([&] { return gdn_args("gdn_chunk", d, false, a); }) != SC_OK) return 0;
-    return 256;
+    sc::ChunkArgs c;
+    return sc::plan_gdn_chunks(a, int(d->state_size), d->dtype == SC_DTYPE_F16, c);
 }
 
 int sc_gdn_chunk_async(const sc_gdn* d, void* workspace, uint64_t workspace_bytes, void* stream) {
