@@ -28,6 +28,7 @@ namespace {
 constexpr int kC = 64;                       // tokens of a chunk
 constexpr int kWaves = 4, kThreadsC = kWaves * 64;
 constexpr float kLeastG = -200.0f;           // a decay of e^-200 is 0 in f32
+constexpr double kLog2e = 1.4426950408889634074;
 constexpr float kUpT = 0x1p10f, kUpX = 0x1p10f, kUpU = 0x1p6f;   // where operands lie in f16's range (T, P and X; U)
 
 // Places of a v head's chunk in the workspace, in 16-byte words: T and P as matrix operands [wave][step][part][lane] (a
@@ -69,6 +70,8 @@ __device__ __forceinline__ float over_rows(float x, F f) {   // over the four la
     r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
+// 2^x by the hardware's instruction, 1 unit in the last place
+__device__ __forceinline__ float exp2_of(double x) { return __builtin_amdgcn_exp2f(float(x)); }
 __device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
 
 // A sequence's rows and chunks: rows [t0, t1), its first chunk of all.
@@ -104,248 +107,314 @@ __device__ __forceinline__ bool seq_of(const GdnArgs& a, uint32_t lane, Find fin
 
 // ---- every chunk's T and P ------------------------------------------------------------------------------------------------
 
-// A workgroup takes one chunk of one key head, for each value head that shares it.  Wave w has the row tile of tokens
-// 16 w .. 16 w + 15 of both products of K with K and Q with K.
+// The largest over the wave of values that are not negative, by row shifts and broadcasts.
+__device__ __forceinline__ float wave_most(float v) {
+    uint32_t x = __float_as_uint(v);
+    x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x111, 0xF, 0xF, false)));   // row_shr 1, 2, 4, 8
+    x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x112, 0xF, 0xF, false)));
+    x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x114, 0xF, 0xF, false)));
+    x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x118, 0xF, 0xF, false)));
+    x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x142, 0xA, 0xF, false)));   // lane 15 of a row to the next one
+    x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x143, 0xC, 0xF, false)));   // lane 31 to the upper half
+    return __uint_as_float(last_lane(x));
+}
+template <int kCtrl, int kRows>
+__device__ __forceinline__ double dpp_add(double x) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(b)), kCtrl, kRows, 0xF, false));
+    const uint32_t hi = uint32_t(__builtin_amdgcn_update_dpp(0, int(uint32_t(b >> 32)), kCtrl, kRows, 0xF, false));
+    return x + __builtin_bit_cast(double, uint64_t(hi) << 32 | lo);
+}
+// Inclusive sums over the lanes.
+__device__ __forceinline__ double scan_add64(double x) {
+    x = dpp_add<0x111, 0xF>(x);
+    x = dpp_add<0x112, 0xF>(x);
+    x = dpp_add<0x114, 0xF>(x);
+    x = dpp_add<0x118, 0xF>(x);
+    x = dpp_add<0x142, 0xA>(x);
+    return dpp_add<0x143, 0xC>(x);
+}
+
+// What one wave writes to LDS the same wave reads in other lanes: its LDS operations stay in this order.
+__device__ __forceinline__ void wave_sync() {
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_wave_barrier();
+}
+
+constexpr int kTileRow = 20, kTileFloats = 16 * kTileRow + 4;   // a 16 x 16 tile in LDS: 16-byte rows, tiles on banks of their own
+constexpr int tile_of(int r, int c) { return r * (r + 1) / 2 + c; }
+
+// A wave takes one chunk of one value head, alone: the products K K^T and Q K^T by tiles of 16 tokens up to the diagonal,
+// A and P from them, and T = (1 + A)^-1: the four diagonal tiles by substitution, a column a lane, the rest by products
+// of tiles, T_10 = - T_11 (A_10 T_00) for tiles of 16 and then of 32, with f32 matrix instructions.  A product's left tile
+// comes from LDS as rows, its right one is a result in registers as it is: the four terms a lane adds are those whose rows
+// it holds.
 template <int S, bool kF16>
-__global__ void __launch_bounds__(kThreadsC) gdn_prepare_kernel(GdnArgs a, ChunkArgs c) {
+__global__ void __launch_bounds__(kThreadsC, 2) gdn_prepare_kernel(GdnArgs a, ChunkArgs c) {
     constexpr int kParts = kF16 ? 1 : 2, kSteps = S / 32;
-    __shared__ ops_u32x4 s_k[kParts][4][kSteps][64];
-    __shared__ __align__(16) float s_a[kC][kC + 4], s_t[kC][kC + 4];
-    __shared__ double s_g[kC];
-    __shared__ float s_beta[kC], s_fk[kC], s_fq[kC], s_kk[kC], s_qq[kC], s_up[2][kC];
+    struct Mine {
+        float tile[10 * kTileFloats];
+        float p[4 * kTileFloats];
+        double G[kC];
+        float beta[kC], fk[kC], fq[kC], up[2][kC], row_down[kC], squares[kC];
+    };
+    __shared__ __align__(16) Mine s_all[kWaves];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t g = lane >> 4, col = lane & 15;
-    const uint32_t kh = blockIdx.x % c.k_heads, chunk = c.first + blockIdx.x / c.k_heads;
+    const uint32_t item = blockIdx.x * kWaves + wave;
+    if (item >= c.count * a.v_heads) return;
+    const uint32_t piece = item / a.v_heads, h = item - piece * a.v_heads, kh = ops_div(h, a.share), chunk = c.first + piece;
+    Mine& s = s_all[wave];
     Seq q;
     if (!seq_of(a, lane, [&](uint32_t, uint32_t lo, uint32_t hi) { return chunk >= lo && chunk < hi; }, q)) return;
     const uint32_t t0 = q.t0 + (chunk - q.chunk0) * kC, n = q.t1 - t0 < kC ? q.t1 - t0 : kC;
-    const uint64_t slot = chunk - c.first;
+    ops_u32x4* out = c.chunks + (uint64_t(piece) * a.v_heads + h) * kChunkWords;
+    uint8_t* rows = reinterpret_cast<uint8_t*>(c.rows + (uint64_t(piece) * c.k_heads + kh) * (4 * kC * S / 8));
+    const bool write_rows = !kF16 && h == kh * a.share.d;
 
-    // this wave's rows: token 16 w + col, values 32 step + 8 g .. + 7
-    const uint32_t mine = wave * 16 + col, row = mine < n ? mine : n - 1;
-    ops_u32x4 kf[kParts][kSteps], qf[kParts][kSteps];
-    if constexpr (kF16) {
-        const uint8_t* kp = a.k + int64_t(t0 + row) * a.k_ld + (kh * S + g * 8) * 2;
-        const uint8_t* qp = a.q + int64_t(t0 + row) * a.q_ld + (kh * S + g * 8) * 2;
+    const bool in = lane < n;
+    const int64_t gates = int64_t(t0 + (in ? lane : 0)) * a.gate_ld + h;
+    const float g_in = ld_global<float>(a.g + gates), beta_in = ld_global<float>(a.beta + gates);
+
+    // tile t of keys or queries: token 16 t + col, values 32 step + 8 g .. + 7: as they lie in memory, then as operands, rows
+    // past the chunk zero
+    auto load_raw = [&](const uint8_t* from, int64_t ld, int t, ops_u32x4 (&x)[kParts * kSteps]) {
+        const uint32_t mine = t * 16 + col, row = mine < n ? mine : n - 1;
+        const uint8_t* p = from + int64_t(t0 + row) * ld + (kh * S + g * 8) * (kF16 ? 2 : 4);
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) kf[0][i] = ld_global<ops_u32x4>(kp + i * 64), qf[0][i] = ld_global<ops_u32x4>(qp + i * 64);
+        for (int i = 0; i < kParts * kSteps; ++i) x[i] = ld_global<ops_u32x4>(p + (kF16 ? i * 64 : i / 2 * 128 + i % 2 * 16));
+    };
+    auto to_tile = [&](const ops_u32x4 (&raw)[kParts * kSteps], int t, ops_u32x4 (&x)[kParts][kSteps], float* up, uint32_t which) {
+        const uint32_t mine = t * 16 + col;
+        if constexpr (kF16) {
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i)
-            if (mine >= n) kf[0][i] = ops_u32x4{}, qf[0][i] = ops_u32x4{};
-        if (g == 0) s_up[0][mine] = 1.0f, s_up[1][mine] = 1.0f;
-    } else {
+            for (int i = 0; i < kSteps; ++i) x[0][i] = raw[i];
 #pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            const uint8_t* p = which ? a.q + int64_t(t0 + row) * a.q_ld : a.k + int64_t(t0 + row) * a.k_ld;
-            f32x4 x[kSteps][2];
+            for (int i = 0; i < kSteps; ++i)
+                if (mine >= n) x[0][i] = ops_u32x4{};
+        } else {
+            // scaled by a power of two to a largest value of 1 .. 2, in two parts, which the second kernel reads
+            f32x4 y[kSteps][2];
             float top = 0;
 #pragma unroll
             for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) x[i][j] = ld_act4<false>(p, kh * S + i * 32 + g * 8 + j * 4);
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i)
-#pragma unroll
                 for (int j = 0; j < 2; ++j) {
-                    if (mine >= n) x[i][j] = f32x4{};
+                    y[i][j] = mine < n ? __builtin_bit_cast(f32x4, raw[(i * 2 + j) % (kParts * kSteps)]) : f32x4{};
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) top = fmaxf(top, fabsf(x[i][j][k]));
+                    for (int k = 0; k < 4; ++k) top = fmaxf(top, fabsf(y[i][j][k]));
                 }
             top = over_rows(top, max_of);
+            float down, back;
+            power_of(top, down, back);
+            if (g == 0) up[mine] = back;
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                uint32_t hi[4], lo[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) split2(y[i][j / 2][j % 2 * 2] * down, y[i][j / 2][j % 2 * 2 + 1] * down, hi[j], lo[j]);
+                x[0][i] = ops_u32x4{hi[0], hi[1], hi[2], hi[3]};
+                x[kParts - 1][i] = ops_u32x4{lo[0], lo[1], lo[2], lo[3]};
+                if (write_rows)
+#pragma unroll
+                    for (int part = 0; part < kParts; ++part)
+                        st_global<ops_u32x4>(rows + (((which * kParts + part) * kC + mine) * S + i * 32 + g * 8) * 2, x[part][i]);
+            }
+        }
+    };
+    auto dot = [&](const ops_u32x4 (&x)[kParts][kSteps], const ops_u32x4 (&y)[kParts][kSteps], f32x4 acc) {
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            acc = mfma(x[0][i], y[0][i], acc);
+            if constexpr (!kF16) acc = mfma(x[0][i], y[kParts - 1][i], acc), acc = mfma(x[kParts - 1][i], y[0][i], acc);
+        }
+        return acc;
+    };
+    // f16 queries are all asked for now, f32 ones a tile ahead (registers)
+    constexpr int kAhead = kF16 ? 4 : 1;
+    ops_u32x4 k_raw[4][kParts * kSteps], q_raw[kAhead][kParts * kSteps], kf[4][kParts][kSteps];
+#pragma unroll
+    for (int t = 0; t < 4; ++t) load_raw(a.k, a.k_ld, t, k_raw[t]);
+#pragma unroll
+    for (int t = 0; t < kAhead; ++t) load_raw(a.q, a.q_ld, t, q_raw[t]);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) to_tile(k_raw[t], t, kf[t], s.up[0], 0);
+
+    // sums of the log decays, to base 2, lane = token
+    const double G = scan_add64(in ? double(g_in < kLeastG ? kLeastG : g_in) * kLog2e : 0.0);
+    const float beta = in ? beta_in : 0.0f;
+    s.G[lane] = G;
+    s.beta[lane] = beta;
+    const uint64_t G_bits = __builtin_bit_cast(uint64_t, G);
+    const double G_all = __builtin_bit_cast(double, uint64_t(last_lane(uint32_t(G_bits >> 32))) << 32 | last_lane(uint32_t(G_bits)));
+
+    // K K^T, element (4 g + i, col) of a tile; its diagonal has the squares of the lengths
+    f32x4 kk[10];
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int cc = 0; cc <= r; ++cc) kk[tile_of(r, cc)] = dot(kf[r], kf[cc], f32x4{});
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (g * 4 + i == col) s.squares[t * 16 + col] = kk[tile_of(t, t)][i];
+    wave_sync();
+    // the factor that brings a row as multiplied to its length, unit or its own, and that length
+    auto factor = [&](float squares, const float* up, float& length) {
+        const float by = kF16 ? 1.0f : up[lane];
+        const float f = !in ? 0.0f : a.l2norm ? __builtin_amdgcn_rsqf(squares + a.eps / by / by) : by;
+        length = in ? __builtin_amdgcn_sqrtf(squares) * f : 0.0f;
+        return f;
+    };
+    float k_length;
+    const float fk = factor(s.squares[lane], s.up[0], k_length), k_most = wave_most(k_length);
+    s.fk[lane] = fk;
+    const float e = exp2_of(G), write = exp2_of(G_all - G) * fk;
+    float* f = reinterpret_cast<float*>(out + 2 * kOperand);
+    {
+        float down, up;
+        power_of(wave_most(write), down, up);
+        const float beta_most = wave_most(fabsf(beta));
+        f[kFState + lane] = beta * fk * e;
+        f[kFBeta + lane] = beta;
+        f[kFWrite + lane] = write * down;
+        if (lane == 0) f[kFDecay] = exp2_of(G_all), f[kFUp] = up, f[kFBetaMost] = beta_most;
+    }
+    wave_sync();
+
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        ops_u32x4 qf[kParts][kSteps];
+        to_tile(q_raw[r % kAhead], r, qf, s.up[1], 1);
+        if (!kF16 && r < 3) load_raw(a.q, a.q_ld, r + 1, q_raw[0]);
+        f32x4 qq = dot(qf, qf, f32x4{}), qk[4];
+#pragma unroll
+        for (int cc = 0; cc <= r; ++cc) qk[cc] = dot(qf, kf[cc], f32x4{});
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (g * 4 + i == col) s.squares[col] = qq[i];
+        wave_sync();
+        if (lane < 16) {
+            // token 16 r + lane: this lane's own place in the chunk is another one
+            const uint32_t t = r * 16 + lane;
+            const float by = kF16 ? 1.0f : s.up[1][t], squares = s.squares[lane];
+            const float fq = t >= n ? 0.0f : a.l2norm ? __builtin_amdgcn_rsqf(squares + a.eps / by / by) : by;
             float down, up;
-            power_of(top, down, up);
-            if (g == 0) s_up[which][mine] = up;
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                uint32_t h[4], l[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) split2(x[i][j / 2][j % 2 * 2] * down, x[i][j / 2][j % 2 * 2 + 1] * down, h[j], l[j]);
-                (which ? qf : kf)[0][i] = ops_u32x4{h[0], h[1], h[2], h[3]};
-                (which ? qf : kf)[kParts - 1][i] = ops_u32x4{l[0], l[1], l[2], l[3]};
-            }
+            power_of(t >= n ? 0.0f : fabsf(a.scale) * __builtin_amdgcn_sqrtf(squares) * fq * k_most, down, up);
+            s.fq[t] = fq * a.scale;
+            s.row_down[t] = down * kUpT;
+            f[kFQuery + t] = a.scale * fq * exp2_of(s.G[t]);
+            f[kFRow + t] = up;
         }
-        // the second kernel reads rows of f16 parts: [k, q][part][64][S]
-        uint8_t* to = reinterpret_cast<uint8_t*>(c.rows + (slot * c.k_heads + kh) * (4 * kC * S / 8));
-#pragma unroll
-        for (int part = 0; part < kParts; ++part)
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                st_global<ops_u32x4>(to + ((part * kC + mine) * S + i * 32 + g * 8) * 2, kf[part][i]);
-                st_global<ops_u32x4>(to + (((kParts + part) * kC + mine) * S + i * 32 + g * 8) * 2, qf[part][i]);
-            }
-    }
-#pragma unroll
-    for (int part = 0; part < kParts; ++part)
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i) s_k[part][wave][i][lane] = kf[part][i];
-    __syncthreads();
-
-    // products of the row tile with the key tiles up to its own: element (4 g + i, col)
-    f32x4 kk[4], qk[4], qq{};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        kk[j] = f32x4{}, qk[j] = f32x4{};
-        if (uint32_t(j) > wave) continue;
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i)
-#pragma unroll
-            for (int x = 0; x < kParts; ++x)
-#pragma unroll
-                for (int y = 0; y < kParts; ++y) {
-                    if (x + y > 1) continue;   // both low parts: below 2^-22
-                    const ops_u32x4 b = s_k[y][j][i][lane];
-                    kk[j] = mfma(kf[x][i], b, kk[j]);
-                    qk[j] = mfma(qf[x][i], b, qk[j]);
-                }
-    }
-#pragma unroll
-    for (int i = 0; i < kSteps; ++i)
-#pragma unroll
-        for (int x = 0; x < kParts; ++x)
-#pragma unroll
-            for (int y = 0; y < kParts; ++y)
-                if (x + y <= 1) qq = mfma(qf[x][i], qf[y][i], qq);
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-        if (uint32_t(j) == wave)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (g * 4 + i == col) s_kk[mine] = kk[j][i], s_qq[mine] = qq[i];
-    __syncthreads();
-    // factors that bring the rows as multiplied to their length: unit, or their own
-    if (threadIdx.x < 2 * kC) {
-        const uint32_t t = threadIdx.x % kC;
-        const bool is_q = threadIdx.x >= kC;
-        const float up = s_up[is_q][t], squares = is_q ? s_qq[t] : s_kk[t];
-        const float f = t >= n ? 0.0f : a.l2norm ? 1.0f / sqrtf(squares + a.eps / up / up) : up;
-        (is_q ? s_fq : s_fk)[t] = f;
-        // lengths, for the bound of P's rows
-        (is_q ? s_qq : s_kk)[t] = t >= n ? 0.0f : sqrtf(squares) * f;
-    }
-
-    for (uint32_t each = 0; each < a.share.d; ++each) {
-        const uint32_t h = kh * a.share.d + each;
-        __syncthreads();
-        float k_most = s_kk[lane];
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) k_most = fmaxf(k_most, __shfl_xor(k_most, m));
-        // sums of the log decays, lane = token
-        const bool in = lane < n;
-        const float* gates = a.g + int64_t(t0 + (in ? lane : 0)) * a.gate_ld + h;
-        const float g1 = in ? ld_global<float>(gates) : 0.0f;
-        const float beta = in ? ld_global<float>(a.beta + int64_t(t0 + (in ? lane : 0)) * a.gate_ld + h) : 0.0f;
-        double G = double(g1 < kLeastG ? kLeastG : g1);
-#pragma unroll
-        for (int m = 1; m < 64; m <<= 1) {
-            const double o = __shfl_up(G, m);
-            if (lane >= uint32_t(m)) G += o;
-        }
-        const double G_all = __shfl(G, 63);
-        ops_u32x4* out = c.chunks + (slot * a.v_heads + h) * kChunkWords;
-        if (wave == 0) {
-            s_g[lane] = G;
-            s_beta[lane] = beta;
-            float* f = reinterpret_cast<float*>(out + 2 * kOperand);
-            const float fk = s_fk[lane], e = expf(float(G)), write = expf(float(G_all - G)) * fk;
-            float most = write, beta_most = fabsf(beta);
-#pragma unroll
-            for (int m = 1; m < 64; m <<= 1) {
-                most = fmaxf(most, __shfl_xor(most, m));
-                beta_most = fmaxf(beta_most, __shfl_xor(beta_most, m));
-            }
-            float down, up, row_down, row_up;
-            power_of(most, down, up);
-            power_of(fabsf(a.scale) * s_qq[lane] * k_most, row_down, row_up);
-            s_up[0][lane] = row_down;
-            f[kFState + lane] = beta * fk * e;
-            f[kFBeta + lane] = beta;
-            f[kFWrite + lane] = write * down;
-            f[kFQuery + lane] = a.scale * s_fq[lane] * e;
-            f[kFRow + lane] = row_up;
-            if (lane == 0) f[kFDecay] = expf(float(G_all)), f[kFUp] = up, f[kFBetaMost] = beta_most;
-        }
-        __syncthreads();
+        wave_sync();
         // A below the diagonal, and P
-        f32x4 p[4];
+        double Gr[4];
+        float br[4], qr[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const double Gj = s_g[j * 16 + col];
-            const float fj = s_fk[j * 16 + col];
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t t = r * 16 + g * 4 + i;
+            Gr[i] = s.G[t];
+            br[i] = s.beta[t] * s.fk[t];
+            qr[i] = s.fq[t] * s.row_down[t];
+        }
+#pragma unroll
+        for (int cc = 0; cc <= r; ++cc) {
+            const double Gc = s.G[cc * 16 + col];
+            const float fc = s.fk[cc * 16 + col];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                const uint32_t r = wave * 16 + g * 4 + i, t = j * 16 + col;
-                const float fade = r >= t ? expf(float(s_g[r] - Gj)) * fj : 0.0f;
-                s_a[r][t] = r > t ? s_beta[r] * s_fk[r] * fade * kk[j][i] : 0.0f;
-                p[j][i] = a.scale * s_fq[r] * fade * qk[j][i] * s_up[0][r] * kUpT;
+                const uint32_t row = g * 4 + i;
+                const float fade = cc < r || row >= col ? exp2_of(Gr[i] - Gc) * fc : 0.0f;
+                s.tile[tile_of(r, cc) * kTileFloats + row * kTileRow + col] = cc < r || row > col ? br[i] * fade * kk[tile_of(r, cc)][i] : 0.0f;
+                s.p[cc * kTileFloats + row * kTileRow + col] = qr[i] * fade * qk[cc][i];
             }
         }
-        __syncthreads();
-        // T: the diagonal tiles by substitution (lane = column of the inverse) ...
-        {
-            float x[16];
+        wave_sync();
+        // P as the second kernel's operand: row 16 r + col, places 0 .. 3 tokens 32 step + 4 g, 4 .. 7 16 more
 #pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                float sum = uint32_t(i) == col ? 1.0f : 0.0f;
-#pragma unroll
-                for (int k = 0; k < i; ++k) sum -= s_a[wave * 16 + i][wave * 16 + k] * x[k];
-                x[i] = sum;
-            }
-            if (g == 0)
-#pragma unroll
-                for (int i = 0; i < 16; ++i) s_t[wave * 16 + i][wave * 16 + col] = x[i];
+        for (int step = 0; step <= r / 2; ++step) {
+            const f32x4 u = *reinterpret_cast<const f32x4*>(&s.p[step * 2 * kTileFloats + col * kTileRow + g * 4]);
+            const f32x4 v = step * 2 + 1 <= r ? *reinterpret_cast<const f32x4*>(&s.p[(step * 2 + 1) * kTileFloats + col * kTileRow + g * 4]) : f32x4{};
+            uint32_t hi[4], lo[4];
+            split2(u.x, u.y, hi[0], lo[0]);
+            split2(u.z, u.w, hi[1], lo[1]);
+            split2(v.x, v.y, hi[2], lo[2]);
+            split2(v.z, v.w, hi[3], lo[3]);
+            st_global<ops_u32x4>(out + kOperand + operand_at(r, step, 0) + lane, ops_u32x4{hi[0], hi[1], hi[2], hi[3]});
+            st_global<ops_u32x4>(out + kOperand + operand_at(r, step, 1) + lane, ops_u32x4{lo[0], lo[1], lo[2], lo[3]});
         }
-        __syncthreads();
-        // ... then T_21 = - T_22 (A_21 T_11) for tiles of 16 and of 32.  product(): 16 x 16 of rows r of X by columns c of Y
-        auto product = [&](const float (&X)[kC][kC + 4], uint32_t r, uint32_t m, const float (&Y)[kC][kC + 4], uint32_t cc, f32x4 acc) {
+        wave_sync();
+    }
+
+    // the diagonal tiles of T: column col of tile g
+    auto tile_at = [&](int t) { return s.tile + t * kTileFloats; };
+    {
+        const float* d = s.tile + (g * (g + 1) / 2 + g) * kTileFloats;
+        float x[16];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) acc = mfma_f32(X[r * 16 + col][m * 16 + k * 4 + g], Y[m * 16 + k * 4 + g][cc * 16 + col], acc);
-            return acc;
-        };
-        auto store = [&](float (&X)[kC][kC + 4], uint32_t r, uint32_t cc, f32x4 v, float by) {
+        for (int i = 0; i < 16; ++i) {
+            f32x4 sum{uint32_t(i) == col ? 1.0f : 0.0f, 0, 0, 0};   // four sums: a chain a quarter as long
 #pragma unroll
-            for (int i = 0; i < 4; ++i) X[r * 16 + g * 4 + i][cc * 16 + col] = v[i] * by;
-        };
-        if (wave == 1 || wave == 3) store(s_a, wave, wave - 1, product(s_a, wave, wave - 1, s_t, wave - 1, f32x4{}), 1.0f);
-        __syncthreads();
-        if (wave == 1 || wave == 3) store(s_t, wave, wave - 1, product(s_t, wave, wave, s_a, wave - 1, f32x4{}), -1.0f);
-        __syncthreads();
-        const uint32_t tr = 2 + wave / 2, tc = wave % 2;
-        f32x4 y = product(s_a, tr, 1, s_t, tc, f32x4{});   // T_01 is zero, as is A's part above
-        if (tc == 0) y = product(s_a, tr, 0, s_t, 0, y);
-        __syncthreads();
-        store(s_a, tr, tc, y, 1.0f);
-        __syncthreads();
-        f32x4 z = product(s_t, tr, 2, s_a, tc, f32x4{});
-        if (tr == 3) z = product(s_t, 3, 3, s_a, tc, z);
-        store(s_t, tr, tc, z, -1.0f);
-        __syncthreads();
-        // both as the second kernel's operands: row 16 w + col, places 0 .. 3 tokens 32 step + 4 g, 4 .. 7 16 more
-#pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            if (which) {
-                __syncthreads();
+            for (int k = 0; k < i; k += 4) {
+                const f32x4 row = *reinterpret_cast<const f32x4*>(&d[i * kTileRow + k]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) s_t[wave * 16 + g * 4 + i][j * 16 + col] = p[j][i];
-                __syncthreads();
+                    if (k + j < i) sum[j] -= row[j] * x[k + j];
             }
-            for (uint32_t step = 0; step <= wave / 2; ++step) {
-                // above the diagonal T's tiles were never written
-                const bool upper = !which && step * 2 + 1 > wave;
-                const f32x4 u = *reinterpret_cast<const f32x4*>(&s_t[wave * 16 + col][step * 32 + g * 4]) * (which ? 1.0f : kUpT);
-                const f32x4 v = upper ? f32x4{} : *reinterpret_cast<const f32x4*>(&s_t[wave * 16 + col][step * 32 + 16 + g * 4]) * (which ? 1.0f : kUpT);
-                uint32_t hi[4], lo[4];
-                split2(u.x, u.y, hi[0], lo[0]);
-                split2(u.z, u.w, hi[1], lo[1]);
-                split2(v.x, v.y, hi[2], lo[2]);
-                split2(v.z, v.w, hi[3], lo[3]);
-                ops_u32x4* to = out + which * kOperand + lane;
-                st_global<ops_u32x4>(to + operand_at(wave, step, 0), ops_u32x4{hi[0], hi[1], hi[2], hi[3]});
-                st_global<ops_u32x4>(to + operand_at(wave, step, 1), ops_u32x4{lo[0], lo[1], lo[2], lo[3]});
-            }
+            x[i] = (sum.x + sum.y) + (sum.z + sum.w);
         }
+        wave_sync();
+#pragma unroll
+        for (int i = 0; i < 16; ++i) s.tile[(g * (g + 1) / 2 + g) * kTileFloats + i * kTileRow + col] = x[i];
+        wave_sync();
     }
+    auto left = [&](int t) { return *reinterpret_cast<const f32x4*>(tile_at(t) + col * kTileRow + g * 4); };
+    auto right = [&](int t) {
+        f32x4 x;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) x[i] = tile_at(t)[(g * 4 + i) * kTileRow + col];
+        return x;
+    };
+    auto product = [&](f32x4 x, f32x4 y, f32x4 acc) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc = mfma_f32(x[i], y[i], acc);
+        return acc;
+    };
+    auto put = [&](int t, f32x4 x) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) tile_at(t)[(g * 4 + i) * kTileRow + col] = x[i];
+    };
+    {
+        const f32x4 zero{}, t00 = right(tile_of(0, 0)), t11 = right(tile_of(1, 1)), t22 = right(tile_of(2, 2));
+        const f32x4 y10 = product(left(tile_of(1, 0)), t00, zero), y32 = product(left(tile_of(3, 2)), t22, zero);
+        const f32x4 t10 = -product(left(tile_of(1, 1)), y10, zero), t32 = -product(left(tile_of(3, 3)), y32, zero);
+        wave_sync();
+        put(tile_of(1, 0), t10);
+        put(tile_of(3, 2), t32);
+        const f32x4 y20 = product(left(tile_of(2, 1)), t10, product(left(tile_of(2, 0)), t00, zero)), y21 = product(left(tile_of(2, 1)), t11, zero);
+        const f32x4 y30 = product(left(tile_of(3, 1)), t10, product(left(tile_of(3, 0)), t00, zero)), y31 = product(left(tile_of(3, 1)), t11, zero);
+        wave_sync();
+        const f32x4 l22 = left(tile_of(2, 2)), l32 = left(tile_of(3, 2)), l33 = left(tile_of(3, 3));
+        put(tile_of(2, 0), -product(l22, y20, zero));
+        put(tile_of(2, 1), -product(l22, y21, zero));
+        put(tile_of(3, 0), -product(l33, y30, product(l32, y20, zero)));
+        put(tile_of(3, 1), -product(l33, y31, product(l32, y21, zero)));
+        wave_sync();
+    }
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+#pragma unroll
+        for (int step = 0; step <= r / 2; ++step) {
+            const f32x4 u = left(tile_of(r, step * 2)) * kUpT, v = step * 2 + 1 <= r ? left(tile_of(r, step * 2 + 1)) * kUpT : f32x4{};
+            uint32_t hi[4], lo[4];
+            split2(u.x, u.y, hi[0], lo[0]);
+            split2(u.z, u.w, hi[1], lo[1]);
+            split2(v.x, v.y, hi[2], lo[2]);
+            split2(v.z, v.w, hi[3], lo[3]);
+            st_global<ops_u32x4>(out + operand_at(r, step, 0) + lane, ops_u32x4{hi[0], hi[1], hi[2], hi[3]});
+            st_global<ops_u32x4>(out + operand_at(r, step, 1) + lane, ops_u32x4{lo[0], lo[1], lo[2], lo[3]});
+        }
 }
 
 // ---- the chunks of a sequence in order ------------------------------------------------------------------------------------
@@ -357,14 +426,19 @@ struct ChunkRows {
     ops_u32x4 k[kParts][kSteps], q[kParts][kSteps];   // its row tile
     uint32_t kt[kParts][2][8];                        // its 32 keys: pairs of keys of the eight tokens of a step
     ops_u32x4 t[2][2], p[2][2];                       // T and P: [step][part]
-    float f_state[4], beta[4], write[4], f_query[4], f_row[4];
-    float decay, up, beta_most;
+    f32x4 f_state, beta, write, f_query, f_row;
+    f32x4 all;                                        // the chunk's decay, the scale of `write`, the largest beta
 };
 
 template <int S, int kCols, bool kF16>
 __global__ void __launch_bounds__(kThreadsC, 1) gdn_chunk_kernel(GdnArgs a, ChunkArgs c) {
     constexpr int kParts = kF16 ? 1 : 2, kSteps = S / 32, kN = kCols / 16;
     using R = ChunkRows<S, kParts>;
+    struct Values {
+        f32x4 beta;
+        uint32_t raw[kN][4];
+        f32x4 by[kN];
+    };
     __shared__ ops_u32x4 s_m[kN][kSteps][2][64];         // the state as an operand: [step][part][lane]
     __shared__ float s_scale[kN][kSteps][16];
     __shared__ ops_u32x2 s_x[kN][2][2][64][2], s_u[kN][2][2][64][2], s_w[kN][2][2][64][2];   // [step][part][lane][tile]
@@ -443,7 +517,6 @@ __global__ void __launch_bounds__(kThreadsC, 1) gdn_chunk_kernel(GdnArgs a, Chun
                         const uint32_t t = step * 32 + (j / 4) * 16 + g * 4 + j % 4, u = t < n ? t : n - 1;
                         const uint8_t* p = kF16 ? a.k + int64_t(t0 + u) * a.k_ld + kh * S * 2 : rows + (part * kC + t) * S * 2;
                         r.kt[part][step][j] = ld_global<uint32_t>(p + (wave * 32 + col * 2) * 2);
-                        if (kF16 && t >= n) r.kt[part][step][j] = 0;
                     }
         }
         const ops_u32x4* from = c.chunks + (slot * a.v_heads + h) * kChunkWords;
@@ -457,37 +530,42 @@ __global__ void __launch_bounds__(kThreadsC, 1) gdn_chunk_kernel(GdnArgs a, Chun
                 }
         const float* f = reinterpret_cast<const float*>(from + 2 * kOperand);
         const uint32_t mine4 = wave * 16 + g * 4;
-        const f32x4 fs = ld_global<f32x4>(f + kFState + mine4), fb = ld_global<f32x4>(f + kFBeta + mine4), fw = ld_global<f32x4>(f + kFWrite + mine4);
-        const f32x4 fq = ld_global<f32x4>(f + kFQuery + mine4), fr = ld_global<f32x4>(f + kFRow + mine4);
-        const f32x4 one = ld_global<f32x4>(f + kFDecay);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) r.f_state[i] = fs[i], r.beta[i] = fb[i], r.write[i] = fw[i], r.f_query[i] = fq[i], r.f_row[i] = fr[i];
-        r.decay = one.x, r.up = one.y, r.beta_most = one.z;
+        r.f_state = ld_global<f32x4>(f + kFState + mine4);
+        r.write = ld_global<f32x4>(f + kFWrite + mine4);
+        r.f_query = ld_global<f32x4>(f + kFQuery + mine4);
+        r.f_row = ld_global<f32x4>(f + kFRow + mine4);
+        r.all = ld_global<f32x4>(f + kFDecay);
     };
-    // beta V of the wave's rows, and its largest value a column, for the scale of X
-    auto load_v = [&](f32x4 (&v)[kN], uint32_t chunk, const float (&beta)[4]) {
+    // the wave's rows of V, and their largest value a column times beta, for the scale of X
+    auto load_v = [&](Values& v, uint32_t chunk) {
         const uint32_t t0 = q.t0 + (chunk - q.chunk0) * kC, n = q.t1 - t0 < kC ? q.t1 - t0 : kC;
+        v.beta = ld_global<f32x4>(reinterpret_cast<const float*>(c.chunks + (uint64_t(chunk - c.first) * a.v_heads + h) * kChunkWords + 2 * kOperand) +
+                                  kFBeta + wave * 16 + g * 4);
 #pragma unroll
-        for (int b = 0; b < kN; ++b)
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t t = wave * 16 + g * 4 + i;
+            const uint8_t* p = a.v + int64_t(t0 + (t < n ? t : n - 1)) * a.v_ld;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t t = wave * 16 + g * 4 + i;
-                const uint8_t* p = a.v + int64_t(t0 + (t < n ? t : n - 1)) * a.v_ld;
+            for (int b = 0; b < kN; ++b) {
                 const uint32_t at = h * S + block * kCols + b * 16 + col;
-                float x;
-                if constexpr (kF16) x = float(__builtin_bit_cast(_Float16, ld_global<uint16_t>(p + at * 2)));
-                else x = ld_global<float>(p + at * 4);
-                v[b][i] = t < n ? x * beta[i] : 0.0f;
+                if constexpr (kF16) v.raw[b][i] = ld_global<uint16_t>(p + at * 2);
+                else v.raw[b][i] = ld_global<uint32_t>(p + at * 4);
             }
+        }
     };
-    auto put_v = [&](const f32x4 (&v)[kN], uint32_t which) {
+    auto put_v = [&](Values& v, uint32_t chunk) {
+        const uint32_t t0 = q.t0 + (chunk - q.chunk0) * kC, n = q.t1 - t0 < kC ? q.t1 - t0 : kC;
 #pragma unroll
         for (int b = 0; b < kN; ++b) {
             float top = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(v[b][i]));
+            for (int i = 0; i < 4; ++i) {
+                const float x = kF16 ? float(__builtin_bit_cast(_Float16, uint16_t(v.raw[b][i]))) : __uint_as_float(v.raw[b][i]);
+                v.by[b][i] = wave * 16 + g * 4 + i < n ? x * v.beta[i] : 0.0f;
+                top = fmaxf(top, fabsf(v.by[b][i]));
+            }
             top = over_rows(top, max_of);
-            if (g == 0) s_v[which][b][wave][col] = top;
+            if (g == 0) s_v[(chunk - c0) & 1][b][wave][col] = top;
         }
     };
     // a tile of 16 tokens of X, U or the weighted U as an operand: the wave's half of a step
@@ -502,14 +580,21 @@ __global__ void __launch_bounds__(kThreadsC, 1) gdn_chunk_kernel(GdnArgs a, Chun
         return *reinterpret_cast<const ops_u32x4*>(&from[step][part][lane][0]);
     };
 
-    R r;
-    f32x4 v[kN];
-    load(r, c0);
-    load_v(v, c0, r.beta);
+    // a chunk's rows are asked for a whole chunk before they are used
+    R ra, rb;
+    Values v;
+    load_v(v, c0);
+    load(ra, c0);
     put_state();
-    put_v(v, 0);
-    for (uint32_t chunk = c0; chunk < c1; ++chunk) {
+    put_v(v, c0);
+    auto turn = [&](const uint32_t chunk, R& r, R& next) {
         const uint32_t t0 = q.t0 + (chunk - q.chunk0) * kC, n = q.t1 - t0 < kC ? q.t1 - t0 : kC;
+        const bool more = chunk + 1 < c1;
+        Values nv;
+        if (more) {
+            load_v(nv, chunk + 1);
+            load(next, chunk + 1);
+        }
         __syncthreads();
         // K M0 and Q M0, a step's sum by its own scale
         f32x4 qm[kN];
@@ -533,13 +618,13 @@ __global__ void __launch_bounds__(kThreadsC, 1) gdn_chunk_kernel(GdnArgs a, Chun
                 qm[b] += scale * qs;
                 most = fmaxf(most, scale);
             }
-            most *= r.beta_most;
+            most *= r.all.z;
 #pragma unroll
             for (int w = 0; w < kWaves; ++w) most = fmaxf(most, s_v[(chunk - c0) & 1][b][w][col]);
             power_of(most, x_down[b], x_up[b]);
             f32x4 x;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = wave * 16 + g * 4 + i < n ? (v[b][i] - r.f_state[i] * km[i]) * (x_down[b] * kUpX) : 0.0f;
+            for (int i = 0; i < 4; ++i) x[i] = wave * 16 + g * 4 + i < n ? (v.by[b][i] - r.f_state[i] * km[i]) * (x_down[b] * kUpX) : 0.0f;
             put(s_x[b], x);
         }
         __syncthreads();
@@ -565,6 +650,12 @@ __global__ void __launch_bounds__(kThreadsC, 1) gdn_chunk_kernel(GdnArgs a, Chun
         __syncthreads();
         // the state after the chunk
         if (keys) {
+            if (kF16 && n < uint32_t(kC))   // the last, partial chunk: whatever lies in the rows past it stays out
+#pragma unroll
+                for (int step = 0; step < 2; ++step)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        if (step * 32 + (j / 4) * 16 + g * 4 + j % 4 >= n) r.kt[0][step][j] = 0;
 #pragma unroll
             for (int b = 0; b < kN; ++b) {
                 f32x4 add[2]{};
@@ -583,9 +674,9 @@ __global__ void __launch_bounds__(kThreadsC, 1) gdn_chunk_kernel(GdnArgs a, Chun
                             if (part == 0) add[e] = mfma(key, lo, add[e]);
                         }
                 }
-                const float by = x_up[b] * r.up * (1.0f / kUpU);
+                const float by = x_up[b] * r.all.y * (1.0f / kUpU);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) m[b][e] = r.decay * m[b][e] + by * add[e];
+                for (int e = 0; e < 2; ++e) m[b][e] = r.all.x * m[b][e] + by * add[e];
             }
         }
         put_state();
@@ -613,11 +704,14 @@ __global__ void __launch_bounds__(kThreadsC, 1) gdn_chunk_kernel(GdnArgs a, Chun
                 else st_global<float>(to + at * 4, o);
             }
         }
-        if (chunk + 1 < c1) {
-            load(r, chunk + 1);
-            load_v(v, chunk + 1, r.beta);
-            put_v(v, (chunk + 1 - c0) & 1);
+        if (more) {
+            put_v(nv, chunk + 1);
+            v = nv;
         }
+    };
+    for (uint32_t chunk = c0; chunk < c1; chunk += 2) {
+        turn(chunk, ra, rb);
+        if (chunk + 1 < c1) turn(chunk + 1, rb, ra);
     }
     if (keys)
 #pragma unroll
@@ -631,7 +725,7 @@ __global__ void __launch_bounds__(kThreadsC, 1) gdn_chunk_kernel(GdnArgs a, Chun
 template <int S, int kCols, bool kF16>
 void launch_chunks(const GdnArgs& a, const ChunkArgs& c, hipStream_t stream) {
     const uint32_t pairs = (a.n_seqs * a.v_heads + 7) / 8 * 8;
-    hipLaunchKernelGGL((gdn_prepare_kernel<S, kF16>), dim3(c.count * c.k_heads), dim3(kThreadsC), 0, stream, a, c);
+    hipLaunchKernelGGL((gdn_prepare_kernel<S, kF16>), dim3((c.count * a.v_heads + kWaves - 1) / kWaves), dim3(kThreadsC), 0, stream, a, c);
     hipLaunchKernelGGL((gdn_chunk_kernel<S, kCols, kF16>), dim3(pairs * (S / kCols)), dim3(kThreadsC), 0, stream, a, c);
 }
 template <int S>
