@@ -64,7 +64,7 @@ typedef struct sc_rope_append {
     const void* v;
     const void* q;            /* [tokens][n_head][head_dim], or NULL: no queries */
     void* q_out;              /* the rotated queries; may be q itself (then q_out_ld == q_ld) */
-    int64_t k_ld, v_ld, q_ld, q_out_ld;  /* multiples of 4 (f32) or 8 (f16) values */
+    int64_t k_ld, v_ld, q_ld, q_out_ld;  /* multiples of 4 (f32) or 8 (f16) values, at most 2^22 */
     int64_t n_head;           /* query heads, 0 without q, at most 4096 */
     int32_t pairing;          /* SC_ROPE_* */
     int64_t rot_dim;          /* the first rot_dim values of a head are rotated: a multiple of 8, 0 .. head_dim */
@@ -89,7 +89,7 @@ typedef struct sc_attn_decode {
     int64_t n_head;           /* query heads, a multiple of n_head_kv: head i reads kv head i / (n_head / n_head_kv) */
     const void* q;            /* [n_seqs][n_head][head_dim], q_ld values from sequence to sequence, 16-byte aligned */
     void* out;                /* likewise with out_ld; must not overlap q */
-    int64_t q_ld, out_ld;     /* multiples of 4 (f32) or 8 (f16) values */
+    int64_t q_ld, out_ld;     /* multiples of 4 (f32) or 8 (f16) values, at most 2^22 */
     float* lse;               /* [n_seqs][n_head], or NULL */
     float scale;              /* scores are scale * q . k */
 } sc_attn_decode;
@@ -123,10 +123,10 @@ typedef struct sc_gdn {
     const void* k;
     const void* v;            /* [tokens][v_heads][S] */
     void* out;                /* [tokens][v_heads][S] */
-    int64_t q_ld, k_ld, v_ld, out_ld;   /* multiples of 4 (f32) or 8 (f16) values */
+    int64_t q_ld, k_ld, v_ld, out_ld;   /* multiples of 4 (f32) or 8 (f16) values, at most 2^22 */
     const float* g;           /* [tokens][v_heads], <= 0 (below -200 counts as -200, whose decay is 0 as well) */
     const float* beta;        /* [tokens][v_heads] */
-    int64_t gate_ld;          /* values from token to token of g and beta */
+    int64_t gate_ld;          /* values from token to token of g and beta, at most 2^22 */
     float scale;
     int32_t l2norm;
     float eps;

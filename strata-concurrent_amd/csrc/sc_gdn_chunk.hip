@@ -6,15 +6,16 @@
 //     M1 = e^(G_C) M0 + sum_j e^(G_C - G_j) k_j u_j^T
 // Everything but M0 is known beforehand, so a first kernel forms T = (1 + A)^-1 and P of every chunk at once, and a second
 // one takes the chunks of a sequence in order with products only.  Columns of the state (values) do not meet: a workgroup
-// of the second kernel takes 16 or 32 of them.  Its four waves share the chunk's 64 tokens (16 rows each of K M0, X, U, O)
-// and the state's keys (32 each, in registers); what the others need of a wave's result goes through LDS, three times a
-// chunk.
+// of the second kernel takes 16 or 32 of them with two waves.  One carries the state, whole columns in its registers: a
+// result of a product (column = lane % 16, rows in registers) is the right operand of the next one as it stands, so nothing
+// it needs crosses lanes but a column's largest value.  The other is a chunk behind and forms the outputs from the state and
+// U that the first left in LDS; it also brings V and the factors of rows.  They meet once a chunk.
 //
 // Accuracy: the products run as f16 matrix instructions with sums in 32 bits, and keep f32 accuracy: an f32 operand is
 // two f16 parts (22 bits) after a scaling by a power of two that puts its largest values near f16's upper end, where small
 // ones keep their digits too.  f16 keys and queries enter as they are, exactly, and f32 ones scaled by row; unit length,
-// decays and write strengths are factors of rows in f32.  The scalings: the state by column and wave, X and U by column,
-// from bounds: with beta |k|^2 <= 2 (where the rule does not diverge) X stays below 2^5 and U below 2^8 of the largest of
+// decays and write strengths are factors of rows in f32.  The scalings: the state by column, X and U by column
+// too, from bounds: with beta |k|^2 <= 2 (where the rule does not diverge) X stays below 2^5 and U below 2^8 of the largest of
 // beta |V| and beta |M0|.  Sums of log decays are in 64 bits: what counts is their differences.
 #include <hip/hip_runtime.h>
 
@@ -29,7 +30,7 @@ constexpr int kC = 64;                       // tokens of a chunk
 constexpr int kWaves = 4, kThreadsC = kWaves * 64;
 constexpr float kLeastG = -200.0f;           // a decay of e^-200 is 0 in f32
 constexpr double kLog2e = 1.4426950408889634074;
-constexpr float kUpT = 0x1p10f, kUpX = 0x1p10f, kUpU = 0x1p6f;   // where operands lie in f16's range (T, P and X; U)
+constexpr float kUpT = 0x1p3f, kUpX = 0x1p3f, kUpU = kUpT * kUpX;   // where operands lie in f16's range: T, P; X; U
 
 // Places of a v head's chunk in the workspace, in 16-byte words: T and P as matrix operands [wave][step][part][lane] (a
 // wave's row tile w has steps 0 .. w / 2 of 32 tokens), then the factors of rows.
@@ -37,8 +38,22 @@ constexpr uint32_t kOperand = 6 * 2 * 64;
 constexpr uint32_t operand_at(uint32_t wave, uint32_t step, uint32_t part) {
     return ((wave < 2 ? wave : wave == 2 ? 2 : 4) + step) * 128 + part * 64;
 }
-enum { kFState = 0, kFBeta = 64, kFWrite = 128, kFQuery = 192, kFRow = 256, kFDecay = 320, kFUp, kFBetaMost, kFactors = 384 };
+enum { kFState = 0, kFBeta = 64, kFWrite = 128, kFQuery = 192, kFRow = 256, kFDecay = 320, kFUp, kFBetaMost, kFactors = 324 };
 constexpr uint32_t kChunkWords = 2 * kOperand + kFactors / 4;
+
+// Places of a key head's chunk in the workspace, in 16-byte words: its keys as the left operand of the state's update
+// [part][step of 32 keys][odd keys][step of 32 tokens][lane], then, where keys and queries are f32, their f16 parts as left
+// operands [keys, queries][part][tile of tokens][step][lane] (f16 ones are read from where they are).
+template <int S, int kParts>
+constexpr uint32_t key_operand(uint32_t part, uint32_t i, uint32_t e, uint32_t step) {
+    return (((part * (S / 32) + i) * 2 + e) * 2 + step) * 64;
+}
+template <int S, int kParts>
+constexpr uint32_t row_operand(uint32_t which, uint32_t part, uint32_t tile, uint32_t i) {
+    return kParts * S * 8 + (((which * kParts + part) * 4 + tile) * (S / 32) + i) * 64;
+}
+template <int S, int kParts>
+constexpr uint32_t kRowWords = kParts * S * 8 * (kParts == 1 ? 1 : 3);
 
 __device__ __forceinline__ f32x4 mfma(ops_u32x4 a, ops_u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
@@ -169,8 +184,8 @@ __global__ void __launch_bounds__(kThreadsC, 2) gdn_prepare_kernel(GdnArgs a, Ch
     if (!seq_of(a, lane, [&](uint32_t, uint32_t lo, uint32_t hi) { return chunk >= lo && chunk < hi; }, q)) return;
     const uint32_t t0 = q.t0 + (chunk - q.chunk0) * kC, n = q.t1 - t0 < kC ? q.t1 - t0 : kC;
     ops_u32x4* out = c.chunks + (uint64_t(piece) * a.v_heads + h) * kChunkWords;
-    uint8_t* rows = reinterpret_cast<uint8_t*>(c.rows + (uint64_t(piece) * c.k_heads + kh) * (4 * kC * S / 8));
-    const bool write_rows = !kF16 && h == kh * a.share.d;
+    ops_u32x4* rows = c.rows + (uint64_t(piece) * c.k_heads + kh) * kRowWords<S, kParts>;
+    const bool write_rows = h == kh * a.share.d;   // one of the value heads that share the keys
 
     const bool in = lane < n;
     const int64_t gates = int64_t(t0 + (in ? lane : 0)) * a.gate_ld + h;
@@ -218,7 +233,7 @@ __global__ void __launch_bounds__(kThreadsC, 2) gdn_prepare_kernel(GdnArgs a, Ch
                 if (write_rows)
 #pragma unroll
                     for (int part = 0; part < kParts; ++part)
-                        st_global<ops_u32x4>(rows + (((which * kParts + part) * kC + mine) * S + i * 32 + g * 8) * 2, x[part][i]);
+                        st_global<ops_u32x4>(rows + row_operand<S, kParts>(which, part, t, i) + lane, x[part][i]);
             }
         }
     };
@@ -239,6 +254,39 @@ __global__ void __launch_bounds__(kThreadsC, 2) gdn_prepare_kernel(GdnArgs a, Ch
     for (int t = 0; t < kAhead; ++t) load_raw(a.q, a.q_ld, t, q_raw[t]);
 #pragma unroll
     for (int t = 0; t < 4; ++t) to_tile(k_raw[t], t, kf[t], s.up[0], 0);
+
+    // the keys as the left operand of the state's update: key 32 i + 2 col + e, tokens 32 step + 4 g + j and 16 more, by way
+    // of LDS, where the tiles will be
+    if (write_rows) {
+        constexpr uint32_t kRow = S * 2 + 16;
+        static_assert(kC * kRow <= sizeof(s.tile) + sizeof(s.p));
+        uint8_t* lds = reinterpret_cast<uint8_t*>(s.tile);
+#pragma unroll
+        for (int part = 0; part < kParts; ++part) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t)
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) *reinterpret_cast<ops_u32x4*>(lds + (t * 16 + col) * kRow + i * 64 + g * 16) = kf[t][part][i];
+            wave_sync();
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+                for (int step = 0; step < 2; ++step) {
+                    uint32_t w[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j)
+                        w[j] = *reinterpret_cast<const uint32_t*>(lds + (step * 32 + (j / 4) * 16 + g * 4 + j % 4) * kRow + (i * 32 + col * 2) * 2);
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        const uint32_t sel = e ? 0x07060302u : 0x05040100u;
+                        st_global<ops_u32x4>(rows + key_operand<S, kParts>(part, i, e, step) + lane,
+                                             ops_u32x4{__builtin_amdgcn_perm(w[1], w[0], sel), __builtin_amdgcn_perm(w[3], w[2], sel),
+                                                       __builtin_amdgcn_perm(w[5], w[4], sel), __builtin_amdgcn_perm(w[7], w[6], sel)});
+                    }
+                }
+            wave_sync();
+        }
+    }
 
     // sums of the log decays, to base 2, lane = token
     const double G = scan_add64(in ? double(g_in < kLeastG ? kLeastG : g_in) * kLog2e : 0.0);
@@ -419,31 +467,34 @@ __global__ void __launch_bounds__(kThreadsC, 2) gdn_prepare_kernel(GdnArgs a, Ch
 
 // ---- the chunks of a sequence in order ------------------------------------------------------------------------------------
 
-// What a wave reads of a chunk before it can start on it.
-template <int S, int kParts>
-struct ChunkRows {
-    static constexpr int kSteps = S / 32;
-    ops_u32x4 k[kParts][kSteps], q[kParts][kSteps];   // its row tile
-    uint32_t kt[kParts][2][8];                        // its 32 keys: pairs of keys of the eight tokens of a step
-    ops_u32x4 t[2][2], p[2][2];                       // T and P: [step][part]
-    f32x4 f_state, beta, write, f_query, f_row;
-    f32x4 all;                                        // the chunk's decay, the scale of `write`, the largest beta
-};
+// Eight values, four each of two tiles, as a right operand in two parts.
+__device__ __forceinline__ void split_pair(f32x4 a, f32x4 b, ops_u32x4& hi, ops_u32x4& lo) {
+    uint32_t h[4], l[4];
+    split2(a.x, a.y, h[0], l[0]);
+    split2(a.z, a.w, h[1], l[1]);
+    split2(b.x, b.y, h[2], l[2]);
+    split2(b.z, b.w, h[3], l[3]);
+    hi = ops_u32x4{h[0], h[1], h[2], h[3]};
+    lo = ops_u32x4{l[0], l[1], l[2], l[3]};
+}
 
 template <int S, int kCols, bool kF16>
-__global__ void __launch_bounds__(kThreadsC, 1) gdn_chunk_kernel(GdnArgs a, ChunkArgs c) {
+__global__ void __launch_bounds__(128, 1) gdn_chunk_kernel(GdnArgs a, ChunkArgs c) {
     constexpr int kParts = kF16 ? 1 : 2, kSteps = S / 32, kN = kCols / 16;
-    using R = ChunkRows<S, kParts>;
-    struct Values {
-        f32x4 beta;
-        uint32_t raw[kN][4];
-        f32x4 by[kN];
+    constexpr uint32_t kBytes = kF16 ? 2 : 4;                            // of an activation
+    constexpr uint32_t kRowV = kCols * kBytes, kPieces = kRowV / 16;     // a row of V or O of this workgroup, in 16-byte pieces
+    constexpr uint32_t kEach = kC * kPieces / 64;                        // pieces of a lane
+    constexpr uint32_t kFLanes = (kFactors + 63) / 64;
+    // what one wave leaves for the other, by the chunk's parity
+    struct Left {
+        ops_u32x4 m[kN][kSteps][2][64], u[kN][2][2][64];   // the state before the chunk and U as right operands: [step][part]
+        float m_up[kN][16], x_up[kN][16];                  // what they were scaled down by, by column
     };
-    __shared__ ops_u32x4 s_m[kN][kSteps][2][64];         // the state as an operand: [step][part][lane]
-    __shared__ float s_scale[kN][kSteps][16];
-    __shared__ ops_u32x2 s_x[kN][2][2][64][2], s_u[kN][2][2][64][2], s_w[kN][2][2][64][2];   // [step][part][lane][tile]
-    __shared__ float s_v[2][kN][kWaves][16];
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    __shared__ Left s_left[2];
+    __shared__ __align__(16) uint8_t s_vin[2][kC * kRowV], s_out[kC * kRowV];
+    __shared__ __align__(16) float s_f[3][kFLanes * 64];
+    const uint32_t tid = threadIdx.x, lane = tid & 63;
+    const bool carries = __builtin_amdgcn_readfirstlane(tid >> 6) == 0;
     const uint32_t g = lane >> 4, col = lane & 15;
     // workgroups go to the eight XCDs in turn: the column blocks of a head are kept on one, whose L2 has its operands
     constexpr uint32_t kBlocks = S / kCols;
@@ -459,274 +510,319 @@ __global__ void __launch_bounds__(kThreadsC, 1) gdn_chunk_kernel(GdnArgs a, Chun
     float* base = a.state[seq];
     if (!base) {
         const uint32_t from = q.t0 + (c0 - q.chunk0) * kC, to = q.t0 + (c1 - q.chunk0) * kC < q.t1 ? q.t0 + (c1 - q.chunk0) * kC : q.t1;
-        for (uint32_t t = from + threadIdx.x / (kCols / 4); t < to; t += kThreadsC / (kCols / 4))
-            st_act4<kF16>(a.out + int64_t(t) * a.out_ld, h * S + block * kCols + threadIdx.x % (kCols / 4) * 4, f32x4{});
+        for (uint32_t t = from + tid / (kCols / 4); t < to; t += 128 / (kCols / 4))
+            st_act4<kF16>(a.out + int64_t(t) * a.out_ld, h * S + block * kCols + tid % (kCols / 4) * 4, f32x4{});
         return;
     }
-    // the state: keys 32 w + 8 g + 2 i + e in m[.][e][i], a column a lane; waves past the keys have none
-    const bool keys = wave < uint32_t(kSteps);
-    float* state = base + a.state_offset + h * a.head_ld + block * kCols + col + (wave * 32 + g * 8) * a.key_ld;
-    f32x4 m[kN][2];
-#pragma unroll
-    for (int b = 0; b < kN; ++b)
-#pragma unroll
-        for (int e = 0; e < 2; ++e)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) m[b][e][i] = keys ? ld_global<float>(state + (2 * i + e) * a.key_ld + b * 16) : 0.0f;
 
-    auto put_state = [&] {
-        if (!keys) return;
-#pragma unroll
-        for (int b = 0; b < kN; ++b) {
-            float top = 0;
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) top = fmaxf(top, fabsf(m[b][e][i]));
-            top = over_rows(top, max_of);
-            float down, up;
-            power_of(top, down, up);
-            if (g == 0) s_scale[b][wave][col] = top == 0 ? 0.0f : up;
-            uint32_t hi[4], lo[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) split2(m[b][0][i] * down, m[b][1][i] * down, hi[i], lo[i]);
-            s_m[b][wave][0][lane] = ops_u32x4{hi[0], hi[1], hi[2], hi[3]};
-            s_m[b][wave][1][lane] = ops_u32x4{lo[0], lo[1], lo[2], lo[3]};
-        }
+    // Loads are asked for where the registers that they fill have been used, a chunk ahead.  What a lane reads past the
+    // sequence's end is its last row again (a minimum of byte offsets, which row strides leave below 2^31), past the last
+    // chunk that chunk again: no branch decides what is in flight.
+    auto last_row = [&](uint32_t chunk) {
+        const uint32_t t0 = (chunk - q.chunk0) * kC;
+        return q.t1 - q.t0 - t0 < kC ? q.t1 - q.t0 - t0 - 1 : kC - 1;
     };
-
-    auto load = [&](R& r, uint32_t chunk) {
-        const uint32_t t0 = q.t0 + (chunk - q.chunk0) * kC, n = q.t1 - t0 < kC ? q.t1 - t0 : kC;
-        const uint64_t slot = chunk - c.first;
-        const uint8_t* rows = reinterpret_cast<const uint8_t*>(c.rows + (slot * c.k_heads + kh) * (4 * kC * S / 8));
-        const uint32_t mine = wave * 16 + col, at = mine < n ? mine : n - 1;
+    auto clamped = [&](uint32_t chunk) { return chunk < c1 ? chunk : c1 - 1; };
+    auto operands_of = [&](uint32_t chunk) { return c.chunks + (uint64_t(chunk - c.first) * a.v_heads + h) * kChunkWords; };
+    auto rows_of = [&](uint32_t chunk) { return c.rows + (uint64_t(chunk - c.first) * c.k_heads + kh) * kRowWords<S, kParts>; };
+    // keys or queries as left operands
+    auto load_rows = [&](ops_u32x4 (&x)[4][kParts][kSteps], uint32_t chunk, uint32_t which) {
+        if constexpr (kF16) {
+            const uint32_t ld = uint32_t(which ? a.q_ld : a.k_ld), last = last_row(chunk) * ld;
+            const uint8_t* p = (which ? a.q : a.k) + int64_t(q.t0 + (chunk - q.chunk0) * kC) * ld + kh * S * 2;
 #pragma unroll
-        for (int part = 0; part < kParts; ++part) {
-            const uint8_t* kp = kF16 ? a.k + int64_t(t0 + at) * a.k_ld + kh * S * 2 : rows + (part * kC + mine) * S * 2;
-            const uint8_t* qp = kF16 ? a.q + int64_t(t0 + at) * a.q_ld + kh * S * 2 : rows + ((kParts + part) * kC + mine) * S * 2;
+            for (int t = 0; t < 4; ++t) {
+                const uint32_t at = min((t * 16 + col) * ld, last) + g * 16;
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                r.k[part][i] = ld_global<ops_u32x4>(kp + i * 64 + g * 16);
-                r.q[part][i] = ld_global<ops_u32x4>(qp + i * 64 + g * 16);
+                for (int i = 0; i < kSteps; ++i) x[t][0][i] = ld_global<ops_u32x4>(p + at + i * 64);
             }
-            if (keys)
+        } else {
+            const ops_u32x4* p = rows_of(chunk) + lane;
 #pragma unroll
-                for (int step = 0; step < 2; ++step)
+            for (int t = 0; t < 4; ++t)
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        const uint32_t t = step * 32 + (j / 4) * 16 + g * 4 + j % 4, u = t < n ? t : n - 1;
-                        const uint8_t* p = kF16 ? a.k + int64_t(t0 + u) * a.k_ld + kh * S * 2 : rows + (part * kC + t) * S * 2;
-                        r.kt[part][step][j] = ld_global<uint32_t>(p + (wave * 32 + col * 2) * 2);
-                    }
-        }
-        const ops_u32x4* from = c.chunks + (slot * a.v_heads + h) * kChunkWords;
+                for (int part = 0; part < kParts; ++part)
 #pragma unroll
-        for (int step = 0; step < 2; ++step)
-            if (uint32_t(step) <= wave / 2)
-#pragma unroll
-                for (int part = 0; part < 2; ++part) {
-                    r.t[step][part] = ld_global<ops_u32x4>(from + operand_at(wave, step, part) + lane);
-                    r.p[step][part] = ld_global<ops_u32x4>(from + kOperand + operand_at(wave, step, part) + lane);
-                }
-        const float* f = reinterpret_cast<const float*>(from + 2 * kOperand);
-        const uint32_t mine4 = wave * 16 + g * 4;
-        r.f_state = ld_global<f32x4>(f + kFState + mine4);
-        r.write = ld_global<f32x4>(f + kFWrite + mine4);
-        r.f_query = ld_global<f32x4>(f + kFQuery + mine4);
-        r.f_row = ld_global<f32x4>(f + kFRow + mine4);
-        r.all = ld_global<f32x4>(f + kFDecay);
-    };
-    // the wave's rows of V, and their largest value a column times beta, for the scale of X
-    auto load_v = [&](Values& v, uint32_t chunk) {
-        const uint32_t t0 = q.t0 + (chunk - q.chunk0) * kC, n = q.t1 - t0 < kC ? q.t1 - t0 : kC;
-        v.beta = ld_global<f32x4>(reinterpret_cast<const float*>(c.chunks + (uint64_t(chunk - c.first) * a.v_heads + h) * kChunkWords + 2 * kOperand) +
-                                  kFBeta + wave * 16 + g * 4);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t t = wave * 16 + g * 4 + i;
-            const uint8_t* p = a.v + int64_t(t0 + (t < n ? t : n - 1)) * a.v_ld;
-#pragma unroll
-            for (int b = 0; b < kN; ++b) {
-                const uint32_t at = h * S + block * kCols + b * 16 + col;
-                if constexpr (kF16) v.raw[b][i] = ld_global<uint16_t>(p + at * 2);
-                else v.raw[b][i] = ld_global<uint32_t>(p + at * 4);
-            }
+                    for (int i = 0; i < kSteps; ++i) x[t][part][i] = ld_global<ops_u32x4>(p + row_operand<S, kParts>(which, part, t, i));
         }
     };
-    auto put_v = [&](Values& v, uint32_t chunk) {
-        const uint32_t t0 = q.t0 + (chunk - q.chunk0) * kC, n = q.t1 - t0 < kC ? q.t1 - t0 : kC;
+    // T or P: operand w of operand_at's six, in two parts
+    auto load_operand = [&](ops_u32x4 (&x)[6][2], uint32_t chunk, uint32_t which) {
+        const ops_u32x4* p = operands_of(chunk) + which * kOperand + lane;
 #pragma unroll
-        for (int b = 0; b < kN; ++b) {
-            float top = 0;
+        for (int i = 0; i < 6; ++i)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float x = kF16 ? float(__builtin_bit_cast(_Float16, uint16_t(v.raw[b][i]))) : __uint_as_float(v.raw[b][i]);
-                v.by[b][i] = wave * 16 + g * 4 + i < n ? x * v.beta[i] : 0.0f;
-                top = fmaxf(top, fabsf(v.by[b][i]));
-            }
-            top = over_rows(top, max_of);
-            if (g == 0) s_v[(chunk - c0) & 1][b][wave][col] = top;
+            for (int part = 0; part < 2; ++part) x[i][part] = ld_global<ops_u32x4>(p + i * 128 + part * 64);
+    };
+    // the product with T or P of a right operand [step][part]
+    auto triangle = [&](const ops_u32x4 (&x)[6][2], const ops_u32x4 (&y)[2][2], int tile) {
+        const int first = tile < 2 ? tile : tile == 2 ? 2 : 4;
+        f32x4 hi{}, lo{};
+#pragma unroll
+        for (int step = 0; step <= tile / 2; ++step) {
+            hi = mfma(x[first + step][0], y[step][0], hi);
+            lo = mfma(x[first + step][0], y[step][1], lo);
+            lo = mfma(x[first + step][1], y[step][0], lo);
         }
-    };
-    // a tile of 16 tokens of X, U or the weighted U as an operand: the wave's half of a step
-    auto put = [&](ops_u32x2 (&to)[2][2][64][2], f32x4 x) {
-        uint32_t h0, l0, h1, l1;
-        split2(x.x, x.y, h0, l0);
-        split2(x.z, x.w, h1, l1);
-        to[wave / 2][0][lane][wave % 2] = ops_u32x2{h0, h1};
-        to[wave / 2][1][lane][wave % 2] = ops_u32x2{l0, l1};
-    };
-    auto get = [&](const ops_u32x2 (&from)[2][2][64][2], int step, int part) {
-        return *reinterpret_cast<const ops_u32x4*>(&from[step][part][lane][0]);
+        return hi + lo;
     };
 
-    // a chunk's rows are asked for a whole chunk before they are used
-    R ra, rb;
-    Values v;
-    load_v(v, c0);
-    load(ra, c0);
-    put_state();
-    put_v(v, c0);
-    auto turn = [&](const uint32_t chunk, R& r, R& next) {
-        const uint32_t t0 = q.t0 + (chunk - q.chunk0) * kC, n = q.t1 - t0 < kC ? q.t1 - t0 : kC;
-        const bool more = chunk + 1 < c1;
-        Values nv;
-        if (more) {
-            load_v(nv, chunk + 1);
-            load(next, chunk + 1);
-        }
-        __syncthreads();
-        // K M0 and Q M0, a step's sum by its own scale
-        f32x4 qm[kN];
-        float x_down[kN], x_up[kN];
-#pragma unroll
-        for (int b = 0; b < kN; ++b) {
-            f32x4 km{};
-            qm[b] = f32x4{};
-            float most = 0;
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                const ops_u32x4 hi = s_m[b][i][0][lane], lo = s_m[b][i][1][lane];
-                const float scale = s_scale[b][i][col];
-                f32x4 ks{}, qs{};
-                ks = mfma(r.k[0][i], hi, ks);
-                qs = mfma(r.q[0][i], hi, qs);
-                ks = mfma(r.k[0][i], lo, ks);
-                qs = mfma(r.q[0][i], lo, qs);
-                if constexpr (!kF16) ks = mfma(r.k[kParts - 1][i], hi, ks), qs = mfma(r.q[kParts - 1][i], hi, qs);
-                km += scale * ks;
-                qm[b] += scale * qs;
-                most = fmaxf(most, scale);
-            }
-            most *= r.all.z;
-#pragma unroll
-            for (int w = 0; w < kWaves; ++w) most = fmaxf(most, s_v[(chunk - c0) & 1][b][w][col]);
-            power_of(most, x_down[b], x_up[b]);
-            f32x4 x;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[i] = wave * 16 + g * 4 + i < n ? (v.by[b][i] - r.f_state[i] * km[i]) * (x_down[b] * kUpX) : 0.0f;
-            put(s_x[b], x);
-        }
-        __syncthreads();
-        // U = T X, and the same weighted for the state
-#pragma unroll
-        for (int b = 0; b < kN; ++b) {
-            f32x4 u{};
-#pragma unroll
-            for (int step = 0; step < 2; ++step)
-                if (uint32_t(step) <= wave / 2) {
-                    const ops_u32x4 hi = get(s_x[b], step, 0), lo = get(s_x[b], step, 1);
-                    u = mfma(r.t[step][0], hi, u);
-                    u = mfma(r.t[step][0], lo, u);
-                    u = mfma(r.t[step][1], hi, u);
-                }
-            u *= kUpU / (kUpT * kUpX);
-            put(s_u[b], u);
-            f32x4 w;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = u[i] * r.write[i];
-            put(s_w[b], w);
-        }
-        __syncthreads();
-        // the state after the chunk
-        if (keys) {
-            if (kF16 && n < uint32_t(kC))   // the last, partial chunk: whatever lies in the rows past it stays out
-#pragma unroll
-                for (int step = 0; step < 2; ++step)
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        if (step * 32 + (j / 4) * 16 + g * 4 + j % 4 >= n) r.kt[0][step][j] = 0;
-#pragma unroll
-            for (int b = 0; b < kN; ++b) {
-                f32x4 add[2]{};
-#pragma unroll
-                for (int step = 0; step < 2; ++step) {
-                    const ops_u32x4 hi = get(s_w[b], step, 0), lo = get(s_w[b], step, 1);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-#pragma unroll
-                        for (int part = 0; part < kParts; ++part) {
-                            const uint32_t sel = e ? 0x07060302u : 0x05040100u;
-                            const uint32_t (&t)[8] = r.kt[part][step];
-                            const ops_u32x4 key{__builtin_amdgcn_perm(t[1], t[0], sel), __builtin_amdgcn_perm(t[3], t[2], sel),
-                                                __builtin_amdgcn_perm(t[5], t[4], sel), __builtin_amdgcn_perm(t[7], t[6], sel)};
-                            add[e] = mfma(key, hi, add[e]);
-                            if (part == 0) add[e] = mfma(key, lo, add[e]);
-                        }
-                }
-                const float by = x_up[b] * r.all.y * (1.0f / kUpU);
-#pragma unroll
-                for (int e = 0; e < 2; ++e) m[b][e] = r.all.x * m[b][e] + by * add[e];
-            }
-        }
-        put_state();
-        // outputs
-#pragma unroll
-        for (int b = 0; b < kN; ++b) {
-            f32x4 pu{};
-#pragma unroll
-            for (int step = 0; step < 2; ++step)
-                if (uint32_t(step) <= wave / 2) {
-                    const ops_u32x4 hi = get(s_u[b], step, 0), lo = get(s_u[b], step, 1);
-                    pu = mfma(r.p[step][0], hi, pu);
-                    pu = mfma(r.p[step][0], lo, pu);
-                    pu = mfma(r.p[step][1], hi, pu);
-                }
-            const float by = x_up[b] * (1.0f / (kUpU * kUpT));
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t t = wave * 16 + g * 4 + i;
-                if (t >= n) continue;
-                const float o = r.f_query[i] * qm[b][i] + r.f_row[i] * by * pu[i];
-                uint8_t* to = a.out + int64_t(t0 + t) * a.out_ld;
-                const uint32_t at = h * S + block * kCols + b * 16 + col;
-                if constexpr (kF16) st_global<uint16_t>(to + at * 2, __builtin_bit_cast(uint16_t, _Float16(o)));
-                else st_global<float>(to + at * 4, o);
-            }
-        }
-        if (more) {
-            put_v(nv, chunk + 1);
-            v = nv;
-        }
-    };
-    for (uint32_t chunk = c0; chunk < c1; chunk += 2) {
-        turn(chunk, ra, rb);
-        if (chunk + 1 < c1) turn(chunk + 1, rb, ra);
-    }
-    if (keys)
+    if (carries) {
+        // the state: keys 32 i + 8 g + 2 j + e in m[.][i][e][j], a column a lane
+        float* state = base + a.state_offset + h * a.head_ld + block * kCols + col + g * 8 * a.key_ld;
+        f32x4 m[kN][kSteps][2];
 #pragma unroll
         for (int b = 0; b < kN; ++b)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) st_global<float>(state + (2 * i + e) * a.key_ld + b * 16, m[b][e][i]);
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) m[b][i][e][j] = ld_global<float>(state + (i * 32 + 2 * j + e) * a.key_ld + b * 16);
+        ops_u32x4 k[4][kParts][kSteps], t[6][2], kt[kParts][kSteps][2][2];
+        auto load_keys = [&](uint32_t chunk) {
+            const ops_u32x4* p = rows_of(chunk) + lane;
+#pragma unroll
+            for (int part = 0; part < kParts; ++part)
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int step = 0; step < 2; ++step) kt[part][i][e][step] = ld_global<ops_u32x4>(p + key_operand<S, kParts>(part, i, e, step));
+        };
+        load_rows(k, c0, 0);
+        load_operand(t, c0, 0);
+        load_keys(c0);
+        for (uint32_t chunk = c0; chunk < c1; ++chunk) {
+            const uint32_t which = (chunk - c0) & 1, last = last_row(chunk), ahead = clamped(chunk + 1);
+            Left& left = s_left[which];
+            __syncthreads();   // V and the factors are here, and the outputs of the chunk before the last are done
+            const float* f = s_f[(chunk - c0) % 3];
+            // the state as a right operand, scaled by column
+            ops_u32x4 mh[kN][kSteps], ml[kN][kSteps];
+            float m_up[kN];
+#pragma unroll
+            for (int b = 0; b < kN; ++b) {
+                float top = 0;
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(m[b][i][e][j]));
+                top = over_rows(top, max_of);
+                float down;
+                power_of(top, down, m_up[b]);
+                if (top == 0) m_up[b] = 0.0f;
+#pragma unroll
+                for (int i = 0; i < kSteps; ++i) {
+                    // keys 8 g .. 8 g + 7 in order: the even ones and the odd ones take turns
+                    const f32x4 even = m[b][i][0] * down, odd = m[b][i][1] * down;
+                    split_pair(f32x4{even.x, odd.x, even.y, odd.y}, f32x4{even.z, odd.z, even.w, odd.w}, mh[b][i], ml[b][i]);
+                    left.m[b][i][0][lane] = mh[b][i];
+                    left.m[b][i][1][lane] = ml[b][i];
+                }
+                if (g == 0) left.m_up[b][col] = m_up[b];
+            }
+            // K M0
+            f32x4 km[kN][4];
+#pragma unroll
+            for (int b = 0; b < kN; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) km[b][r] = f32x4{};
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+                for (int x = 0; x < kParts + 1; ++x)   // high by high, high by low, low by high
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+#pragma unroll
+                        for (int b = 0; b < kN; ++b) km[b][r] = mfma(k[r][x == 2][i], x == 1 ? ml[b][i] : mh[b][i], km[b][r]);
+            load_rows(k, ahead, 0);
+            // X, scaled by column
+            ops_u32x4 xs[kN][2][2];
+            float x_up[kN];
+#pragma unroll
+            for (int b = 0; b < kN; ++b) {
+                f32x4 v[4];
+                float top = 0;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const f32x4 beta = *reinterpret_cast<const f32x4*>(&f[kFBeta + r * 16 + g * 4]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint32_t row = r * 16 + g * 4 + j;
+                        const uint8_t* p = &s_vin[which][row * kRowV + (b * 16 + col) * kBytes];
+                        float x;
+                        if constexpr (kF16) x = float(*reinterpret_cast<const _Float16*>(p));
+                        else x = *reinterpret_cast<const float*>(p);
+                        v[r][j] = row <= last ? x * beta[j] : 0.0f;
+                        top = fmaxf(top, fabsf(v[r][j]));
+                    }
+                }
+                top = over_rows(top, max_of);
+                float down;
+                power_of(fmaxf(top, m_up[b] * f[kFBetaMost]), down, x_up[b]);
+                if (g == 0) left.x_up[b][col] = x_up[b];
+                down *= kUpX;
+                const float by = m_up[b] * down;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const f32x4 fs = *reinterpret_cast<const f32x4*>(&f[kFState + r * 16 + g * 4]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        v[r][j] = int(r * 16 + g * 4 + j) <= int(last) ? v[r][j] * down - fs[j] * by * km[b][r][j] : 0.0f;
+                }
+                split_pair(v[0], v[1], xs[b][0][0], xs[b][0][1]);
+                split_pair(v[2], v[3], xs[b][1][0], xs[b][1][1]);
+            }
+            // U = T X, and the same weighted for the state
+            ops_u32x4 ws[kN][2][2];
+#pragma unroll
+            for (int b = 0; b < kN; ++b) {
+                f32x4 u[4];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) u[r] = triangle(t, xs[b], r);
+                ops_u32x4 us[2][2];
+                split_pair(u[0], u[1], us[0][0], us[0][1]);
+                split_pair(u[2], u[3], us[1][0], us[1][1]);
+#pragma unroll
+                for (int step = 0; step < 2; ++step)
+#pragma unroll
+                    for (int part = 0; part < 2; ++part) left.u[b][step][part][lane] = us[step][part];
+#pragma unroll
+                for (int r = 0; r < 4; ++r) u[r] *= *reinterpret_cast<const f32x4*>(&f[kFWrite + r * 16 + g * 4]);
+                split_pair(u[0], u[1], ws[b][0][0], ws[b][0][1]);
+                split_pair(u[2], u[3], ws[b][1][0], ws[b][1][1]);
+            }
+            load_operand(t, ahead, 0);
+            // the state after the chunk
+            const float decay = f[kFDecay], up = f[kFUp] * (1.0f / kUpU);
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                f32x4 add[kN][2];
+#pragma unroll
+                for (int b = 0; b < kN; ++b) add[b][0] = f32x4{}, add[b][1] = f32x4{};
+#pragma unroll
+                for (int step = 0; step < 2; ++step)
+#pragma unroll
+                    for (int x = 0; x < kParts + 1; ++x)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e)
+#pragma unroll
+                            for (int b = 0; b < kN; ++b)
+                                add[b][e] = mfma(kt[x == 2][i][e][step], ws[b][step][x == 1], add[b][e]);
+#pragma unroll
+                for (int b = 0; b < kN; ++b)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) m[b][i][e] = decay * m[b][i][e] + (x_up[b] * up) * add[b][e];
+            }
+            load_keys(ahead);
+        }
+        __syncthreads();   // the last chunk's outputs
+#pragma unroll
+        for (int b = 0; b < kN; ++b)
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) st_global<float>(state + (i * 32 + 2 * j + e) * a.key_ld + b * 16, m[b][i][e][j]);
+        return;
+    }
+
+    // the other wave: V and the factors of the chunk after the next, outputs of the chunk before
+    const uint32_t v_ld = uint32_t(a.v_ld);
+    ops_u32x4 v_in[kEach];
+    float f_in[kFLanes];
+    auto load_early = [&](uint32_t chunk) {
+        const uint32_t last = last_row(chunk) * v_ld;
+        const uint8_t* p = a.v + int64_t(q.t0 + (chunk - q.chunk0) * kC) * a.v_ld + (h * S + block * kCols) * kBytes;
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            const uint32_t at = lane + i * 64;
+            v_in[i] = ld_global<ops_u32x4>(p + min(at / kPieces * v_ld, last) + at % kPieces * 16);
+        }
+        const float* f = reinterpret_cast<const float*>(operands_of(chunk) + 2 * kOperand);
+#pragma unroll
+        for (uint32_t i = 0; i < kFLanes; ++i) f_in[i] = ld_global<float>(f + min(lane + i * 64, uint32_t(kFactors - 1)));
+    };
+    auto put_early = [&](uint32_t n) {
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) *reinterpret_cast<ops_u32x4*>(&s_vin[n & 1][(lane + i * 64) * 16]) = v_in[i];
+#pragma unroll
+        for (uint32_t i = 0; i < kFLanes; ++i) s_f[n % 3][lane + i * 64] = f_in[i];
+    };
+    ops_u32x4 qs[4][kParts][kSteps], p[6][2];
+    load_early(c0);
+    put_early(0);
+    load_early(clamped(c0 + 1));
+    load_rows(qs, c0, 1);
+    load_operand(p, c0, 1);
+    for (uint32_t chunk = c0; chunk <= c1; ++chunk) {
+        const uint32_t n = chunk - c0;
+        __syncthreads();
+        // the first wave reads the places of chunk n now, and this one the factors of chunk n - 1
+        if (chunk < c1) {
+            put_early(n + 1);
+            load_early(clamped(chunk + 2));
+        }
+        if (chunk == c0) continue;
+        const uint32_t done = chunk - 1, last = last_row(done);
+        const Left& left = s_left[(n - 1) & 1];
+        const float* f = s_f[(n - 1) % 3];
+#pragma unroll
+        for (int b = 0; b < kN; ++b) {
+            f32x4 qm[4];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) qm[r] = f32x4{};
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) {
+                const ops_u32x4 hi = left.m[b][i][0][lane], lo = left.m[b][i][1][lane];
+#pragma unroll
+                for (int x = 0; x < kParts + 1; ++x)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) qm[r] = mfma(qs[r][x == 2][i], x == 1 ? lo : hi, qm[r]);
+            }
+            ops_u32x4 us[2][2];
+#pragma unroll
+            for (int step = 0; step < 2; ++step)
+#pragma unroll
+                for (int part = 0; part < 2; ++part) us[step][part] = left.u[b][step][part][lane];
+            const float m_up = left.m_up[b][col], by = left.x_up[b][col] * (1.0f / (kUpU * kUpT));
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const f32x4 pu = triangle(p, us, r);
+                const f32x4 fq = *reinterpret_cast<const f32x4*>(&f[kFQuery + r * 16 + g * 4]), fr = *reinterpret_cast<const f32x4*>(&f[kFRow + r * 16 + g * 4]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float o = fq[j] * m_up * qm[r][j] + fr[j] * by * pu[j];
+                    uint8_t* to = &s_out[(r * 16 + g * 4 + j) * kRowV + (b * 16 + col) * kBytes];
+                    if constexpr (kF16) *reinterpret_cast<_Float16*>(to) = _Float16(o);
+                    else *reinterpret_cast<float*>(to) = o;
+                }
+            }
+        }
+        load_rows(qs, clamped(chunk), 1);
+        load_operand(p, clamped(chunk), 1);
+        wave_sync();
+        uint8_t* to = a.out + int64_t(q.t0 + (done - q.chunk0) * kC) * a.out_ld + (h * S + block * kCols) * kBytes;
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            const uint32_t at = lane + i * 64;
+            if (at / kPieces <= last)
+                st_global<ops_u32x4>(to + int64_t(at / kPieces) * a.out_ld + at % kPieces * 16, *reinterpret_cast<const ops_u32x4*>(&s_out[at * 16]));
+        }
+        wave_sync();
+    }
 }
 
 template <int S, int kCols, bool kF16>
 void launch_chunks(const GdnArgs& a, const ChunkArgs& c, hipStream_t stream) {
     const uint32_t pairs = (a.n_seqs * a.v_heads + 7) / 8 * 8;
     hipLaunchKernelGGL((gdn_prepare_kernel<S, kF16>), dim3((c.count * a.v_heads + kWaves - 1) / kWaves), dim3(kThreadsC), 0, stream, a, c);
-    hipLaunchKernelGGL((gdn_chunk_kernel<S, kCols, kF16>), dim3(pairs * (S / kCols)), dim3(kThreadsC), 0, stream, a, c);
+    hipLaunchKernelGGL((gdn_chunk_kernel<S, kCols, kF16>), dim3(pairs * (S / kCols)), dim3(128), 0, stream, a, c);
 }
 template <int S>
 hipError_t launch_of(const GdnArgs& a, const ChunkArgs& plan, bool f16, hipStream_t stream) {
@@ -751,7 +847,7 @@ uint64_t plan_gdn_chunks(const GdnArgs& a, int size, bool f16, ChunkArgs& c) {
     c.count = c.total < kMostChunks ? c.total : kMostChunks;
     c.first = 0;
     c.k_heads = a.v_heads / a.share.d;
-    const uint64_t chunks = uint64_t(c.count) * a.v_heads * kChunkWords, rows = f16 ? 0 : uint64_t(c.count) * c.k_heads * (4 * kC * size / 8);
+    const uint64_t chunks = uint64_t(c.count) * a.v_heads * kChunkWords, rows = uint64_t(c.count) * c.k_heads * size * (f16 ? 8 : 48);
     c.rows_at = chunks;
     const uint64_t bytes = (chunks + rows) * 16;
     return bytes ? bytes : 256;

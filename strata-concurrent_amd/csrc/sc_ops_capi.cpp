@@ -32,9 +32,10 @@ int launched(hipError_t e, const char* op) {
 
 bool off(const void* p, uintptr_t align) { return (reinterpret_cast<uintptr_t>(p) & (align - 1)) != 0; }
 
-// The row stride of an activation tensor: whole 16 bytes from row to row, at least a row, in bytes below 2^31 values.
+// The row stride of an activation tensor: whole 16 bytes from row to row, at least a row, at most 2^22 values (the rows
+// of a chunk of 64 lie within 2^31 bytes).
 bool row_stride(int64_t ld, int64_t row, int32_t dtype) {
-    return ld >= row && ld <= (int64_t(1) << 31) && ld % (dtype == SC_DTYPE_F16 ? 8 : 4) == 0;
+    return ld >= row && ld <= (int64_t(1) << 22) && ld % (dtype == SC_DTYPE_F16 ? 8 : 4) == 0;
 }
 int64_t value_bytes(int32_t dtype) { return dtype == SC_DTYPE_F16 ? 2 : 4; }
 
@@ -114,7 +115,7 @@ int gdn_args(const char* op, const sc_gdn* d, bool step, sc::GdnArgs& a) {
     if (!row_stride(d->q_ld, d->k_heads * S, d->dtype) || !row_stride(d->k_ld, d->k_heads * S, d->dtype) ||
         !row_stride(d->v_ld, d->v_heads * S, d->dtype) || !row_stride(d->out_ld, d->v_heads * S, d->dtype))
         return bad(op, "row strides must be whole 16 bytes and hold a row");
-    if (!d->g || !d->beta || off(d->g, 4) || off(d->beta, 4) || d->gate_ld < d->v_heads || d->gate_ld > (int64_t(1) << 31))
+    if (!d->g || !d->beta || off(d->g, 4) || off(d->beta, 4) || d->gate_ld < d->v_heads || d->gate_ld > (int64_t(1) << 22))
         return bad(op, "g and beta must be given, 4-byte aligned, gate_ld at least v_heads");
     if (!d->state || off(d->state, 8)) return bad(op, "state must be given, 8-byte aligned");
     if (d->state_offset < 0 || d->state_offset % 4 || d->state_head_ld < S || d->state_head_ld % 4 || d->state_key_ld < S ||
