@@ -12,11 +12,11 @@
 // U that the first left in LDS; it also brings V and the factors of rows.  They meet once a chunk.
 //
 // Accuracy: the products run as f16 matrix instructions with sums in 32 bits, and keep f32 accuracy: an f32 operand is
-// two f16 parts (22 bits) after a scaling by a power of two that puts its largest values near f16's upper end, where small
-// ones keep their digits too.  f16 keys and queries enter as they are, exactly, and f32 ones scaled by row; unit length,
-// decays and write strengths are factors of rows in f32.  The scalings: the state by column, X and U by column
-// too, from bounds: with beta |k|^2 <= 2 (where the rule does not diverge) X stays below 2^5 and U below 2^8 of the largest of
-// beta |V| and beta |M0|.  Sums of log decays are in 64 bits: what counts is their differences.
+// two f16 parts (22 bits).  f16 keys and queries enter as they are, exactly, f32 ones scaled by row with a power of two;
+// unit length, decays and write strengths are factors of rows in f32.  The state, X and U share one power of two a column,
+// which changes only when the column's largest of |M0| and beta |V| leaves a window: with beta |k|^2 <= 2 (where the rule
+// does not diverge) X stays below 2^5 and U below 2^8 of that, inside f16's range, and what is lost of small values is
+// below 2^-25 of the window's lower end.  Sums of log decays are in 64 bits: what counts is their differences.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -30,7 +30,9 @@ constexpr int kC = 64;                       // tokens of a chunk
 constexpr int kWaves = 4, kThreadsC = kWaves * 64;
 constexpr float kLeastG = -200.0f;           // a decay of e^-200 is 0 in f32
 constexpr double kLog2e = 1.4426950408889634074;
-constexpr float kUpT = 0x1p3f, kUpX = 0x1p3f, kUpU = kUpT * kUpX;   // where operands lie in f16's range: T, P; X; U
+// Where a column's largest of |M0| and beta |V| lies as operands: below 2^kTop and not below 2^kLeast, else it is scaled
+// anew, to 2^kAim.
+constexpr int kTop = 7, kLeast = -3, kAim = 3;
 
 // Places of a v head's chunk in the workspace, in 16-byte words: T and P as matrix operands [wave][step][part][lane] (a
 // wave's row tile w has steps 0 .. w / 2 of 32 tokens), then the factors of rows.
@@ -60,16 +62,23 @@ __device__ __forceinline__ f32x4 mfma(ops_u32x4 a, ops_u32x4 b, f32x4 c) {
 }
 __device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
-__device__ __forceinline__ uint32_t pack_f16(float a, float b) {
-    return __builtin_bit_cast(uint32_t, f16x2{_Float16(a), _Float16(b)});
+// Two values, each times `by`, as two f16 parts: the product truncated, and what that left out.  The high part is taken by
+// the instruction that packs two, so that what is subtracted is what is multiplied later; the low part is one fused
+// multiply-add a value that rounds to f16 (which is why `by` is never the literal one: that would be a subtraction and a
+// conversion).
+__device__ __forceinline__ void split2(float a, float b, float by_a, float by_b, uint32_t& hi, uint32_t& lo) {
+    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a * by_a, b * by_b));
+    const f16x2 h = __builtin_bit_cast(f16x2, hi);
+    const f16x2 l{_Float16(__builtin_fmaf(a, by_a, -float(h.x))), _Float16(__builtin_fmaf(b, by_b, -float(h.y)))};
+    lo = __builtin_bit_cast(uint32_t, l);
 }
-// Two values as two f16 parts: truncated, and what that left out.  The high part is taken by the instruction that packs
-// two, so that what is subtracted is what is multiplied later (a conversion the compiler folds into the product before it
-// may round another way).
 __device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    float one = 1.0f;
+    asm("" : "+s"(one));
     hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
     const f16x2 h = __builtin_bit_cast(f16x2, hi);
-    lo = pack_f16(a - float(h.x), b - float(h.y));
+    const f16x2 l{_Float16(__builtin_fmaf(a, one, -float(h.x))), _Float16(__builtin_fmaf(b, one, -float(h.y)))};
+    lo = __builtin_bit_cast(uint32_t, l);
 }
 // 2^-e and 2^e for the exponent of x >= 0 (its largest power of two not above), within f32's normal range; 1 for 0.
 __device__ __forceinline__ void power_of(float x, float& down, float& up) {
@@ -159,27 +168,47 @@ __device__ __forceinline__ void wave_sync() {
 constexpr int kTileRow = 20, kTileFloats = 16 * kTileRow + 4;   // a 16 x 16 tile in LDS: 16-byte rows, tiles on banks of their own
 constexpr int tile_of(int r, int c) { return r * (r + 1) / 2 + c; }
 
-// A wave takes one chunk of one value head, alone: the products K K^T and Q K^T by tiles of 16 tokens up to the diagonal,
-// A and P from them, and T = (1 + A)^-1: the four diagonal tiles by substitution, a column a lane, the rest by products
-// of tiles, T_10 = - T_11 (A_10 T_00) for tiles of 16 and then of 32, with f32 matrix instructions.  A product's left tile
-// comes from LDS as rows, its right one is a result in registers as it is: the four terms a lane adds are those whose rows
-// it holds.
+// Eight values, four each of two tiles, as a right operand in two parts.
+__device__ __forceinline__ void split_pair(f32x4 a, f32x4 b, ops_u32x4& hi, ops_u32x4& lo) {
+    uint32_t h[4], l[4];
+    split2(a.x, a.y, h[0], l[0]);
+    split2(a.z, a.w, h[1], l[1]);
+    split2(b.x, b.y, h[2], l[2]);
+    split2(b.z, b.w, h[3], l[3]);
+    hi = ops_u32x4{h[0], h[1], h[2], h[3]};
+    lo = ops_u32x4{l[0], l[1], l[2], l[3]};
+}
+
+// The same of values times `by`.
+__device__ __forceinline__ void split_pair(f32x4 a, f32x4 b, f32x4 by_a, f32x4 by_b, ops_u32x4& hi, ops_u32x4& lo) {
+    uint32_t h[4], l[4];
+    split2(a.x, a.y, by_a.x, by_a.y, h[0], l[0]);
+    split2(a.z, a.w, by_a.z, by_a.w, h[1], l[1]);
+    split2(b.x, b.y, by_b.x, by_b.y, h[2], l[2]);
+    split2(b.z, b.w, by_b.z, by_b.w, h[3], l[3]);
+    hi = ops_u32x4{h[0], h[1], h[2], h[3]};
+    lo = ops_u32x4{l[0], l[1], l[2], l[3]};
+}
+
+// A workgroup takes one chunk of one value head; wave w has its row tile w, tokens 16 w .. 16 w + 15: K K^T and Q K^T by
+// tiles up to the diagonal, A and P from them, and of T = (1 + A)^-1 the diagonal tile by substitution, a column a lane; the
+// rest of T by products of tiles, T_10 = - T_11 (A_10 T_00) for tiles of 16 and then of 32, with f32 matrix instructions.  A
+// product's left tile comes from LDS as rows, its right one is a result in registers as it is: the four terms a lane adds are
+// those whose rows it holds.  Latency bounds it, not any of its units: a chunk of one head is a chain of small steps.
 template <int S, bool kF16>
-__global__ void __launch_bounds__(kThreadsC, 2) gdn_prepare_kernel(GdnArgs a, ChunkArgs c) {
+__global__ void __launch_bounds__(kThreadsC, 3) gdn_prepare_kernel(GdnArgs a, ChunkArgs c) {
     constexpr int kParts = kF16 ? 1 : 2, kSteps = S / 32;
-    struct Mine {
-        float tile[10 * kTileFloats];
-        float p[4 * kTileFloats];
-        double G[kC];
-        float beta[kC], fk[kC], fq[kC], up[2][kC], row_down[kC], squares[kC];
-    };
-    __shared__ __align__(16) Mine s_all[kWaves];
+    __shared__ union {
+        ops_u32x4 k[kParts][4][kSteps][64];   // keys as operands: [part][tile][step][lane]
+        float p[10 * kTileFloats];            // then P, by tiles
+    } s_u;
+    __shared__ __align__(16) float s_tile[10 * kTileFloats];
+    auto& s_k = s_u.k;
+    __shared__ double s_G[kC];
+    __shared__ float s_beta[kC], s_fk[kC], s_kk[kC], s_up[kC], s_q[kWaves][5][16];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t g = lane >> 4, col = lane & 15;
-    const uint32_t item = blockIdx.x * kWaves + wave;
-    if (item >= c.count * a.v_heads) return;
-    const uint32_t piece = item / a.v_heads, h = item - piece * a.v_heads, kh = ops_div(h, a.share), chunk = c.first + piece;
-    Mine& s = s_all[wave];
+    const uint32_t piece = blockIdx.x / a.v_heads, h = blockIdx.x - piece * a.v_heads, kh = ops_div(h, a.share), chunk = c.first + piece;
     Seq q;
     if (!seq_of(a, lane, [&](uint32_t, uint32_t lo, uint32_t hi) { return chunk >= lo && chunk < hi; }, q)) return;
     const uint32_t t0 = q.t0 + (chunk - q.chunk0) * kC, n = q.t1 - t0 < kC ? q.t1 - t0 : kC;
@@ -187,28 +216,30 @@ __global__ void __launch_bounds__(kThreadsC, 2) gdn_prepare_kernel(GdnArgs a, Ch
     ops_u32x4* rows = c.rows + (uint64_t(piece) * c.k_heads + kh) * kRowWords<S, kParts>;
     const bool write_rows = h == kh * a.share.d;   // one of the value heads that share the keys
 
+    // the wave's rows of keys and queries as they lie in memory: token 16 w + col, values 32 step + 8 g .. + 7
+    const uint32_t mine = wave * 16 + col, row = mine < n ? mine : n - 1;
+    ops_u32x4 k_raw[kParts * kSteps], q_raw[kParts * kSteps], kf[kParts][kSteps], qf[kParts][kSteps];
+    {
+        const uint8_t* p = a.k + int64_t(t0 + row) * a.k_ld + (kh * S + g * 8) * (kF16 ? 2 : 4);
+#pragma unroll
+        for (int i = 0; i < kParts * kSteps; ++i) k_raw[i] = ld_global<ops_u32x4>(p + (kF16 ? i * 64 : i / 2 * 128 + i % 2 * 16));
+        p = a.q + int64_t(t0 + row) * a.q_ld + (kh * S + g * 8) * (kF16 ? 2 : 4);
+#pragma unroll
+        for (int i = 0; i < kParts * kSteps; ++i) q_raw[i] = ld_global<ops_u32x4>(p + (kF16 ? i * 64 : i / 2 * 128 + i % 2 * 16));
+    }
+    // the gates, lane = token
     const bool in = lane < n;
     const int64_t gates = int64_t(t0 + (in ? lane : 0)) * a.gate_ld + h;
     const float g_in = ld_global<float>(a.g + gates), beta_in = ld_global<float>(a.beta + gates);
 
-    // tile t of keys or queries: token 16 t + col, values 32 step + 8 g .. + 7: as they lie in memory, then as operands, rows
-    // past the chunk zero
-    auto load_raw = [&](const uint8_t* from, int64_t ld, int t, ops_u32x4 (&x)[kParts * kSteps]) {
-        const uint32_t mine = t * 16 + col, row = mine < n ? mine : n - 1;
-        const uint8_t* p = from + int64_t(t0 + row) * ld + (kh * S + g * 8) * (kF16 ? 2 : 4);
-#pragma unroll
-        for (int i = 0; i < kParts * kSteps; ++i) x[i] = ld_global<ops_u32x4>(p + (kF16 ? i * 64 : i / 2 * 128 + i % 2 * 16));
-    };
-    auto to_tile = [&](const ops_u32x4 (&raw)[kParts * kSteps], int t, ops_u32x4 (&x)[kParts][kSteps], float* up, uint32_t which) {
-        const uint32_t mine = t * 16 + col;
+    // as operands, rows past the chunk zero; f32 ones scaled by a power of two to a largest value of 1 .. 2, in two parts,
+    // which the second kernel reads.  The power of two is returned.
+    auto to_operand = [&](const ops_u32x4 (&raw)[kParts * kSteps], ops_u32x4 (&x)[kParts][kSteps], uint32_t which) {
+        float back = 1.0f;
         if constexpr (kF16) {
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) x[0][i] = raw[i];
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i)
-                if (mine >= n) x[0][i] = ops_u32x4{};
+            for (int i = 0; i < kSteps; ++i) x[0][i] = mine < n ? raw[i] : ops_u32x4{};
         } else {
-            // scaled by a power of two to a largest value of 1 .. 2, in two parts, which the second kernel reads
             f32x4 y[kSteps][2];
             float top = 0;
 #pragma unroll
@@ -220,202 +251,173 @@ __global__ void __launch_bounds__(kThreadsC, 2) gdn_prepare_kernel(GdnArgs a, Ch
                     for (int k = 0; k < 4; ++k) top = fmaxf(top, fabsf(y[i][j][k]));
                 }
             top = over_rows(top, max_of);
-            float down, back;
+            float down;
             power_of(top, down, back);
-            if (g == 0) up[mine] = back;
+            const f32x4 by{down, down, down, down};
 #pragma unroll
             for (int i = 0; i < kSteps; ++i) {
-                uint32_t hi[4], lo[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) split2(y[i][j / 2][j % 2 * 2] * down, y[i][j / 2][j % 2 * 2 + 1] * down, hi[j], lo[j]);
-                x[0][i] = ops_u32x4{hi[0], hi[1], hi[2], hi[3]};
-                x[kParts - 1][i] = ops_u32x4{lo[0], lo[1], lo[2], lo[3]};
+                split_pair(y[i][0], y[i][1], by, by, x[0][i], x[kParts - 1][i]);
                 if (write_rows)
 #pragma unroll
                     for (int part = 0; part < kParts; ++part)
-                        st_global<ops_u32x4>(rows + row_operand<S, kParts>(which, part, t, i) + lane, x[part][i]);
+                        st_global<ops_u32x4>(rows + row_operand<S, kParts>(which, part, wave, i) + lane, x[part][i]);
             }
         }
+        return back;
     };
-    auto dot = [&](const ops_u32x4 (&x)[kParts][kSteps], const ops_u32x4 (&y)[kParts][kSteps], f32x4 acc) {
+    const float k_up = to_operand(k_raw, kf, 0);
+    if (g == 0) s_up[mine] = k_up;
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            acc = mfma(x[0][i], y[0][i], acc);
-            if constexpr (!kF16) acc = mfma(x[0][i], y[kParts - 1][i], acc), acc = mfma(x[kParts - 1][i], y[0][i], acc);
-        }
-        return acc;
-    };
-    // f16 queries are all asked for now, f32 ones a tile ahead (registers)
-    constexpr int kAhead = kF16 ? 4 : 1;
-    ops_u32x4 k_raw[4][kParts * kSteps], q_raw[kAhead][kParts * kSteps], kf[4][kParts][kSteps];
+    for (int part = 0; part < kParts; ++part)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) load_raw(a.k, a.k_ld, t, k_raw[t]);
-#pragma unroll
-    for (int t = 0; t < kAhead; ++t) load_raw(a.q, a.q_ld, t, q_raw[t]);
-#pragma unroll
-    for (int t = 0; t < 4; ++t) to_tile(k_raw[t], t, kf[t], s.up[0], 0);
-
-    // the keys as the left operand of the state's update: key 32 i + 2 col + e, tokens 32 step + 4 g + j and 16 more, by way
-    // of LDS, where the tiles will be
-    if (write_rows) {
-        constexpr uint32_t kRow = S * 2 + 16;
-        static_assert(kC * kRow <= sizeof(s.tile) + sizeof(s.p));
-        uint8_t* lds = reinterpret_cast<uint8_t*>(s.tile);
-#pragma unroll
-        for (int part = 0; part < kParts; ++part) {
-#pragma unroll
-            for (int t = 0; t < 4; ++t)
-#pragma unroll
-                for (int i = 0; i < kSteps; ++i) *reinterpret_cast<ops_u32x4*>(lds + (t * 16 + col) * kRow + i * 64 + g * 16) = kf[t][part][i];
-            wave_sync();
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i)
-#pragma unroll
-                for (int step = 0; step < 2; ++step) {
-                    uint32_t w[8];
-#pragma unroll
-                    for (int j = 0; j < 8; ++j)
-                        w[j] = *reinterpret_cast<const uint32_t*>(lds + (step * 32 + (j / 4) * 16 + g * 4 + j % 4) * kRow + (i * 32 + col * 2) * 2);
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const uint32_t sel = e ? 0x07060302u : 0x05040100u;
-                        st_global<ops_u32x4>(rows + key_operand<S, kParts>(part, i, e, step) + lane,
-                                             ops_u32x4{__builtin_amdgcn_perm(w[1], w[0], sel), __builtin_amdgcn_perm(w[3], w[2], sel),
-                                                       __builtin_amdgcn_perm(w[5], w[4], sel), __builtin_amdgcn_perm(w[7], w[6], sel)});
-                    }
-                }
-            wave_sync();
-        }
-    }
-
-    // sums of the log decays, to base 2, lane = token
+        for (int i = 0; i < kSteps; ++i) s_k[part][wave][i][lane] = kf[part][i];
+    const float q_up = to_operand(q_raw, qf, 1);
+    // sums of the log decays, to base 2
     const double G = scan_add64(in ? double(g_in < kLeastG ? kLeastG : g_in) * kLog2e : 0.0);
     const float beta = in ? beta_in : 0.0f;
-    s.G[lane] = G;
-    s.beta[lane] = beta;
     const uint64_t G_bits = __builtin_bit_cast(uint64_t, G);
     const double G_all = __builtin_bit_cast(double, uint64_t(last_lane(uint32_t(G_bits >> 32))) << 32 | last_lane(uint32_t(G_bits)));
+    if (wave == 0) s_G[lane] = G, s_beta[lane] = beta;
+    __syncthreads();
 
-    // K K^T, element (4 g + i, col) of a tile; its diagonal has the squares of the lengths
-    f32x4 kk[10];
+    // the row tile's products, element (4 g + i, col) of a tile; the diagonals have the squares of the lengths
+    f32x4 kk[4], qk[4], qq{};
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
+    for (int t = 0; t < 4; ++t) {
+        kk[t] = f32x4{}, qk[t] = f32x4{};
+        if (uint32_t(t) > wave) continue;
 #pragma unroll
-        for (int cc = 0; cc <= r; ++cc) kk[tile_of(r, cc)] = dot(kf[r], kf[cc], f32x4{});
+        for (int i = 0; i < kSteps; ++i) {
+            const ops_u32x4 hi = s_k[0][t][i][lane];
+            kk[t] = mfma(kf[0][i], hi, kk[t]);
+            qk[t] = mfma(qf[0][i], hi, qk[t]);
+            if constexpr (!kF16) {
+                const ops_u32x4 lo = s_k[kParts - 1][t][i][lane];
+                kk[t] = mfma(kf[0][i], lo, kk[t]);
+                qk[t] = mfma(qf[0][i], lo, qk[t]);
+                kk[t] = mfma(kf[kParts - 1][i], hi, kk[t]);
+                qk[t] = mfma(qf[kParts - 1][i], hi, qk[t]);
+            }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i) {
+        qq = mfma(qf[0][i], qf[0][i], qq);
+        if constexpr (!kF16) qq = mfma(qf[0][i], qf[kParts - 1][i], qq), qq = mfma(qf[kParts - 1][i], qf[0][i], qq);
+    }
+    f32x4 own{};
 #pragma unroll
     for (int t = 0; t < 4; ++t)
+        if (uint32_t(t) == wave) own = kk[t];
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (g * 4 + i == col) s.squares[t * 16 + col] = kk[tile_of(t, t)][i];
-    wave_sync();
+    for (int i = 0; i < 4; ++i)
+        if (g * 4 + i == col) s_kk[mine] = own[i], s_q[wave][0][col] = qq[i];
+    // the keys as the left operand of the state's update: keys 32 w + 2 col + e, tokens 32 step + 4 g + j and 16 more
+    if (write_rows && wave < uint32_t(kSteps)) {
+#pragma unroll
+        for (int part = 0; part < kParts; ++part)
+#pragma unroll
+            for (int step = 0; step < 2; ++step) {
+                uint32_t w[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    w[j] = reinterpret_cast<const uint32_t*>(&s_k[part][step * 2 + j / 4][wave][col / 4 * 16 + g * 4 + j % 4])[col % 4];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    const uint32_t sel = e ? 0x07060302u : 0x05040100u;
+                    st_global<ops_u32x4>(rows + key_operand<S, kParts>(part, wave, e, step) + lane,
+                                         ops_u32x4{__builtin_amdgcn_perm(w[1], w[0], sel), __builtin_amdgcn_perm(w[3], w[2], sel),
+                                                   __builtin_amdgcn_perm(w[5], w[4], sel), __builtin_amdgcn_perm(w[7], w[6], sel)});
+                }
+            }
+    }
+    __syncthreads();
     // the factor that brings a row as multiplied to its length, unit or its own, and that length
-    auto factor = [&](float squares, const float* up, float& length) {
-        const float by = kF16 ? 1.0f : up[lane];
-        const float f = !in ? 0.0f : a.l2norm ? __builtin_amdgcn_rsqf(squares + a.eps / by / by) : by;
-        length = in ? __builtin_amdgcn_sqrtf(squares) * f : 0.0f;
-        return f;
+    auto factor = [&](float squares, float by, bool there) {
+        return !there ? 0.0f : a.l2norm ? __builtin_amdgcn_rsqf(squares + a.eps / by / by) : by;
     };
-    float k_length;
-    const float fk = factor(s.squares[lane], s.up[0], k_length), k_most = wave_most(k_length);
-    s.fk[lane] = fk;
-    const float e = exp2_of(G), write = exp2_of(G_all - G) * fk;
+    const float fk = factor(s_kk[lane], s_up[lane], in), k_most = wave_most(in ? __builtin_amdgcn_sqrtf(s_kk[lane]) * fk : 0.0f);
     float* f = reinterpret_cast<float*>(out + 2 * kOperand);
-    {
+    if (wave == 0) {
+        s_fk[lane] = fk;
+        // the weights of writes, at most 2 as an operand; scaled only where they need it
+        const float write = exp2_of(G_all - G) * fk, most = wave_most(write), beta_most = wave_most(fabsf(beta));
         float down, up;
-        power_of(wave_most(write), down, up);
-        const float beta_most = wave_most(fabsf(beta));
-        f[kFState + lane] = beta * fk * e;
+        power_of(most >= 0x1p-10f && most < 2.0f ? 1.0f : most, down, up);
+        f[kFState + lane] = beta * fk * exp2_of(G);
         f[kFBeta + lane] = beta;
         f[kFWrite + lane] = write * down;
         if (lane == 0) f[kFDecay] = exp2_of(G_all), f[kFUp] = up, f[kFBetaMost] = beta_most;
     }
-    wave_sync();
-
+    if (g == 0) {
+        const bool there = mine < n;
+        const float squares = s_q[wave][0][col], fq = factor(squares, q_up, there);
+        float down, up;
+        power_of(there ? fabsf(a.scale) * __builtin_amdgcn_sqrtf(squares) * fq * k_most : 0.0f, down, up);
+        s_q[wave][1][col] = fq * a.scale * down;
+        f[kFQuery + mine] = a.scale * fq * exp2_of(s_G[mine]);
+        f[kFRow + mine] = up;
+    }
+    __syncthreads();
+    // A below the diagonal, and P, by way of LDS
+    double Gr[4];
+    float br[4], qr[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        ops_u32x4 qf[kParts][kSteps];
-        to_tile(q_raw[r % kAhead], r, qf, s.up[1], 1);
-        if (!kF16 && r < 3) load_raw(a.q, a.q_ld, r + 1, q_raw[0]);
-        f32x4 qq = dot(qf, qf, f32x4{}), qk[4];
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t t = wave * 16 + g * 4 + i;
+        Gr[i] = s_G[t];
+        br[i] = s_beta[t] * s_fk[t];
+        qr[i] = s_q[wave][1][g * 4 + i];
+    }
+    float* tiles = s_tile + wave * (wave + 1) / 2 * kTileFloats;   // the wave's row of them
 #pragma unroll
-        for (int cc = 0; cc <= r; ++cc) qk[cc] = dot(qf, kf[cc], f32x4{});
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (g * 4 + i == col) s.squares[col] = qq[i];
-        wave_sync();
-        if (lane < 16) {
-            // token 16 r + lane: this lane's own place in the chunk is another one
-            const uint32_t t = r * 16 + lane;
-            const float by = kF16 ? 1.0f : s.up[1][t], squares = s.squares[lane];
-            const float fq = t >= n ? 0.0f : a.l2norm ? __builtin_amdgcn_rsqf(squares + a.eps / by / by) : by;
-            float down, up;
-            power_of(t >= n ? 0.0f : fabsf(a.scale) * __builtin_amdgcn_sqrtf(squares) * fq * k_most, down, up);
-            s.fq[t] = fq * a.scale;
-            s.row_down[t] = down * kUpT;
-            f[kFQuery + t] = a.scale * fq * exp2_of(s.G[t]);
-            f[kFRow + t] = up;
-        }
-        wave_sync();
-        // A below the diagonal, and P
-        double Gr[4];
-        float br[4], qr[4];
+    for (int t = 0; t < 4; ++t) {
+        if (uint32_t(t) > wave) continue;
+        const double Gc = s_G[t * 16 + col];
+        const float fc = s_fk[t * 16 + col];
+        const bool below = uint32_t(t) < wave;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const uint32_t t = r * 16 + g * 4 + i;
-            Gr[i] = s.G[t];
-            br[i] = s.beta[t] * s.fk[t];
-            qr[i] = s.fq[t] * s.row_down[t];
+            const uint32_t r = g * 4 + i;
+            const float fade = below || r >= col ? exp2_of(Gr[i] - Gc) * fc : 0.0f;
+            tiles[t * kTileFloats + r * kTileRow + col] = below || r > col ? br[i] * fade * kk[t][i] : 0.0f;
+            s_u.p[(wave * (wave + 1) / 2 + t) * kTileFloats + r * kTileRow + col] = qr[i] * fade * qk[t][i];
         }
-#pragma unroll
-        for (int cc = 0; cc <= r; ++cc) {
-            const double Gc = s.G[cc * 16 + col];
-            const float fc = s.fk[cc * 16 + col];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t row = g * 4 + i;
-                const float fade = cc < r || row >= col ? exp2_of(Gr[i] - Gc) * fc : 0.0f;
-                s.tile[tile_of(r, cc) * kTileFloats + row * kTileRow + col] = cc < r || row > col ? br[i] * fade * kk[tile_of(r, cc)][i] : 0.0f;
-                s.p[cc * kTileFloats + row * kTileRow + col] = qr[i] * fade * qk[cc][i];
-            }
-        }
-        wave_sync();
-        // P as the second kernel's operand: row 16 r + col, places 0 .. 3 tokens 32 step + 4 g, 4 .. 7 16 more
-#pragma unroll
-        for (int step = 0; step <= r / 2; ++step) {
-            const f32x4 u = *reinterpret_cast<const f32x4*>(&s.p[step * 2 * kTileFloats + col * kTileRow + g * 4]);
-            const f32x4 v = step * 2 + 1 <= r ? *reinterpret_cast<const f32x4*>(&s.p[(step * 2 + 1) * kTileFloats + col * kTileRow + g * 4]) : f32x4{};
-            uint32_t hi[4], lo[4];
-            split2(u.x, u.y, hi[0], lo[0]);
-            split2(u.z, u.w, hi[1], lo[1]);
-            split2(v.x, v.y, hi[2], lo[2]);
-            split2(v.z, v.w, hi[3], lo[3]);
-            st_global<ops_u32x4>(out + kOperand + operand_at(r, step, 0) + lane, ops_u32x4{hi[0], hi[1], hi[2], hi[3]});
-            st_global<ops_u32x4>(out + kOperand + operand_at(r, step, 1) + lane, ops_u32x4{lo[0], lo[1], lo[2], lo[3]});
-        }
-        wave_sync();
     }
-
-    // the diagonal tiles of T: column col of tile g
-    auto tile_at = [&](int t) { return s.tile + t * kTileFloats; };
+    wave_sync();
+    // a row tile of P or T as the second kernel's operand: row col, places 0 .. 3 tokens 32 step + 4 g, 4 .. 7 16 more
+    auto write_operand = [&](const float* from, uint32_t which) {
+        for (uint32_t step = 0; step <= wave / 2; ++step) {
+            const f32x4 u = *reinterpret_cast<const f32x4*>(&from[step * 2 * kTileFloats + col * kTileRow + g * 4]);
+            const f32x4 v = step * 2 + 1 <= wave ? *reinterpret_cast<const f32x4*>(&from[(step * 2 + 1) * kTileFloats + col * kTileRow + g * 4]) : f32x4{};
+            ops_u32x4 hi, lo;
+            split_pair(u, v, hi, lo);
+            st_global<ops_u32x4>(out + which * kOperand + operand_at(wave, step, 0) + lane, hi);
+            st_global<ops_u32x4>(out + which * kOperand + operand_at(wave, step, 1) + lane, lo);
+        }
+    };
+    write_operand(s_u.p + wave * (wave + 1) / 2 * kTileFloats, 1);
+    // the diagonal tile of T, column col (the same in each group of lanes)
+    auto tile_at = [&](int t) { return s_tile + t * kTileFloats; };
     {
-        const float* d = s.tile + (g * (g + 1) / 2 + g) * kTileFloats;
+        float* d = tiles + wave * kTileFloats;
         float x[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             f32x4 sum{uint32_t(i) == col ? 1.0f : 0.0f, 0, 0, 0};   // four sums: a chain a quarter as long
 #pragma unroll
             for (int k = 0; k < i; k += 4) {
-                const f32x4 row = *reinterpret_cast<const f32x4*>(&d[i * kTileRow + k]);
+                const f32x4 r = *reinterpret_cast<const f32x4*>(&d[i * kTileRow + k]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    if (k + j < i) sum[j] -= row[j] * x[k + j];
+                    if (k + j < i) sum[j] -= r[j] * x[k + j];
             }
             x[i] = (sum.x + sum.y) + (sum.z + sum.w);
         }
         wave_sync();
+        if (g == 0)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) s.tile[(g * (g + 1) / 2 + g) * kTileFloats + i * kTileRow + col] = x[i];
-        wave_sync();
+            for (int i = 0; i < 16; ++i) d[i * kTileRow + col] = x[i];
     }
     auto left = [&](int t) { return *reinterpret_cast<const f32x4*>(tile_at(t) + col * kTileRow + g * 4); };
     auto right = [&](int t) {
@@ -433,49 +435,69 @@ __global__ void __launch_bounds__(kThreadsC, 2) gdn_prepare_kernel(GdnArgs a, Ch
 #pragma unroll
         for (int i = 0; i < 4; ++i) tile_at(t)[(g * 4 + i) * kTileRow + col] = x[i];
     };
-    {
-        const f32x4 zero{}, t00 = right(tile_of(0, 0)), t11 = right(tile_of(1, 1)), t22 = right(tile_of(2, 2));
-        const f32x4 y10 = product(left(tile_of(1, 0)), t00, zero), y32 = product(left(tile_of(3, 2)), t22, zero);
-        const f32x4 t10 = -product(left(tile_of(1, 1)), y10, zero), t32 = -product(left(tile_of(3, 3)), y32, zero);
+    __syncthreads();
+    const f32x4 zero{};
+    if (wave & 1) {   // T_10 and T_32
+        const int w = int(wave), at = tile_of(w, w - 1);
+        const f32x4 x = product(left(at), right(tile_of(w - 1, w - 1)), zero);
+        const f32x4 y = -product(left(tile_of(w, w)), x, zero);
         wave_sync();
-        put(tile_of(1, 0), t10);
-        put(tile_of(3, 2), t32);
-        const f32x4 y20 = product(left(tile_of(2, 1)), t10, product(left(tile_of(2, 0)), t00, zero)), y21 = product(left(tile_of(2, 1)), t11, zero);
-        const f32x4 y30 = product(left(tile_of(3, 1)), t10, product(left(tile_of(3, 0)), t00, zero)), y31 = product(left(tile_of(3, 1)), t11, zero);
-        wave_sync();
-        const f32x4 l22 = left(tile_of(2, 2)), l32 = left(tile_of(3, 2)), l33 = left(tile_of(3, 3));
-        put(tile_of(2, 0), -product(l22, y20, zero));
-        put(tile_of(2, 1), -product(l22, y21, zero));
-        put(tile_of(3, 0), -product(l33, y30, product(l32, y20, zero)));
-        put(tile_of(3, 1), -product(l33, y31, product(l32, y21, zero)));
-        wave_sync();
+        put(at, y);
     }
-#pragma unroll
-    for (int r = 0; r < 4; ++r)
-#pragma unroll
-        for (int step = 0; step <= r / 2; ++step) {
-            const f32x4 u = left(tile_of(r, step * 2)) * kUpT, v = step * 2 + 1 <= r ? left(tile_of(r, step * 2 + 1)) * kUpT : f32x4{};
-            uint32_t hi[4], lo[4];
-            split2(u.x, u.y, hi[0], lo[0]);
-            split2(u.z, u.w, hi[1], lo[1]);
-            split2(v.x, v.y, hi[2], lo[2]);
-            split2(v.z, v.w, hi[3], lo[3]);
-            st_global<ops_u32x4>(out + operand_at(r, step, 0) + lane, ops_u32x4{hi[0], hi[1], hi[2], hi[3]});
-            st_global<ops_u32x4>(out + operand_at(r, step, 1) + lane, ops_u32x4{lo[0], lo[1], lo[2], lo[3]});
+    __syncthreads();
+    {
+        // T_rc of the lower left half, r = 2, 3 and c = 0, 1, from the column y of A T there
+        const int r = 2 + int(wave >> 1), cc = int(wave & 1);
+        f32x4 y2 = product(left(tile_of(2, 1)), right(tile_of(1, cc)), zero), y3{};
+        if (cc == 0) y2 = product(left(tile_of(2, 0)), right(tile_of(0, 0)), y2);
+        f32x4 z;
+        if (r == 2) {
+            z = product(left(tile_of(2, 2)), y2, zero);
+        } else {
+            y3 = product(left(tile_of(3, 1)), right(tile_of(1, cc)), zero);
+            if (cc == 0) y3 = product(left(tile_of(3, 0)), right(tile_of(0, 0)), y3);
+            z = product(left(tile_of(3, 3)), y3, product(left(tile_of(3, 2)), y2, zero));
         }
+        __syncthreads();   // everyone has read A there
+        put(tile_of(r, cc), -z);
+    }
+    __syncthreads();
+    write_operand(tiles, 0);
 }
 
 // ---- the chunks of a sequence in order ------------------------------------------------------------------------------------
 
-// Eight values, four each of two tiles, as a right operand in two parts.
-__device__ __forceinline__ void split_pair(f32x4 a, f32x4 b, ops_u32x4& hi, ops_u32x4& lo) {
-    uint32_t h[4], l[4];
-    split2(a.x, a.y, h[0], l[0]);
-    split2(a.z, a.w, h[1], l[1]);
-    split2(b.x, b.y, h[2], l[2]);
-    split2(b.z, b.w, h[3], l[3]);
-    hi = ops_u32x4{h[0], h[1], h[2], h[3]};
-    lo = ops_u32x4{l[0], l[1], l[2], l[3]};
+// A column's state m times 2^up, scaled anew where the largest of it and of beta V (`v_top`, unscaled) leaves the window;
+// `down` is 2^-up.
+template <int kSteps>
+__device__ __forceinline__ void fit_scale(f32x4 (&m)[kSteps][2], int& up, float& down, float v_top, float beta_most) {
+    float top = 0;
+#pragma unroll
+    for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+            for (int j = 0; j < 4; j += 2) top = fmaxf(fmaxf(top, fabsf(m[i][e][j])), fabsf(m[i][e][j + 1]));
+    top = over_rows(top, max_of) * beta_most;
+    down = __builtin_amdgcn_ldexpf(1.0f, -up);
+    top = fmaxf(top, v_top * down);
+    if (__any(top >= float(1 << kTop) || (top > 0 && top < 1.0f / float(1 << -kLeast)))) {
+        // to 2^kAim, within what f32 can scale by
+        const int e = int(__float_as_uint(top) >> 23) - 127 - kAim, to = up + e;
+        const int by = top == 0 ? 0 : (to > 120 ? 120 : to < -120 ? -120 : to) - up;
+        up += by;
+        down = __builtin_amdgcn_ldexpf(1.0f, -up);
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) m[i][e][j] = __builtin_amdgcn_ldexpf(m[i][e][j], -by);
+    }
+}
+// Keys 32 i + 8 g .. + 7 of the state as a right operand: the even ones and the odd ones take turns.
+__device__ __forceinline__ void split_state(const f32x4 (&m)[2], ops_u32x4& hi, ops_u32x4& lo) {
+    split_pair(f32x4{m[0].x, m[1].x, m[0].y, m[1].y}, f32x4{m[0].z, m[1].z, m[0].w, m[1].w}, hi, lo);
 }
 
 template <int S, int kCols, bool kF16>
@@ -488,19 +510,27 @@ __global__ void __launch_bounds__(128, 1) gdn_chunk_kernel(GdnArgs a, ChunkArgs 
     // what one wave leaves for the other, by the chunk's parity
     struct Left {
         ops_u32x4 m[kN][kSteps][2][64], u[kN][2][2][64];   // the state before the chunk and U as right operands: [step][part]
-        float m_up[kN][16], x_up[kN][16];                  // what they were scaled down by, by column
+        int up[kN][16];                                    // the power of two that a column of both is to be scaled up by
     };
-    __shared__ Left s_left[2];
-    __shared__ __align__(16) uint8_t s_vin[2][kC * kRowV], s_out[kC * kRowV];
-    __shared__ __align__(16) float s_f[3][kFLanes * 64];
-    const uint32_t tid = threadIdx.x, lane = tid & 63;
-    const bool carries = __builtin_amdgcn_readfirstlane(tid >> 6) == 0;
+    struct Values {
+        f32x4 v[kN][4][64];                                // beta V as results lie: [tile][lane]
+        float most[kN][16];                                // its largest magnitude by column
+    };
+    struct Shared {
+        Left left[2];
+        Values values[2];
+        alignas(16) uint8_t vin[kC * kRowV], out[kC * kRowV];
+        alignas(16) float f[3][kFLanes * 64];
+    };
+    __shared__ Shared s;
+    const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const bool carries = wave == 0;
     const uint32_t g = lane >> 4, col = lane & 15;
     // workgroups go to the eight XCDs in turn: the column blocks of a head are kept on one, whose L2 has its operands
     constexpr uint32_t kBlocks = S / kCols;
-    const uint32_t within = blockIdx.x / 8, pair = within / kBlocks * 8 + blockIdx.x % 8, block = within % kBlocks;
-    if (pair >= a.n_seqs * a.v_heads) return;
-    const uint32_t seq = pair / a.v_heads, h = pair - seq * a.v_heads, kh = ops_div(h, a.share);
+    const uint32_t within = blockIdx.x / 8, head = within / kBlocks * 8 + blockIdx.x % 8, block = within % kBlocks;
+    if (head >= a.n_seqs * a.v_heads) return;
+    const uint32_t seq = head / a.v_heads, h = head - seq * a.v_heads, kh = ops_div(h, a.share);
     Seq q;
     if (!seq_of(a, lane, [&](uint32_t s, uint32_t, uint32_t) { return s == seq; }, q)) return;
     // this launch's chunks of the sequence
@@ -579,6 +609,11 @@ __global__ void __launch_bounds__(128, 1) gdn_chunk_kernel(GdnArgs a, ChunkArgs 
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) m[b][i][e][j] = ld_global<float>(state + (i * 32 + 2 * j + e) * a.key_ld + b * 16);
+        // waited for here: the loop would wait for it every time around
+#pragma unroll
+        for (int b = 0; b < kN; ++b)
+#pragma unroll
+            for (int i = 0; i < kSteps; ++i) asm volatile("" : "+v"(m[b][i][0]), "+v"(m[b][i][1]));
         ops_u32x4 k[4][kParts][kSteps], t[6][2], kt[kParts][kSteps][2][2];
         auto load_keys = [&](uint32_t chunk) {
             const ops_u32x4* p = rows_of(chunk) + lane;
@@ -594,36 +629,29 @@ __global__ void __launch_bounds__(128, 1) gdn_chunk_kernel(GdnArgs a, ChunkArgs 
         load_rows(k, c0, 0);
         load_operand(t, c0, 0);
         load_keys(c0);
+        int up[kN];   // a column's state is m times 2^up
+#pragma unroll
+        for (int b = 0; b < kN; ++b) up[b] = 0;
         for (uint32_t chunk = c0; chunk < c1; ++chunk) {
-            const uint32_t which = (chunk - c0) & 1, last = last_row(chunk), ahead = clamped(chunk + 1);
-            Left& left = s_left[which];
+            const uint32_t which = (chunk - c0) & 1, ahead = clamped(chunk + 1);
+            Left& left = s.left[which];
             __syncthreads();   // V and the factors are here, and the outputs of the chunk before the last are done
-            const float* f = s_f[(chunk - c0) % 3];
-            // the state as a right operand, scaled by column
+            const float* f = s.f[(chunk - c0) % 3];
+            const Values& values = s.values[which];
+            // the state as a right operand
+            const float beta_most = fmaxf(f[kFBetaMost], 1.0f);
             ops_u32x4 mh[kN][kSteps], ml[kN][kSteps];
-            float m_up[kN];
+            float down[kN];
 #pragma unroll
             for (int b = 0; b < kN; ++b) {
-                float top = 0;
-#pragma unroll
-                for (int i = 0; i < kSteps; ++i)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e)
-#pragma unroll
-                        for (int j = 0; j < 4; ++j) top = fmaxf(top, fabsf(m[b][i][e][j]));
-                top = over_rows(top, max_of);
-                float down;
-                power_of(top, down, m_up[b]);
-                if (top == 0) m_up[b] = 0.0f;
+                fit_scale<kSteps>(m[b], up[b], down[b], values.most[b][col], beta_most);
 #pragma unroll
                 for (int i = 0; i < kSteps; ++i) {
-                    // keys 8 g .. 8 g + 7 in order: the even ones and the odd ones take turns
-                    const f32x4 even = m[b][i][0] * down, odd = m[b][i][1] * down;
-                    split_pair(f32x4{even.x, odd.x, even.y, odd.y}, f32x4{even.z, odd.z, even.w, odd.w}, mh[b][i], ml[b][i]);
+                    split_state(m[b][i], mh[b][i], ml[b][i]);
                     left.m[b][i][0][lane] = mh[b][i];
                     left.m[b][i][1][lane] = ml[b][i];
                 }
-                if (g == 0) left.m_up[b][col] = m_up[b];
+                if (g == 0) left.up[b][col] = up[b];
             }
             // K M0
             f32x4 km[kN][4];
@@ -640,42 +668,19 @@ __global__ void __launch_bounds__(128, 1) gdn_chunk_kernel(GdnArgs a, ChunkArgs 
 #pragma unroll
                         for (int b = 0; b < kN; ++b) km[b][r] = mfma(k[r][x == 2][i], x == 1 ? ml[b][i] : mh[b][i], km[b][r]);
             load_rows(k, ahead, 0);
-            // X, scaled by column
+            // X; rows past the sequence's end are zero, as their V and factors are
             ops_u32x4 xs[kN][2][2];
-            float x_up[kN];
 #pragma unroll
             for (int b = 0; b < kN; ++b) {
-                f32x4 v[4];
-                float top = 0;
+                f32x4 x[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const f32x4 beta = *reinterpret_cast<const f32x4*>(&f[kFBeta + r * 16 + g * 4]);
+                    const f32x4 fs = *reinterpret_cast<const f32x4*>(&f[kFState + r * 16 + g * 4]), v = values.v[b][r][lane];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const uint32_t row = r * 16 + g * 4 + j;
-                        const uint8_t* p = &s_vin[which][row * kRowV + (b * 16 + col) * kBytes];
-                        float x;
-                        if constexpr (kF16) x = float(*reinterpret_cast<const _Float16*>(p));
-                        else x = *reinterpret_cast<const float*>(p);
-                        v[r][j] = row <= last ? x * beta[j] : 0.0f;
-                        top = fmaxf(top, fabsf(v[r][j]));
-                    }
+                    for (int j = 0; j < 4; ++j) x[r][j] = __builtin_fmaf(-fs[j], km[b][r][j], v[j] * down[b]);
                 }
-                top = over_rows(top, max_of);
-                float down;
-                power_of(fmaxf(top, m_up[b] * f[kFBetaMost]), down, x_up[b]);
-                if (g == 0) left.x_up[b][col] = x_up[b];
-                down *= kUpX;
-                const float by = m_up[b] * down;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const f32x4 fs = *reinterpret_cast<const f32x4*>(&f[kFState + r * 16 + g * 4]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        v[r][j] = int(r * 16 + g * 4 + j) <= int(last) ? v[r][j] * down - fs[j] * by * km[b][r][j] : 0.0f;
-                }
-                split_pair(v[0], v[1], xs[b][0][0], xs[b][0][1]);
-                split_pair(v[2], v[3], xs[b][1][0], xs[b][1][1]);
+                split_pair(x[0], x[1], xs[b][0][0], xs[b][0][1]);
+                split_pair(x[2], x[3], xs[b][1][0], xs[b][1][1]);
             }
             // U = T X, and the same weighted for the state
             ops_u32x4 ws[kN][2][2];
@@ -684,39 +689,49 @@ __global__ void __launch_bounds__(128, 1) gdn_chunk_kernel(GdnArgs a, ChunkArgs 
                 f32x4 u[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) u[r] = triangle(t, xs[b], r);
-                ops_u32x4 us[2][2];
-                split_pair(u[0], u[1], us[0][0], us[0][1]);
-                split_pair(u[2], u[3], us[1][0], us[1][1]);
 #pragma unroll
-                for (int step = 0; step < 2; ++step)
-#pragma unroll
-                    for (int part = 0; part < 2; ++part) left.u[b][step][part][lane] = us[step][part];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) u[r] *= *reinterpret_cast<const f32x4*>(&f[kFWrite + r * 16 + g * 4]);
-                split_pair(u[0], u[1], ws[b][0][0], ws[b][0][1]);
-                split_pair(u[2], u[3], ws[b][1][0], ws[b][1][1]);
+                for (int step = 0; step < 2; ++step) {
+                    ops_u32x4 hi, lo;
+                    split_pair(u[step * 2], u[step * 2 + 1], hi, lo);
+                    left.u[b][step][0][lane] = hi;
+                    left.u[b][step][1][lane] = lo;
+                    const f32x4 w0 = *reinterpret_cast<const f32x4*>(&f[kFWrite + step * 32 + g * 4]), w1 = *reinterpret_cast<const f32x4*>(&f[kFWrite + step * 32 + 16 + g * 4]);
+                    split_pair(u[step * 2], u[step * 2 + 1], w0, w1, ws[b][step][0], ws[b][step][1]);
+                }
             }
             load_operand(t, ahead, 0);
             // the state after the chunk
-            const float decay = f[kFDecay], up = f[kFUp] * (1.0f / kUpU);
+            const float decay = f[kFDecay], w_up = f[kFUp];
+            const bool plain = __builtin_amdgcn_readfirstlane(int(w_up == 1.0f));   // nearly always
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                f32x4 add[kN][2];
+            for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-                for (int b = 0; b < kN; ++b) add[b][0] = f32x4{}, add[b][1] = f32x4{};
+                for (int b = 0; b < kN; ++b)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) m[b][i][e] *= decay;
+            auto update = [&](f32x4 (&add)[kN][kSteps][2]) {
 #pragma unroll
                 for (int step = 0; step < 2; ++step)
 #pragma unroll
                     for (int x = 0; x < kParts + 1; ++x)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e)
+                        for (int i = 0; i < kSteps; ++i)
 #pragma unroll
-                            for (int b = 0; b < kN; ++b)
-                                add[b][e] = mfma(kt[x == 2][i][e][step], ws[b][step][x == 1], add[b][e]);
+                            for (int e = 0; e < 2; ++e)
 #pragma unroll
-                for (int b = 0; b < kN; ++b)
+                                for (int b = 0; b < kN; ++b) add[b][i][e] = mfma(kt[x == 2][i][e][step], ws[b][step][x == 1], add[b][i][e]);
+            };
+            if (plain) {
+                update(m);
+            } else {
+                f32x4 add[kN][kSteps][2]{};
+                update(add);
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) m[b][i][e] = decay * m[b][i][e] + (x_up[b] * up) * add[b][e];
+                for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+                    for (int b = 0; b < kN; ++b)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) m[b][i][e] += w_up * add[b][i][e];
             }
             load_keys(ahead);
         }
@@ -728,7 +743,8 @@ __global__ void __launch_bounds__(128, 1) gdn_chunk_kernel(GdnArgs a, ChunkArgs 
 #pragma unroll
                 for (int e = 0; e < 2; ++e)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) st_global<float>(state + (i * 32 + 2 * j + e) * a.key_ld + b * 16, m[b][i][e][j]);
+                    for (int j = 0; j < 4; ++j)
+                        st_global<float>(state + (i * 32 + 2 * j + e) * a.key_ld + b * 16, __builtin_amdgcn_ldexpf(m[b][i][e][j], up[b]));
         return;
     }
 
@@ -748,15 +764,42 @@ __global__ void __launch_bounds__(128, 1) gdn_chunk_kernel(GdnArgs a, ChunkArgs 
 #pragma unroll
         for (uint32_t i = 0; i < kFLanes; ++i) f_in[i] = ld_global<float>(f + min(lane + i * 64, uint32_t(kFactors - 1)));
     };
-    auto put_early = [&](uint32_t n) {
+    // V as the first wave takes it, by way of LDS: times beta, rows past the sequence's end zero, a lane's four rows together
+    auto put_early = [&](uint32_t chunk, uint32_t n) {
+        const uint32_t last = last_row(chunk);
+        float* f = s.f[n % 3];
+        Values& to = s.values[n & 1];
 #pragma unroll
-        for (uint32_t i = 0; i < kEach; ++i) *reinterpret_cast<ops_u32x4*>(&s_vin[n & 1][(lane + i * 64) * 16]) = v_in[i];
+        for (uint32_t i = 0; i < kEach; ++i) {
+            const uint32_t at = lane + i * 64;
+            *reinterpret_cast<ops_u32x4*>(&s.vin[at * 16]) = at / kPieces <= last ? v_in[i] : ops_u32x4{};
+        }
 #pragma unroll
-        for (uint32_t i = 0; i < kFLanes; ++i) s_f[n % 3][lane + i * 64] = f_in[i];
+        for (uint32_t i = 0; i < kFLanes; ++i) f[lane + i * 64] = f_in[i];
+        wave_sync();
+#pragma unroll
+        for (int b = 0; b < kN; ++b) {
+            float top = 0;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                f32x4 v = *reinterpret_cast<const f32x4*>(&f[kFBeta + r * 16 + g * 4]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint8_t* p = &s.vin[(r * 16 + g * 4 + j) * kRowV + (b * 16 + col) * kBytes];
+                    if constexpr (kF16) v[j] *= float(*reinterpret_cast<const _Float16*>(p));
+                    else v[j] *= *reinterpret_cast<const float*>(p);
+                    top = fmaxf(top, fabsf(v[j]));
+                }
+                to.v[b][r][lane] = v;
+            }
+            top = over_rows(top, max_of);
+            if (g == 0) to.most[b][col] = top;
+        }
+        wave_sync();
     };
     ops_u32x4 qs[4][kParts][kSteps], p[6][2];
     load_early(c0);
-    put_early(0);
+    put_early(c0, 0);
     load_early(clamped(c0 + 1));
     load_rows(qs, c0, 1);
     load_operand(p, c0, 1);
@@ -765,13 +808,13 @@ __global__ void __launch_bounds__(128, 1) gdn_chunk_kernel(GdnArgs a, ChunkArgs 
         __syncthreads();
         // the first wave reads the places of chunk n now, and this one the factors of chunk n - 1
         if (chunk < c1) {
-            put_early(n + 1);
+            put_early(clamped(chunk + 1), n + 1);
             load_early(clamped(chunk + 2));
         }
         if (chunk == c0) continue;
         const uint32_t done = chunk - 1, last = last_row(done);
-        const Left& left = s_left[(n - 1) & 1];
-        const float* f = s_f[(n - 1) % 3];
+        const Left& left = s.left[(n - 1) & 1];
+        const float* f = s.f[(n - 1) % 3];
 #pragma unroll
         for (int b = 0; b < kN; ++b) {
             f32x4 qm[4];
@@ -790,15 +833,15 @@ __global__ void __launch_bounds__(128, 1) gdn_chunk_kernel(GdnArgs a, ChunkArgs 
             for (int step = 0; step < 2; ++step)
 #pragma unroll
                 for (int part = 0; part < 2; ++part) us[step][part] = left.u[b][step][part][lane];
-            const float m_up = left.m_up[b][col], by = left.x_up[b][col] * (1.0f / (kUpU * kUpT));
+            const int up = left.up[b][col];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const f32x4 pu = triangle(p, us, r);
                 const f32x4 fq = *reinterpret_cast<const f32x4*>(&f[kFQuery + r * 16 + g * 4]), fr = *reinterpret_cast<const f32x4*>(&f[kFRow + r * 16 + g * 4]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float o = fq[j] * m_up * qm[r][j] + fr[j] * by * pu[j];
-                    uint8_t* to = &s_out[(r * 16 + g * 4 + j) * kRowV + (b * 16 + col) * kBytes];
+                    const float o = __builtin_amdgcn_ldexpf(fq[j] * qm[r][j] + fr[j] * pu[j], up);
+                    uint8_t* to = &s.out[(r * 16 + g * 4 + j) * kRowV + (b * 16 + col) * kBytes];
                     if constexpr (kF16) *reinterpret_cast<_Float16*>(to) = _Float16(o);
                     else *reinterpret_cast<float*>(to) = o;
                 }
@@ -812,24 +855,24 @@ __global__ void __launch_bounds__(128, 1) gdn_chunk_kernel(GdnArgs a, ChunkArgs 
         for (uint32_t i = 0; i < kEach; ++i) {
             const uint32_t at = lane + i * 64;
             if (at / kPieces <= last)
-                st_global<ops_u32x4>(to + int64_t(at / kPieces) * a.out_ld + at % kPieces * 16, *reinterpret_cast<const ops_u32x4*>(&s_out[at * 16]));
+                st_global<ops_u32x4>(to + int64_t(at / kPieces) * a.out_ld + at % kPieces * 16, *reinterpret_cast<const ops_u32x4*>(&s.out[at * 16]));
         }
         wave_sync();
     }
 }
 
-template <int S, int kCols, bool kF16>
+template <int S, bool kF16>
 void launch_chunks(const GdnArgs& a, const ChunkArgs& c, hipStream_t stream) {
-    const uint32_t pairs = (a.n_seqs * a.v_heads + 7) / 8 * 8;
-    hipLaunchKernelGGL((gdn_prepare_kernel<S, kF16>), dim3((c.count * a.v_heads + kWaves - 1) / kWaves), dim3(kThreadsC), 0, stream, a, c);
-    hipLaunchKernelGGL((gdn_chunk_kernel<S, kCols, kF16>), dim3(pairs * (S / kCols)), dim3(128), 0, stream, a, c);
+    const uint32_t heads = (a.n_seqs * a.v_heads + 7) / 8 * 8;
+    hipLaunchKernelGGL((gdn_prepare_kernel<S, kF16>), dim3(c.count * a.v_heads), dim3(kThreadsC), 0, stream, a, c);
+    hipLaunchKernelGGL((gdn_chunk_kernel<S, 16, kF16>), dim3(heads * (S / 16)), dim3(128), 0, stream, a, c);
 }
 template <int S>
 hipError_t launch_of(const GdnArgs& a, const ChunkArgs& plan, bool f16, hipStream_t stream) {
     for (ChunkArgs c = plan; c.first < plan.total; c.first += plan.count) {
         c.count = plan.total - c.first < plan.count ? plan.total - c.first : plan.count;
-        if (f16) launch_chunks<S, 16, true>(a, c, stream);
-        else launch_chunks<S, 16, false>(a, c, stream);
+        if (f16) launch_chunks<S, true>(a, c, stream);
+        else launch_chunks<S, false>(a, c, stream);
         const hipError_t e = hipGetLastError();
         if (e != hipSuccess) return e;
     }
