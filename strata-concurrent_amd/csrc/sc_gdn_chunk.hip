@@ -6,10 +6,10 @@
 //     M1 = e^(G_C) M0 + sum_j e^(G_C - G_j) k_j u_j^T
 // Everything but M0 is known beforehand, so a first kernel forms T = (1 + A)^-1 and P of every chunk at once, and a second
 // one takes the chunks of a sequence in order with products only.  Columns of the state (values) do not meet: a workgroup
-// of the second kernel takes 16 or 32 of them with two waves.  One carries the state, whole columns in its registers: a
+// of the second kernel takes 16 of them with four waves.  Two carry the state, half the keys each, in their registers: a
 // result of a product (column = lane % 16, rows in registers) is the right operand of the next one as it stands, so nothing
-// it needs crosses lanes but a column's largest value.  The other is a chunk behind and forms the outputs from the state and
-// U that the first left in LDS; it also brings V and the factors of rows.  They meet once a chunk.
+// crosses lanes but a column's largest value, and only the two halves of K M0 are exchanged.  The two others are a chunk
+// behind and form the outputs from the state and U that the first left in LDS; they also bring V, T and the factors of rows.
 //
 // Accuracy: the products run as f16 matrix instructions with sums in 32 bits, and keep f32 accuracy: an f32 operand is
 // two f16 parts (22 bits).  f16 keys and queries enter as they are, exactly, f32 ones scaled by row with a power of two;
@@ -467,10 +467,15 @@ __global__ void __launch_bounds__(kThreadsC, 3) gdn_prepare_kernel(GdnArgs a, Ch
 
 // ---- the chunks of a sequence in order ------------------------------------------------------------------------------------
 
-// A column's state m times 2^up, scaled anew where the largest of it and of beta V (`v_top`, unscaled) leaves the window;
-// `down` is 2^-up.
+// The columns of the state of a workgroup of the second kernel
+constexpr int kCols = 16;
+// Its waves: the state's keys are shared by two where there are 64 or more, two others form the outputs.
+template <int S>
+constexpr int kStateWaves = S >= 64 ? 2 : 1;
+constexpr int kOutWaves = 2;
+
 template <int kSteps>
-__device__ __forceinline__ void fit_scale(f32x4 (&m)[kSteps][2], int& up, float& down, float v_top, float beta_most) {
+__device__ __forceinline__ float most_of(const f32x4 (&m)[kSteps][2]) {
     float top = 0;
 #pragma unroll
     for (int i = 0; i < kSteps; ++i)
@@ -478,9 +483,14 @@ __device__ __forceinline__ void fit_scale(f32x4 (&m)[kSteps][2], int& up, float&
         for (int e = 0; e < 2; ++e)
 #pragma unroll
             for (int j = 0; j < 4; j += 2) top = fmaxf(fmaxf(top, fabsf(m[i][e][j])), fabsf(m[i][e][j + 1]));
-    top = over_rows(top, max_of) * beta_most;
+    return over_rows(top, max_of);
+}
+// A column's state is m times 2^up; scaled anew where its largest or that of beta V (`v_top`, unscaled) leaves the window.
+// `m_top` is the larger of m's in the column, in every wave that has a part of it; `down` is 2^-up.
+template <int kSteps>
+__device__ __forceinline__ void fit_scale(f32x4 (&m)[kSteps][2], int& up, float& down, float m_top, float v_top, float beta_most) {
     down = __builtin_amdgcn_ldexpf(1.0f, -up);
-    top = fmaxf(top, v_top * down);
+    const float top = fmaxf(m_top * beta_most, v_top * down);
     if (__any(top >= float(1 << kTop) || (top > 0 && top < 1.0f / float(1 << -kLeast)))) {
         // to 2^kAim, within what f32 can scale by
         const int e = int(__float_as_uint(top) >> 23) - 127 - kAim, to = up + e;
@@ -500,31 +510,31 @@ __device__ __forceinline__ void split_state(const f32x4 (&m)[2], ops_u32x4& hi, 
     split_pair(f32x4{m[0].x, m[1].x, m[0].y, m[1].y}, f32x4{m[0].z, m[1].z, m[0].w, m[1].w}, hi, lo);
 }
 
-template <int S, int kCols, bool kF16>
-__global__ void __launch_bounds__(128, 1) gdn_chunk_kernel(GdnArgs a, ChunkArgs c) {
-    constexpr int kParts = kF16 ? 1 : 2, kSteps = S / 32, kN = kCols / 16;
+template <int S, bool kF16>
+__global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chunk_kernel(GdnArgs a, ChunkArgs c) {
+    constexpr int kParts = kF16 ? 1 : 2, kSteps = S / 32, kShares = kStateWaves<S>, kMine = kSteps / kShares;
+    constexpr uint32_t kThreads = (kShares + kOutWaves) * 64;
     constexpr uint32_t kBytes = kF16 ? 2 : 4;                            // of an activation
     constexpr uint32_t kRowV = kCols * kBytes, kPieces = kRowV / 16;     // a row of V or O of this workgroup, in 16-byte pieces
-    constexpr uint32_t kEach = kC * kPieces / 64;                        // pieces of a lane
-    constexpr uint32_t kFLanes = (kFactors + 63) / 64;
-    // what one wave leaves for the other, by the chunk's parity
+    constexpr uint32_t kEach = kC * kPieces / (kOutWaves * 64);          // pieces of a lane
+    // what the state's waves leave for the others, by the chunk's parity
     struct Left {
-        ops_u32x4 m[kN][kSteps][2][64], u[kN][2][2][64];   // the state before the chunk and U as right operands: [step][part]
-        int up[kN][16];                                    // the power of two that a column of both is to be scaled up by
+        ops_u32x4 m[kSteps][2][64], u[2][2][64];   // the state before the chunk and U as right operands: [step][part]
+        int up[16];                                // the power of two that a column of both is to be scaled up by
     };
+    // and the others for them
     struct Values {
-        f32x4 v[kN][4][64];                                // beta V as results lie: [tile][lane]
-        float most[kN][16];                                // its largest magnitude by column
+        f32x4 v[4][64];                            // beta V as results lie: [tile][lane]
+        float most[kOutWaves][16];                 // its largest magnitude by column, of two tiles each
+        ops_u32x4 t[6][2][64];                     // T
     };
-    struct Shared {
-        Left left[2];
-        Values values[2];
-        alignas(16) uint8_t vin[kC * kRowV], out[kC * kRowV];
-        alignas(16) float f[3][kFLanes * 64];
-    };
-    __shared__ Shared s;
+    __shared__ Left s_left[2];
+    __shared__ Values s_values[2];
+    __shared__ __align__(16) uint8_t s_vin[kC * kRowV], s_out[kC * kRowV];
+    __shared__ __align__(16) float s_f[3][(kFactors + 63) / 64 * 64];
+    __shared__ f32x4 s_km[kShares][4][64];         // K M0 by a wave's keys
+    __shared__ float s_top[kShares][16];           // the largest of a wave's state by column
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const bool carries = wave == 0;
     const uint32_t g = lane >> 4, col = lane & 15;
     // workgroups go to the eight XCDs in turn: the column blocks of a head are kept on one, whose L2 has its operands
     constexpr uint32_t kBlocks = S / kCols;
@@ -540,7 +550,7 @@ __global__ void __launch_bounds__(128, 1) gdn_chunk_kernel(GdnArgs a, ChunkArgs 
     float* base = a.state[seq];
     if (!base) {
         const uint32_t from = q.t0 + (c0 - q.chunk0) * kC, to = q.t0 + (c1 - q.chunk0) * kC < q.t1 ? q.t0 + (c1 - q.chunk0) * kC : q.t1;
-        for (uint32_t t = from + tid / (kCols / 4); t < to; t += 128 / (kCols / 4))
+        for (uint32_t t = from + tid / (kCols / 4); t < to; t += kThreads / (kCols / 4))
             st_act4<kF16>(a.out + int64_t(t) * a.out_ld, h * S + block * kCols + tid % (kCols / 4) * 4, f32x4{});
         return;
     }
@@ -555,41 +565,36 @@ __global__ void __launch_bounds__(128, 1) gdn_chunk_kernel(GdnArgs a, ChunkArgs 
     auto clamped = [&](uint32_t chunk) { return chunk < c1 ? chunk : c1 - 1; };
     auto operands_of = [&](uint32_t chunk) { return c.chunks + (uint64_t(chunk - c.first) * a.v_heads + h) * kChunkWords; };
     auto rows_of = [&](uint32_t chunk) { return c.rows + (uint64_t(chunk - c.first) * c.k_heads + kh) * kRowWords<S, kParts>; };
-    // keys or queries as left operands
-    auto load_rows = [&](ops_u32x4 (&x)[4][kParts][kSteps], uint32_t chunk, uint32_t which) {
+    // a tile of keys or queries as left operands, N steps from `first` on
+    auto load_rows = [&](auto& x, uint32_t chunk, uint32_t which, uint32_t tile, uint32_t first) {
+        constexpr int N = sizeof(x[0]) / sizeof(x[0][0]);
         if constexpr (kF16) {
-            const uint32_t ld = uint32_t(which ? a.q_ld : a.k_ld), last = last_row(chunk) * ld;
-            const uint8_t* p = (which ? a.q : a.k) + int64_t(q.t0 + (chunk - q.chunk0) * kC) * ld + kh * S * 2;
+            const uint32_t ld = uint32_t(which ? a.q_ld : a.k_ld);
+            const uint8_t* p = (which ? a.q : a.k) + int64_t(q.t0 + (chunk - q.chunk0) * kC) * ld + kh * S * 2 + first * 64;
+            const uint32_t at = min((tile * 16 + col) * ld, last_row(chunk) * ld) + g * 16;
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                const uint32_t at = min((t * 16 + col) * ld, last) + g * 16;
-#pragma unroll
-                for (int i = 0; i < kSteps; ++i) x[t][0][i] = ld_global<ops_u32x4>(p + at + i * 64);
-            }
+            for (int i = 0; i < N; ++i) x[0][i] = ld_global<ops_u32x4>(p + at + i * 64);
         } else {
             const ops_u32x4* p = rows_of(chunk) + lane;
 #pragma unroll
-            for (int t = 0; t < 4; ++t)
+            for (int part = 0; part < kParts; ++part)
 #pragma unroll
-                for (int part = 0; part < kParts; ++part)
-#pragma unroll
-                    for (int i = 0; i < kSteps; ++i) x[t][part][i] = ld_global<ops_u32x4>(p + row_operand<S, kParts>(which, part, t, i));
+                for (int i = 0; i < N; ++i) x[part][i] = ld_global<ops_u32x4>(p + row_operand<S, kParts>(which, part, tile, first + i));
         }
     };
-    // T or P: operand w of operand_at's six, in two parts
-    auto load_operand = [&](ops_u32x4 (&x)[6][2], uint32_t chunk, uint32_t which) {
-        const ops_u32x4* p = operands_of(chunk) + which * kOperand + lane;
+    // n of P's six operands (operand_at's order) from `first` on, in two parts
+    auto load_operand = [&](auto& x, int at, int n, uint32_t chunk, uint32_t first) {
+        const ops_u32x4* p = operands_of(chunk) + kOperand + first * 128 + lane;
 #pragma unroll
-        for (int i = 0; i < 6; ++i)
+        for (int i = 0; i < n; ++i)
 #pragma unroll
-            for (int part = 0; part < 2; ++part) x[i][part] = ld_global<ops_u32x4>(p + i * 128 + part * 64);
+            for (int part = 0; part < 2; ++part) x[at + i][part] = ld_global<ops_u32x4>(p + i * 128 + part * 64);
     };
-    // the product with T or P of a right operand [step][part]
-    auto triangle = [&](const ops_u32x4 (&x)[6][2], const ops_u32x4 (&y)[2][2], int tile) {
-        const int first = tile < 2 ? tile : tile == 2 ? 2 : 4;
+    // the product of n operands of a row tile from `first` on with a right operand [step][part]
+    auto triangle = [&](const auto& x, int first, int n, const ops_u32x4 (&y)[2][2]) {
         f32x4 hi{}, lo{};
 #pragma unroll
-        for (int step = 0; step <= tile / 2; ++step) {
+        for (int step = 0; step < n; ++step) {
             hi = mfma(x[first + step][0], y[step][0], hi);
             lo = mfma(x[first + step][0], y[step][1], lo);
             lo = mfma(x[first + step][1], y[step][0], lo);
@@ -597,275 +602,279 @@ __global__ void __launch_bounds__(128, 1) gdn_chunk_kernel(GdnArgs a, ChunkArgs 
         return hi + lo;
     };
 
-    if (carries) {
-        // the state: keys 32 i + 8 g + 2 j + e in m[.][i][e][j], a column a lane
-        float* state = base + a.state_offset + h * a.head_ld + block * kCols + col + g * 8 * a.key_ld;
-        f32x4 m[kN][kSteps][2];
+    if (wave < kShares) {
+        // the state: keys 32 (first + i) + 8 g + 2 j + e in m[i][e][j], a column a lane
+        const uint32_t first = wave * kMine;
+        float* state = base + a.state_offset + h * a.head_ld + block * kCols + col + (first * 32 + g * 8) * a.key_ld;
+        f32x4 m[kMine][2];
 #pragma unroll
-        for (int b = 0; b < kN; ++b)
+        for (int i = 0; i < kMine; ++i)
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i)
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) m[b][i][e][j] = ld_global<float>(state + (i * 32 + 2 * j + e) * a.key_ld + b * 16);
+                for (int j = 0; j < 4; ++j) m[i][e][j] = ld_global<float>(state + (i * 32 + 2 * j + e) * a.key_ld);
         // waited for here: the loop would wait for it every time around
 #pragma unroll
-        for (int b = 0; b < kN; ++b)
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i) asm volatile("" : "+v"(m[b][i][0]), "+v"(m[b][i][1]));
-        ops_u32x4 k[4][kParts][kSteps], t[6][2], kt[kParts][kSteps][2][2];
+        for (int i = 0; i < kMine; ++i) asm volatile("" : "+v"(m[i][0]), "+v"(m[i][1]));
+        ops_u32x4 k[4][kParts][kMine], kt[kParts][kMine][2][2];
         auto load_keys = [&](uint32_t chunk) {
             const ops_u32x4* p = rows_of(chunk) + lane;
 #pragma unroll
             for (int part = 0; part < kParts; ++part)
 #pragma unroll
-                for (int i = 0; i < kSteps; ++i)
+                for (int i = 0; i < kMine; ++i)
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
 #pragma unroll
-                        for (int step = 0; step < 2; ++step) kt[part][i][e][step] = ld_global<ops_u32x4>(p + key_operand<S, kParts>(part, i, e, step));
+                        for (int step = 0; step < 2; ++step) kt[part][i][e][step] = ld_global<ops_u32x4>(p + key_operand<S, kParts>(part, first + i, e, step));
         };
-        load_rows(k, c0, 0);
-        load_operand(t, c0, 0);
-        load_keys(c0);
-        int up[kN];   // a column's state is m times 2^up
 #pragma unroll
-        for (int b = 0; b < kN; ++b) up[b] = 0;
+        for (int r = 0; r < 4; ++r) load_rows(k[r], c0, 0, r, first);
+        load_keys(c0);
+        int up = 0;   // a column's state is m times 2^up
+        float top = most_of<kMine>(m);
+        if (g == 0) s_top[wave][col] = top;
         for (uint32_t chunk = c0; chunk < c1; ++chunk) {
             const uint32_t which = (chunk - c0) & 1, ahead = clamped(chunk + 1);
-            Left& left = s.left[which];
+            Left& left = s_left[which];
             __syncthreads();   // V and the factors are here, and the outputs of the chunk before the last are done
-            const float* f = s.f[(chunk - c0) % 3];
-            const Values& values = s.values[which];
+            const float* f = s_f[(chunk - c0) % 3];
+            const Values& values = s_values[which];
             // the state as a right operand
-            const float beta_most = fmaxf(f[kFBetaMost], 1.0f);
-            ops_u32x4 mh[kN][kSteps], ml[kN][kSteps];
-            float down[kN];
+            ops_u32x4 mh[kMine], ml[kMine];
+            float down;
+            if constexpr (kShares > 1) top = fmaxf(s_top[0][col], s_top[kShares - 1][col]);
+            fit_scale<kMine>(m, up, down, top, fmaxf(values.most[0][col], values.most[1][col]), fmaxf(f[kFBetaMost], 1.0f));
 #pragma unroll
-            for (int b = 0; b < kN; ++b) {
-                fit_scale<kSteps>(m[b], up[b], down[b], values.most[b][col], beta_most);
-#pragma unroll
-                for (int i = 0; i < kSteps; ++i) {
-                    split_state(m[b][i], mh[b][i], ml[b][i]);
-                    left.m[b][i][0][lane] = mh[b][i];
-                    left.m[b][i][1][lane] = ml[b][i];
-                }
-                if (g == 0) left.up[b][col] = up[b];
+            for (int i = 0; i < kMine; ++i) {
+                split_state(m[i], mh[i], ml[i]);
+                left.m[first + i][0][lane] = mh[i];
+                left.m[first + i][1][lane] = ml[i];
             }
+            if (wave == 0 && g == 0) left.up[col] = up;
             // K M0
-            f32x4 km[kN][4];
+            f32x4 km[4];
 #pragma unroll
-            for (int b = 0; b < kN; ++b)
+            for (int r = 0; r < 4; ++r) km[r] = f32x4{};
 #pragma unroll
-                for (int r = 0; r < 4; ++r) km[b][r] = f32x4{};
-#pragma unroll
-            for (int i = 0; i < kSteps; ++i)
+            for (int i = 0; i < kMine; ++i)
 #pragma unroll
                 for (int x = 0; x < kParts + 1; ++x)   // high by high, high by low, low by high
 #pragma unroll
-                    for (int r = 0; r < 4; ++r)
+                    for (int r = 0; r < 4; ++r) km[r] = mfma(k[r][x == 2][i], x == 1 ? ml[i] : mh[i], km[r]);
 #pragma unroll
-                        for (int b = 0; b < kN; ++b) km[b][r] = mfma(k[r][x == 2][i], x == 1 ? ml[b][i] : mh[b][i], km[b][r]);
-            load_rows(k, ahead, 0);
+            for (int r = 0; r < 4; ++r) load_rows(k[r], ahead, 0, r, first);
+            if constexpr (kShares > 1) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s_km[wave][r][lane] = km[r];
+                __syncthreads();
+#pragma unroll
+                for (int r = 0; r < 4; ++r) km[r] += s_km[wave ^ 1][r][lane];   // the same sum in both waves
+            }
             // X; rows past the sequence's end are zero, as their V and factors are
-            ops_u32x4 xs[kN][2][2];
-#pragma unroll
-            for (int b = 0; b < kN; ++b) {
+            ops_u32x4 xs[2][2];
+            {
                 f32x4 x[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const f32x4 fs = *reinterpret_cast<const f32x4*>(&f[kFState + r * 16 + g * 4]), v = values.v[b][r][lane];
+                    const f32x4 fs = *reinterpret_cast<const f32x4*>(&f[kFState + r * 16 + g * 4]), v = values.v[r][lane];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) x[r][j] = __builtin_fmaf(-fs[j], km[b][r][j], v[j] * down[b]);
+                    for (int j = 0; j < 4; ++j) x[r][j] = __builtin_fmaf(-fs[j], km[r][j], v[j] * down);
                 }
-                split_pair(x[0], x[1], xs[b][0][0], xs[b][0][1]);
-                split_pair(x[2], x[3], xs[b][1][0], xs[b][1][1]);
+                split_pair(x[0], x[1], xs[0][0], xs[0][1]);
+                split_pair(x[2], x[3], xs[1][0], xs[1][1]);
             }
             // U = T X, and the same weighted for the state
-            ops_u32x4 ws[kN][2][2];
+            ops_u32x4 ws[2][2];
+            {
+                ops_u32x4 t[6][2];
 #pragma unroll
-            for (int b = 0; b < kN; ++b) {
-                f32x4 u[4];
+                for (int i = 0; i < 6; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) u[r] = triangle(t, xs[b], r);
+                    for (int part = 0; part < 2; ++part) t[i][part] = values.t[i][part][lane];
+                f32x4 u[4]{triangle(t, 0, 1, xs), triangle(t, 1, 1, xs), triangle(t, 2, 2, xs), triangle(t, 4, 2, xs)};
 #pragma unroll
                 for (int step = 0; step < 2; ++step) {
-                    ops_u32x4 hi, lo;
-                    split_pair(u[step * 2], u[step * 2 + 1], hi, lo);
-                    left.u[b][step][0][lane] = hi;
-                    left.u[b][step][1][lane] = lo;
                     const f32x4 w0 = *reinterpret_cast<const f32x4*>(&f[kFWrite + step * 32 + g * 4]), w1 = *reinterpret_cast<const f32x4*>(&f[kFWrite + step * 32 + 16 + g * 4]);
-                    split_pair(u[step * 2], u[step * 2 + 1], w0, w1, ws[b][step][0], ws[b][step][1]);
+                    split_pair(u[step * 2], u[step * 2 + 1], w0, w1, ws[step][0], ws[step][1]);
+                    if (kShares == 1 || uint32_t(step) == wave) {
+                        ops_u32x4 hi, lo;
+                        split_pair(u[step * 2], u[step * 2 + 1], hi, lo);
+                        left.u[step][0][lane] = hi;
+                        left.u[step][1][lane] = lo;
+                    }
                 }
             }
-            load_operand(t, ahead, 0);
             // the state after the chunk
             const float decay = f[kFDecay], w_up = f[kFUp];
             const bool plain = __builtin_amdgcn_readfirstlane(int(w_up == 1.0f));   // nearly always
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i)
+            for (int i = 0; i < kMine; ++i)
 #pragma unroll
-                for (int b = 0; b < kN; ++b)
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) m[b][i][e] *= decay;
-            auto update = [&](f32x4 (&add)[kN][kSteps][2]) {
+                for (int e = 0; e < 2; ++e) m[i][e] *= decay;
+            auto update = [&](f32x4 (&add)[kMine][2]) {
 #pragma unroll
                 for (int step = 0; step < 2; ++step)
 #pragma unroll
                     for (int x = 0; x < kParts + 1; ++x)
 #pragma unroll
-                        for (int i = 0; i < kSteps; ++i)
+                        for (int i = 0; i < kMine; ++i)
 #pragma unroll
-                            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                                for (int b = 0; b < kN; ++b) add[b][i][e] = mfma(kt[x == 2][i][e][step], ws[b][step][x == 1], add[b][i][e]);
+                            for (int e = 0; e < 2; ++e) add[i][e] = mfma(kt[x == 2][i][e][step], ws[step][x == 1], add[i][e]);
             };
             if (plain) {
                 update(m);
             } else {
-                f32x4 add[kN][kSteps][2]{};
+                f32x4 add[kMine][2]{};
                 update(add);
 #pragma unroll
-                for (int i = 0; i < kSteps; ++i)
+                for (int i = 0; i < kMine; ++i)
 #pragma unroll
-                    for (int b = 0; b < kN; ++b)
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) m[b][i][e] += w_up * add[b][i][e];
+                    for (int e = 0; e < 2; ++e) m[i][e] += w_up * add[i][e];
             }
             load_keys(ahead);
+            top = most_of<kMine>(m);
+            if (g == 0) s_top[wave][col] = top;
         }
         __syncthreads();   // the last chunk's outputs
 #pragma unroll
-        for (int b = 0; b < kN; ++b)
+        for (int i = 0; i < kMine; ++i)
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i)
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
-                for (int e = 0; e < 2; ++e)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        st_global<float>(state + (i * 32 + 2 * j + e) * a.key_ld + b * 16, __builtin_amdgcn_ldexpf(m[b][i][e][j], up[b]));
+                for (int j = 0; j < 4; ++j)
+                    st_global<float>(state + (i * 32 + 2 * j + e) * a.key_ld, __builtin_amdgcn_ldexpf(m[i][e][j], up));
         return;
     }
 
-    // the other wave: V and the factors of the chunk after the next, outputs of the chunk before
-    const uint32_t v_ld = uint32_t(a.v_ld);
-    ops_u32x4 v_in[kEach];
-    float f_in[kFLanes];
+    // The other waves: V, T and the factors of the chunk after the next, outputs of the chunk before.  Wave w of the two takes
+    // V's tiles 2 w and 2 w + 1 and the outputs' w and 3 - w, which have three operands of P's six.
+    const uint32_t w = wave - kShares, v_ld = uint32_t(a.v_ld);
+    ops_u32x4 v_in[kEach], t_in[6];
+    float f_in[4];
+    auto factor_at = [&](uint32_t i) { return (i == 0 ? 1 : w ? i + 2 : (i - 1) * 2) * 64 + lane; };   // both have kFBeta's
     auto load_early = [&](uint32_t chunk) {
         const uint32_t last = last_row(chunk) * v_ld;
         const uint8_t* p = a.v + int64_t(q.t0 + (chunk - q.chunk0) * kC) * a.v_ld + (h * S + block * kCols) * kBytes;
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i) {
-            const uint32_t at = lane + i * 64;
+            const uint32_t at = lane + (w * kEach + i) * 64;
             v_in[i] = ld_global<ops_u32x4>(p + min(at / kPieces * v_ld, last) + at % kPieces * 16);
         }
+#pragma unroll
+        for (int i = 0; i < 6; ++i) t_in[i] = ld_global<ops_u32x4>(operands_of(chunk) + (w * 6 + i) * 64 + lane);
         const float* f = reinterpret_cast<const float*>(operands_of(chunk) + 2 * kOperand);
 #pragma unroll
-        for (uint32_t i = 0; i < kFLanes; ++i) f_in[i] = ld_global<float>(f + min(lane + i * 64, uint32_t(kFactors - 1)));
+        for (uint32_t i = 0; i < 4; ++i) f_in[i] = ld_global<float>(f + min(factor_at(i), uint32_t(kFactors - 1)));
     };
-    // V as the first wave takes it, by way of LDS: times beta, rows past the sequence's end zero, a lane's four rows together
+    // V as the state's waves take it, by way of LDS: times beta, rows past the sequence's end zero, a lane's four rows together
     auto put_early = [&](uint32_t chunk, uint32_t n) {
         const uint32_t last = last_row(chunk);
-        float* f = s.f[n % 3];
-        Values& to = s.values[n & 1];
+        float* f = s_f[n % 3];
+        Values& to = s_values[n & 1];
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i) {
-            const uint32_t at = lane + i * 64;
-            *reinterpret_cast<ops_u32x4*>(&s.vin[at * 16]) = at / kPieces <= last ? v_in[i] : ops_u32x4{};
+            const uint32_t at = lane + (w * kEach + i) * 64;
+            *reinterpret_cast<ops_u32x4*>(&s_vin[at * 16]) = at / kPieces <= last ? v_in[i] : ops_u32x4{};
         }
 #pragma unroll
-        for (uint32_t i = 0; i < kFLanes; ++i) f[lane + i * 64] = f_in[i];
+        for (uint32_t i = 0; i < 4; ++i) f[factor_at(i)] = f_in[i];
         wave_sync();
+        float top = 0;
 #pragma unroll
-        for (int b = 0; b < kN; ++b) {
-            float top = 0;
+        for (uint32_t i = 0; i < 2; ++i) {
+            const uint32_t row = (w * 2 + i) * 16 + g * 4;
+            f32x4 v = *reinterpret_cast<const f32x4*>(&f[kFBeta + row]);
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                f32x4 v = *reinterpret_cast<const f32x4*>(&f[kFBeta + r * 16 + g * 4]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint8_t* p = &s.vin[(r * 16 + g * 4 + j) * kRowV + (b * 16 + col) * kBytes];
-                    if constexpr (kF16) v[j] *= float(*reinterpret_cast<const _Float16*>(p));
-                    else v[j] *= *reinterpret_cast<const float*>(p);
-                    top = fmaxf(top, fabsf(v[j]));
-                }
-                to.v[b][r][lane] = v;
+            for (int j = 0; j < 4; ++j) {
+                const uint8_t* p = &s_vin[(row + j) * kRowV + col * kBytes];
+                if constexpr (kF16) v[j] *= float(*reinterpret_cast<const _Float16*>(p));
+                else v[j] *= *reinterpret_cast<const float*>(p);
+                top = fmaxf(top, fabsf(v[j]));
             }
-            top = over_rows(top, max_of);
-            if (g == 0) to.most[b][col] = top;
+            to.v[w * 2 + i][lane] = v;
         }
+        top = over_rows(top, max_of);
+        if (g == 0) to.most[w][col] = top;
+#pragma unroll
+        for (uint32_t i = 0; i < 6; ++i) to.t[(w * 6 + i) / 2][i % 2][lane] = t_in[i];
         wave_sync();
     };
-    ops_u32x4 qs[4][kParts][kSteps], p[6][2];
-    load_early(c0);
-    put_early(c0, 0);
-    load_early(clamped(c0 + 1));
-    load_rows(qs, c0, 1);
-    load_operand(p, c0, 1);
-    for (uint32_t chunk = c0; chunk <= c1; ++chunk) {
-        const uint32_t n = chunk - c0;
-        __syncthreads();
-        // the first wave reads the places of chunk n now, and this one the factors of chunk n - 1
-        if (chunk < c1) {
-            put_early(clamped(chunk + 1), n + 1);
-            load_early(clamped(chunk + 2));
+    ops_u32x4 qs[2][kParts][kSteps], p[3][2];
+    auto load_ahead = [&](uint32_t chunk) {
+        load_rows(qs[0], chunk, 1, w, 0);
+        load_rows(qs[1], chunk, 1, 3 - w, 0);
+        load_operand(p, 0, 1, chunk, w);
+        load_operand(p, 1, 2, chunk, 4 - 2 * w);
+    };
+    auto outputs = [&](uint32_t done) {
+        const uint32_t n = done - c0;
+        const uint32_t last = last_row(done);
+        const Left& left = s_left[n & 1];
+        const float* f = s_f[n % 3];
+        f32x4 qm[2]{};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i) {
+            const ops_u32x4 hi = left.m[i][0][lane], lo = left.m[i][1][lane];
+#pragma unroll
+            for (int x = 0; x < kParts + 1; ++x)
+#pragma unroll
+                for (int r = 0; r < 2; ++r) qm[r] = mfma(qs[r][x == 2][i], x == 1 ? lo : hi, qm[r]);
         }
-        if (chunk == c0) continue;
-        const uint32_t done = chunk - 1, last = last_row(done);
-        const Left& left = s.left[(n - 1) & 1];
-        const float* f = s.f[(n - 1) % 3];
+        ops_u32x4 us[2][2];
 #pragma unroll
-        for (int b = 0; b < kN; ++b) {
-            f32x4 qm[4];
+        for (int step = 0; step < 2; ++step)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) qm[r] = f32x4{};
+            for (int part = 0; part < 2; ++part) us[step][part] = left.u[step][part][lane];
+        const int up = left.up[col];
 #pragma unroll
-            for (int i = 0; i < kSteps; ++i) {
-                const ops_u32x4 hi = left.m[b][i][0][lane], lo = left.m[b][i][1][lane];
+        for (int r = 0; r < 2; ++r) {
+            const uint32_t row = (r ? 3 - w : w) * 16 + g * 4;
+            const f32x4 sum = r ? triangle(p, 1, 2, us) : triangle(p, 0, 1, us);
+            const f32x4 fq = *reinterpret_cast<const f32x4*>(&f[kFQuery + row]), fr = *reinterpret_cast<const f32x4*>(&f[kFRow + row]);
 #pragma unroll
-                for (int x = 0; x < kParts + 1; ++x)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) qm[r] = mfma(qs[r][x == 2][i], x == 1 ? lo : hi, qm[r]);
-            }
-            ops_u32x4 us[2][2];
-#pragma unroll
-            for (int step = 0; step < 2; ++step)
-#pragma unroll
-                for (int part = 0; part < 2; ++part) us[step][part] = left.u[b][step][part][lane];
-            const int up = left.up[b][col];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const f32x4 pu = triangle(p, us, r);
-                const f32x4 fq = *reinterpret_cast<const f32x4*>(&f[kFQuery + r * 16 + g * 4]), fr = *reinterpret_cast<const f32x4*>(&f[kFRow + r * 16 + g * 4]);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float o = __builtin_amdgcn_ldexpf(fq[j] * qm[r][j] + fr[j] * pu[j], up);
-                    uint8_t* to = &s.out[(r * 16 + g * 4 + j) * kRowV + (b * 16 + col) * kBytes];
-                    if constexpr (kF16) *reinterpret_cast<_Float16*>(to) = _Float16(o);
-                    else *reinterpret_cast<float*>(to) = o;
-                }
+            for (int j = 0; j < 4; ++j) {
+                const float o = __builtin_amdgcn_ldexpf(fq[j] * qm[r][j] + fr[j] * sum[j], up);
+                uint8_t* to = &s_out[(row + j) * kRowV + col * kBytes];
+                if constexpr (kF16) *reinterpret_cast<_Float16*>(to) = _Float16(o);
+                else *reinterpret_cast<float*>(to) = o;
             }
         }
-        load_rows(qs, clamped(chunk), 1);
-        load_operand(p, clamped(chunk), 1);
+        load_ahead(clamped(done + 1));
         wave_sync();
         uint8_t* to = a.out + int64_t(q.t0 + (done - q.chunk0) * kC) * a.out_ld + (h * S + block * kCols) * kBytes;
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i) {
-            const uint32_t at = lane + i * 64;
-            if (at / kPieces <= last)
-                st_global<ops_u32x4>(to + int64_t(at / kPieces) * a.out_ld + at % kPieces * 16, *reinterpret_cast<const ops_u32x4*>(&s.out[at * 16]));
+            const uint32_t at = lane + i * 64, half = at / (16 * kPieces), row = (half ? 3 - w : w) * 16 + at / kPieces % 16;
+            if (row <= last) st_global<ops_u32x4>(to + int64_t(row) * a.out_ld + at % kPieces * 16, *reinterpret_cast<const ops_u32x4*>(&s_out[row * kRowV + at % kPieces * 16]));
         }
         wave_sync();
+    };
+    // before a chunk's second barrier the state's waves read the places of that chunk
+    auto meet = [&](uint32_t chunk) {
+        __syncthreads();
+        put_early(clamped(chunk + 1), chunk + 1 - c0);
+        load_early(clamped(chunk + 2));
+        if constexpr (kShares > 1) __syncthreads();
+    };
+    load_early(c0);
+    put_early(c0, 0);
+    load_early(clamped(c0 + 1));
+    meet(c0);
+    load_ahead(c0);
+    for (uint32_t chunk = c0 + 1; chunk < c1; ++chunk) {
+        meet(chunk);
+        outputs(chunk - 1);
     }
+    __syncthreads();
+    outputs(c1 - 1);
 }
 
 template <int S, bool kF16>
 void launch_chunks(const GdnArgs& a, const ChunkArgs& c, hipStream_t stream) {
     const uint32_t heads = (a.n_seqs * a.v_heads + 7) / 8 * 8;
     hipLaunchKernelGGL((gdn_prepare_kernel<S, kF16>), dim3(c.count * a.v_heads), dim3(kThreadsC), 0, stream, a, c);
-    hipLaunchKernelGGL((gdn_chunk_kernel<S, 16, kF16>), dim3(heads * (S / 16)), dim3(128), 0, stream, a, c);
+    hipLaunchKernelGGL((gdn_chunk_kernel<S, kF16>), dim3(heads * (S / kCols)), dim3((kStateWaves<S> + kOutWaves) * 64), 0, stream, a, c);
 }
 template <int S>
 hipError_t launch_of(const GdnArgs& a, const ChunkArgs& plan, bool f16, hipStream_t stream) {
