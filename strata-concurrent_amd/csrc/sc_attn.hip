@@ -191,12 +191,6 @@ __device__ __forceinline__ int32_t row_of(const AttnArgs& a, const Span& p, int3
     return in ? int32_t((uint32_t(entry) * a.c.H + h) * a.c.ps.d + (cell - page * a.c.ps.d)) : -1;
 }
 
-// A load of what is read once, past the caches' keeping.
-template <class T>
-__device__ __forceinline__ T ld_once(const void* p) {
-    return __builtin_nontemporal_load((const __attribute__((address_space(1))) T*) (p));
-}
-
 template <int D, bool kInt8>
 __device__ __forceinline__ void load_keys(Rows<D, kInt8>& r, const AttnArgs& a, int32_t row, uint32_t lane) {
     using R = Rows<D, kInt8>;

@@ -105,25 +105,42 @@ template <class T>
 __device__ __forceinline__ void st_global(void* p, T v) {
     *(__attribute__((address_space(1))) T*) (p) = v;
 }
+// What is read or written once, past the caches' keeping.
+template <class T>
+__device__ __forceinline__ T ld_once(const void* p) {
+    return __builtin_nontemporal_load((const __attribute__((address_space(1))) T*) (p));
+}
+template <class T>
+__device__ __forceinline__ void st_once(void* p, T v) {
+    __builtin_nontemporal_store(v, (__attribute__((address_space(1))) T*) (p));
+}
 
-// Four consecutive values of an activation row, in f32.
-template <bool kF16>
+// Four consecutive values of an activation row, in f32; kOnce: past the caches' keeping.
+template <bool kF16, bool kOnce = false>
 __device__ __forceinline__ f32x4 ld_act4(const uint8_t* row, uint32_t at) {
     if constexpr (kF16) {
-        const f16x4 h = __builtin_bit_cast(f16x4, ld_global<ops_u32x2>(row + uint64_t(at) * 2));
+        const uint8_t* p = row + uint64_t(at) * 2;
+        const f16x4 h = __builtin_bit_cast(f16x4, kOnce ? ld_once<ops_u32x2>(p) : ld_global<ops_u32x2>(p));
         return f32x4{float(h.x), float(h.y), float(h.z), float(h.w)};
     } else {
-        return __builtin_bit_cast(f32x4, ld_global<ops_u32x4>(row + uint64_t(at) * 4));
+        const uint8_t* p = row + uint64_t(at) * 4;
+        return __builtin_bit_cast(f32x4, kOnce ? ld_once<ops_u32x4>(p) : ld_global<ops_u32x4>(p));
     }
 }
-template <bool kF16>
+template <bool kF16, bool kOnce = false>
 __device__ __forceinline__ void st_act4(uint8_t* row, uint32_t at, f32x4 v) {
     if constexpr (kF16) {
         // round to nearest even: the results' type holds 11 bits
         const f16x4 h{_Float16(v.x), _Float16(v.y), _Float16(v.z), _Float16(v.w)};
-        st_global<ops_u32x2>(row + uint64_t(at) * 2, __builtin_bit_cast(ops_u32x2, h));
+        const ops_u32x2 bits = __builtin_bit_cast(ops_u32x2, h);
+        uint8_t* p = row + uint64_t(at) * 2;
+        if constexpr (kOnce) st_once<ops_u32x2>(p, bits);
+        else st_global<ops_u32x2>(p, bits);
     } else {
-        st_global<ops_u32x4>(row + uint64_t(at) * 4, __builtin_bit_cast(ops_u32x4, v));
+        const ops_u32x4 bits = __builtin_bit_cast(ops_u32x4, v);
+        uint8_t* p = row + uint64_t(at) * 4;
+        if constexpr (kOnce) st_once<ops_u32x4>(p, bits);
+        else st_global<ops_u32x4>(p, bits);
     }
 }
 

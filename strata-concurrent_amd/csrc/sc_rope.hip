@@ -17,6 +17,11 @@ namespace sc {
 namespace {
 
 constexpr int kRopeThreads = 256;
+// Calls with as many tokens fill the chip with a workgroup a token, and their queries do not stay in the caches until they
+// are read: they are stored past them (10 K tokens of 24 heads of 256, f32: 118 us by plain stores, 109 past the caches).
+// With fewer, a token's rows are shared by workgroups and the queries left in the caches for the attention that follows
+// (one token of 28 rows: 3.6 us in shares, 4.5 by one workgroup).
+constexpr uint32_t kManyTokens = 512;
 constexpr double kTwoPi = 6.283185307179586476925286766559;
 
 // Writes four values of a pool row at `d` in the cache's format; `row` is the pool row.
@@ -36,7 +41,7 @@ __device__ __forceinline__ void st_cache4(uint8_t* pool, uint16_t* scales, uint6
     }
 }
 
-template <int D, bool kInt8, bool kF16>
+template <int D, bool kInt8, bool kF16, bool kMany>
 __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(RopeArgs a) {
     constexpr uint32_t kLanes = D / 4, kRows = 64 / kLanes;   // lanes of a row, rows of a wave
     __shared__ float s_cos[D / 2], s_sin[D / 2];
@@ -69,7 +74,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(RopeArgs a) {
         const bool there = r < total, is_q = r < a.n_head, is_k = !is_q && r < a.n_head + a.c.H;
         const uint32_t h = !there ? 0 : is_q ? r : is_k ? r - a.n_head : r - a.n_head - a.c.H;
         const uint8_t* src = is_q ? a.q + t * a.q_ld : is_k ? a.k + t * a.k_ld : a.v + t * a.v_ld;
-        f32x4 x = ld_act4<kF16>(src, h * D + d);
+        f32x4 x = ld_act4<kF16, true>(src, h * D + d);
         if (a.rot) {
             f32x4 o{};
             uint32_t i[4];
@@ -88,7 +93,7 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(RopeArgs a) {
             if (d < a.rot && (is_q || is_k))
                 for (int j = 0; j < 4; ++j) x[j] = x[j] * s_cos[i[j]] + sign[j] * o[j] * s_sin[i[j]];
         }
-        if (there && is_q) st_act4<kF16>(a.q_out + t * a.q_out_ld, h * D + d, x);
+        if (there && is_q) st_act4<kF16, kMany>(a.q_out + t * a.q_out_ld, h * D + d, x);
         const bool keep = there && !is_q && row0 >= 0;
         const uint64_t row = keep ? uint64_t(row0) + uint64_t(h) * a.c.ps.d : 0;
         st_cache4<D, kInt8>(is_k ? a.c.k : a.c.v, is_k ? a.c.k_scale : a.c.v_scale, row, d, x, keep);
@@ -99,11 +104,13 @@ template <int D, bool kInt8>
 hipError_t launch_of(const RopeArgs& a, bool f16, hipStream_t stream) {
     constexpr uint32_t per_wg = kRopeThreads / 64 * (64 / (D / 4));
     const uint32_t total = a.n_head + 2 * a.c.H, most = (total + per_wg - 1) / per_wg;
-    // a share of a token's rows each while tokens alone leave the chip's 256 units without work
-    const uint32_t y = a.tokens >= 512 ? 1 : most < (512 + a.tokens - 1) / a.tokens ? most : (512 + a.tokens - 1) / a.tokens;
+    const uint32_t shares = (kManyTokens + a.tokens - 1) / a.tokens, y = most < shares ? most : shares;
+    const bool many = a.tokens >= kManyTokens;
     const dim3 grid(a.tokens, y), block(kRopeThreads);
-    if (f16) hipLaunchKernelGGL((rope_append_kernel<D, kInt8, true>), grid, block, 0, stream, a);
-    else hipLaunchKernelGGL((rope_append_kernel<D, kInt8, false>), grid, block, 0, stream, a);
+    if (f16 && many) hipLaunchKernelGGL((rope_append_kernel<D, kInt8, true, true>), grid, block, 0, stream, a);
+    else if (f16) hipLaunchKernelGGL((rope_append_kernel<D, kInt8, true, false>), grid, block, 0, stream, a);
+    else if (many) hipLaunchKernelGGL((rope_append_kernel<D, kInt8, false, true>), grid, block, 0, stream, a);
+    else hipLaunchKernelGGL((rope_append_kernel<D, kInt8, false, false>), grid, block, 0, stream, a);
     return hipGetLastError();
 }
 
