@@ -85,7 +85,8 @@ class Layer:
 
 
 STEPS = [(128, 16, 32, 1, "f32", "slot"), (128, 16, 32, 5, "f16", "prefill"), (128, 16, 48, 2, "f32", "slot"),
-         (64, 4, 8, 3, "f16", "slot"), (32, 4, 8, 7, "f32", "prefill"), (64, 1, 1, 1, "f32", "slot"), (128, 8, 8, 70, "f32", "slot")]
+         (64, 4, 8, 3, "f16", "slot"), (32, 4, 8, 7, "f32", "prefill"), (64, 1, 1, 1, "f32", "slot"), (128, 8, 8, 70, "f32", "slot"),
+         (64, 8, 16, 40, "f16", "prefill"), (128, 2, 4, 66, "f16", "slot")]   # the last three by 64 columns
 
 
 @pytest.mark.parametrize("l2norm", [True, False], ids=["unit", "as-is"])

@@ -40,6 +40,8 @@ CASES = [
     ("int8", "f16", 1, 64, 8, 16, 64, "neighbours", [1] * 70, list(range(0, 700, 10))),
     ("int8", "f32", 4, 128, 1, 32, 128, "halves", [3, 9], [0, 1]),
     ("int8", "f32", 2, 128, 5, 2, 0, "halves", [600], [1]),
+    ("f16", "f16", 2, 64, 4, 5, 32, "neighbours", [511, 2], [9, 0]),
+    ("f16", "f32", 1, 256, 16, 3, 256, "halves", [512], [100]),
 ]
 
 
