@@ -129,6 +129,21 @@ def test_a_long_prompt(sc, ops, plain, cuda, dtype):
 
 
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
+def test_a_state_as_a_whole(sc, ops, plain, cuda, dtype):
+    """The error of a state in its norm: every token's write is known to 2^-22 of itself and 2^-27 of the column's largest
+    value, errors of either sign in 128 keys and of some tens of tokens that the state still holds: below 2^-20."""
+    x = Layer(sc, ops, 14, 128, 2, 4, [2050], dtype)
+    x.v, x.v64 = act(x.v64 * np.exp2(-np.arange(128) / 16), dtype)   # columns of other sizes
+    x.build().launch()
+    sc.device_sync()
+    _, M = x.read()
+    for h in range(x.vh):
+        _, want = plain.delta_rule(x.M[0, h], x.q64[:, h // 2], x.k64[:, h // 2], x.v64[:, h], x.g[:, h], x.beta[:, h], x.scale, True, x.eps)
+        err = np.linalg.norm(M[0, h] - want, axis=0) / np.linalg.norm(want, axis=0)
+        assert err.max() <= 2.0 ** -20, (h, err.max())
+
+
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
 @pytest.mark.parametrize("by", [2.0 ** -9, 2.0 ** 9])
 def test_small_and_large_values(sc, ops, plain, cuda, by, dtype):
     """The rule is linear in its values and its state: results keep their accuracy whatever their size."""
