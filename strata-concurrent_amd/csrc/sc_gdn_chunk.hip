@@ -6,10 +6,10 @@
 //     M1 = e^(G_C) M0 + sum_j e^(G_C - G_j) k_j u_j^T
 // Everything but M0 is known beforehand, so a first kernel forms T = (1 + A)^-1 and P of every chunk at once, and a second
 // one takes the chunks of a sequence in order with products only.  Columns of the state (values) do not meet: a workgroup
-// of the second kernel takes 16 of them with four waves.  Two carry the state, half the keys each, in their registers: a
+// of the second kernel takes 16 or 32 of them with four waves.  Two carry the state, half the keys each, in their registers: a
 // result of a product (column = lane % 16, rows in registers) is the right operand of the next one as it stands, so nothing
-// crosses lanes but a column's largest value, and only the two halves of K M0 are exchanged.  The two others are a chunk
-// behind and form the outputs from the state and U that the first left in LDS; they also bring V, T and the factors of rows.
+// crosses lanes but a column's largest value, and only parts of K M0 are exchanged.  The two others form the outputs from
+// the state and U that the first left in LDS; they also bring V, T and the factors of rows.
 //
 // Accuracy: the products run as f16 matrix instructions with sums in 32 bits, and keep f32 accuracy: an f32 operand is
 // two f16 parts (22 bits).  f16 keys and queries enter as they are, exactly, f32 ones scaled by row with a power of two;
@@ -128,6 +128,26 @@ __device__ __forceinline__ bool seq_of(const GdnArgs& a, uint32_t lane, Find fin
         chunks += last_lane(sum);
     }
     return false;
+}
+// The sequence that has the place `rank` by its chunks of [c0, c1), most first: the longest begin first, so that no long one
+// is left to run alone at the end.  Batches of more than 64 are taken as they come.
+__device__ __forceinline__ bool seq_of_rank(const GdnArgs& a, uint32_t lane, uint32_t rank, uint32_t c0, uint32_t c1, Seq& q) {
+    if (a.n_seqs > 64) return seq_of(a, lane, [&](uint32_t s, uint32_t, uint32_t) { return s == rank; }, q);
+    const bool in = lane < a.n_seqs;
+    const uint32_t t0 = in ? rows_from(a, lane) : 0u, t1 = in ? rows_from(a, lane + 1) : 0u;
+    const uint32_t n = t1 > t0 ? (t1 - t0 + kC - 1) / kC : 0u, hi = scan_add(n), lo = hi - n;
+    const uint32_t from = lo > c0 ? lo : c0, to = hi < c1 ? hi : c1;
+    const uint32_t key = in ? (from < to ? to - from : 0u) * 64 + 64 - lane : 0u;
+    uint32_t before = 0;
+    for (uint32_t i = 0; i < a.n_seqs; ++i) before += uint32_t(__builtin_amdgcn_readlane(int(key), int(i))) > key;
+    const uint64_t here = __ballot(in && before == rank);
+    if (!here) return false;
+    const int at = __builtin_ctzll(here);
+    q.s = uint32_t(at);
+    q.t0 = __builtin_amdgcn_readlane(t0, at);
+    q.t1 = __builtin_amdgcn_readlane(t1, at);
+    q.chunk0 = __builtin_amdgcn_readlane(lo, at);
+    return true;
 }
 
 // ---- every chunk's T and P ------------------------------------------------------------------------------------------------
@@ -468,12 +488,14 @@ __global__ void __launch_bounds__(kThreadsC, 3) gdn_prepare_kernel(GdnArgs a, Ch
 
 // ---- the chunks of a sequence in order ------------------------------------------------------------------------------------
 
-// The columns of the state of a workgroup of the second kernel
-constexpr int kCols = 16;
-// Its waves: the state's keys are shared by two where there are 64 or more, two others form the outputs.
+// Waves of a workgroup of the second kernel: the state's keys are shared by two where there are 64 or more, two others form
+// the outputs.
 template <int S>
 constexpr int kStateWaves = S >= 64 ? 2 : 1;
 constexpr int kOutWaves = 2;
+
+template <class T>
+__device__ __forceinline__ T pick(bool first, T a, T b) { return first ? a : b; }
 
 template <int kSteps>
 __device__ __forceinline__ float most_of(const f32x4 (&m)[kSteps][2]) {
@@ -511,44 +533,45 @@ __device__ __forceinline__ void split_state(const f32x4 (&m)[2], ops_u32x4& hi, 
     split_pair(f32x4{m[0].x, m[1].x, m[0].y, m[1].y}, f32x4{m[0].z, m[1].z, m[0].w, m[1].w}, hi, lo);
 }
 
-template <int S, bool kF16>
+// kN tiles of 16 columns.  With one, both waves of the state form U from the whole of K M0; with two, each forms the one of
+// its tile and they exchange what the update needs.
+template <int S, int kN, bool kF16>
 __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chunk_kernel(GdnArgs a, ChunkArgs c) {
     constexpr int kParts = kF16 ? 1 : 2, kSteps = S / 32, kShares = kStateWaves<S>, kMine = kSteps / kShares;
-    constexpr uint32_t kThreads = (kShares + kOutWaves) * 64;
+    static_assert(kN == 1 || kShares == 2);
+    constexpr uint32_t kCols = kN * 16, kThreads = (kShares + kOutWaves) * 64;
     constexpr uint32_t kBytes = kF16 ? 2 : 4;                            // of an activation
     constexpr uint32_t kRowV = kCols * kBytes, kPieces = kRowV / 16;     // a row of V or O of this workgroup, in 16-byte pieces
     constexpr uint32_t kEach = kC * kPieces / (kOutWaves * 64);          // pieces of a lane
-    // what the state's waves leave for the others, by the chunk's parity
-    struct Left {
-        ops_u32x4 m[kSteps][2][64], u[2][2][64];   // the state before the chunk and U as right operands: [step][part]
-        int up[16];                                // the power of two that a column of both is to be scaled up by
-    };
-    // and the others for them
-    struct Values {
-        f32x4 v[4][64];                            // beta V as results lie: [tile][lane]
-        float most[kOutWaves][16];                 // its largest magnitude by column, of two tiles each
-        ops_u32x4 t[6][2][64];                     // T
-    };
-    __shared__ Left s_left[2];
-    __shared__ Values s_values[2];
-    __shared__ __align__(16) uint8_t s_vin[kC * kRowV], s_out[kC * kRowV];
-    __shared__ __align__(16) float s_f[3][(kFactors + 63) / 64 * 64];
-    __shared__ f32x4 s_km[kShares][4][64];         // K M0 by a wave's keys
-    __shared__ float s_top[kShares][16];           // the largest of a wave's state by column
+    // where registers are few, the keys' second form is asked for within its chunk and the first one at its end
+    constexpr bool kAhead = kF16;
+    // Right operands are [tile][step][part][lane], results [tile of columns][tile of rows][lane].  A barrier opens a chunk and
+    // another is in its middle; what lies here is written in one half and read in the other, or the next chunk's first.
+    __shared__ ops_u32x4 s_m[kN][kSteps][2][64];              // the state before the chunk: first half, second
+    __shared__ ops_u32x4 s_u[kN][2][2][64];                   // U: second half, first
+    __shared__ f32x4 s_v[kN][4][64];                          // beta V: first half, second
+    __shared__ ops_u32x4 s_t[6][2][64];                       // T: first half, second
+    __shared__ f32x4 s_km[kShares][4][64];                    // K M0 by a wave's keys: first half, second
+    __shared__ ops_u32x4 s_w[kN == 1 ? 1 : kN][2][2][64];     // U weighted for the state, with two tiles
+    __shared__ __align__(16) uint8_t s_stage[kOutWaves][32 * kRowV];   // a wave's rows of V or O on their way
+    __shared__ __align__(16) float s_f[2][(kFactors + 63) / 64 * 64];  // factors of rows: second half, all of the next and its next first
+    __shared__ int s_up[kN][16];                              // the power of two by which a column's m and u are to be scaled up
+    __shared__ float s_most[kOutWaves][kN][16];               // the largest of beta V by column: second half, first
+    __shared__ float s_top[kShares][kN][16];                  // the largest of a wave's state by column: second half, first
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t g = lane >> 4, col = lane & 15;
     // workgroups go to the eight XCDs in turn: the column blocks of a head are kept on one, whose L2 has its operands
     constexpr uint32_t kBlocks = S / kCols;
     const uint32_t within = blockIdx.x / 8, head = within / kBlocks * 8 + blockIdx.x % 8, block = within % kBlocks;
     if (head >= a.n_seqs * a.v_heads) return;
-    const uint32_t seq = head / a.v_heads, h = head - seq * a.v_heads, kh = ops_div(h, a.share);
+    const uint32_t rank = head / a.v_heads, h = head - rank * a.v_heads, kh = ops_div(h, a.share);
     Seq q;
-    if (!seq_of(a, lane, [&](uint32_t s, uint32_t, uint32_t) { return s == seq; }, q)) return;
+    if (!seq_of_rank(a, lane, rank, c.first, c.first + c.count, q)) return;
     // this launch's chunks of the sequence
     const uint32_t all = q.t1 > q.t0 ? (q.t1 - q.t0 + kC - 1) / kC : 0u;
     const uint32_t c0 = q.chunk0 > c.first ? q.chunk0 : c.first, c1 = q.chunk0 + all < c.first + c.count ? q.chunk0 + all : c.first + c.count;
     if (c0 >= c1) return;
-    float* base = a.state[seq];
+    float* base = a.state[q.s];
     if (!base) {
         const uint32_t from = q.t0 + (c0 - q.chunk0) * kC, to = q.t0 + (c1 - q.chunk0) * kC < q.t1 ? q.t0 + (c1 - q.chunk0) * kC : q.t1;
         for (uint32_t t = from + tid / (kCols / 4); t < to; t += kThreads / (kCols / 4))
@@ -566,6 +589,13 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
     auto clamped = [&](uint32_t chunk) { return chunk < c1 ? chunk : c1 - 1; };
     auto operands_of = [&](uint32_t chunk) { return c.chunks + (uint64_t(chunk - c.first) * a.v_heads + h) * kChunkWords; };
     auto rows_of = [&](uint32_t chunk) { return c.rows + (uint64_t(chunk - c.first) * c.k_heads + kh) * kRowWords<S, kParts>; };
+    // Operand `word / 64` of a key head's: the lane's offset holds what an instruction's own offset cannot, a scalar address
+    // each would take more scalar registers than there are.
+    auto row_word = [&](const ops_u32x4* from, uint32_t word) {
+        uint32_t at = lane * 16 + (word / 512 * 8 + 4) * 1024;
+        asm("" : "+v"(at));
+        return reinterpret_cast<const uint8_t*>(from) + at + (int(word / 64 % 8) - 4) * 1024;
+    };
     // a tile of keys or queries as left operands, N steps from `first` on
     auto load_rows = [&](auto& x, uint32_t chunk, uint32_t which, uint32_t tile, uint32_t first) {
         constexpr int N = sizeof(x[0]) / sizeof(x[0][0]);
@@ -576,20 +606,12 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
 #pragma unroll
             for (int i = 0; i < N; ++i) x[0][i] = ld_global<ops_u32x4>(p + at + i * 64);
         } else {
-            const ops_u32x4* p = rows_of(chunk) + lane;
+            const ops_u32x4* p = rows_of(chunk) + (tile * kSteps + first) * 64;
 #pragma unroll
             for (int part = 0; part < kParts; ++part)
 #pragma unroll
-                for (int i = 0; i < N; ++i) x[part][i] = ld_global<ops_u32x4>(p + row_operand<S, kParts>(which, part, tile, first + i));
+                for (int i = 0; i < N; ++i) x[part][i] = ld_global<ops_u32x4>(row_word(p, row_operand<S, kParts>(which, part, 0, i)));
         }
-    };
-    // n of P's six operands (operand_at's order) from `first` on, in two parts
-    auto load_operand = [&](auto& x, int at, int n, uint32_t chunk, uint32_t first) {
-        const ops_u32x4* p = operands_of(chunk) + kOperand + first * 128 + lane;
-#pragma unroll
-        for (int i = 0; i < n; ++i)
-#pragma unroll
-            for (int part = 0; part < 2; ++part) x[at + i][part] = ld_global<ops_u32x4>(p + i * 128 + part * 64);
     };
     // the product of n operands of a row tile from `first` on with a right operand [step][part]
     auto triangle = [&](const auto& x, int first, int n, const ops_u32x4 (&y)[2][2]) {
@@ -604,22 +626,30 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
     };
 
     if (wave < kShares) {
-        // the state: keys 32 (first + i) + 8 g + 2 j + e in m[i][e][j], a column a lane
+        // the state: keys 32 (first + i) + 8 g + 2 j + e in m[b][i][e][j], a column a lane
         const uint32_t first = wave * kMine;
         float* state = base + a.state_offset + h * a.head_ld + block * kCols + col + (first * 32 + g * 8) * a.key_ld;
-        f32x4 m[kMine][2];
+        f32x4 m[kN][kMine][2];
 #pragma unroll
-        for (int i = 0; i < kMine; ++i)
+        for (int b = 0; b < kN; ++b)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int i = 0; i < kMine; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) m[i][e][j] = ld_global<float>(state + (i * 32 + 2 * j + e) * a.key_ld);
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) m[b][i][e][j] = ld_global<float>(state + (i * 32 + 2 * j + e) * a.key_ld + b * 16);
         // waited for here: the loop would wait for it every time around
 #pragma unroll
-        for (int i = 0; i < kMine; ++i) asm volatile("" : "+v"(m[i][0]), "+v"(m[i][1]));
+        for (int b = 0; b < kN; ++b)
+#pragma unroll
+            for (int i = 0; i < kMine; ++i) asm volatile("" : "+v"(m[b][i][0]), "+v"(m[b][i][1]));
         ops_u32x4 k[4][kParts][kMine], kt[kParts][kMine][2][2];
         auto load_keys = [&](uint32_t chunk) {
-            const ops_u32x4* p = rows_of(chunk) + lane;
+#pragma unroll
+            for (int r = 0; r < 4; ++r) load_rows(k[r], chunk, 0, r, first);
+        };
+        auto load_turned = [&](uint32_t chunk) {
+            const ops_u32x4* p = rows_of(chunk) + first * 256;
 #pragma unroll
             for (int part = 0; part < kParts; ++part)
 #pragma unroll
@@ -627,93 +657,126 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
 #pragma unroll
                     for (int e = 0; e < 2; ++e)
 #pragma unroll
-                        for (int step = 0; step < 2; ++step) kt[part][i][e][step] = ld_global<ops_u32x4>(p + key_operand<S, kParts>(part, first + i, e, step));
+                        for (int step = 0; step < 2; ++step) kt[part][i][e][step] = ld_global<ops_u32x4>(row_word(p, key_operand<S, kParts>(part, i, e, step)));
         };
-#pragma unroll
-        for (int r = 0; r < 4; ++r) load_rows(k[r], c0, 0, r, first);
         load_keys(c0);
-        int up = 0;   // a column's state is m times 2^up
-        float top = most_of<kMine>(m);
-        if (g == 0) s_top[wave][col] = top;
+        if (kAhead) load_turned(c0);
+        int up[kN];   // a column's state is m times 2^up
+#pragma unroll
+        for (int b = 0; b < kN; ++b) {
+            up[b] = 0;
+            const float top = most_of<kMine>(m[b]);
+            if (g == 0) s_top[wave][b][col] = top;
+        }
         for (uint32_t chunk = c0; chunk < c1; ++chunk) {
-            const uint32_t which = (chunk - c0) & 1, ahead = clamped(chunk + 1);
-            Left& left = s_left[which];
-            __syncthreads();   // V and the factors are here, and the outputs of the chunk before the last are done
-            const float* f = s_f[(chunk - c0) % 3];
-            const Values& values = s_values[which];
+            const uint32_t ahead = clamped(chunk + 1);
+            __syncthreads();
+            const float* f = s_f[(chunk - c0) & 1];
             // the state as a right operand
-            ops_u32x4 mh[kMine], ml[kMine];
-            float down;
-            if constexpr (kShares > 1) top = fmaxf(s_top[0][col], s_top[kShares - 1][col]);
-            fit_scale<kMine>(m, up, down, top, fmaxf(values.most[0][col], values.most[1][col]), fmaxf(f[kFBetaMost], 1.0f));
+            ops_u32x4 mh[kN][kMine], ml[kN][kMine];
+            float down[kN];
+            const float beta_most = fmaxf(f[kFBetaMost], 1.0f);
 #pragma unroll
-            for (int i = 0; i < kMine; ++i) {
-                split_state(m[i], mh[i], ml[i]);
-                left.m[first + i][0][lane] = mh[i];
-                left.m[first + i][1][lane] = ml[i];
+            for (int b = 0; b < kN; ++b) {
+                fit_scale<kMine>(m[b], up[b], down[b], fmaxf(s_top[0][b][col], s_top[kShares - 1][b][col]),
+                                 fmaxf(s_most[0][b][col], s_most[1][b][col]), beta_most);
+#pragma unroll
+                for (int i = 0; i < kMine; ++i) {
+                    split_state(m[b][i], mh[b][i], ml[b][i]);
+                    s_m[b][first + i][0][lane] = mh[b][i];
+                    s_m[b][first + i][1][lane] = ml[b][i];
+                }
+                if (wave == 0 && g == 0) s_up[b][col] = up[b];
             }
-            if (wave == 0 && g == 0) left.up[col] = up;
             // K M0
-            f32x4 km[4];
+            f32x4 km[kN][4];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) km[r] = f32x4{};
+            for (int b = 0; b < kN; ++b)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) km[b][r] = f32x4{};
 #pragma unroll
             for (int i = 0; i < kMine; ++i)
 #pragma unroll
                 for (int x = 0; x < kParts + 1; ++x)   // high by high, high by low, low by high
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) km[r] = mfma(k[r][x == 2][i], x == 1 ? ml[i] : mh[i], km[r]);
+                    for (int r = 0; r < 4; ++r)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) load_rows(k[r], ahead, 0, r, first);
+                        for (int b = 0; b < kN; ++b) km[b][r] = mfma(k[r][x == 2][i], x == 1 ? ml[b][i] : mh[b][i], km[b][r]);
+            if (kAhead) load_keys(ahead);
+            else load_turned(chunk);
+            // with one tile each wave's part goes to the other, with two the part of the other's tile
+            const uint32_t tile = kN == 1 ? 0 : wave;
             if constexpr (kShares > 1) {
 #pragma unroll
-                for (int r = 0; r < 4; ++r) s_km[wave][r][lane] = km[r];
-                __syncthreads();
+                for (int r = 0; r < 4; ++r) s_km[wave][r][lane] = kN == 1 ? f32x4(km[0][r]) : pick(wave, km[0][r], km[kN - 1][r]);
+            }
+            __syncthreads();
 #pragma unroll
-                for (int r = 0; r < 4; ++r) km[r] += s_km[wave ^ 1][r][lane];   // the same sum in both waves
+            for (int r = 0; r < 4; ++r) {
+                if (kN > 1) km[0][r] = pick(wave, km[kN - 1][r], km[0][r]);
+                if constexpr (kShares > 1) km[0][r] += s_km[wave ^ 1][r][lane];   // the same sum in both waves
             }
             // X; rows past the sequence's end are zero, as their V and factors are
             ops_u32x4 xs[2][2];
             {
+                const float by = kN == 1 ? float(down[0]) : pick(wave, down[kN - 1], down[0]);
                 f32x4 x[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const f32x4 fs = *reinterpret_cast<const f32x4*>(&f[kFState + r * 16 + g * 4]), v = values.v[r][lane];
+                    const f32x4 fs = *reinterpret_cast<const f32x4*>(&f[kFState + r * 16 + g * 4]), v = s_v[tile][r][lane];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) x[r][j] = __builtin_fmaf(-fs[j], km[r][j], v[j] * down);
+                    for (int j = 0; j < 4; ++j) x[r][j] = __builtin_fmaf(-fs[j], km[0][r][j], v[j] * by);
                 }
                 split_pair(x[0], x[1], xs[0][0], xs[0][1]);
                 split_pair(x[2], x[3], xs[1][0], xs[1][1]);
             }
             // U = T X, and the same weighted for the state
-            ops_u32x4 ws[2][2];
+            ops_u32x4 ws[kN][2][2];
             {
-                ops_u32x4 t[6][2];
+                f32x4 u[4];
 #pragma unroll
-                for (int i = 0; i < 6; ++i)
+                for (int r = 0; r < 4; ++r) {
+                    const int n = 1 + r / 2, from = r < 2 ? r : r * 2 - 2;
+                    ops_u32x4 t[2][2];
 #pragma unroll
-                    for (int part = 0; part < 2; ++part) t[i][part] = values.t[i][part][lane];
-                f32x4 u[4]{triangle(t, 0, 1, xs), triangle(t, 1, 1, xs), triangle(t, 2, 2, xs), triangle(t, 4, 2, xs)};
+                    for (int i = 0; i < n; ++i)
+#pragma unroll
+                        for (int part = 0; part < 2; ++part) t[i][part] = s_t[from + i][part][lane];
+                    u[r] = triangle(t, 0, n, xs);
+                    if (!kAhead) asm volatile("" ::: "memory");   // not all of T at once
+                }
 #pragma unroll
                 for (int step = 0; step < 2; ++step) {
                     const f32x4 w0 = *reinterpret_cast<const f32x4*>(&f[kFWrite + step * 32 + g * 4]), w1 = *reinterpret_cast<const f32x4*>(&f[kFWrite + step * 32 + 16 + g * 4]);
-                    split_pair(u[step * 2], u[step * 2 + 1], w0, w1, ws[step][0], ws[step][1]);
-                    if (kShares == 1 || uint32_t(step) == wave) {
+                    split_pair(u[step * 2], u[step * 2 + 1], w0, w1, ws[0][step][0], ws[0][step][1]);
+                    if (kN > 1) s_w[tile][step][0][lane] = ws[0][step][0], s_w[tile][step][1][lane] = ws[0][step][1];
+                    if (kN > 1 || kShares == 1 || uint32_t(step) == wave) {
                         ops_u32x4 hi, lo;
                         split_pair(u[step * 2], u[step * 2 + 1], hi, lo);
-                        left.u[step][0][lane] = hi;
-                        left.u[step][1][lane] = lo;
+                        s_u[tile][step][0][lane] = hi;
+                        s_u[tile][step][1][lane] = lo;
                     }
                 }
+            }
+            if constexpr (kN > 1) {
+                __syncthreads();
+#pragma unroll
+                for (int b = 0; b < kN; ++b)
+#pragma unroll
+                    for (int step = 0; step < 2; ++step)
+#pragma unroll
+                        for (int part = 0; part < 2; ++part) ws[b][step][part] = s_w[b][step][part][lane];
             }
             // the state after the chunk
             const float decay = f[kFDecay], w_up = f[kFUp];
             const bool plain = __builtin_amdgcn_readfirstlane(int(w_up == 1.0f));   // nearly always
 #pragma unroll
-            for (int i = 0; i < kMine; ++i)
+            for (int b = 0; b < kN; ++b)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) m[i][e] *= decay;
-            auto update = [&](f32x4 (&add)[kMine][2]) {
+                for (int i = 0; i < kMine; ++i)
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) m[b][i][e] *= decay;
+            auto update = [&](f32x4 (&add)[kN][kMine][2]) {
 #pragma unroll
                 for (int step = 0; step < 2; ++step)
 #pragma unroll
@@ -721,49 +784,61 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
 #pragma unroll
                         for (int i = 0; i < kMine; ++i)
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) add[i][e] = mfma(kt[x == 2][i][e][step], ws[step][x == 1], add[i][e]);
+                            for (int e = 0; e < 2; ++e)
+#pragma unroll
+                                for (int b = 0; b < kN; ++b) add[b][i][e] = mfma(kt[x == 2][i][e][step], ws[b][step][x == 1], add[b][i][e]);
             };
             if (plain) {
                 update(m);
             } else {
-                f32x4 add[kMine][2]{};
+                f32x4 add[kN][kMine][2]{};
                 update(add);
 #pragma unroll
-                for (int i = 0; i < kMine; ++i)
+                for (int b = 0; b < kN; ++b)
 #pragma unroll
-                    for (int e = 0; e < 2; ++e) m[i][e] += w_up * add[i][e];
+                    for (int i = 0; i < kMine; ++i)
+#pragma unroll
+                        for (int e = 0; e < 2; ++e) m[b][i][e] += w_up * add[b][i][e];
             }
-            load_keys(ahead);
-            top = most_of<kMine>(m);
-            if (g == 0) s_top[wave][col] = top;
+            if (kAhead) load_turned(ahead);
+            else load_keys(ahead);
+#pragma unroll
+            for (int b = 0; b < kN; ++b) {
+                const float top = most_of<kMine>(m[b]);
+                if (g == 0) s_top[wave][b][col] = top;
+            }
         }
         __syncthreads();   // the last chunk's outputs
 #pragma unroll
-        for (int i = 0; i < kMine; ++i)
+        for (int b = 0; b < kN; ++b)
 #pragma unroll
-            for (int e = 0; e < 2; ++e)
+            for (int i = 0; i < kMine; ++i)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    st_global<float>(state + (i * 32 + 2 * j + e) * a.key_ld, __builtin_amdgcn_ldexpf(m[i][e][j], up));
+                for (int e = 0; e < 2; ++e)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        st_global<float>(state + (i * 32 + 2 * j + e) * a.key_ld + b * 16, __builtin_amdgcn_ldexpf(m[b][i][e][j], up[b]));
         return;
     }
 
-    // The other waves: V, T and the factors of the chunk after the next, outputs of the chunk before.  Wave w of the two takes
-    // V's tiles 2 w and 2 w + 1 and the outputs' w and 3 - w, which have three operands of P's six.
+    // The other waves: V, T and the factors, and the outputs, whose part from U is formed a chunk behind.  Wave w of the two
+    // takes the row tiles w and 3 - w, which have three operands of P's six.
     const uint32_t w = wave - kShares, v_ld = uint32_t(a.v_ld);
+    uint8_t* stage = s_stage[w];
+    auto tile_of = [&](uint32_t i) { return i ? 3 - w : w; };
+    auto row_at = [&](uint32_t at) { return tile_of(at / (16 * kPieces)) * 16 + at / kPieces % 16; };   // of piece `at` of the wave's rows
     ops_u32x4 v_in[kEach], t_in[6];
     float f_in[4];
+    f32x4 v[kN][2];
     auto factor_at = [&](uint32_t i) { return (i == 0 ? 1 : w ? i + 2 : (i - 1) * 2) * 64 + lane; };   // both have kFBeta's
     auto load_early = [&](uint32_t chunk) {
         const uint32_t last = last_row(chunk) * v_ld;
         const uint8_t* p = a.v + int64_t(q.t0 + (chunk - q.chunk0) * kC) * a.v_ld + (h * S + block * kCols) * kBytes;
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i) {
-            const uint32_t at = lane + (w * kEach + i) * 64;
-            v_in[i] = ld_global<ops_u32x4>(p + min(at / kPieces * v_ld, last) + at % kPieces * 16);
+            const uint32_t at = lane + i * 64;
+            v_in[i] = ld_global<ops_u32x4>(p + min(row_at(at) * v_ld, last) + at % kPieces * 16);
         }
-#pragma unroll
-        for (int i = 0; i < 6; ++i) t_in[i] = ld_global<ops_u32x4>(operands_of(chunk) + (w * 6 + i) * 64 + lane);
         const float* f = reinterpret_cast<const float*>(operands_of(chunk) + 2 * kOperand);
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) f_in[i] = ld_global<float>(f + min(factor_at(i), uint32_t(kFactors - 1)));
@@ -771,111 +846,160 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
     // V as the state's waves take it, by way of LDS: times beta, rows past the sequence's end zero, a lane's four rows together
     auto put_early = [&](uint32_t chunk, uint32_t n) {
         const uint32_t last = last_row(chunk);
-        float* f = s_f[n % 3];
-        Values& to = s_values[n & 1];
+        float* f = s_f[n & 1];
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i) {
-            const uint32_t at = lane + (w * kEach + i) * 64;
-            *reinterpret_cast<ops_u32x4*>(&s_vin[at * 16]) = at / kPieces <= last ? v_in[i] : ops_u32x4{};
+            const uint32_t at = lane + i * 64;
+            *reinterpret_cast<ops_u32x4*>(&stage[at * 16]) = row_at(at) <= last ? v_in[i] : ops_u32x4{};
         }
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) f[factor_at(i)] = f_in[i];
         wave_sync();
-        float top = 0;
 #pragma unroll
-        for (uint32_t i = 0; i < 2; ++i) {
-            const uint32_t row = (w * 2 + i) * 16 + g * 4;
-            f32x4 v = *reinterpret_cast<const f32x4*>(&f[kFBeta + row]);
+        for (int b = 0; b < kN; ++b) {
+            float top = 0;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint8_t* p = &s_vin[(row + j) * kRowV + col * kBytes];
-                if constexpr (kF16) v[j] *= float(*reinterpret_cast<const _Float16*>(p));
-                else v[j] *= *reinterpret_cast<const float*>(p);
-                top = fmaxf(top, fabsf(v[j]));
+            for (uint32_t i = 0; i < 2; ++i) {
+                f32x4 x = *reinterpret_cast<const f32x4*>(&f[kFBeta + tile_of(i) * 16 + g * 4]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint8_t* p = &stage[(i * 16 + g * 4 + j) * kRowV + (b * 16 + col) * kBytes];
+                    if constexpr (kF16) x[j] *= float(*reinterpret_cast<const _Float16*>(p));
+                    else x[j] *= *reinterpret_cast<const float*>(p);
+                    top = fmaxf(top, fabsf(x[j]));
+                }
+                v[b][i] = x;
             }
-            to.v[w * 2 + i][lane] = v;
+            top = over_rows(top, max_of);
+            if (g == 0) s_most[w][b][col] = top;
         }
-        top = over_rows(top, max_of);
-        if (g == 0) to.most[w][col] = top;
-#pragma unroll
-        for (uint32_t i = 0; i < 6; ++i) to.t[(w * 6 + i) / 2][i % 2][lane] = t_in[i];
         wave_sync();
+    };
+    auto load_t = [&](uint32_t chunk) {
+#pragma unroll
+        for (int i = 0; i < 6; ++i) t_in[i] = ld_global<ops_u32x4>(operands_of(chunk) + (w * 6 + i) * 64 + lane);
     };
     ops_u32x4 qs[2][kParts][kSteps], p[3][2];
-    auto load_ahead = [&](uint32_t chunk) {
+    auto load_queries = [&](uint32_t chunk) {
         load_rows(qs[0], chunk, 1, w, 0);
         load_rows(qs[1], chunk, 1, 3 - w, 0);
-        load_operand(p, 0, 1, chunk, w);
-        load_operand(p, 1, 2, chunk, 4 - 2 * w);
     };
-    auto outputs = [&](uint32_t done) {
-        const uint32_t n = done - c0;
-        const uint32_t last = last_row(done);
-        const Left& left = s_left[n & 1];
-        const float* f = s_f[n % 3];
-        f32x4 qm[2]{};
+    // P's operand w, and the two of tile 3 - w
+    auto load_p = [&](uint32_t chunk) {
+        const ops_u32x4* from = operands_of(chunk) + kOperand + lane;
 #pragma unroll
-        for (int i = 0; i < kSteps; ++i) {
-            const ops_u32x4 hi = left.m[i][0][lane], lo = left.m[i][1][lane];
+        for (int i = 0; i < 3; ++i)
 #pragma unroll
-            for (int x = 0; x < kParts + 1; ++x)
-#pragma unroll
-                for (int r = 0; r < 2; ++r) qm[r] = mfma(qs[r][x == 2][i], x == 1 ? lo : hi, qm[r]);
-        }
-        ops_u32x4 us[2][2];
-#pragma unroll
-        for (int step = 0; step < 2; ++step)
-#pragma unroll
-            for (int part = 0; part < 2; ++part) us[step][part] = left.u[step][part][lane];
-        const int up = left.up[col];
-#pragma unroll
-        for (int r = 0; r < 2; ++r) {
-            const uint32_t row = (r ? 3 - w : w) * 16 + g * 4;
-            const f32x4 sum = r ? triangle(p, 1, 2, us) : triangle(p, 0, 1, us);
-            const f32x4 fq = *reinterpret_cast<const f32x4*>(&f[kFQuery + row]), fr = *reinterpret_cast<const f32x4*>(&f[kFRow + row]);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float o = __builtin_amdgcn_ldexpf(fq[j] * qm[r][j] + fr[j] * sum[j], up);
-                uint8_t* to = &s_out[(row + j) * kRowV + col * kBytes];
-                if constexpr (kF16) *reinterpret_cast<_Float16*>(to) = _Float16(o);
-                else *reinterpret_cast<float*>(to) = o;
-            }
-        }
-        load_ahead(clamped(done + 1));
-        wave_sync();
-        uint8_t* to = a.out + int64_t(q.t0 + (done - q.chunk0) * kC) * a.out_ld + (h * S + block * kCols) * kBytes;
-#pragma unroll
-        for (uint32_t i = 0; i < kEach; ++i) {
-            const uint32_t at = lane + i * 64, half = at / (16 * kPieces), row = (half ? 3 - w : w) * 16 + at / kPieces % 16;
-            if (row <= last) st_global<ops_u32x4>(to + int64_t(row) * a.out_ld + at % kPieces * 16, *reinterpret_cast<const ops_u32x4*>(&s_out[row * kRowV + at % kPieces * 16]));
-        }
-        wave_sync();
+            for (int part = 0; part < 2; ++part) p[i][part] = ld_global<ops_u32x4>(from + ((i == 0 ? w : 3 - 2 * w + i) * 2 + part) * 64);
     };
-    // before a chunk's second barrier the state's waves read the places of that chunk
-    auto meet = [&](uint32_t chunk) {
+    f32x4 qm[kN][2];
+    int up[kN];
+    auto first_half = [&](uint32_t chunk) {
+#pragma unroll
+        for (int b = 0; b < kN; ++b)
+#pragma unroll
+            for (uint32_t i = 0; i < 2; ++i) s_v[b][tile_of(i)][lane] = v[b][i];
+#pragma unroll
+        for (uint32_t i = 0; i < 6; ++i) s_t[(w * 6 + i) / 2][i % 2][lane] = t_in[i];
+        load_t(clamped(chunk + 1));
+    };
+    auto second_half = [&](uint32_t chunk) {
         __syncthreads();
+#pragma unroll
+        for (int b = 0; b < kN; ++b)
+#pragma unroll
+            for (int r = 0; r < 2; ++r) qm[b][r] = f32x4{};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int b = 0; b < kN; ++b) {
+                const ops_u32x4 hi = s_m[b][i][0][lane], lo = s_m[b][i][1][lane];
+#pragma unroll
+                for (int x = 0; x < kParts + 1; ++x)
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) qm[b][r] = mfma(qs[r][x == 2][i], x == 1 ? lo : hi, qm[b][r]);
+            }
+#pragma unroll
+        for (int b = 0; b < kN; ++b) up[b] = s_up[b][col];
+        load_queries(clamped(chunk + 1));
+        if constexpr (kN > 1) __syncthreads();
         put_early(clamped(chunk + 1), chunk + 1 - c0);
         load_early(clamped(chunk + 2));
-        if constexpr (kShares > 1) __syncthreads();
+    };
+    auto outputs = [&](uint32_t done) {
+        const uint32_t last = last_row(done);
+        const float* f = s_f[(done - c0) & 1];
+#pragma unroll
+        for (int b = 0; b < kN; ++b) {
+            ops_u32x4 us[2][2];
+#pragma unroll
+            for (int step = 0; step < 2; ++step)
+#pragma unroll
+                for (int part = 0; part < 2; ++part) us[step][part] = s_u[b][step][part][lane];
+#pragma unroll
+            for (uint32_t r = 0; r < 2; ++r) {
+                const f32x4 sum = r ? triangle(p, 1, 2, us) : triangle(p, 0, 1, us);
+                const uint32_t row = tile_of(r) * 16 + g * 4;
+                const f32x4 fq = *reinterpret_cast<const f32x4*>(&f[kFQuery + row]), fr = *reinterpret_cast<const f32x4*>(&f[kFRow + row]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float o = __builtin_amdgcn_ldexpf(fq[j] * qm[b][r][j] + fr[j] * sum[j], up[b]);
+                    uint8_t* to = &stage[(r * 16 + g * 4 + j) * kRowV + (b * 16 + col) * kBytes];
+                    if constexpr (kF16) *reinterpret_cast<_Float16*>(to) = _Float16(o);
+                    else *reinterpret_cast<float*>(to) = o;
+                }
+            }
+        }
+        load_p(clamped(done + 1));
+        wave_sync();
+        uint8_t* to = a.out + int64_t(q.t0 + (done - q.chunk0) * kC) * a.out_ld + (h * S + block * kCols) * kBytes;
+        uint32_t o_ld = uint32_t(a.out_ld);
+        asm volatile("" : "+s"(o_ld));   // the rows' offsets formed here: kept, they would have to be read from memory
+#pragma unroll
+        for (uint32_t i = 0; i < kEach; ++i) {
+            const uint32_t at = lane + i * 64, row = row_at(at);
+            if (row <= last) st_global<ops_u32x4>(to + (row * o_ld + at % kPieces * 16), *reinterpret_cast<const ops_u32x4*>(&stage[at * 16]));
+        }
+        wave_sync();
     };
     load_early(c0);
+    load_t(c0);
     put_early(c0, 0);
+    load_queries(c0);
     load_early(clamped(c0 + 1));
-    meet(c0);
-    load_ahead(c0);
+    __syncthreads();
+    first_half(c0);
+    load_p(c0);
+    second_half(c0);
     for (uint32_t chunk = c0 + 1; chunk < c1; ++chunk) {
-        meet(chunk);
+        __syncthreads();
+        first_half(chunk);
         outputs(chunk - 1);
+        second_half(chunk);
     }
     __syncthreads();
     outputs(c1 - 1);
 }
 
+// Two tiles of columns a workgroup halve what a chunk's operands cost in reads (132 KB for f32, 72 for f16), one gives twice
+// as many workgroups, each with less to do between its barriers.  Measured in us for both kernels, sequences of 32 heads of
+// 128 and up to 1024 tokens, two tiles against one: f16 55 : 45 for one sequence, 62 : 65 for two, 97 : 129 for eight; f32
+// 67 : 52, 78 : 70, 83 : 82 for three, 151 : 178 for eight.  So two where that leaves three quarters of the chip's 256 units a
+// workgroup (f16), or two to each (f32).
+template <bool kF16>
+constexpr uint32_t kWideFrom = kF16 ? 192 : 512;
+
 template <int S, bool kF16>
 void launch_chunks(const GdnArgs& a, const ChunkArgs& c, hipStream_t stream) {
     const uint32_t heads = (a.n_seqs * a.v_heads + 7) / 8 * 8;
+    const dim3 threads((kStateWaves<S> + kOutWaves) * 64);
     hipLaunchKernelGGL((gdn_prepare_kernel<S, kF16>), dim3(c.count * a.v_heads), dim3(kThreadsC), 0, stream, a, c);
-    hipLaunchKernelGGL((gdn_chunk_kernel<S, kF16>), dim3(heads * (S / kCols)), dim3((kStateWaves<S> + kOutWaves) * 64), 0, stream, a, c);
+    if constexpr (S >= 64)
+        if (heads * (S / 32) >= kWideFrom<kF16>) {
+            hipLaunchKernelGGL((gdn_chunk_kernel<S, 2, kF16>), dim3(heads * (S / 32)), threads, 0, stream, a, c);
+            return;
+        }
+    hipLaunchKernelGGL((gdn_chunk_kernel<S, 1, kF16>), dim3(heads * (S / 16)), threads, 0, stream, a, c);
 }
 template <int S>
 hipError_t launch_of(const GdnArgs& a, const ChunkArgs& plan, bool f16, hipStream_t stream) {

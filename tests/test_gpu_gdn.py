@@ -105,11 +105,16 @@ CHUNKS = [
     (128, 16, 32, [61], "f32", "slot"), (128, 2, 4, [1, 0, 64, 65, 127, 128, 129], "f32", "prefill"),
     (128, 2, 4, [300, 1, 15, 16, 17], "f16", "slot"), (64, 4, 8, [33, 200, 2], "f32", "slot"), (64, 2, 2, [130], "f16", "prefill"),
     (32, 4, 8, [77, 64, 3], "f32", "slot"), (32, 1, 2, [200], "f16", "prefill"), (128, 1, 3, [500, 63], "f16", "slot"),
+    # enough heads for workgroups of 32 columns, and more sequences than a wave sorts
+    (128, 2, 4, [1, 0, 64, 65, 127, 128, 129, 33, 3, 200, 63, 66], "f16", "slot"),
+    (128, 4, 8, [1, 0, 64, 65, 127, 128, 129, 33, 3, 200, 63, 66, 2, 5, 70, 9], "f32", "prefill"),
+    (64, 8, 16, [70, 64, 1, 130, 0, 17], "f16", "prefill"), (64, 8, 16, [70, 64, 1, 130, 0, 17, 65, 2, 3, 4, 5, 6, 7, 8, 9, 60], "f32", "slot"),
+    (64, 1, 2, [5, 0, 66, 1, 64] * 14, "f32", "slot"), (64, 1, 4, [5, 0, 66, 1, 64] * 14, "f16", "slot"),
 ]
 
 
 @pytest.mark.parametrize("l2norm", [True, False], ids=["unit", "as-is"])
-@pytest.mark.parametrize("case", CHUNKS, ids=[f"S{c[0]}-{c[1]}-{c[2]}-{max(c[3])}-{c[4]}-{c[5]}" for c in CHUNKS])
+@pytest.mark.parametrize("case", CHUNKS, ids=[f"S{c[0]}-{c[1]}-{c[2]}-n{len(c[3])}-{max(c[3])}-{c[4]}-{c[5]}" for c in CHUNKS])
 def test_chunk_against_64_bits(sc, ops, plain, cuda, case, l2norm):
     S, kh, vh, lens, dtype, layout = case
     print(f"chunk {case}", flush=True)
