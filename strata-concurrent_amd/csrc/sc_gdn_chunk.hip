@@ -229,7 +229,11 @@ __global__ void __launch_bounds__(kThreadsC, 3) gdn_prepare_kernel(GdnArgs a, Ch
     __shared__ float s_beta[kC], s_fk[kC], s_kk[kC], s_up[kC], s_q[kWaves][5][16];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t g = lane >> 4, col = lane & 15;
-    const uint32_t piece = blockIdx.x / a.v_heads, h = blockIdx.x - piece * a.v_heads, kh = ops_div(h, a.share), chunk = c.first + piece;
+    // workgroups go to the eight XCDs in turn: the value heads of a key head are kept on one, whose L2 then has its rows
+    const uint32_t within = blockIdx.x / 8, group = ops_div(within, a.share) * 8 + blockIdx.x % 8;
+    const uint32_t piece = group / c.k_heads, kh = group - piece * c.k_heads, h = kh * a.share.d + within % a.share.d;
+    const uint32_t chunk = c.first + piece;
+    if (piece >= c.count) return;
     Seq q;
     if (!seq_of(a, lane, [&](uint32_t, uint32_t lo, uint32_t hi) { return chunk >= lo && chunk < hi; }, q)) return;
     const uint32_t t0 = q.t0 + (chunk - q.chunk0) * kC, n = q.t1 - t0 < kC ? q.t1 - t0 : kC;
@@ -560,11 +564,12 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
     __shared__ float s_top[kShares][kN][16];                  // the largest of a wave's state by column: second half, first
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t g = lane >> 4, col = lane & 15;
-    // workgroups go to the eight XCDs in turn: the column blocks of a head are kept on one, whose L2 has its operands
+    // workgroups go to the eight XCDs in turn: the column blocks of the value heads of a key head are kept on one
     constexpr uint32_t kBlocks = S / kCols;
-    const uint32_t within = blockIdx.x / 8, head = within / kBlocks * 8 + blockIdx.x % 8, block = within % kBlocks;
-    if (head >= a.n_seqs * a.v_heads) return;
-    const uint32_t rank = head / a.v_heads, h = head - rank * a.v_heads, kh = ops_div(h, a.share);
+    const uint32_t within = blockIdx.x / 8, heads8 = within / kBlocks, block = within % kBlocks;
+    const uint32_t group = ops_div(heads8, a.share) * 8 + blockIdx.x % 8, rank = group / c.k_heads;
+    if (rank >= a.n_seqs) return;
+    const uint32_t kh = group - rank * c.k_heads, h = kh * a.share.d + heads8 % a.share.d;
     Seq q;
     if (!seq_of_rank(a, lane, rank, c.first, c.first + c.count, q)) return;
     // this launch's chunks of the sequence
@@ -991,11 +996,12 @@ constexpr uint32_t kWideFrom = kF16 ? 192 : 512;
 
 template <int S, bool kF16>
 void launch_chunks(const GdnArgs& a, const ChunkArgs& c, hipStream_t stream) {
-    const uint32_t heads = (a.n_seqs * a.v_heads + 7) / 8 * 8;
+    auto by_eight = [&](uint32_t rows) { return (rows * c.k_heads + 7) / 8 * 8 * a.share.d; };   // value heads, key heads by eights
+    const uint32_t heads = by_eight(a.n_seqs);
     const dim3 threads((kStateWaves<S> + kOutWaves) * 64);
-    hipLaunchKernelGGL((gdn_prepare_kernel<S, kF16>), dim3(c.count * a.v_heads), dim3(kThreadsC), 0, stream, a, c);
+    hipLaunchKernelGGL((gdn_prepare_kernel<S, kF16>), dim3(by_eight(c.count)), dim3(kThreadsC), 0, stream, a, c);
     if constexpr (S >= 64)
-        if (heads * (S / 32) >= kWideFrom<kF16>) {
+        if (a.n_seqs * a.v_heads * (S / 32) >= kWideFrom<kF16>) {
             hipLaunchKernelGGL((gdn_chunk_kernel<S, 2, kF16>), dim3(heads * (S / 32)), threads, 0, stream, a, c);
             return;
         }
