@@ -14,6 +14,12 @@
 // The head is the lane's column in both results, so the running statistics are the lane's own: only the largest score of a
 // turn crosses lanes (two swaps), and bringing o to a new m is a product by the lane's own factor.
 //
+// Rows that are read once go past the caches' keeping: values always (267 us for 1.5 GB of eight sequences where they do
+// not, 241 where they do), keys in int8 (40.7 and 38.3 us for 135 MB), but not in f16, where a row's 512 bytes are read by
+// instructions of 64 of them (248 and 241 us).  Measured, 2 kv heads of 256 and 24 query heads: 1.5 GB of f16 rows in 236 us,
+// 6.4 TB/s where reading alone reaches 6.9; 135 MB of int8 rows in 37 us, where a call whose
+// workgroups take one turn each takes 12.
+//
 // Accuracy: probabilities and f32 queries enter the matrix instructions as two f16 parts (high part truncated, the rest
 // rounded likewise: 22 bits), keys, values and f16 queries are exact, int8 codes are exact in f16 and their scales are
 // applied in f32; sums are in 32 bits.  m leaves the largest probability at 2^10, so that small ones stay in f16's normal
@@ -33,7 +39,11 @@ constexpr float kInf = __builtin_inff();
 constexpr int kAttnWaves = 4, kAttnThreads = kAttnWaves * 64;
 constexpr int kTurn = 32;                       // cells of a wave's turn
 constexpr uint32_t kUnit = kTurn * kAttnWaves;  // cells of a workgroup's turn
-constexpr uint32_t kAttnSlots = 512;            // workgroups that the units are shared out among
+// Workgroups that the units are shared out among, one to each of the chip's 256 units, whose next turn's rows are in flight
+// while this one's are worked on.  Two to each have more in flight, but give twice the parts to write and to join; between
+// the two some run alone at the end.  Eight sequences of 1 K to 128 K cells: 236 us with 256, 273 with 384, 242 with 512; one
+// of 128 K 51, 61, 54; 32 of up to 8 K in int8 37, 41, 38.
+constexpr uint32_t kAttnSlots = 256;
 constexpr float kTop = 10.0f, kMost = 15.0f;    // log2 of the largest probability after a new m, and before one is needed
 
 // 2^x by the hardware's instruction (1 unit in the last place; results below the normal range are 0).
@@ -609,9 +619,11 @@ __global__ void __launch_bounds__(kAttnThreads) attn_join_kernel(AttnArgs a) {
 template <int D, bool kInt8, bool kF16>
 hipError_t launch_of(const AttnArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL((attn_part_kernel<D, kInt8, kF16>), dim3(a.grid), dim3(kAttnThreads), 0, stream, a);
-    // a head's parts by one workgroup where the heads fill the chip, by one for 64 values each where they do not
+    // A head's parts by one workgroup where the heads fill the chip or its threads have all the parts in flight at once, else by
+    // one for 64 values each: with 24 heads 11.0 us against 11.6 for 1 K cells, 11.6 against 12.2 for 4 K (both kernels), but
+    // 56.6 against 53.7 for 128 K; with 768 heads 38.3 against 41.5
     const uint32_t rows = a.n_seqs * a.n_head;
-    if (a.join && rows >= 128) hipLaunchKernelGGL((attn_join_kernel<D, D, kF16>), dim3(rows), dim3(kAttnThreads), 0, stream, a);
+    if (a.join && (rows >= 128 || a.parts <= 32)) hipLaunchKernelGGL((attn_join_kernel<D, D, kF16>), dim3(rows), dim3(kAttnThreads), 0, stream, a);
     else if (a.join) hipLaunchKernelGGL((attn_join_kernel<D, 64, kF16>), dim3(rows, D / 64), dim3(kAttnThreads), 0, stream, a);
     return hipGetLastError();
 }
@@ -631,7 +643,9 @@ uint64_t plan_attn(AttnArgs& a, int head_dim) {
     a.slots = kAttnSlots;
     a.least = 1;
     a.join = most > a.least;
+    // With a workgroup for every unit that there can be, none has to find its place: 12.4 us for 1 K cells, 13.3 without.
     a.direct = a.join && !a.window && rows * most <= a.slots ? uint32_t(most) : 0;
+    a.parts = uint32_t(most < a.slots ? most : a.slots + 1);
     // parts of all sequences: at most a slot's share each, and one more a sequence
     const uint64_t shares = a.slots < rows * most ? a.slots : rows * most;
     a.grid = uint32_t(a.direct ? rows * most : rows + (a.join ? shares : 0));

@@ -49,6 +49,7 @@ struct AttnArgs {
     uint32_t slots, least;                // workgroups the units are shared out among, units of a part at least
     uint32_t grid, join;                  // workgroups of the launch, whether a sequence can have more than one part
     uint32_t direct;                      // units a sequence can have, where each is a workgroup of its own; else 0
+    uint32_t parts;                       // parts a sequence can have
     float* ws;                            // the parts' results
     ops_u32x2* where;                     // [n_seqs] parts of a sequence and its first one's place
 };
