@@ -16,9 +16,9 @@
 //
 // Rows that are read once go past the caches' keeping: values always (267 us for 1.5 GB of eight sequences where they do
 // not, 241 where they do), keys in int8 (40.7 and 38.3 us for 135 MB), but not in f16, where a row's 512 bytes are read by
-// instructions of 64 of them (248 and 241 us).  Measured, 2 kv heads of 256 and 24 query heads: 1.5 GB of f16 rows in 236 us,
-// 6.4 TB/s where reading alone reaches 6.9; 135 MB of int8 rows in 37 us, where a call whose
-// workgroups take one turn each takes 12.
+// instructions of 64 of them (248 and 241 us).  Measured, 2 kv heads of 256 and 24 query heads: 1.5 GB of f16 rows in 238 us,
+// 6.3 TB/s where reading alone reaches 6.9; 135 MB of int8 rows in 37 us, where a call whose workgroups take one turn each
+// takes 12.
 //
 // Accuracy: probabilities and f32 queries enter the matrix instructions as two f16 parts (high part truncated, the rest
 // rounded likewise: 22 bits), keys, values and f16 queries are exact, int8 codes are exact in f16 and their scales are

@@ -4,7 +4,9 @@
 // both products taken of the state as it was, x = M^T k and y = M^T q, the token needs one pass over it:
 //     u = beta (v - e^g x),   out = scale (e^g y + (q . k) u),   M <- e^g M + k u^T.
 // Columns of the state (values) do not meet, so a workgroup takes a head's columns, or some of them, and keeps them in
-// registers: four columns a lane, the keys spread over the lanes and waves and summed over them.
+// registers: four columns a lane, the keys spread over the lanes and waves and summed over them.  Reading and writing the
+// state bounds it, past the caches' keeping (53 us; 58 through them): 64 sequences of 32 heads of 128, 270 MB in 48 us, 5.6 TB/s
+// where this library's plain copy reaches 5.7.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

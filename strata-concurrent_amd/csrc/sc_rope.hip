@@ -6,6 +6,9 @@
 // tokens are few, a share of its rows): the token's cosines and sines are formed once in 64 bits, where the angle at
 // position 10^5 still has its low digits, and its rows of queries, keys and values are then taken a wave each, four values
 // a lane.  A pair's other value is in the lane itself (neighbours) or rot / 8 lanes away (halves: one lane exchange).
+// 10 854 tokens of 24 + 2 x 2 heads of 256 (f32 into an f16 cache): 600 MB in 109 us, 5.5 TB/s where this library's plain copy
+// reaches 5.7.  Rows asked for several at a time, before they are turned, made it slower (119 us by twos, 127 by fours): many
+// waves with a row each keep memory busier than fewer with more.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>

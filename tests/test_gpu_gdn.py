@@ -190,6 +190,30 @@ def test_gates_at_their_ends(sc, ops, plain, cuda, step):
     x.check(plain)
 
 
+@pytest.mark.parametrize("dtype", ["f16", "f32"])
+@pytest.mark.parametrize("step", [True, False], ids=["step", "chunk"])
+def test_values_that_are_no_numbers(sc, ops, cuda, step, dtype):
+    """Infinities and NaN in a sequence's values, keys, gates or state change no bit of other heads and sequences."""
+    def run(spoil):
+        x = Layer(sc, ops, 15, 64, 2, 4, [1] * 5 if step else [70, 130, 64, 65, 3], dtype, step=step)
+        if spoil:
+            x.v[x.cu[0], 1, 3], x.k[x.cu[1] + 0, 1, 5], x.M[2, 0, 7, 9] = np.nan, np.inf, -np.inf
+            x.beta[x.cu[3], 2], x.q[x.cu[4], 0, 1] = np.nan, np.inf
+        x.build().launch()
+        sc.device_sync()
+        return x, *x.read()
+
+    (x, a, m), (_, b, n) = run(False), run(True)
+    spoiled = {(0, 1), (1, 2), (1, 3), (2, 0), (3, 2), (4, 0), (4, 1)}
+    for s in range(5):
+        for h in range(4):
+            same = (a[x.cu[s]:x.cu[s + 1], h].tobytes() == b[x.cu[s]:x.cu[s + 1], h].tobytes(), m[s, h].tobytes() == n[s, h].tobytes())
+            if (s, h) not in spoiled:
+                assert same == (True, True), (s, h)
+            else:
+                assert not same[0] and not np.isfinite(b[x.cu[s]:x.cu[s + 1], h]).all(), (s, h)
+
+
 def test_pieces_of_a_prompt(sc, ops, plain, cuda):
     """A prompt in three calls, the last tokens one by one, goes on from the state that each leaves."""
     S, kh, vh, T = 64, 2, 4, 200
