@@ -216,9 +216,9 @@ __device__ __forceinline__ void split_pair(f32x4 a, f32x4 b, f32x4 by_a, f32x4 b
 // rest of T by products of tiles, T_10 = - T_11 (A_10 T_00) for tiles of 16 and then of 32, with f32 matrix instructions.  A
 // product's left tile comes from LDS as rows, its right one is a result in registers as it is: the four terms a lane adds are
 // those whose rows it holds.  A chunk of one head is a chain of small steps whose latency bounds a small call (11 us for one
-// chunk of 32 heads of 128, f32; 20 by a single wave) and one in f16 (4096 of them in 67 us, 4.3 TB/s; 50 by single waves, which
-// is not worth a kernel more); in f32 the parts of keys and queries that it writes do (5568 in 153 us, 5.2 TB/s).  Three
-// workgroups share a unit; room for a fourth would take registers that it needs (81 us).
+// chunk of 32 heads of 128, f32; 20 by a single wave) and a large one (4096 of them in 67 us, f16, 3.3 TB/s; 50 by single waves,
+// which is not worth a kernel more; 5568 in about 140 us, f32, where it also writes the parts of keys and queries, 4 TB/s).
+// Three workgroups share a unit; room for a fourth would take registers that it needs (81 us).
 template <int S, bool kF16>
 __global__ void __launch_bounds__(kThreadsC, 3) gdn_prepare_kernel(GdnArgs a, ChunkArgs c) {
     constexpr int kParts = kF16 ? 1 : 2, kSteps = S / 32;
@@ -543,7 +543,7 @@ __device__ __forceinline__ void split_state(const f32x4 (&m)[2], ops_u32x4& hi, 
 // kN tiles of 16 columns.  With one, both waves of the state form U from the whole of K M0; with two, each forms the one of
 // its tile and they exchange what the update needs.  One sequence is bound by the chain of a chunk's products, splits and
 // barriers, 1.9 us each (8192 tokens, 32 heads of 128, f16: 238 us), many by the operands that their workgroups read through
-// their caches (10 854 tokens of eight sequences, f32: 286 us, 10 TB/s of them).
+// their caches (10 854 tokens of eight sequences, f32: 250-290 us, 10-12 TB/s of them).
 template <int S, int kN, bool kF16>
 __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chunk_kernel(GdnArgs a, ChunkArgs c) {
     constexpr int kParts = kF16 ? 1 : 2, kSteps = S / 32, kShares = kStateWaves<S>, kMine = kSteps / kShares;
