@@ -103,9 +103,12 @@ __device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); 
 struct Seq {
     uint32_t s, t0, t1, chunk0;
 };
-__device__ __forceinline__ uint32_t rows_from(const GdnArgs& a, uint32_t s) {
-    const int64_t t = ld_global<int64_t>(a.cu + s);
-    return t < 0 ? 0u : t > int64_t(a.tokens) ? a.tokens : uint32_t(t);
+// The rows of sequence s, of the last one past it: two loads at once.
+__device__ __forceinline__ void ends_of(const GdnArgs& a, uint32_t s, uint32_t& t0, uint32_t& t1) {
+    const int64_t* p = a.cu + (s < a.n_seqs ? s : a.n_seqs - 1);
+    const int64_t from = ld_global<int64_t>(p), to = ld_global<int64_t>(p + 1);
+    auto bounded = [&](int64_t t) { return t < 0 ? 0u : t > int64_t(a.tokens) ? a.tokens : uint32_t(t); };
+    t0 = bounded(from), t1 = bounded(to);
 }
 // The sequence that `find` (of a sequence and the range of its chunks) looks for; one load a lane and a scan for 64.
 template <class Find>
@@ -113,8 +116,9 @@ __device__ __forceinline__ bool seq_of(const GdnArgs& a, uint32_t lane, Find fin
     uint32_t chunks = 0;
     for (uint32_t base = 0; base < a.n_seqs; base += 64) {
         const bool in = base + lane < a.n_seqs;
-        const uint32_t t0 = in ? rows_from(a, base + lane) : 0u, t1 = in ? rows_from(a, base + lane + 1) : 0u;
-        const uint32_t n = t1 > t0 ? (t1 - t0 + kC - 1) / kC : 0u;
+        uint32_t t0, t1;
+        ends_of(a, base + lane, t0, t1);
+        const uint32_t n = in && t1 > t0 ? (t1 - t0 + kC - 1) / kC : 0u;
         const uint32_t sum = scan_add(n), lo = chunks + sum - n;
         const uint64_t here = __ballot(in && find(base + lane, lo, lo + n));
         if (here) {
@@ -134,8 +138,9 @@ __device__ __forceinline__ bool seq_of(const GdnArgs& a, uint32_t lane, Find fin
 __device__ __forceinline__ bool seq_of_rank(const GdnArgs& a, uint32_t lane, uint32_t rank, uint32_t c0, uint32_t c1, Seq& q) {
     if (a.n_seqs > 64) return seq_of(a, lane, [&](uint32_t s, uint32_t, uint32_t) { return s == rank; }, q);
     const bool in = lane < a.n_seqs;
-    const uint32_t t0 = in ? rows_from(a, lane) : 0u, t1 = in ? rows_from(a, lane + 1) : 0u;
-    const uint32_t n = t1 > t0 ? (t1 - t0 + kC - 1) / kC : 0u, hi = scan_add(n), lo = hi - n;
+    uint32_t t0, t1;
+    ends_of(a, lane, t0, t1);
+    const uint32_t n = in && t1 > t0 ? (t1 - t0 + kC - 1) / kC : 0u, hi = scan_add(n), lo = hi - n;
     const uint32_t from = lo > c0 ? lo : c0, to = hi < c1 ? hi : c1;
     const uint32_t key = in ? (from < to ? to - from : 0u) * 64 + 64 - lane : 0u;
     uint32_t before = 0;
