@@ -221,18 +221,21 @@ __device__ __forceinline__ void split_pair(f32x4 a, f32x4 b, f32x4 by_a, f32x4 b
 // rest of T by products of tiles, T_10 = - T_11 (A_10 T_00) for tiles of 16 and then of 32, with f32 matrix instructions.  A
 // product's left tile comes from LDS as rows, its right one is a result in registers as it is: the four terms a lane adds are
 // those whose rows it holds.  A chunk of one head is a chain of small steps whose latency bounds a small call (11 us for one
-// chunk of 32 heads of 128, f32; 20 by a single wave) and a large one (4096 of them in 67 us, f16, 3.3 TB/s; 50 by single waves,
-// which is not worth a kernel more; 5568 in about 140 us, f32, where it also writes the parts of keys and queries, 4 TB/s).
-// Three workgroups share a unit; room for a fourth would take registers that it needs (81 us).
+// chunk of 32 heads of 128, f32; 20 by a single wave) and a large one (4096 of them in 60 us, f16, 3.7 TB/s; 50 by single waves,
+// which is not worth a kernel more; 5568 in 127 to 150 us, f32, where it also writes the parts of keys and queries, 4.4 TB/s).
+// So it keeps room for four workgroups a unit: A, T and P lie where the keys were, and the substitution asks for its rows a few
+// at a time (by three workgroups, with all of them at once: 68 and 132 to 165 us).
 template <int S, bool kF16>
-__global__ void __launch_bounds__(kThreadsC, 3) gdn_prepare_kernel(GdnArgs a, ChunkArgs c) {
+__global__ void __launch_bounds__(kThreadsC, 4) gdn_prepare_kernel(GdnArgs a, ChunkArgs c) {
     constexpr int kParts = kF16 ? 1 : 2, kSteps = S / 32;
     __shared__ union {
         ops_u32x4 k[kParts][4][kSteps][64];   // keys as operands: [part][tile][step][lane]
-        float p[10 * kTileFloats];            // then P, by tiles
+        struct {
+            float t[10 * kTileFloats], p[10 * kTileFloats];   // then A, which becomes T, and P, by tiles
+        } f;
     } s_u;
-    __shared__ __align__(16) float s_tile[10 * kTileFloats];
     auto& s_k = s_u.k;
+    float* s_tile = s_u.f.t;
     __shared__ double s_G[kC];
     __shared__ float s_beta[kC], s_fk[kC], s_kk[kC], s_up[kC], s_q[kWaves][5][16];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -414,7 +417,7 @@ __global__ void __launch_bounds__(kThreadsC, 3) gdn_prepare_kernel(GdnArgs a, Ch
             const uint32_t r = g * 4 + i;
             const float fade = below || r >= col ? exp2_of(Gr[i] - Gc) * fc : 0.0f;
             tiles[t * kTileFloats + r * kTileRow + col] = below || r > col ? br[i] * fade * kk[t][i] : 0.0f;
-            s_u.p[(wave * (wave + 1) / 2 + t) * kTileFloats + r * kTileRow + col] = qr[i] * fade * qk[t][i];
+            s_u.f.p[(wave * (wave + 1) / 2 + t) * kTileFloats + r * kTileRow + col] = qr[i] * fade * qk[t][i];
         }
     }
     wave_sync();
@@ -429,23 +432,25 @@ __global__ void __launch_bounds__(kThreadsC, 3) gdn_prepare_kernel(GdnArgs a, Ch
             st_global<ops_u32x4>(out + which * kOperand + operand_at(wave, step, 1) + lane, lo);
         }
     };
-    write_operand(s_u.p + wave * (wave + 1) / 2 * kTileFloats, 1);
+    write_operand(s_u.f.p + wave * (wave + 1) / 2 * kTileFloats, 1);
     // the diagonal tile of T, column col (the same in each group of lanes)
     auto tile_at = [&](int t) { return s_tile + t * kTileFloats; };
     {
         float* d = tiles + wave * kTileFloats;
+        uint32_t row0 = 0;
         float x[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             f32x4 sum{uint32_t(i) == col ? 1.0f : 0.0f, 0, 0, 0};   // four sums: a chain a quarter as long
 #pragma unroll
             for (int k = 0; k < i; k += 4) {
-                const f32x4 r = *reinterpret_cast<const f32x4*>(&d[i * kTileRow + k]);
+                const f32x4 r = *reinterpret_cast<const f32x4*>(&d[row0 + i * kTileRow + k]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     if (k + j < i) sum[j] -= r[j] * x[k + j];
             }
             x[i] = (sum.x + sum.y) + (sum.z + sum.w);
+            if (i == 3 || i == 7 || i == 11) asm volatile("" : "+v"(row0), "+v"(x[i]));   // not all rows at once
         }
         wave_sync();
         if (g == 0)
