@@ -973,7 +973,7 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
         load_p(clamped(done + 1));
         wave_sync();
         uint8_t* to = a.out + int64_t(q.t0 + (done - q.chunk0) * kC) * a.out_ld + (h * S + block * kCols) * kBytes;
-        uint32_t o_ld = uint32_t(a.out_ld);
+        uint32_t o_ld = __builtin_amdgcn_readfirstlane(uint32_t(a.out_ld));
         asm volatile("" : "+s"(o_ld));   // the rows' offsets formed here: kept, they would have to be read from memory
 #pragma unroll
         for (uint32_t i = 0; i < kEach; ++i) {
