@@ -552,7 +552,7 @@ __device__ __forceinline__ void split_state(const f32x4 (&m)[2], ops_u32x4& hi, 
 
 // kN tiles of 16 columns.  With one, both waves of the state form U from the whole of K M0; with two, each forms the one of
 // its tile and they exchange what the update needs.  One sequence is bound by the chain of a chunk's products, splits and
-// barriers, 1.9 us each (8192 tokens, 32 heads of 128, f16: 238 us), many by the operands that their workgroups read through
+// barriers, 1.8 us each (8192 tokens, 32 heads of 128, f16: 236 us), many by the operands that their workgroups read through
 // their caches (10 854 tokens of eight sequences, f32: 250-290 us, 10-12 TB/s of them).
 template <int S, int kN, bool kF16>
 __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chunk_kernel(GdnArgs a, ChunkArgs c) {
@@ -1003,8 +1003,8 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
 
 // Two tiles of columns a workgroup halve what a chunk's operands cost in reads (132 KB for f32, 72 for f16), one gives twice
 // as many workgroups, each with less to do between its barriers.  Measured in us for both kernels, sequences of 32 heads of
-// 128 and up to 1024 tokens, two tiles against one: f16 55 : 45 for one sequence, 62 : 65 for two, 97 : 129 for eight; f32
-// 67 : 52, 78 : 70, 83 : 82 for three, 151 : 178 for eight.  So two where that leaves three quarters of the chip's 256 units a
+// 128 and up to 1024 tokens, two tiles against one: f16 56 : 44 for one sequence, 60 : 62 for two, 93 : 123 for eight; f32
+// 67 : 51, 76 : 68, 78 : 78 for three, 149 : 172 for eight.  So two where that leaves three quarters of the chip's 256 units a
 // workgroup (f16), or two to each (f32).
 template <bool kF16>
 constexpr uint32_t kWideFrom = kF16 ? 192 : 512;
@@ -1034,17 +1034,20 @@ hipError_t launch_of(const GdnArgs& a, const ChunkArgs& plan, bool f16, hipStrea
     return hipSuccess;
 }
 
-// Chunks of one pair of launches: a long prompt goes through the workspace in pieces, which bounds it (0.6 GB for 32 heads of
-// 128 in f32).  Pieces of 64 chunks stay in the caches, those of 512 leave more sequences to run at once: 32 768 tokens of one
-// sequence (f16) take 1125, 1181 and 1165 us by pieces of 64, 256 and 512, eight sequences of up to 8192 (f32) 2042, 1624, 1473.
-constexpr uint32_t kMostChunks = 256;
+// Chunks of one pair of launches: a long prompt goes through the workspace in pieces, which bounds it (1.2 GB at most for 32
+// heads of 128 in f32).  A piece of one sequence stays in the memory's own cache, 256 MB, until it has been read: 32 768 tokens
+// of 32 heads of 128 take 1093, 1060, 1149 and 1126 us by pieces of 64, 128, 256 and 512 chunks in f16, 1430, 1643, 1587 and
+// 1550 in f32, whose pieces are twice as large.  Each further sequence adds as many, so that all have something to do: eight of
+// up to 8192 (f32) 2029, 1605 and 1490 by 64, 256 and 512.
+constexpr uint32_t kMostChunks = 512;
 
 }  // namespace
 
 uint64_t plan_gdn_chunks(const GdnArgs& a, int size, bool f16, ChunkArgs& c) {
     // a sequence has at most one chunk that is not full
     c.total = a.tokens / kC + (a.n_seqs < a.tokens ? a.n_seqs : a.tokens);
-    c.count = c.total < kMostChunks ? c.total : kMostChunks;
+    const uint32_t each = f16 ? 128 : 64, most = a.n_seqs < kMostChunks / each ? a.n_seqs * each : kMostChunks;
+    c.count = c.total < most ? c.total : most;
     c.first = 0;
     c.k_heads = a.v_heads / a.share.d;
     const uint64_t chunks = uint64_t(c.count) * a.v_heads * kChunkWords, rows = uint64_t(c.count) * c.k_heads * size * (f16 ? 8 : 48);

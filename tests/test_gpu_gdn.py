@@ -133,6 +133,15 @@ def test_a_long_prompt(sc, ops, plain, cuda, dtype):
     x.check(plain, heads=[0, 3])
 
 
+@pytest.mark.parametrize("dtype,lens", [("f16", [8300]), ("f32", [9000, 3000, 1000]), ("f16", [100, 13000, 70, 4000])])
+def test_prompts_of_several_pieces(sc, ops, plain, cuda, dtype, lens):
+    """Prompts that go through the workspace in pieces, a piece's end inside a sequence or between two."""
+    x = Layer(sc, ops, 16, 64, 1, 2, lens, dtype)
+    x.build().launch()
+    sc.device_sync()
+    x.check(plain, heads=[1])
+
+
 @pytest.mark.parametrize("dtype", ["f16", "f32"])
 def test_a_state_as_a_whole(sc, ops, plain, cuda, dtype):
     """The error of a state in its norm: every token's write is known to 2^-22 of itself and 2^-27 of the column's largest
