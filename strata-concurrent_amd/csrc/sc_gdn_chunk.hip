@@ -237,7 +237,7 @@ __global__ void __launch_bounds__(kThreadsC, 4) gdn_prepare_kernel(GdnArgs a, Ch
     auto& s_k = s_u.k;
     float* s_tile = s_u.f.t;
     __shared__ double s_G[kC];
-    __shared__ float s_beta[kC], s_fk[kC], s_kk[kC], s_up[kC], s_q[kWaves][5][16];
+    __shared__ float s_beta[kC], s_fk[kC], s_kk[kC], s_up[kC], s_q[kWaves][2][16];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t g = lane >> 4, col = lane & 15;
     // workgroups go to the eight XCDs in turn: the value heads of a key head are kept on one, whose L2 then has its rows
@@ -1036,16 +1036,16 @@ hipError_t launch_of(const GdnArgs& a, const ChunkArgs& plan, bool f16, hipStrea
 
 // Chunks of one pair of launches: a long prompt goes through the workspace in pieces, which bounds it (1.2 GB at most for 32
 // heads of 128 in f32).  A piece of one sequence stays in the memory's own cache, 256 MB, until it has been read: 32 768 tokens
-// of 32 heads of 128 take 1093, 1060, 1149 and 1126 us by pieces of 64, 128, 256 and 512 chunks in f16, 1430, 1643, 1587 and
+// of 32 heads of 128 take 1093, 1050, 1149 and 1126 us by pieces of 64, 128, 256 and 512 chunks in f16, 1421, 1643, 1587 and
 // 1550 in f32, whose pieces are twice as large.  Each further sequence adds as many, so that all have something to do: eight of
-// up to 8192 (f32) 2029, 1605 and 1490 by 64, 256 and 512.
+// up to 8192 (f32) 2029, 1605 and 1455 by 64, 256 and 512.
 constexpr uint32_t kMostChunks = 512;
 
 }  // namespace
 
 uint64_t plan_gdn_chunks(const GdnArgs& a, int size, bool f16, ChunkArgs& c) {
-    // a sequence has at most one chunk that is not full
-    c.total = a.tokens / kC + (a.n_seqs < a.tokens ? a.n_seqs : a.tokens);
+    // a sequence has at most one chunk that is not full, of one token at least
+    c.total = uint32_t((a.tokens + uint64_t(kC - 1) * (a.n_seqs < a.tokens ? a.n_seqs : a.tokens)) / kC);
     const uint32_t each = f16 ? 128 : 64, most = a.n_seqs < kMostChunks / each ? a.n_seqs * each : kMostChunks;
     c.count = c.total < most ? c.total : most;
     c.first = 0;
