@@ -29,6 +29,7 @@
 
 #include <cstdint>
 
+#include "sc_attn_split.hpp"
 #include "sc_ops.hpp"
 
 namespace sc {
@@ -36,14 +37,7 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr float kInf = __builtin_inff();
-constexpr int kAttnWaves = 4, kAttnThreads = kAttnWaves * 64;
-constexpr int kTurn = 32;                       // cells of a wave's turn
-constexpr uint32_t kUnit = kTurn * kAttnWaves;  // cells of a workgroup's turn
-// Workgroups that the units are shared out among, one to each of the chip's 256 units, whose next turn's rows are in flight
-// while this one's are worked on.  Two to each have more in flight, but give twice the parts to write and to join; between
-// the two some run alone at the end.  Eight sequences of 1 K to 128 K cells: 236 us with 256, 273 with 384, 242 with 512; one
-// of 128 K 51, 61, 54; 32 of up to 8 K in int8 37, 41, 38.
-constexpr uint32_t kAttnSlots = 256;
+constexpr int kAttnThreads = kAttnWaves * 64;
 constexpr float kTop = 10.0f, kMost = 15.0f;    // log2 of the largest probability after a new m, and before one is needed
 
 // 2^x by the hardware's instruction (1 unit in the last place; results below the normal range are 0).
@@ -62,17 +56,7 @@ __device__ __forceinline__ float over_rows(float x, F f) {
 
 // ---- which cells a workgroup takes ------------------------------------------------------------------------------------
 
-struct Span {
-    uint32_t first, len, begin, units;   // cells [first, len), counted in units from `begin`, a multiple of a turn
-};
-__device__ __forceinline__ Span span_of(const AttnArgs& a, int64_t n) {
-    Span p;
-    p.len = n < 0 ? 0u : n > int64_t(a.max_len) ? a.max_len : uint32_t(n);
-    p.first = a.window && p.len > a.window ? p.len - a.window : 0u;
-    p.begin = p.first & ~uint32_t(kTurn - 1);
-    p.units = (p.len - p.begin + kUnit - 1) / kUnit;
-    return p;
-}
+__device__ __forceinline__ Span span_of(const AttnArgs& a, int64_t n) { return cells_of(n, a.max_len, a.window); }
 
 // The workgroups of a sequence are its parts times its tiles (kv heads and tiles of query heads), the tiles of a part next
 // to each other: they read the same pages.
@@ -91,12 +75,10 @@ __device__ __forceinline__ bool place_of(const AttnArgs& a, uint32_t lane, uint3
     uint32_t sum = my_units;             // at most 2^24 units a sequence and 16 sequences a lane
     for (uint32_t base = 64; base < a.n_seqs; base += 64) sum += span_of(a, length(base + lane)).units;
     const uint64_t total = uint64_t(last_lane(scan_add(sum & 0xFFFFFFu))) + (uint64_t(last_lane(scan_add(sum >> 24))) << 24);
-    uint64_t share = (total * a.tiles + a.slots - 1) / a.slots;
-    uint32_t per = share < a.least ? a.least : uint32_t(share);   // below 2^31: a sequence has at most 2^24 units
-    auto parts_of = [&](uint32_t s, uint32_t units) { return s >= a.n_seqs ? 0u : units <= per ? 1u : (units + per - 1) / per; };
-    // a few workgroups more than run at once would run alone at the end; twice the share is always enough here
-    if (a.n_seqs <= 64 && a.n_seqs * a.tiles * 2 <= a.slots)
-        while (last_lane(scan_add(parts_of(lane, my_units))) * a.tiles > a.slots) per += per / 32 + 1;
+    uint32_t per = units_of_part(total, a.tiles, a.slots, a.least);
+    auto parts_of = [&](uint32_t s, uint32_t units) { return s >= a.n_seqs ? 0u : parts_of_units(units, per); };
+    if (parts_fit(a.n_seqs, a.tiles, a.slots))
+        while (last_lane(scan_add(parts_of(lane, my_units))) * a.tiles > a.slots) per = wider_part(per);
     uint32_t wgs = 0, ids = 0;
     for (uint32_t base = 0; base < a.n_seqs; base += 64) {
         const int64_t n = base ? length(base + lane) : mine;
@@ -637,19 +619,14 @@ hipError_t launch_of(const AttnArgs& a, int format, bool f16, hipStream_t stream
 
 uint64_t plan_attn(AttnArgs& a, int head_dim) {
     a.tiles = a.c.H * ((a.n_head / a.c.H + 15) / 16);
-    const uint64_t rows = uint64_t(a.n_seqs) * a.tiles;
-    // a window may begin anywhere in a turn, so it can touch a unit more
-    const uint64_t most = ((a.window ? a.window + kTurn : a.max_len) + kUnit - 1) / kUnit;
     a.slots = kAttnSlots;
     a.least = 1;
-    a.join = most > a.least;
-    // With a workgroup for every unit that there can be, none has to find its place: 12.4 us for 1 K cells, 13.3 without.
-    a.direct = a.join && !a.window && rows * most <= a.slots ? uint32_t(most) : 0;
-    a.parts = uint32_t(most < a.slots ? most : a.slots + 1);
-    // parts of all sequences: at most a slot's share each, and one more a sequence
-    const uint64_t shares = a.slots < rows * most ? a.slots : rows * most;
-    a.grid = uint32_t(a.direct ? rows * most : rows + (a.join ? shares : 0));
-    return a.join ? 2 * shares * 16 * uint64_t(head_dim + 4) * 4 + (uint64_t(a.n_seqs) * 8 + 15) / 16 * 16 : 16;
+    const SplitPlan p = plan_split(a.n_seqs, a.tiles, a.max_len, a.window, a.slots);
+    a.join = p.join;
+    a.direct = p.direct;
+    a.parts = p.parts;
+    a.grid = uint32_t(p.grid);
+    return a.join ? p.places * 16 * uint64_t(head_dim + 4) * 4 + (uint64_t(a.n_seqs) * 8 + 15) / 16 * 16 : 16;
 }
 
 void place_attn(AttnArgs& a, void* workspace, uint64_t bytes) {
