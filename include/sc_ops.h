@@ -122,7 +122,8 @@ typedef struct sc_gdn {
     const void* q;            /* [tokens][k_heads][S], q_ld values from token to token, 16-byte aligned */
     const void* k;
     const void* v;            /* [tokens][v_heads][S] */
-    void* out;                /* [tokens][v_heads][S] */
+    void* out;                /* [tokens][v_heads][S]; may be v itself (then out_ld == v_ld), and shares no byte with q, k or
+                                 the rest of v: refused by the calls that enqueue */
     int64_t q_ld, k_ld, v_ld, out_ld;   /* multiples of 4 (f32) or 8 (f16) values, at most 2^22 */
     const float* g;           /* [tokens][v_heads], <= 0 (below -200 counts as -200, whose decay is 0 as well) */
     const float* beta;        /* [tokens][v_heads] */
@@ -130,8 +131,8 @@ typedef struct sc_gdn {
     float scale;
     int32_t l2norm;
     float eps;
-    float* const* state;      /* device [n_seqs]: each sequence's base; a NULL entry is a sequence without a slot: its
-                                 out rows are zeros */
+    float* const* state;      /* device [n_seqs]: each sequence's base, 16-byte aligned; a NULL entry is a sequence without
+                                 a slot: its out rows are zeros */
     int64_t state_offset;     /* floats from the base to this layer's state (e.g. a multiple of sc_gdn_row_floats) */
     int64_t state_head_ld;    /* floats between heads: S in a slot's (S, HV, S) row, S * S in the prefill layout */
     int64_t state_key_ld;     /* floats between keys: HV * S in a slot's row, S in the prefill layout */

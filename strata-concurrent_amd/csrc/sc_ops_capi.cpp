@@ -39,6 +39,17 @@ bool row_stride(int64_t ld, int64_t row, int32_t dtype) {
 }
 int64_t value_bytes(int32_t dtype) { return dtype == SC_DTYPE_F16 ? 2 : 4; }
 
+// Whether two tensors of `rows` rows have a byte in common, rows [p + t * ld, + row).  Rows side by side in one buffer, such
+// as the parts of a fused projection, have one stride and none in common.
+bool share_bytes(const void* a, int64_t a_ld, int64_t a_row, const void* b, int64_t b_ld, int64_t b_row, int64_t rows) {
+    if (rows == 0) return false;
+    const uint64_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+    if (p <= q ? q - p >= uint64_t((rows - 1) * a_ld + a_row) : p - q >= uint64_t((rows - 1) * b_ld + b_row)) return false;
+    if (a_ld != b_ld) return true;
+    const int64_t into = p <= q ? int64_t((q - p) % a_ld) : (a_ld - int64_t((p - q) % a_ld)) % a_ld;   // b's rows into a's
+    return into < a_row || into + b_row > a_ld;
+}
+
 // Checks a cache and lays it out for the kernels; an SC_ status.
 int cache_args(const char* op, const sc_kv_cache* c, int64_t n_seqs, sc::CacheArgs& o) {
     if (!c) return bad(op, "missing cache");
@@ -152,6 +163,18 @@ int gdn_args(const char* op, const sc_gdn* d, bool step, sc::GdnArgs& a) {
     return SC_OK;
 }
 
+// Workgroups of other columns read queries and keys of rows that one has written the outputs of; a row's values are read by
+// the one that writes its outputs, before it does, so those may lie in one place.
+bool outputs_apart(const sc_gdn* d) {
+    const int64_t b = value_bytes(d->dtype), row = d->v_heads * d->state_size * b, key_row = d->k_heads * d->state_size * b;
+    auto meets = [&](const void* x, int64_t ld, int64_t x_row) {
+        return share_bytes(d->out, d->out_ld * b, row, x, ld * b, x_row, d->tokens);
+    };
+    return !meets(d->q, d->q_ld, key_row) && !meets(d->k, d->k_ld, key_row) &&
+           ((d->out == d->v && d->out_ld == d->v_ld) || !meets(d->v, d->v_ld, row));
+}
+constexpr const char* kOutputsMeet = "out must not overlap q or k, nor v unless it is v";
+
 }  // namespace
 
 int sc_rope_append_async(const sc_kv_cache* cache, const sc_rope_append* d, void* stream) {
@@ -228,6 +251,7 @@ int sc_gdn_step_async(const sc_gdn* d, void* stream) {
     return guarded([&] {
         sc::GdnArgs a{};
         if (const int e = gdn_args("gdn_step", d, true, a)) return e;
+        if (!outputs_apart(d)) return bad("gdn_step", kOutputsMeet);
         return launched(sc::launch_gdn_step(a, int(d->state_size), d->dtype == SC_DTYPE_F16, static_cast<hipStream_t>(stream)),
                         "gdn_step");
     });
@@ -247,6 +271,7 @@ int sc_gdn_chunk_async(const sc_gdn* d, void* workspace, uint64_t workspace_byte
         if (const int e = gdn_args(op, d, false, a)) return e;
         if (!workspace || off(workspace, 256) || workspace_bytes < sc_gdn_chunk_workspace_bytes(d))
             return bad(op, "workspace missing, not 256-byte aligned or below sc_gdn_chunk_workspace_bytes");
+        if (!outputs_apart(d)) return bad(op, kOutputsMeet);
         if (d->tokens == 0) return sc::record_ok();
         return launched(sc::launch_gdn_chunk(a, int(d->state_size), d->dtype == SC_DTYPE_F16, workspace,
                                              static_cast<hipStream_t>(stream)), op);
