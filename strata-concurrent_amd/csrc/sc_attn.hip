@@ -20,14 +20,17 @@
 // 6.3 TB/s where reading alone reaches 6.9; 135 MB of int8 rows in 37 us, where a call whose workgroups take one turn each
 // takes 12.
 //
-// Accuracy: probabilities and f32 queries enter the matrix instructions as two f16 parts (high part truncated, the rest
-// rounded likewise: 22 bits), keys, values and f16 queries are exact, int8 codes are exact in f16 and their scales are
-// applied in f32; sums are in 32 bits.  m leaves the largest probability at 2^10, so that small ones stay in f16's normal
-// range; an f32 query head is first scaled by a power of two.  The low part of a probability is at least 2^-24, so that an
-// infinite value in the cache meets no zero: it would make a NaN where the formula has an infinity.
+// Accuracy: weights and f32 queries enter the matrix instructions as two f16 parts, each rounded to nearest; keys, values and
+// f16 queries are exact, int8 codes are exact in f16 and their scales are applied in f32; sums are in 32 bits.  f16 is a fixed
+// point below 2^-14, so the reference m follows the turn's weights (the constants below): a cell that outweighs the rest by
+// 2^80 takes no bit from them.  Infinities: an infinite value may meet a weight's part that is 0, an infinite key a query's
+// second part of the other sign, and make a NaN where the formula has an infinity.  A wave whose sums are no finite numbers goes
+// over its turns again with weights as they are, by 32-bit products; no weight is 0 there, unless it is below 2^-126 of the
+// part's largest.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
+#include <type_traits>
 
 #include "sc_attn_split.hpp"
 #include "sc_ops.hpp"
@@ -38,12 +41,20 @@ namespace {
 constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
 constexpr float kInf = __builtin_inff();
 constexpr int kAttnThreads = kAttnWaves * 64;
-constexpr float kTop = 10.0f, kMost = 15.0f;    // log2 of the largest probability after a new m, and before one is needed
+// Log2 of a turn's weights, relative to m: at most kMost, at least kLeast.  Two f16 parts keep a weight to 2^-23 of itself from
+// 2^-2 on, and to 2^-17 from 2^kLeast on.  Where a turn's leave that range m moves, up or down by whole numbers, so that the
+// largest is about kTop, or kDeep where the least would be too small; but it is never more than kFar below the largest of all:
+// what is summed stays below 2^125.  Cells that are too small even then, and below kWait (an int8 cell's weights differ by its
+// blocks' scales), wait for another go at the same turn, with an m of their own: each go takes its largest, so there is an end.
+constexpr float kTop = 11.0f, kDeep = 14.0f, kMost = 15.0f, kLeast = -8.0f, kWait = 5.0f, kFar = 76.0f;
+constexpr float kTiny = 0x1p-126f;
 
 // 2^x by the hardware's instruction (1 unit in the last place; results below the normal range are 0).
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-// 2^(a - b) for a <= b or -inf: nothing weighs nothing.
-__device__ __forceinline__ float weight(float a, float b) { return a == -kInf ? 0.0f : exp2_fast(a - b); }
+__device__ __forceinline__ bool rarely(bool x) { return __builtin_expect(x, false); }
+// 2^(a - b), at least the smallest normal number, which changes no sum but leaves infinities what they are; nothing weighs
+// nothing.
+__device__ __forceinline__ float weight(float a, float b) { return a == -kInf ? 0.0f : fmaxf(exp2_fast(a - b), kTiny); }
 
 // The maximum and the sum over the four lanes that share lane % 16 (the 16-lane rows of the wave), in every one of them.
 template <class F>
@@ -53,6 +64,9 @@ __device__ __forceinline__ float over_rows(float x, F f) {
     r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
     return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
+
+__device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
+__device__ __forceinline__ float min_of(float a, float b) { return fminf(a, b); }
 
 // ---- which cells a workgroup takes ------------------------------------------------------------------------------------
 
@@ -104,6 +118,7 @@ __device__ __forceinline__ bool place_of(const AttnArgs& a, uint32_t lane, uint3
 
 // ---- a wave's turn ------------------------------------------------------------------------------------------------------
 
+using u16x2 = __attribute__((ext_vector_type(2))) uint16_t;
 __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
 __device__ __forceinline__ f16x2 two(uint32_t w) { return __builtin_bit_cast(f16x2, w); }
@@ -111,20 +126,47 @@ __device__ __forceinline__ uint32_t bits(f16x2 h) { return __builtin_bit_cast(ui
 __device__ __forceinline__ f16x8 eight(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __builtin_bit_cast(f16x8, ops_u32x4{a, b, c, d});
 }
-__device__ __forceinline__ uint32_t pack_rtz(float a, float b) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
-}
-// Two f16 parts of eight values that are not negative: the truncated value, and what it left out, at least 2^-24.
+__device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+// Two f16 parts of eight values: the value rounded to nearest, and what that left out rounded likewise.
 __device__ __forceinline__ void split8(const float (&p)[8], f16x8& hi, f16x8& lo) {
     uint32_t h[4], r[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        h[i] = pack_rtz(p[2 * i], p[2 * i + 1]);
+        h[i] = bits(f16x2{_Float16(p[2 * i]), _Float16(p[2 * i + 1])});
+        asm("" : "+v"(h[i]));   // what is left out is of this, not of a product that the compiler would round once more
         const f16x2 t = two(h[i]);
-        r[i] = bits(__builtin_elementwise_max(two(pack_rtz(p[2 * i] - float(t.x), p[2 * i + 1] - float(t.y))), two(0x00010001u)));
+        r[i] = bits(f16x2{_Float16(p[2 * i] - float(t.x)), _Float16(p[2 * i + 1] - float(t.y))});
     }
     hi = eight(h[0], h[1], h[2], h[3]);
     lo = eight(r[0], r[1], r[2], r[3]);
+}
+// The largest of a cell's f16 scales, which are not negative, and the least but one less; and their exponents, as bounds.
+template <int kBlocks>
+__device__ __forceinline__ void scales_of(const uint32_t (&s)[2], u16x2& hi, u16x2& lo) {
+#pragma unroll
+    for (int i = 0; i < (kBlocks > 2 ? 2 : 1); ++i) {
+        const uint32_t w = (kBlocks == 1 ? s[i] | s[i] << 16 : s[i]) & 0x7FFF7FFFu;
+        const u16x2 a = __builtin_bit_cast(u16x2, w);
+        hi = __builtin_elementwise_max(hi, a);
+        lo = __builtin_elementwise_min(lo, u16x2(a - u16x2{1, 1}));
+    }
+}
+__device__ __forceinline__ float exponent_most(u16x2 hi) { return float(int(max(uint32_t(hi.x), uint32_t(hi.y)) >> 10) - 14); }
+__device__ __forceinline__ float exponent_least(u16x2 lo) {
+    const uint32_t e = min(uint32_t(lo.x), uint32_t(lo.y)) >> 10;
+    return e ? float(int(e) - 15) : -24.0f;
+}
+// A tile of values by eight cells' weights, in two parts; or as they are, by 32-bit products at a quarter of the rate, where no
+// weight is 0, so that an infinite value of little weight is infinite.
+template <bool kAsIs>
+__device__ __forceinline__ void add_values(f32x4& o, f16x8 v, const float (&p)[8], f16x8 hi, f16x8 lo) {
+    if constexpr (kAsIs) {
+#pragma unroll
+        for (int n = 0; n < 8; ++n) o = mfma_f32(float(v[n]), fmaxf(p[n], kTiny), o);
+    } else {
+        o = mfma(v, hi, o);
+        o = mfma(v, lo, o);
+    }
 }
 
 // Four int8 codes with 128 added (one exclusive or) as f16: 0x64 above a byte is 1024 + the byte, exactly.
@@ -342,159 +384,217 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_part_kernel(AttnArgs a) 
     const float c = s_c[col];
 
     f32x4 o[kOut];
+    float m, l;
+    // the rows of turn u, by way of the table's entries
+    auto load_row = [&](uint32_t u) {
+        row = row_of(a, span, entry_of(a, p.s, base0 + u * kUnit, lane), h, base0 + u * kUnit, lane);
+        there = uint32_t(__ballot(row >= 0));
+        row = row < 0 ? 0 : row;
+        entry = entry_of(a, p.s, base0 + (u + 1) * kUnit, lane);
+    };
+    // The part's turns: weights in two parts, or as they are.
+    auto turns = [&](auto form) {
+        constexpr bool kAsIs = decltype(form)::value;
 #pragma unroll
-    for (int j = 0; j < kOut; ++j) o[j] = f32x4{};
-    float m = -kInf, l = 0;
-    // a turn's table entries are asked for before the rows of the turn before it: asked for after them, they would only
-    // come when all of those have
-    for (uint32_t u = u0; u < u1; ++u) {
-        // scores: x[t * 4 + i] of cell 16 t + 4 g + i.  The queries are read from LDS every turn, two steps at a time (the
-        // barriers to the compiler): kept in registers they would take the place of rows in flight
-        float x[8], ks_top[8];
-        f32x4 hi[2]{}, lo[2]{};
+        for (int j = 0; j < kOut; ++j) o[j] = f32x4{};
+        m = -kInf, l = 0;
+        // the largest weight of all; of a turn that is gone at again, the m of the cells that waited
+        float high = -kInf, waited = 0;
+        bool again = false;
+        // a turn's table entries are asked for before the rows of the turn before it: asked for after them, they would only
+        // come when all of those have
+        for (uint32_t u = u0; u < u1;) {
+            // scores: x[t * 4 + i] of cell 16 t + 4 g + i.  The queries are read from LDS every turn, two steps at a time (the
+            // barriers to the compiler): kept in registers they would take the place of rows in flight
+            float x[8];
+            f32x4 hi[2]{}, lo[2]{};   // the low part's products apart only where infinities are looked for
 #pragma unroll
-        for (int b = 0; b < kBlocks; ++b) {
-            asm volatile("" ::: "memory");
-            f16x8 q[kParts][2];
+            for (int b = 0; b < kBlocks; ++b) {
+                asm volatile("" ::: "memory");
+                f16x8 q[kParts][2];
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
+                for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int i = 0; i < kParts; ++i) q[i][k] = __builtin_bit_cast(f16x8, s.q.q[i][2 * b + k][lane]);
+                    for (int i = 0; i < kParts; ++i) q[i][k] = __builtin_bit_cast(f16x8, s.q.q[i][2 * b + k][lane]);
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                if constexpr (kInt8) {
-                    f32x4 bh{}, bl{};
-                    uint32_t w[8];
+                for (int t = 0; t < 2; ++t) {
+                    if constexpr (kInt8) {
+                        f32x4 bh{}, bl{};
+                        uint32_t w[8];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k) codes4(r.k[t][b][k] ^ 0x80808080u, w[2 * k], w[2 * k + 1]);
+                        for (int k = 0; k < 4; ++k) codes4(r.k[t][b][k] ^ 0x80808080u, w[2 * k], w[2 * k + 1]);
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const f16x8 key = eight(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-                        bh = mfma(key, q[0][k], bh);
-                        if constexpr (!kF16) bl = mfma(key, q[kParts - 1][k], bl);
-                    }
+                        for (int k = 0; k < 2; ++k) {
+                            const f16x8 key = eight(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+                            bh = mfma(key, q[0][k], bh);
+                            if constexpr (!kF16) (kAsIs ? bl : bh) = mfma(key, q[kParts - 1][k], kAsIs ? bl : bh);
+                        }
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float ks = scale_of(r.ks[t * 4 + i], b);
-                        hi[t][i] += ks * bh[i];
-                        if constexpr (!kF16) lo[t][i] += ks * bl[i];
-                    }
-                } else {
+                        for (int i = 0; i < 4; ++i) {
+                            const float ks = scale_of(r.ks[t * 4 + i], b);
+                            hi[t][i] += ks * bh[i];
+                            if constexpr (!kF16 && kAsIs) lo[t][i] += ks * bl[i];
+                        }
+                    } else {
 #pragma unroll
-                    for (int k = 0; k < 2; ++k) {
-                        const f16x8 key = __builtin_bit_cast(f16x8, r.k[t][2 * b + k]);
-                        hi[t] = mfma(key, q[0][k], hi[t]);
-                        if constexpr (!kF16) lo[t] = mfma(key, q[kParts - 1][k], lo[t]);
+                        for (int k = 0; k < 2; ++k) {
+                            const f16x8 key = __builtin_bit_cast(f16x8, r.k[t][2 * b + k]);
+                            hi[t] = mfma(key, q[0][k], hi[t]);
+                            if constexpr (!kF16) (kAsIs ? lo[t] : hi[t]) = mfma(key, q[kParts - 1][k], kAsIs ? lo[t] : hi[t]);
+                        }
                     }
                 }
             }
-        }
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            // an infinite key makes the low part's product NaN: the high part has the score
-            const float high = hi[n / 4][n % 4], sum = kF16 || !(fabsf(high) < kInf) ? high : high + lo[n / 4][n % 4];
-            x[n] = sum * c;
-        }
-        // the next turn's keys take the place of this one's
-        const uint32_t seen = there;
-        const bool more = u + 1 < u1;
-        if (more) {
-            row = row_of(a, span, entry, h, base0 + (u + 1) * kUnit, lane);
-            there = uint32_t(__ballot(row >= 0));
-            row = row < 0 ? 0 : row;
-            entry = entry_of(a, p.s, base0 + (u + 2) * kUnit, lane);
-            load_keys<D, kInt8>(r, a, row, lane);
-        }
-        uint32_t gone[8];   // all ones where a cell is not there
-        const bool whole = seen == 0xFFFFFFFFu;
-        if (!whole) {
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
-                gone[n] = (seen >> ((n & 3) + g * 4 + (n >> 2) * 16)) & 1u ? 0u : ~0u;
-                if (gone[n]) x[n] = -kInf;
+                // an infinite key makes the low part's product NaN: the high part has the score
+                const float high = hi[n / 4][n % 4], sum = kF16 || !kAsIs || !(fabsf(high) < kInf) ? high : high + lo[n / 4][n % 4];
+                x[n] = sum * c;
+            }
+            // the next turn's keys take the place of this one's
+            const uint32_t seen = there;
+            const bool more = u + 1 < u1;
+            if (more) {
+                row = row_of(a, span, entry, h, base0 + (u + 1) * kUnit, lane);
+                there = uint32_t(__ballot(row >= 0));
+                row = row < 0 ? 0 : row;
+                entry = entry_of(a, p.s, base0 + (u + 2) * kUnit, lane);
+                load_keys<D, kInt8>(r, a, row, lane);
+            }
+            uint32_t gone[8];   // all ones where a cell is not there
+            const bool whole = seen == 0xFFFFFFFFu;
+            if (!whole) {
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    gone[n] = (seen >> ((n & 3) + g * 4 + (n >> 2) * 16)) & 1u ? 0u : ~0u;
+                    if (gone[n]) x[n] = -kInf;
+#pragma unroll
+                    for (int i = 0; i < R::kValPieces; ++i)
+#pragma unroll
+                        for (int k = 0; k < R::kValWords; ++k) r.v[n][i][k] = gone[n] ? 0u : r.v[n][i][k];
+                    if constexpr (kInt8) r.vs[n][0] = gone[n] ? 0u : r.vs[n][0], r.vs[n][1] = gone[n] ? 0u : r.vs[n][1];
+                }
+            }
+            // Where the turn's weights lie: the largest of the column, the least of the lane's own cells.  An int8 weight is
+            // multiplied with its blocks' scales before it becomes f16: their exponents count, bounds over the lane's cells, or
+            // cell by cell where cells wait.
+            float top = -kInf, low = kInf;
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                top = fmaxf(top, x[n]);
+                low = fminf(low, x[n] == -kInf ? kInf : x[n]);
+            }
+            if constexpr (kInt8) {
+                u16x2 hi{}, lo{0xFFFF, 0xFFFF};   // one less for the least, so that scales that are 0 do not count
+#pragma unroll
+                for (int n = 0; n < 8; ++n) scales_of<kBlocks>(r.vs[n], hi, lo);
+                top += exponent_most(hi);
+                low += exponent_least(lo);
+            }
+            auto waits = [&](int n, float m, float& y) {
+                float z = y = x[n];
+                if constexpr (kInt8) {
+                    u16x2 hi{}, lo{0xFFFF, 0xFFFF};
+                    scales_of<kBlocks>(r.vs[n], hi, lo);
+                    y += exponent_most(hi);
+                    z += exponent_least(lo);
+                }
+                return z < m + kLeast && y < m + kWait;
+            };
+            if (rarely(again)) {
+                top = -kInf, low = kInf;
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    float y;
+                    x[n] = waits(n, waited, y) ? x[n] : -kInf;
+                    top = fmaxf(top, x[n] == -kInf ? -kInf : y);
+                    low = x[n] == -kInf ? low : -kInf;   // it will be looked for
+                }
+            }
+            top = over_rows(top, max_of);
+            if (const bool out = top > m + kMost || low < m + kLeast; rarely(__any(out))) {
+                const float f = floorf(top), least = over_rows(low, min_of);
+                high = fmaxf(high, f);
+                const bool moves = over_rows(out ? 1.0f : 0.0f, max_of) > 0 && top > -kInf;
+                const float to = moves ? fmaxf(f - (least < f - kTop + kLeast ? kDeep : kTop), high - kFar) : m;
+                const float w = m == -kInf ? 0.0f : fmaxf(__builtin_amdgcn_ldexpf(1.0f, min(int(m - to), 100)), kTiny);
+                m = to;
+                l *= w;
+#pragma unroll
+                for (int j = 0; j < kOut; ++j) o[j] *= w;
+            }
+            const float ref = m == -kInf ? 0.0f : m;
+            float pr[8];
+#pragma unroll
+            for (int n = 0; n < 8; ++n) pr[n] = exp2_fast(x[n] - ref);
+            again = false;
+            if (!kAsIs && rarely(__any(low < m + kLeast))) {
+                bool left = false;
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    float y;
+                    const bool w = m > high - kFar && x[n] > -kInf && waits(n, m, y);
+                    pr[n] = w ? 0.0f : pr[n];
+                    left |= w;
+                }
+                waited = over_rows(left ? 1.0f : 0.0f, max_of) > 0 ? m : -kInf;
+                again = __any(left);
+            }
+#pragma unroll
+            for (int n = 0; n < 8; ++n) l += pr[n];
+            if constexpr (kInt8) {
+#pragma unroll
+                for (int b = 0; b < kBlocks; ++b) {
+                    float pb[8];
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) pb[n] = pr[n] * scale_of(r.vs[n], b);
+                    f16x8 hi{}, lo{};
+                    if constexpr (!kAsIs) split8(pb, hi, lo);
+                    uint32_t w[8];
+#pragma unroll
+                    for (int n = 0; n < 8; ++n) w[n] = r.v[n][b][0] ^ 0x80808080u;
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        uint32_t e0[4], e1[4];   // the pair of places 2 k, 2 k + 1 of cells 2 i, 2 i + 1
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+                            codes4(__builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], k ? 0x07030602u : 0x05010400u), e0[i], e1[i]);
+                        add_values<kAsIs>(o[b * 4 + 2 * k], eight(e0[0], e0[1], e0[2], e0[3]), pb, hi, lo);
+                        add_values<kAsIs>(o[b * 4 + 2 * k + 1], eight(e1[0], e1[1], e1[2], e1[3]), pb, hi, lo);
+                    }
+                }
+            } else {
+                f16x8 hi{}, lo{};
+                if constexpr (!kAsIs) split8(pr, hi, lo);
 #pragma unroll
                 for (int i = 0; i < R::kValPieces; ++i)
 #pragma unroll
-                    for (int k = 0; k < R::kValWords; ++k) r.v[n][i][k] = gone[n] ? 0u : r.v[n][i][k];
-                if constexpr (kInt8) r.vs[n][0] = gone[n] ? 0u : r.vs[n][0], r.vs[n][1] = gone[n] ? 0u : r.vs[n][1];
-            }
-        }
-        // what a probability is multiplied with before it becomes f16: int8 values' scales, by their exponent
-        float top = -kInf;
+                    for (int k = 0; k < R::kValWords; ++k) {
 #pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            ks_top[n] = 0;
-            if constexpr (kInt8) {
-                uint32_t e = 0;   // exponents of the scales, which are not negative
+                        for (int e = 0; e < 2; ++e) {
+                            const uint32_t sel = e ? 0x07060302u : 0x05040100u;
+                            uint32_t w[4];
 #pragma unroll
-                for (int b = 0; b < kBlocks; ++b) {
-                    const uint32_t s = (r.vs[n][b / 2] >> (b & 1 ? 16 : 0)) & 0x7FFFu;
-                    e = e > s ? e : s;
-                }
-                ks_top[n] = float(int(e >> 10) - 14);
-            }
-            top = fmaxf(top, x[n] + ks_top[n]);
-        }
-        top = over_rows(top, [](float p, float q) { return fmaxf(p, q); });
-        if (__any(top > m + kMost)) {
-            const float to = top > m + kMost ? top - kTop : m, w = weight(m, to);
-            m = to;
-            l *= w;
-#pragma unroll
-            for (int j = 0; j < kOut; ++j) o[j] *= w;
-        }
-        const float ref = m == -kInf ? 0.0f : m;
-        float pr[8];
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            pr[n] = exp2_fast(x[n] - ref);
-            l += pr[n];
-        }
-        if constexpr (kInt8) {
-#pragma unroll
-            for (int b = 0; b < kBlocks; ++b) {
-                float pb[8];
-#pragma unroll
-                for (int n = 0; n < 8; ++n) pb[n] = pr[n] * scale_of(r.vs[n], b);
-                f16x8 hi, lo;
-                split8(pb, hi, lo);
-                uint32_t w[8];
-#pragma unroll
-                for (int n = 0; n < 8; ++n) w[n] = r.v[n][b][0] ^ 0x80808080u;
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    uint32_t e0[4], e1[4];   // the pair of places 2 k, 2 k + 1 of cells 2 i, 2 i + 1
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        codes4(__builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], k ? 0x07030602u : 0x05010400u), e0[i], e1[i]);
-                    const f16x8 v0 = eight(e0[0], e0[1], e0[2], e0[3]), v1 = eight(e1[0], e1[1], e1[2], e1[3]);
-                    o[b * 4 + 2 * k] = mfma(v0, hi, o[b * 4 + 2 * k]);
-                    o[b * 4 + 2 * k] = mfma(v0, lo, o[b * 4 + 2 * k]);
-                    o[b * 4 + 2 * k + 1] = mfma(v1, hi, o[b * 4 + 2 * k + 1]);
-                    o[b * 4 + 2 * k + 1] = mfma(v1, lo, o[b * 4 + 2 * k + 1]);
-                }
-            }
-        } else {
-            f16x8 hi, lo;
-            split8(pr, hi, lo);
-#pragma unroll
-            for (int i = 0; i < R::kValPieces; ++i)
-#pragma unroll
-                for (int k = 0; k < R::kValWords; ++k) {
-#pragma unroll
-                    for (int e = 0; e < 2; ++e) {
-                        const uint32_t sel = e ? 0x07060302u : 0x05040100u;
-                        uint32_t w[4];
-#pragma unroll
-                        for (int n = 0; n < 4; ++n) w[n] = __builtin_amdgcn_perm(r.v[2 * n + 1][i][k], r.v[2 * n][i][k], sel);
-                        const f16x8 v = eight(w[0], w[1], w[2], w[3]);
-                        const int j = (i * R::kValWords + k) * 2 + e;
-                        o[j] = mfma(v, hi, o[j]);
-                        o[j] = mfma(v, lo, o[j]);
+                            for (int n = 0; n < 4; ++n) w[n] = __builtin_amdgcn_perm(r.v[2 * n + 1][i][k], r.v[2 * n][i][k], sel);
+                            add_values<kAsIs>(o[(i * R::kValWords + k) * 2 + e], eight(w[0], w[1], w[2], w[3]), pr, hi, lo);
+                        }
                     }
-                }
+            }
+            if (rarely(again)) load_row(u), load_keys<D, kInt8>(r, a, row, lane);
+            else ++u;
+            if (again || more) load_values<D, kInt8>(r, a, row, lane);
         }
-        if (more) load_values<D, kInt8>(r, a, row, lane);
+    };
+    turns(std::false_type{});
+    // an infinite value may have met a part that is 0 (a value that is no number shows either way)
+    bool odd = false;
+#pragma unroll
+    for (int j = 0; j < kOut; ++j) odd |= !(fabsf((o[j].x + o[j].y) + (o[j].z + o[j].w)) < kInf);
+    if (rarely(__any(odd))) {
+        load_row(u0);
+        load_keys<D, kInt8>(r, a, row, lane);
+        load_values<D, kInt8>(r, a, row, lane);
+        turns(std::true_type{});
     }
 
     // the waves' results to one m, summed through LDS
