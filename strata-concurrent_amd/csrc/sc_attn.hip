@@ -349,7 +349,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_part_kernel(AttnArgs a) 
     }
 #pragma unroll
     for (uint32_t i4 = 0; i4 < 4; ++i4) {
-        // an f32 head is scaled by a power of two to a largest value of 1 .. 2
+        // an f32 head is scaled by a power of two to a largest value of 2^14 .. 2^15, so that the two parts of values down to
+        // 2^-16 of that keep all bits: a key can be as much larger there
         const uint32_t i = i4 * 4 + wave;
         float x[D / 64], top = 0;
 #pragma unroll
@@ -361,11 +362,11 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_part_kernel(AttnArgs a) 
         if constexpr (!kF16) {
 #pragma unroll
             for (int m = 1; m < 64; m <<= 1) top = fmaxf(top, __shfl_xor(top, m));
-            if (top > 0 && top < kInf) {
-                const int e = int(__float_as_uint(top) >> 23) - 127;   // -127 for a subnormal: it stays below 1
-                const int f = e > 126 ? 126 : e < -126 ? -126 : e;
-                by = __uint_as_float(uint32_t(127 - f) << 23);
-                back = __uint_as_float(uint32_t(127 + f) << 23);
+            if (top > 0) {
+                // within what a power of two and its inverse can be; infinite for an infinite value, which stays one
+                const int e = int(__float_as_uint(top) >> 23) - 127, f = e > 127 ? 127 : e < -112 ? -112 : e;
+                by = __uint_as_float(uint32_t(127 + 14 - f) << 23);
+                back = __uint_as_float(uint32_t(127 - 14 + f) << 23);
             }
         }
         if (lane == 0) s_c[i] = a.scale * kLog2e * back;

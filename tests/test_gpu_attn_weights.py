@@ -193,3 +193,41 @@ def test_scores_beyond_all_measure(sc, ops, cuda, size):
     assert (np.abs(got[0, 0] - v[n - 1]) <= 2.0 ** -19 * np.abs(v[n - 1])).all() and (np.abs(got[0, 1] - v[0]) <= 2.0 ** -19 * np.abs(v[0])).all()
     assert abs(lse[0, 0] / (256 * (n - 1) * size * D ** -0.5) - 1) < 2.0 ** -22 and lse[0, 1] == 0
     assert np.abs(got[0, 2] - v[:n].mean(0)).max() < 2.0 ** -19
+
+
+@pytest.mark.parametrize("fmt", ["f16", "int8"])
+def test_queries_and_keys_of_many_sizes(sc, ops, cuda, fmt):
+    """A value of a query a million times smaller than its largest, where the keys are as much larger: the products count."""
+    rng = np.random.default_rng(8)
+    n, H, D, heads = 90, 1, 128, 8
+    cache = Cache(sc, ops, rng, fmt, H, D, 4, 1, 23, table=None, n_pages=23)
+    q = rng.standard_normal((1, heads, D)).astype(np.float32)
+    if fmt == "f16":
+        k = cache.host["k"].astype(np.float32) / 16
+        k[:, 0] = rng.uniform(-60000, 60000, len(k))
+        cache.host["k"] = k.astype(np.float16)
+        q[0, :, 0] = 1.37 * 2.0 ** -16
+    else:
+        cache.host["ks"][:, 0] = np.float16(500).view(np.uint16)
+        cache.host["ks"][:, 1] = np.float16(0.001).view(np.uint16)
+        q[0, :, :64] *= 2.0 ** -16
+    _put(cache)
+    got, lse = _run(sc, ops, cache, q, [n], 92)
+    _check(cache, q, n, got.astype(np.float64), lse)
+
+
+@pytest.mark.parametrize("fmt", ["f16", "int8"])
+def test_infinite_queries(sc, ops, cuda, fmt):
+    """An infinite value of a query makes every score an infinity of its key's sign: nothing is left where they are all negative,
+    no number where one is positive; values next to it that f16 does not hold change nothing."""
+    rng = np.random.default_rng(10)
+    n, H, D, heads = 40, 1, 64, 3
+    cache = Cache(sc, ops, rng, fmt, H, D, 4, 1, 10, table=None, n_pages=10)
+    cache.host["k"][:, 5] = -1 - np.arange(40) % 3
+    cache.host["k"][:, 6] = 1
+    _put(cache)
+    q = (rng.standard_normal((1, heads, D)) * 1e6).astype(np.float32)
+    q[0, 0, 5], q[0, 1, 5], q[0, 2, 5] = np.inf, -np.inf, 1
+    got, lse = _run(sc, ops, cache, q, [n], 40)
+    assert (got[0, 0] == 0).all() and lse[0, 0] == -np.inf
+    assert np.isnan(got[0, 1]).all() and np.isfinite(got[0, 2]).all()
