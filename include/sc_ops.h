@@ -141,10 +141,10 @@ typedef struct sc_gdn {
 /* One token of every sequence (tokens == n_seqs): state read, updated in place, one launch. */
 int sc_gdn_step_async(const sc_gdn* a, void* stream);
 /* Every sequence's tokens in order (a prompt, or a piece of one: the state goes on from what it holds).  A sequence
- * without tokens keeps its state; rows past cu[n_seqs] are left out.  Sums and states in 32 bits: the products of the
- * chunks run on the matrix cores in parts that keep f32 accuracy, for keys with beta * |k|^2 <= 2 (of unit length: beta <= 2),
- * which is where the rule itself does not diverge; beyond, a value may overflow.  Infinities and NaN stay in the
- * heads that they belong to.  The result does not depend on timing. */
+ * without tokens keeps its state; rows past cu[n_seqs] are left out.  Sums, states and the products of a chunk's rows with each
+ * other in 32 bits; products with the state run on the matrix cores in two f16 parts of each column's own size, which keep f32
+ * accuracy.  Infinities and NaN stay in the heads that they belong to, and reach no output before the 16 tokens (of a chunk of 64,
+ * from the sequence's first) that they are among.  The result does not depend on timing. */
 uint64_t sc_gdn_chunk_workspace_bytes(const sc_gdn* a);
 int sc_gdn_chunk_async(const sc_gdn* a, void* workspace, uint64_t workspace_bytes, void* stream);
 

@@ -11,15 +11,15 @@
 // crosses lanes but a column's largest value, and only parts of K M0 are exchanged.  The two others form the outputs from
 // the state and U that the first left in LDS; they also bring V, T and the factors of rows.
 //
-// Accuracy: the products run as f16 matrix instructions with sums in 32 bits, and keep f32 accuracy: an f32 operand is
-// two f16 parts (22 bits).  f16 keys and queries enter as they are, exactly, f32 ones scaled by row with a power of two;
-// unit length, decays and write strengths are factors of rows in f32.  The state, X and U share one power of two a column,
-// which changes only when the column's largest of |M0| and beta |V| leaves a window: with beta |k|^2 <= 2 (where the rule
-// does not diverge) X stays below 2^5 and U below 2^8 of that, inside f16's range, and what is lost of small values is
-// below 2^-27 of the largest (a window that began at 2^-3 instead of 2^2 made a state's error three times as large, 1.3e-6
-// after 8192 tokens).  Sums of log decays are in 64 bits: what counts is their differences.
+// Accuracy: T X and P U are products of 32-bit numbers, since a chunk's rows differ by whatever its gates leave of them.  The
+// other products run as f16 matrix instructions with sums in 32 bits, an f32 operand as two f16 parts: f16 keys and queries
+// enter as they are, f32 ones scaled by row with a power of two; unit length, decays and write strengths are factors of rows
+// in f32.  The state before a chunk and the writes U that are added to it have a power of two a column each, from its largest,
+// so that neither takes bits from the other.  A column of the state is held in the units that its last writes came in.  Sums of
+// log decays are in 64 bits: what counts is their differences.
 #include <hip/hip_runtime.h>
 
+#include <climits>
 #include <cstdint>
 
 #include "sc_ops.hpp"
@@ -31,17 +31,13 @@ constexpr int kC = 64;                       // tokens of a chunk
 constexpr int kWaves = 4, kThreadsC = kWaves * 64;
 constexpr float kLeastG = -200.0f;           // a decay of e^-200 is 0 in f32
 constexpr double kLog2e = 1.4426950408889634074;
-// Where a column's largest of |M0| and beta |V| lies as operands: below 2^kTop and not below 2^kLeast, else it is scaled
-// anew, to 2^kAim.
-constexpr int kTop = 7, kLeast = 2, kAim = 5;
+// A column's largest lies at 2^kAim to twice that as an f16 operand; its state is kept below 2^kFar of its units.
+constexpr int kAim = 14, kFar = 100;
 
-// Places of a v head's chunk in the workspace, in 16-byte words: T and P as matrix operands [wave][step][part][lane] (a
-// wave's row tile w has steps 0 .. w / 2 of 32 tokens), then the factors of rows.
-constexpr uint32_t kOperand = 6 * 2 * 64;
-constexpr uint32_t operand_at(uint32_t wave, uint32_t step, uint32_t part) {
-    return ((wave < 2 ? wave : wave == 2 ? 2 : 4) + step) * 128 + part * 64;
-}
-enum { kFState = 0, kFBeta = 64, kFWrite = 128, kFQuery = 192, kFRow = 256, kFDecay = 320, kFUp, kFBetaMost, kFactors = 324 };
+constexpr int tile_of(int r, int c) { return r * (r + 1) / 2 + c; }   // of the tiles of 16 x 16 up to the diagonal
+// Places of a v head's chunk in the workspace, in 16-byte words: T and P by tiles [tile][lane], then the factors of rows.
+constexpr uint32_t kOperand = 10 * 64;
+enum { kFState = 0, kFBeta = 64, kFWrite = 128, kFQuery = 192, kFDecay = 256, kFactors = 260 };
 constexpr uint32_t kChunkWords = 2 * kOperand + kFactors / 4;
 
 // Places of a key head's chunk in the workspace, in 16-byte words: its keys as the left operand of the state's update
@@ -62,23 +58,22 @@ __device__ __forceinline__ f32x4 mfma(ops_u32x4 a, ops_u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 __device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+// The product of two tiles of 32-bit numbers: a lane has four values of its row of the left one and, as results lie, of its
+// column of the right one.
+__device__ __forceinline__ f32x4 product(f32x4 x, f32x4 y, f32x4 acc) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) acc = mfma_f32(x[i], y[i], acc);
+    return acc;
+}
 
-// Two values, each times `by`, as two f16 parts: the product truncated, and what that left out.  The high part is taken by
-// the instruction that packs two, so that what is subtracted is what is multiplied later; the low part is one fused
-// multiply-add a value that rounds to f16 (which is why `by` is never the literal one: that would be a subtraction and a
-// conversion).
+// Two values, each times `by`, as two f16 parts: the product rounded to nearest, and what that left out rounded likewise (a
+// fused multiply-add a value).  What is subtracted is what is multiplied later, not a product that the compiler would round
+// once more.
 __device__ __forceinline__ void split2(float a, float b, float by_a, float by_b, uint32_t& hi, uint32_t& lo) {
-    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a * by_a, b * by_b));
+    hi = __builtin_bit_cast(uint32_t, f16x2{_Float16(a * by_a), _Float16(b * by_b)});
+    asm("" : "+v"(hi));
     const f16x2 h = __builtin_bit_cast(f16x2, hi);
     const f16x2 l{_Float16(__builtin_fmaf(a, by_a, -float(h.x))), _Float16(__builtin_fmaf(b, by_b, -float(h.y)))};
-    lo = __builtin_bit_cast(uint32_t, l);
-}
-__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
-    float one = 1.0f;
-    asm("" : "+s"(one));
-    hi = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(a, b));
-    const f16x2 h = __builtin_bit_cast(f16x2, hi);
-    const f16x2 l{_Float16(__builtin_fmaf(a, one, -float(h.x))), _Float16(__builtin_fmaf(b, one, -float(h.y)))};
     lo = __builtin_bit_cast(uint32_t, l);
 }
 // 2^-e and 2^e for the exponent of x >= 0 (its largest power of two not above), within f32's normal range; 1 for 0.
@@ -157,17 +152,6 @@ __device__ __forceinline__ bool seq_of_rank(const GdnArgs& a, uint32_t lane, uin
 
 // ---- every chunk's T and P ------------------------------------------------------------------------------------------------
 
-// The largest over the wave of values that are not negative, by row shifts and broadcasts.
-__device__ __forceinline__ float wave_most(float v) {
-    uint32_t x = __float_as_uint(v);
-    x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x111, 0xF, 0xF, false)));   // row_shr 1, 2, 4, 8
-    x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x112, 0xF, 0xF, false)));
-    x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x114, 0xF, 0xF, false)));
-    x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x118, 0xF, 0xF, false)));
-    x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x142, 0xA, 0xF, false)));   // lane 15 of a row to the next one
-    x = max(x, uint32_t(__builtin_amdgcn_update_dpp(0, int(x), 0x143, 0xC, 0xF, false)));   // lane 31 to the upper half
-    return __uint_as_float(last_lane(x));
-}
 template <int kCtrl, int kRows>
 __device__ __forceinline__ double dpp_add(double x) {
     const uint64_t b = __builtin_bit_cast(uint64_t, x);
@@ -192,20 +176,8 @@ __device__ __forceinline__ void wave_sync() {
 }
 
 constexpr int kTileRow = 20, kTileFloats = 16 * kTileRow + 4;   // a 16 x 16 tile in LDS: 16-byte rows, tiles on banks of their own
-constexpr int tile_of(int r, int c) { return r * (r + 1) / 2 + c; }
 
-// Eight values, four each of two tiles, as a right operand in two parts.
-__device__ __forceinline__ void split_pair(f32x4 a, f32x4 b, ops_u32x4& hi, ops_u32x4& lo) {
-    uint32_t h[4], l[4];
-    split2(a.x, a.y, h[0], l[0]);
-    split2(a.z, a.w, h[1], l[1]);
-    split2(b.x, b.y, h[2], l[2]);
-    split2(b.z, b.w, h[3], l[3]);
-    hi = ops_u32x4{h[0], h[1], h[2], h[3]};
-    lo = ops_u32x4{l[0], l[1], l[2], l[3]};
-}
-
-// The same of values times `by`.
+// Eight values, four each of two tiles, times `by`, as a right operand in two parts.
 __device__ __forceinline__ void split_pair(f32x4 a, f32x4 b, f32x4 by_a, f32x4 by_b, ops_u32x4& hi, ops_u32x4& lo) {
     uint32_t h[4], l[4];
     split2(a.x, a.y, by_a.x, by_a.y, h[0], l[0]);
@@ -372,27 +344,19 @@ __global__ void __launch_bounds__(kThreadsC, 4) gdn_prepare_kernel(GdnArgs a, Ch
     auto factor = [&](float squares, float by, bool there) {
         return !there ? 0.0f : a.l2norm ? __builtin_amdgcn_rsqf(squares + a.eps / by / by) : by;
     };
-    const float fk = factor(s_kk[lane], s_up[lane], in), k_most = wave_most(in ? __builtin_amdgcn_sqrtf(s_kk[lane]) * fk : 0.0f);
+    const float fk = factor(s_kk[lane], s_up[lane], in);
     float* f = reinterpret_cast<float*>(out + 2 * kOperand);
     if (wave == 0) {
         s_fk[lane] = fk;
-        // the weights of writes, at most 2 as an operand; scaled only where they need it
-        const float write = exp2_of(G_all - G) * fk, most = wave_most(write), beta_most = wave_most(fabsf(beta));
-        float down, up;
-        power_of(most >= 0x1p-10f && most < 2.0f ? 1.0f : most, down, up);
         f[kFState + lane] = beta * fk * exp2_of(G);
         f[kFBeta + lane] = beta;
-        f[kFWrite + lane] = write * down;
-        if (lane == 0) f[kFDecay] = exp2_of(G_all), f[kFUp] = up, f[kFBetaMost] = beta_most;
+        f[kFWrite + lane] = exp2_of(G_all - G) * fk;
+        if (lane == 0) f[kFDecay] = exp2_of(G_all);
     }
     if (g == 0) {
-        const bool there = mine < n;
-        const float squares = s_q[wave][0][col], fq = factor(squares, q_up, there);
-        float down, up;
-        power_of(there ? fabsf(a.scale) * __builtin_amdgcn_sqrtf(squares) * fq * k_most : 0.0f, down, up);
-        s_q[wave][1][col] = fq * a.scale * down;
-        f[kFQuery + mine] = a.scale * fq * exp2_of(s_G[mine]);
-        f[kFRow + mine] = up;
+        const float fq = factor(s_q[wave][0][col], q_up, mine < n) * a.scale;
+        s_q[wave][1][col] = fq;
+        f[kFQuery + mine] = fq * exp2_of(s_G[mine]);
     }
     __syncthreads();
     // A below the diagonal, and P, by way of LDS
@@ -421,16 +385,11 @@ __global__ void __launch_bounds__(kThreadsC, 4) gdn_prepare_kernel(GdnArgs a, Ch
         }
     }
     wave_sync();
-    // a row tile of P or T as the second kernel's operand: row col, places 0 .. 3 tokens 32 step + 4 g, 4 .. 7 16 more
+    // a row tile of P or T as the second kernel's left operands: row col, places 4 g .. + 3
     auto write_operand = [&](const float* from, uint32_t which) {
-        for (uint32_t step = 0; step <= wave / 2; ++step) {
-            const f32x4 u = *reinterpret_cast<const f32x4*>(&from[step * 2 * kTileFloats + col * kTileRow + g * 4]);
-            const f32x4 v = step * 2 + 1 <= wave ? *reinterpret_cast<const f32x4*>(&from[(step * 2 + 1) * kTileFloats + col * kTileRow + g * 4]) : f32x4{};
-            ops_u32x4 hi, lo;
-            split_pair(u, v, hi, lo);
-            st_global<ops_u32x4>(out + which * kOperand + operand_at(wave, step, 0) + lane, hi);
-            st_global<ops_u32x4>(out + which * kOperand + operand_at(wave, step, 1) + lane, lo);
-        }
+        for (uint32_t t = 0; t <= wave; ++t)
+            st_global<ops_u32x4>(out + which * kOperand + (wave * (wave + 1) / 2 + t) * 64 + lane,
+                                 *reinterpret_cast<const ops_u32x4*>(&from[t * kTileFloats + col * kTileRow + g * 4]));
     };
     write_operand(s_u.f.p + wave * (wave + 1) / 2 * kTileFloats, 1);
     // the diagonal tile of T, column col (the same in each group of lanes)
@@ -463,11 +422,6 @@ __global__ void __launch_bounds__(kThreadsC, 4) gdn_prepare_kernel(GdnArgs a, Ch
 #pragma unroll
         for (int i = 0; i < 4; ++i) x[i] = tile_at(t)[(g * 4 + i) * kTileRow + col];
         return x;
-    };
-    auto product = [&](f32x4 x, f32x4 y, f32x4 acc) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc = mfma_f32(x[i], y[i], acc);
-        return acc;
     };
     auto put = [&](int t, f32x4 x) {
 #pragma unroll
@@ -525,29 +479,12 @@ __device__ __forceinline__ float most_of(const f32x4 (&m)[kSteps][2]) {
             for (int j = 0; j < 4; j += 2) top = fmaxf(fmaxf(top, fabsf(m[i][e][j])), fabsf(m[i][e][j + 1]));
     return over_rows(top, max_of);
 }
-// A column's state is m times 2^up; scaled anew where its largest or that of beta V (`v_top`, unscaled) leaves the window.
-// `m_top` is the larger of m's in the column, in every wave that has a part of it; `down` is 2^-up.
-template <int kSteps>
-__device__ __forceinline__ void fit_scale(f32x4 (&m)[kSteps][2], int& up, float& down, float m_top, float v_top, float beta_most) {
-    down = __builtin_amdgcn_ldexpf(1.0f, -up);
-    const float top = fmaxf(m_top * beta_most, v_top * down);
-    if (__any(top >= float(1 << kTop) || (top > 0 && top < float(1 << kLeast)))) {
-        // to 2^kAim, within what f32 can scale by
-        const int e = int(__float_as_uint(top) >> 23) - 127 - kAim, to = up + e;
-        const int by = top == 0 ? 0 : (to > 120 ? 120 : to < -120 ? -120 : to) - up;
-        up += by;
-        down = __builtin_amdgcn_ldexpf(1.0f, -up);
-#pragma unroll
-        for (int i = 0; i < kSteps; ++i)
-#pragma unroll
-            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) m[i][e][j] = __builtin_amdgcn_ldexpf(m[i][e][j], -by);
-    }
-}
+// What a largest value is to be scaled down by to lie at 2^kAim, as an exponent whose power f32 holds either way.
+__device__ __forceinline__ int exponent_of(float top) { return max(int(__float_as_uint(top) >> 23) - 127 - kAim, -126); }
 // Keys 32 i + 8 g .. + 7 of the state as a right operand: the even ones and the odd ones take turns.
-__device__ __forceinline__ void split_state(const f32x4 (&m)[2], ops_u32x4& hi, ops_u32x4& lo) {
-    split_pair(f32x4{m[0].x, m[1].x, m[0].y, m[1].y}, f32x4{m[0].z, m[1].z, m[0].w, m[1].w}, hi, lo);
+__device__ __forceinline__ void split_state(const f32x4 (&m)[2], float by, ops_u32x4& hi, ops_u32x4& lo) {
+    const f32x4 four{by, by, by, by};
+    split_pair(f32x4{m[0].x, m[1].x, m[0].y, m[1].y}, f32x4{m[0].z, m[1].z, m[0].w, m[1].w}, four, four, hi, lo);
 }
 
 // kN tiles of 16 columns.  With one, both waves of the state form U from the whole of K M0; with two, each forms the one of
@@ -564,18 +501,18 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
     constexpr uint32_t kEach = kC * kPieces / (kOutWaves * 64);          // pieces of a lane
     // where registers are few, the keys' second form is asked for within its chunk and the first one at its end
     constexpr bool kAhead = kF16;
-    // Right operands are [tile][step][part][lane], results [tile of columns][tile of rows][lane].  A barrier opens a chunk and
-    // another is in its middle; what lies here is written in one half and read in the other, or the next chunk's first.
+    // Right operands are [tile][step][part][lane], results [tile of columns][tile of rows][lane].  A barrier opens a chunk,
+    // another is in its middle, a third where U is known; what lies here is written between two and read after the next.
     __shared__ ops_u32x4 s_m[kN][kSteps][2][64];              // the state before the chunk: first half, second
-    __shared__ ops_u32x4 s_u[kN][2][2][64];                   // U: second half, first
+    __shared__ f32x4 s_u[kN][4][64];                          // U: second half, last part of it
     __shared__ f32x4 s_v[kN][4][64];                          // beta V: first half, second
-    __shared__ ops_u32x4 s_t[6][2][64];                       // T: first half, second
+    __shared__ f32x4 s_t[10][64];                             // T: first half, second
     __shared__ f32x4 s_km[kShares][4][64];                    // K M0 by a wave's keys: first half, second
     __shared__ ops_u32x4 s_w[kN == 1 ? 1 : kN][2][2][64];     // U weighted for the state, with two tiles
     __shared__ __align__(16) uint8_t s_stage[kOutWaves][32 * kRowV];   // a wave's rows of V or O on their way
     __shared__ __align__(16) float s_f[2][(kFactors + 63) / 64 * 64];  // factors of rows: second half, all of the next and its next first
-    __shared__ int s_up[kN][16];                              // the power of two by which a column's m and u are to be scaled up
-    __shared__ float s_most[kOutWaves][kN][16];               // the largest of beta V by column: second half, first
+    __shared__ float s_back[kN][16];                          // what brings a column's products with the state back: first half, second
+    __shared__ int s_up[kN == 1 ? 1 : kN][16];                // the new units of a column's state, with two tiles
     __shared__ float s_top[kShares][kN][16];                  // the largest of a wave's state by column: second half, first
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t g = lane >> 4, col = lane & 15;
@@ -633,18 +570,6 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
                 for (int i = 0; i < N; ++i) x[part][i] = ld_global<ops_u32x4>(row_word(p, row_operand<S, kParts>(which, part, 0, i)));
         }
     };
-    // the product of n operands of a row tile from `first` on with a right operand [step][part]
-    auto triangle = [&](const auto& x, int first, int n, const ops_u32x4 (&y)[2][2]) {
-        f32x4 hi{}, lo{};
-#pragma unroll
-        for (int step = 0; step < n; ++step) {
-            hi = mfma(x[first + step][0], y[step][0], hi);
-            lo = mfma(x[first + step][0], y[step][1], lo);
-            lo = mfma(x[first + step][1], y[step][0], lo);
-        }
-        return hi + lo;
-    };
-
     if (wave < kShares) {
         // the state: keys 32 (first + i) + 8 g + 2 j + e in m[b][i][e][j], a column a lane
         const uint32_t first = wave * kMine;
@@ -692,21 +617,24 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
             const uint32_t ahead = clamped(chunk + 1);
             __syncthreads();
             const float* f = s_f[(chunk - c0) & 1];
-            // the state as a right operand
+            // the state as a right operand, its column's largest at 2^kAim
             ops_u32x4 mh[kN][kMine], ml[kN][kMine];
-            float down[kN];
-            const float beta_most = fmaxf(f[kFBetaMost], 1.0f);
+            float back[kN];
+            int reach[kN];   // the exponent of the column's largest, in all
 #pragma unroll
             for (int b = 0; b < kN; ++b) {
-                fit_scale<kMine>(m[b], up[b], down[b], fmaxf(s_top[0][b][col], s_top[kShares - 1][b][col]),
-                                 fmaxf(s_most[0][b][col], s_most[1][b][col]), beta_most);
+                const float top = fmaxf(s_top[0][b][col], s_top[kShares - 1][b][col]);
+                const int e = top > 0 ? exponent_of(top) : 0;
+                const float by = __builtin_amdgcn_ldexpf(1.0f, -e);
+                reach[b] = top > 0 ? e + up[b] + kAim : INT_MIN;
+                back[b] = __builtin_amdgcn_ldexpf(1.0f, e + up[b]);
 #pragma unroll
                 for (int i = 0; i < kMine; ++i) {
-                    split_state(m[b][i], mh[b][i], ml[b][i]);
+                    split_state(m[b][i], by, mh[b][i], ml[b][i]);
                     s_m[b][first + i][0][lane] = mh[b][i];
                     s_m[b][first + i][1][lane] = ml[b][i];
                 }
-                if (wave == 0 && g == 0) s_up[b][col] = up[b];
+                if (wave == 0 && g == 0) s_back[b][col] = back[b];
             }
             // K M0
             f32x4 km[kN][4];
@@ -724,6 +652,14 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
                         for (int b = 0; b < kN; ++b) km[b][r] = mfma(k[r][x == 2][i], x == 1 ? ml[b][i] : mh[b][i], km[b][r]);
             if (kAhead) load_keys(ahead);
             else load_turned(chunk);
+            // the factors of K M0's rows, with what brings it back; asked for now where there are registers
+            auto factors_of = [&](int r) {
+                return *reinterpret_cast<const f32x4*>(&f[kFState + r * 16 + g * 4]) * (kN == 1 ? float(back[0]) : pick(wave, back[kN - 1], back[0]));
+            };
+            f32x4 fs[4];
+            if constexpr (kN == 1)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) fs[r] = factors_of(r);
             // with one tile each wave's part goes to the other, with two the part of the other's tile
             const uint32_t tile = kN == 1 ? 0 : wave;
             if constexpr (kShares > 1) {
@@ -737,89 +673,119 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
                 if constexpr (kShares > 1) km[0][r] += s_km[wave ^ 1][r][lane];   // the same sum in both waves
             }
             // X; rows past the sequence's end are zero, as their V and factors are
-            ops_u32x4 xs[2][2];
-            {
-                const float by = kN == 1 ? float(down[0]) : pick(wave, down[kN - 1], down[0]);
-                f32x4 x[4];
+            f32x4 x[4], u[4];
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const f32x4 fs = *reinterpret_cast<const f32x4*>(&f[kFState + r * 16 + g * 4]), v = s_v[tile][r][lane];
+            for (int r = 0; r < 4; ++r) {
+                if constexpr (kN > 1) fs[r] = factors_of(r);
+                const f32x4 v = s_v[tile][r][lane];
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) x[r][j] = __builtin_fmaf(-fs[j], km[0][r][j], v[j] * by);
-                }
-                split_pair(x[0], x[1], xs[0][0], xs[0][1]);
-                split_pair(x[2], x[3], xs[1][0], xs[1][1]);
+                for (int j = 0; j < 4; ++j) x[r][j] = __builtin_fmaf(-fs[r][j], km[0][r][j], v[j]);
             }
-            // U = T X, and the same weighted for the state
+            // U = T X; weighted, it is what the state takes, its column's largest at 2^kAim.  With one tile of columns the state's
+            // waves have two row tiles each, five of T's ten tiles, and exchange them; with two, each has its columns'.
             ops_u32x4 ws[kN][2][2];
+            int to[kN];
             {
-                f32x4 u[4];
+                // the products of some of T's tiles with X's, a row's sums side by side
+                auto times = [&](auto& sums, const auto& rows, const auto& cols) {
+                    constexpr int n = sizeof(rows) / sizeof(rows[0]);
+                    f32x4 t[n];
+#pragma unroll
+                    for (int k = 0; k < n; ++k) t[k] = s_t[tile_of(rows[k], cols[k])][lane];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int k = 0; k < n; ++k) sums[k] = mfma_f32(t[k][i], x[cols[k]][i], sums[k]);
+                };
+                f32x4 fw[4];
+                if constexpr (kN == 1)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) fw[r] = *reinterpret_cast<const f32x4*>(&f[kFWrite + r * 16 + g * 4]);
+                if constexpr (kN == 1 && kShares == 2) {
+                    f32x4 y[3]{}, z[2]{};
+                    if (wave) {
+                        constexpr int rows[] = {1, 2, 2}, cols[] = {0, 0, 1}, rows2[] = {1, 2}, cols2[] = {1, 2};
+                        times(y, rows, cols);
+                        z[0] = y[0], z[1] = y[1];
+                        times(z, rows2, cols2);
+                        s_u[0][1][lane] = z[0];
+                        s_u[0][2][lane] = z[1] + y[2];
+                    } else {
+                        constexpr int rows[] = {0, 3, 3}, cols[] = {0, 0, 1}, rows2[] = {3, 3}, cols2[] = {2, 3};
+                        times(y, rows, cols);
+                        z[0] = y[1], z[1] = y[2];
+                        times(z, rows2, cols2);
+                        s_u[0][0][lane] = y[0];
+                        s_u[0][3][lane] = z[0] + z[1];
+                    }
+                    __syncthreads();   // the helpers wait for U here
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) u[r] = s_u[0][r][lane];
+                } else {
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        f32x4 sums[2]{};   // a chain half as long
+#pragma unroll
+                        for (int t = 0; t <= r; ++t) sums[t & 1] = product(s_t[tile_of(r, t)][lane], x[t], sums[t & 1]);
+                        u[r] = sums[0] + sums[1];
+                        s_u[tile][r][lane] = u[r];
+                    }
+                    if constexpr (kN == 1) __syncthreads();
+                }
+                float top = 0;
+                f32x4 w[4];
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int n = 1 + r / 2, from = r < 2 ? r : r * 2 - 2;
-                    ops_u32x4 t[2][2];
+                    if constexpr (kN > 1) fw[r] = *reinterpret_cast<const f32x4*>(&f[kFWrite + r * 16 + g * 4]);
 #pragma unroll
-                    for (int i = 0; i < n; ++i)
-#pragma unroll
-                        for (int part = 0; part < 2; ++part) t[i][part] = s_t[from + i][part][lane];
-                    u[r] = triangle(t, 0, n, xs);
-                    if (!kAhead) asm volatile("" ::: "memory");   // not all of T at once
-                }
-#pragma unroll
-                for (int step = 0; step < 2; ++step) {
-                    const f32x4 w0 = *reinterpret_cast<const f32x4*>(&f[kFWrite + step * 32 + g * 4]), w1 = *reinterpret_cast<const f32x4*>(&f[kFWrite + step * 32 + 16 + g * 4]);
-                    split_pair(u[step * 2], u[step * 2 + 1], w0, w1, ws[0][step][0], ws[0][step][1]);
-                    if (kN > 1) s_w[tile][step][0][lane] = ws[0][step][0], s_w[tile][step][1][lane] = ws[0][step][1];
-                    if (kN > 1 || kShares == 1 || uint32_t(step) == wave) {
-                        ops_u32x4 hi, lo;
-                        split_pair(u[step * 2], u[step * 2 + 1], hi, lo);
-                        s_u[tile][step][0][lane] = hi;
-                        s_u[tile][step][1][lane] = lo;
+                    for (int j = 0; j < 4; ++j) {
+                        w[r][j] = u[r][j] * fw[r][j];
+                        top = fmaxf(top, fabsf(w[r][j]));
                     }
                 }
+                top = over_rows(top, max_of);
+                const int most = kN == 1 ? reach[0] : pick(wave, reach[kN - 1], reach[0]), now = kN == 1 ? up[0] : pick(wave, up[kN - 1], up[0]);
+                to[0] = top > 0 ? max(max(exponent_of(top), most == INT_MIN ? INT_MIN : most - kFar), now - 126) : now;
+                const float by = __builtin_amdgcn_ldexpf(1.0f, -to[0]);
+                const f32x4 four{by, by, by, by};
+#pragma unroll
+                for (int step = 0; step < 2; ++step) {
+                    split_pair(w[step * 2], w[step * 2 + 1], four, four, ws[0][step][0], ws[0][step][1]);
+                    if (kN > 1) s_w[tile][step][0][lane] = ws[0][step][0], s_w[tile][step][1][lane] = ws[0][step][1];
+                }
+                if (kN > 1 && g == 0) s_up[tile][col] = to[0];
             }
             if constexpr (kN > 1) {
                 __syncthreads();
 #pragma unroll
-                for (int b = 0; b < kN; ++b)
+                for (int b = 0; b < kN; ++b) {
+                    to[b] = s_up[b][col];
 #pragma unroll
                     for (int step = 0; step < 2; ++step)
 #pragma unroll
                         for (int part = 0; part < 2; ++part) ws[b][step][part] = s_w[b][step][part][lane];
+                }
             }
-            // the state after the chunk
-            const float decay = f[kFDecay], w_up = f[kFUp];
-            const bool plain = __builtin_amdgcn_readfirstlane(int(w_up == 1.0f));   // nearly always
+            // the state after the chunk, in the units of what is added
 #pragma unroll
-            for (int b = 0; b < kN; ++b)
+            for (int b = 0; b < kN; ++b) {
+                const float decay = __builtin_amdgcn_ldexpf(f[kFDecay], up[b] - to[b]);
+                up[b] = to[b];
 #pragma unroll
                 for (int i = 0; i < kMine; ++i)
 #pragma unroll
                     for (int e = 0; e < 2; ++e) m[b][i][e] *= decay;
-            auto update = [&](f32x4 (&add)[kN][kMine][2]) {
+            }
 #pragma unroll
-                for (int step = 0; step < 2; ++step)
+            for (int step = 0; step < 2; ++step)
 #pragma unroll
-                    for (int x = 0; x < kParts + 1; ++x)
-#pragma unroll
-                        for (int i = 0; i < kMine; ++i)
-#pragma unroll
-                            for (int e = 0; e < 2; ++e)
-#pragma unroll
-                                for (int b = 0; b < kN; ++b) add[b][i][e] = mfma(kt[x == 2][i][e][step], ws[b][step][x == 1], add[b][i][e]);
-            };
-            if (plain) {
-                update(m);
-            } else {
-                f32x4 add[kN][kMine][2]{};
-                update(add);
-#pragma unroll
-                for (int b = 0; b < kN; ++b)
+                for (int x = 0; x < kParts + 1; ++x)
 #pragma unroll
                     for (int i = 0; i < kMine; ++i)
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) m[b][i][e] += w_up * add[b][i][e];
-            }
+                        for (int e = 0; e < 2; ++e)
+#pragma unroll
+                            for (int b = 0; b < kN; ++b) m[b][i][e] = mfma(kt[x == 2][i][e][step], ws[b][step][x == 1], m[b][i][e]);
             if (kAhead) load_turned(ahead);
             else load_keys(ahead);
 #pragma unroll
@@ -841,14 +807,15 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
         return;
     }
 
-    // The other waves: V, T and the factors, and the outputs, whose part from U is formed a chunk behind.  Wave w of the two
-    // takes the row tiles w and 3 - w, which have three operands of P's six.
+    // The other waves: V, T and the factors, and the outputs, whose part from U is formed where U is known.  Wave w of the two
+    // takes the row tiles w and 3 - w, which have five of P's ten.
     const uint32_t w = wave - kShares, v_ld = uint32_t(a.v_ld);
     uint8_t* stage = s_stage[w];
-    auto tile_of = [&](uint32_t i) { return i ? 3 - w : w; };
-    auto row_at = [&](uint32_t at) { return tile_of(at / (16 * kPieces)) * 16 + at / kPieces % 16; };   // of piece `at` of the wave's rows
-    ops_u32x4 v_in[kEach], t_in[6];
-    float f_in[4];
+    auto row_tile = [&](uint32_t i) { return i ? 3 - w : w; };
+    auto row_at = [&](uint32_t at) { return row_tile(at / (16 * kPieces)) * 16 + at / kPieces % 16; };   // of piece `at` of the wave's rows
+    ops_u32x4 v_in[kEach];
+    f32x4 t_in[5];
+    float f_in[3];
     f32x4 v[kN][2];
     auto factor_at = [&](uint32_t i) { return (i == 0 ? 1 : w ? i + 2 : (i - 1) * 2) * 64 + lane; };   // both have kFBeta's
     auto load_early = [&](uint32_t chunk) {
@@ -861,7 +828,7 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
         }
         const float* f = reinterpret_cast<const float*>(operands_of(chunk) + 2 * kOperand);
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) f_in[i] = ld_global<float>(f + min(factor_at(i), uint32_t(kFactors - 1)));
+        for (uint32_t i = 0; i < 3; ++i) f_in[i] = ld_global<float>(f + min(factor_at(i), uint32_t(kFactors - 1)));
     };
     // V as the state's waves take it, by way of LDS: times beta, rows past the sequence's end zero, a lane's four rows together
     auto put_early = [&](uint32_t chunk, uint32_t n) {
@@ -873,54 +840,63 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
             *reinterpret_cast<ops_u32x4*>(&stage[at * 16]) = row_at(at) <= last ? v_in[i] : ops_u32x4{};
         }
 #pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) f[factor_at(i)] = f_in[i];
+        for (uint32_t i = 0; i < 3; ++i) f[factor_at(i)] = f_in[i];
         wave_sync();
 #pragma unroll
         for (int b = 0; b < kN; ++b) {
-            float top = 0;
 #pragma unroll
             for (uint32_t i = 0; i < 2; ++i) {
-                f32x4 x = *reinterpret_cast<const f32x4*>(&f[kFBeta + tile_of(i) * 16 + g * 4]);
+                f32x4 x = *reinterpret_cast<const f32x4*>(&f[kFBeta + row_tile(i) * 16 + g * 4]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const uint8_t* p = &stage[(i * 16 + g * 4 + j) * kRowV + (b * 16 + col) * kBytes];
                     if constexpr (kF16) x[j] *= float(*reinterpret_cast<const _Float16*>(p));
                     else x[j] *= *reinterpret_cast<const float*>(p);
-                    top = fmaxf(top, fabsf(x[j]));
                 }
                 v[b][i] = x;
             }
-            top = over_rows(top, max_of);
-            if (g == 0) s_most[w][b][col] = top;
         }
         wave_sync();
     };
     auto load_t = [&](uint32_t chunk) {
 #pragma unroll
-        for (int i = 0; i < 6; ++i) t_in[i] = ld_global<ops_u32x4>(operands_of(chunk) + (w * 6 + i) * 64 + lane);
+        for (int i = 0; i < 5; ++i) t_in[i] = ld_global<f32x4>(operands_of(chunk) + (w * 5 + i) * 64 + lane);
     };
-    ops_u32x4 qs[2][kParts][kSteps], p[3][2];
+    ops_u32x4 qs[2][kParts][kSteps];
+    f32x4 p[5];
     auto load_queries = [&](uint32_t chunk) {
         load_rows(qs[0], chunk, 1, w, 0);
         load_rows(qs[1], chunk, 1, 3 - w, 0);
     };
-    // P's operand w, and the two of tile 3 - w
+    // P's tiles of rows w, then those of rows 3 - w
     auto load_p = [&](uint32_t chunk) {
         const ops_u32x4* from = operands_of(chunk) + kOperand + lane;
 #pragma unroll
-        for (int i = 0; i < 3; ++i)
-#pragma unroll
-            for (int part = 0; part < 2; ++part) p[i][part] = ld_global<ops_u32x4>(from + ((i == 0 ? w : 3 - 2 * w + i) * 2 + part) * 64);
+        for (uint32_t i = 0; i < 5; ++i) p[i] = ld_global<f32x4>(from + (i <= w ? w * (w + 1) / 2 + i : (3 - w) * (4 - w) / 2 + i - w - 1) * 64);
     };
-    f32x4 qm[kN][2];
-    int up[kN];
+    f32x4 qm[kN][2], sum[kN][2];
+    float back[kN];
+    // P U: a wave's second tile is of rows w or 3 - w
+    auto products = [&] {
+#pragma unroll
+        for (int b = 0; b < kN; ++b) {
+            sum[b][0] = product(p[0], s_u[b][0][lane], f32x4{});
+            const f32x4 x = product(p[1], s_u[b][w][lane], w ? sum[b][0] : f32x4{});
+            sum[b][1] = w ? f32x4{} : x;
+            if (w) sum[b][0] = x;
+            f32x4 odd = product(p[3], s_u[b][2 - w][lane], f32x4{});   // in two sums: a chain half as long
+            sum[b][1] = product(p[2], s_u[b][1 - w][lane], sum[b][1]);
+            odd = product(p[4], s_u[b][3 - w][lane], odd);
+            sum[b][1] += odd;
+        }
+    };
     auto first_half = [&](uint32_t chunk) {
 #pragma unroll
         for (int b = 0; b < kN; ++b)
 #pragma unroll
-            for (uint32_t i = 0; i < 2; ++i) s_v[b][tile_of(i)][lane] = v[b][i];
+            for (uint32_t i = 0; i < 2; ++i) s_v[b][row_tile(i)][lane] = v[b][i];
 #pragma unroll
-        for (uint32_t i = 0; i < 6; ++i) s_t[(w * 6 + i) / 2][i % 2][lane] = t_in[i];
+        for (uint32_t i = 0; i < 5; ++i) s_t[w * 5 + i][lane] = t_in[i];
         load_t(clamped(chunk + 1));
     };
     auto second_half = [&](uint32_t chunk) {
@@ -940,9 +916,11 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
                     for (int r = 0; r < 2; ++r) qm[b][r] = mfma(qs[r][x == 2][i], x == 1 ? lo : hi, qm[b][r]);
             }
 #pragma unroll
-        for (int b = 0; b < kN; ++b) up[b] = s_up[b][col];
+        for (int b = 0; b < kN; ++b) back[b] = s_back[b][col];
         load_queries(clamped(chunk + 1));
-        if constexpr (kN > 1) __syncthreads();
+        __syncthreads();
+        products();
+        load_p(clamped(chunk + 1));
         put_early(clamped(chunk + 1), chunk + 1 - c0);
         load_early(clamped(chunk + 2));
     };
@@ -951,26 +929,19 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
         const float* f = s_f[(done - c0) & 1];
 #pragma unroll
         for (int b = 0; b < kN; ++b) {
-            ops_u32x4 us[2][2];
-#pragma unroll
-            for (int step = 0; step < 2; ++step)
-#pragma unroll
-                for (int part = 0; part < 2; ++part) us[step][part] = s_u[b][step][part][lane];
 #pragma unroll
             for (uint32_t r = 0; r < 2; ++r) {
-                const f32x4 sum = r ? triangle(p, 1, 2, us) : triangle(p, 0, 1, us);
-                const uint32_t row = tile_of(r) * 16 + g * 4;
-                const f32x4 fq = *reinterpret_cast<const f32x4*>(&f[kFQuery + row]), fr = *reinterpret_cast<const f32x4*>(&f[kFRow + row]);
+                const uint32_t row = row_tile(r) * 16 + g * 4;
+                const f32x4 fq = *reinterpret_cast<const f32x4*>(&f[kFQuery + row]);
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float o = __builtin_amdgcn_ldexpf(fq[j] * qm[b][r][j] + fr[j] * sum[j], up[b]);
+                    const float o = __builtin_fmaf(fq[j], qm[b][r][j] * back[b], sum[b][r][j]);
                     uint8_t* to = &stage[(r * 16 + g * 4 + j) * kRowV + (b * 16 + col) * kBytes];
                     if constexpr (kF16) *reinterpret_cast<_Float16*>(to) = _Float16(o);
                     else *reinterpret_cast<float*>(to) = o;
                 }
             }
         }
-        load_p(clamped(done + 1));
         wave_sync();
         uint8_t* to = a.out + int64_t(q.t0 + (done - q.chunk0) * kC) * a.out_ld + (h * S + block * kCols) * kBytes;
         uint32_t o_ld = __builtin_amdgcn_readfirstlane(uint32_t(a.out_ld));
