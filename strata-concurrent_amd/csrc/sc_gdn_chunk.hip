@@ -13,8 +13,8 @@
 //
 // Accuracy: T X and P U are products of 32-bit numbers, since a chunk's rows differ by whatever its gates leave of them.  The
 // other products run as f16 matrix instructions with sums in 32 bits, an f32 operand as two f16 parts: f16 keys and queries
-// enter as they are, f32 ones scaled by row with a power of two; unit length, decays and write strengths are factors of rows
-// in f32.  The state before a chunk and the writes U that are added to it have a power of two a column each, from its largest,
+// enter as they are, f32 ones, and all keys that the state takes, scaled by row with a power of two, so that no row's weight
+// is larger for its key being short; unit length, decays and write strengths are factors of rows in f32.  The state before a chunk and the writes U that are added to it have a power of two a column each, from its largest,
 // so that neither takes bits from the other.  A column of the state is held in the units that its last writes came in.  Sums of
 // log decays are in 64 bits: what counts is their differences.
 #include <hip/hip_runtime.h>
@@ -27,6 +27,7 @@
 namespace sc {
 namespace {
 
+using u16x2 = __attribute__((ext_vector_type(2))) uint16_t;
 constexpr int kC = 64;                       // tokens of a chunk
 constexpr int kWaves = 4, kThreadsC = kWaves * 64;
 constexpr float kLeastG = -200.0f;           // a decay of e^-200 is 0 in f32
@@ -210,6 +211,7 @@ __global__ void __launch_bounds__(kThreadsC, 4) gdn_prepare_kernel(GdnArgs a, Ch
     float* s_tile = s_u.f.t;
     __shared__ double s_G[kC];
     __shared__ float s_beta[kC], s_fk[kC], s_kk[kC], s_up[kC], s_q[kWaves][2][16];
+    __shared__ int s_short[kC];   // f16 keys: the power of two that they are scaled up by for the state's update
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t g = lane >> 4, col = lane & 15;
     // workgroups go to the eight XCDs in turn: the value heads of a key head are kept on one, whose L2 then has its rows
@@ -275,6 +277,15 @@ __global__ void __launch_bounds__(kThreadsC, 4) gdn_prepare_kernel(GdnArgs a, Ch
     };
     const float k_up = to_operand(k_raw, kf, 0);
     if (g == 0) s_up[mine] = k_up;
+    if constexpr (kF16) {   // to a largest value of 2^14 .. 2^15, without loss; longer ones as they are
+        u16x2 most{};
+#pragma unroll
+        for (int i = 0; i < kSteps; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, kf[0][i][j] & 0x7FFF7FFFu));
+        const float top = over_rows(float(__builtin_bit_cast(_Float16, max(most.x, most.y))), max_of);
+        if (g == 0) s_short[mine] = top > 0 ? max(14 + 127 - int(__float_as_uint(top) >> 23), 0) : 0;
+    }
 #pragma unroll
     for (int part = 0; part < kParts; ++part)
 #pragma unroll
@@ -328,8 +339,14 @@ __global__ void __launch_bounds__(kThreadsC, 4) gdn_prepare_kernel(GdnArgs a, Ch
             for (int step = 0; step < 2; ++step) {
                 uint32_t w[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j)
+                for (int j = 0; j < 8; ++j) {
                     w[j] = reinterpret_cast<const uint32_t*>(&s_k[part][step * 2 + j / 4][wave][col / 4 * 16 + g * 4 + j % 4])[col % 4];
+                    if constexpr (kF16) {
+                        const float by = __builtin_amdgcn_ldexpf(1.0f, s_short[step * 32 + j / 4 * 16 + g * 4 + j % 4]);
+                        const f16x2 k = __builtin_bit_cast(f16x2, w[j]);
+                        w[j] = __builtin_bit_cast(uint32_t, f16x2{_Float16(float(k.x) * by), _Float16(float(k.y) * by)});
+                    }
+                }
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     const uint32_t sel = e ? 0x07060302u : 0x05040100u;
@@ -350,7 +367,9 @@ __global__ void __launch_bounds__(kThreadsC, 4) gdn_prepare_kernel(GdnArgs a, Ch
         s_fk[lane] = fk;
         f[kFState + lane] = beta * fk * exp2_of(G);
         f[kFBeta + lane] = beta;
-        f[kFWrite + lane] = exp2_of(G_all - G) * fk;
+        // a key that is 0 writes nothing, whatever its factor
+        const float write = s_kk[lane] == 0 ? 0.0f : exp2_of(G_all - G) * fk;
+        f[kFWrite + lane] = kF16 ? __builtin_amdgcn_ldexpf(write, -s_short[lane]) : write;
         if (lane == 0) f[kFDecay] = exp2_of(G_all);
     }
     if (g == 0) {
