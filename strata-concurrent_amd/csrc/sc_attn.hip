@@ -47,6 +47,7 @@ constexpr int kAttnThreads = kAttnWaves * 64;
 // what is summed stays below 2^125.  Cells that are too small even then, and below kWait (an int8 cell's weights differ by its
 // blocks' scales), wait for another go at the same turn, with an m of their own: each go takes its largest, so there is an end.
 constexpr float kTop = 11.0f, kDeep = 14.0f, kMost = 15.0f, kLeast = -8.0f, kWait = 5.0f, kFar = 76.0f;
+constexpr float kNear = 12.0f, kNearBy = 0x1p12f;
 constexpr float kTiny = 0x1p-126f;
 
 // 2^x by the hardware's instruction (1 unit in the last place; results below the normal range are 0).
@@ -524,10 +525,11 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_part_kernel(AttnArgs a) 
 #pragma unroll
                 for (int j = 0; j < kOut; ++j) o[j] *= w;
             }
-            const float ref = m == -kInf ? 0.0f : m;
+            // by way of a reference near the largest: a difference from m itself would round the exponents of weights near 1
+            const float ref = m == -kInf ? 0.0f : m + kNear;
             float pr[8];
 #pragma unroll
-            for (int n = 0; n < 8; ++n) pr[n] = exp2_fast(x[n] - ref);
+            for (int n = 0; n < 8; ++n) pr[n] = exp2_fast(x[n] - ref) * kNearBy;
             again = false;
             if (!kAsIs && rarely(__any(low < m + kLeast))) {
                 bool left = false;

@@ -231,3 +231,23 @@ def test_infinite_queries(sc, ops, cuda, fmt):
     got, lse = _run(sc, ops, cache, q, [n], 40)
     assert (got[0, 0] == 0).all() and lse[0, 0] == -np.inf
     assert np.isnan(got[0, 1]).all() and np.isfinite(got[0, 2]).all()
+
+
+@pytest.mark.parametrize("fmt", ["f16", "int8"])
+def test_few_cells_as_32_bits_have_them(sc, ops, cuda, fmt):
+    """The root of the mean squared error of 5 cells' outputs, relative to sum w |v| / sum w.  A weight's parts: its score's sum and
+    scaling (a score of one: 2^-23.6), the difference from the reference (at most 4: 2^-24.3), the exponential (2^-24.7), its two f16
+    parts (2^-25), together 2^-23.1, of five cells with weights of like size half as much; 2^-23.5 leaves the rest to the sums."""
+    rng = np.random.default_rng(11)
+    n, H, D, heads = 5, 2, 64, 1024
+    cache = Cache(sc, ops, rng, fmt, H, D, 4, 1, 2, table=None, n_pages=2)
+    q = rng.standard_normal((1, heads, D)).astype(np.float32)
+    got, _ = _run(sc, ops, cache, q, [n], 8)
+    k, v = _rows(cache, n)
+    off = []
+    for i in range(heads):
+        s = (k[:, i // 512] @ q[0, i].astype(np.float64)) * D ** -0.5
+        w = np.exp(s - s.max())
+        off.append((got[0, i] - w @ v[:, i // 512] / w.sum()) / (w @ np.abs(v[:, i // 512]) / w.sum()))
+    rms = np.sqrt(np.mean(np.square(off)))
+    assert rms <= 2.0 ** -23.5, np.log2(rms)
