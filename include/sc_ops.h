@@ -135,7 +135,8 @@ typedef struct sc_gdn {
                                  a slot: its out rows are zeros */
     int64_t state_offset;     /* floats from the base to this layer's state (e.g. a multiple of sc_gdn_row_floats) */
     int64_t state_head_ld;    /* floats between heads: S in a slot's (S, HV, S) row, S * S in the prefill layout */
-    int64_t state_key_ld;     /* floats between keys: HV * S in a slot's row, S in the prefill layout */
+    int64_t state_key_ld;     /* floats between keys: HV * S in a slot's row, S in the prefill layout.  All three multiples of 4, at
+                                 most 2^40; the heads lie inside a key's row or the keys inside a head's block */
 } sc_gdn;
 
 /* One token of every sequence (tokens == n_seqs): state read, updated in place, one launch. */

@@ -132,8 +132,10 @@ int gdn_args(const char* op, const sc_gdn* d, bool step, sc::GdnArgs& a) {
     if (d->state_offset < 0 || d->state_offset % 4 || d->state_head_ld < S || d->state_head_ld % 4 || d->state_key_ld < S ||
         d->state_key_ld % 4)
         return bad(op, "state strides must be multiples of 4 floats and hold a row");
-    // heads inside a key's row, or keys inside a head's block: anything else puts two values in one place
-    if (d->state_key_ld < d->v_heads * d->state_head_ld && d->state_head_ld < S * d->state_key_ld)
+    constexpr int64_t most = int64_t(1) << 40;
+    if (d->state_offset > most || d->state_head_ld > most || d->state_key_ld > most) return bad(op, "state strides must be at most 2^40 floats");
+    // the heads' rows inside a key's, or the keys' inside a head's block: anything else puts two values in one place
+    if (d->state_key_ld < (d->v_heads - 1) * d->state_head_ld + S && d->state_head_ld < (S - 1) * d->state_key_ld + S)
         return bad(op, "state strides overlap");
     if (!(d->eps >= 0)) return bad(op, "eps must not be negative");
     const int64_t b = value_bytes(d->dtype);

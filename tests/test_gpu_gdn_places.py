@@ -44,3 +44,38 @@ def test_outputs_over_the_values_and_in_one_buffer(sc, ops, cuda, lens, step, dt
         found.append((np.ascontiguousarray(got), state.numpy()))
     for got, state in found[1:]:
         assert np.array_equal(got.view(np.uint8), found[0][0].view(np.uint8)) and np.array_equal(state.view(np.uint8), found[0][1].view(np.uint8))
+
+
+@pytest.mark.parametrize("heads,head_ld,key_ld", [(4, 68, 3 * 68 + 64), (4, 63 * 72 + 64, 72), (1, 64 * 64, 72), (1, 68, 64)])
+@pytest.mark.parametrize("step", [True, False], ids=["step", "chunk"])
+def test_states_with_room_between(sc, ops, cuda, step, heads, head_ld, key_ld):
+    """Heads or keys apart by more than their rows, to the last float: the packed states' bits, and the room between untouched."""
+    S, n, N = 64, 3, 3 if step else 100
+    rng = np.random.default_rng(heads + key_ld)
+    q, k, v = (upload(sc, rng.standard_normal((N, heads * S)).astype(np.float32)) for _ in range(3))
+    gates = [upload(sc, x.astype(np.float32)) for x in (-rng.random((N, heads)), rng.random((N, heads)))]
+    cu = None if step else upload(sc, np.array([0, 70, 70, 100], np.int64))
+    M = rng.standard_normal((n, heads, S, S)).astype(np.float32)   # [head][key][value]
+    each = (heads - 1) * head_ld + (S - 1) * key_ld + S
+    flat = np.full((n, each + 4), 7, np.float32)
+    at = (np.arange(heads) * head_ld)[:, None, None] + (np.arange(S) * key_ld)[:, None] + np.arange(S)
+    flat[:, at] = M
+    found = []
+    for packed in (True, False):
+        state = upload(sc, M if packed else flat)
+        if packed:
+            states = ops.gdn_states(state, n_seqs=n, v_heads=heads, state_size=S, layout="prefill")
+        else:
+            states = ops.GdnStates([state.ptr + 4 * i * (each + 4) for i in range(n)], heads, S, 0, head_ld, key_ld, keep=state)
+        out = upload(sc, np.zeros((N, heads * S), np.float32))
+        make = ops.GdnStep if step else ops.GdnChunk
+        make(states, q, k, v, *gates, out, "f32", k_heads=heads, n_seqs=n, tokens=N, cu=cu, scale=S ** -0.5, l2norm=True).launch()
+        sc.device_sync()
+        got = state.numpy()
+        if not packed:
+            rest = np.ones(got.shape, bool)
+            rest[:, at] = False
+            assert (got[rest] == 7).all()
+            got = np.ascontiguousarray(got[:, at])
+        found.append((out.numpy(), got))
+    assert all(np.array_equal(a.view(np.uint8), b.view(np.uint8)) for a, b in zip(*found))

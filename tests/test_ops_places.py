@@ -65,3 +65,34 @@ def test_a_batch_without_tokens_has_no_rows(sc, ops):
                     out=FAKE, q_ld=512, k_ld=512, v_ld=512, out_ld=512, g=FAKE, beta=FAKE, gate_ld=8, scale=0.1, l2norm=1, eps=1e-6,
                     state=FAKE, state_offset=0, state_head_ld=64, state_key_ld=512)
     assert sc.lib.sc_gdn_chunk_async(C.byref(a), FAKE, 1 << 40, None) == sc.SC_OK
+
+
+STRIDES = [(68, 7 * 68 + 64), (64, 512), (64 * 64, 64), (63 * 72 + 64, 72), (1 << 40, 64), (64, 1 << 40)]   # heads, keys
+STRIDES_REFUSED = [(68, 7 * 68 + 60), (63 * 72 + 60, 72), (128, 512), (1 << 62, 64), (64, 1 << 62), ((1 << 40) + 4, 64)]
+
+
+def _strides(sc, ops, step, v_heads, head_ld, key_ld, offset=0):
+    n = 5
+    a = ops.GdnDesc(k_heads=v_heads, v_heads=v_heads, state_size=64, n_seqs=n if step else 1, tokens=n, cu=None if step else FAKE,
+                    dtype=sc.SC_DTYPE_F32, q=FAKE, k=FAKE, v=FAKE + MIB, out=FAKE + 2 * MIB, q_ld=512, k_ld=512, v_ld=512, out_ld=512,
+                    g=FAKE, beta=FAKE, gate_ld=8, scale=0.1, l2norm=1, eps=1e-6, state=FAKE, state_offset=offset, state_head_ld=head_ld,
+                    state_key_ld=key_ld)
+    code = sc.lib.sc_gdn_step_async(C.byref(a), None) if step else sc.lib.sc_gdn_chunk_async(C.byref(a), FAKE, 1 << 40, None)
+    return code, sc.last_error()
+
+
+@pytest.mark.parametrize("step", [True, False], ids=["step", "chunk"])
+@pytest.mark.parametrize("v_heads,head_ld,key_ld", [(8, *x) for x in STRIDES] + [(1, 64, 64), (1, 4096, 72), (1, 68, 64)])
+def test_states_apart_are_taken(sc, ops, step, v_heads, head_ld, key_ld):
+    if sc.device_count() > 0:
+        pytest.skip("the addresses are none: only where nothing can be launched")
+    code, why = _strides(sc, ops, step, v_heads, head_ld, key_ld)
+    assert code == sc.SC_EHIP, why
+
+
+@pytest.mark.parametrize("step", [True, False], ids=["step", "chunk"])
+@pytest.mark.parametrize("head_ld,key_ld", STRIDES_REFUSED)
+def test_states_that_meet_are_refused(sc, ops, step, head_ld, key_ld):
+    code, why = _strides(sc, ops, step, 8, head_ld, key_ld)
+    assert code == sc.SC_EINVAL and "state strides" in why, why
+    assert _strides(sc, ops, step, 8, 64, 512, 1 << 62)[0] == sc.SC_EINVAL
