@@ -519,13 +519,13 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
     constexpr uint32_t kRowV = kCols * kBytes, kPieces = kRowV / 16;     // a row of V or O of this workgroup, in 16-byte pieces
     constexpr uint32_t kEach = kC * kPieces / (kOutWaves * 64);          // pieces of a lane
     // where registers are few, the keys' second form is asked for within its chunk and the first one at its end
-    constexpr bool kAhead = kF16;
+    constexpr bool kAhead = kF16, kOwnT = kF16 && kN == 1 && kShares == 2;
     // Right operands are [tile][step][part][lane], results [tile of columns][tile of rows][lane].  A barrier opens a chunk,
     // another is in its middle, a third where U is known; what lies here is written between two and read after the next.
     __shared__ ops_u32x4 s_m[kN][kSteps][2][64];              // the state before the chunk: first half, second
     __shared__ f32x4 s_u[kN][4][64];                          // U: second half, last part of it
     __shared__ f32x4 s_v[kN][4][64];                          // beta V: first half, second
-    __shared__ f32x4 s_t[10][64];                             // T: first half, second
+    __shared__ f32x4 s_t[kOwnT ? 1 : 10][64];                 // T: first half, second
     __shared__ f32x4 s_km[kShares][4][64];                    // K M0 by a wave's keys: first half, second
     __shared__ ops_u32x4 s_w[kN == 1 ? 1 : kN][2][2][64];     // U weighted for the state, with two tiles
     __shared__ __align__(16) uint8_t s_stage[kOutWaves][32 * kRowV];   // a wave's rows of V or O on their way
@@ -589,6 +589,9 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
                 for (int i = 0; i < N; ++i) x[part][i] = ld_global<ops_u32x4>(row_word(p, row_operand<S, kParts>(which, part, 0, i)));
         }
     };
+    // The five tiles up to the diagonal of rows w and then of rows 3 - w.
+    auto row_and_other = [](uint32_t w, uint32_t i) { return i <= w ? w * (w + 1) / 2 + i : (3 - w) * (4 - w) / 2 + i - w - 1; };
+
     if (wave < kShares) {
         // the state: keys 32 (first + i) + 8 g + 2 j + e in m[b][i][e][j], a column a lane
         const uint32_t first = wave * kMine;
@@ -608,6 +611,12 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
 #pragma unroll
             for (int i = 0; i < kMine; ++i) asm volatile("" : "+v"(m[b][i][0]), "+v"(m[b][i][1]));
         ops_u32x4 k[4][kParts][kMine], kt[kParts][kMine][2][2];
+        f32x4 t_own[kOwnT ? 5 : 1];   // a wave's two rows of T's tiles
+        auto load_t = [&](uint32_t chunk) {
+            const ops_u32x4* from = operands_of(chunk) + lane;
+#pragma unroll
+            for (uint32_t i = 0; i < 5; ++i) t_own[kOwnT ? i : 0] = ld_global<f32x4>(from + row_and_other(wave, i) * 64);
+        };
         auto load_keys = [&](uint32_t chunk) {
 #pragma unroll
             for (int r = 0; r < 4; ++r) load_rows(k[r], chunk, 0, r, first);
@@ -624,6 +633,7 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
                         for (int step = 0; step < 2; ++step) kt[part][i][e][step] = ld_global<ops_u32x4>(row_word(p, key_operand<S, kParts>(part, i, e, step)));
         };
         load_keys(c0);
+        if (kOwnT) load_t(c0);
         if (kAhead) load_turned(c0);
         int up[kN];   // a column's state is m times 2^up
 #pragma unroll
@@ -705,38 +715,34 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
             ops_u32x4 ws[kN][2][2];
             int to[kN];
             {
-                // the products of some of T's tiles with X's, a row's sums side by side
-                auto times = [&](auto& sums, const auto& rows, const auto& cols) {
-                    constexpr int n = sizeof(rows) / sizeof(rows[0]);
-                    f32x4 t[n];
-#pragma unroll
-                    for (int k = 0; k < n; ++k) t[k] = s_t[tile_of(rows[k], cols[k])][lane];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-#pragma unroll
-                        for (int k = 0; k < n; ++k) sums[k] = mfma_f32(t[k][i], x[cols[k]][i], sums[k]);
-                };
                 f32x4 fw[4];
                 if constexpr (kN == 1)
 #pragma unroll
                     for (int r = 0; r < 4; ++r) fw[r] = *reinterpret_cast<const f32x4*>(&f[kFWrite + r * 16 + g * 4]);
                 if constexpr (kN == 1 && kShares == 2) {
-                    f32x4 y[3]{}, z[2]{};
+                    f32x4 t[5];
+#pragma unroll
+                    for (uint32_t i = 0; i < 5; ++i) t[i] = kOwnT ? t_own[i] : s_t[row_and_other(wave, i)][lane];
+                    // the sums of both rows side by side: row `wave`, and in two row 3 - wave
+                    auto times = [&](f32x4 (&y)[3], const f32x4 (&a)[3], const f32x4 (&b)[3], int n) {
+#pragma unroll
+                        for (int i = 0; i < 4; ++i)
+#pragma unroll
+                            for (int j = 0; j < n; ++j) y[j] = mfma_f32(a[j][i], b[j][i], y[j]);
+                    };
+                    f32x4 y[3]{};
                     if (wave) {
-                        constexpr int rows[] = {1, 2, 2}, cols[] = {0, 0, 1}, rows2[] = {1, 2}, cols2[] = {1, 2};
-                        times(y, rows, cols);
-                        z[0] = y[0], z[1] = y[1];
-                        times(z, rows2, cols2);
-                        s_u[0][1][lane] = z[0];
-                        s_u[0][2][lane] = z[1] + y[2];
+                        times(y, {t[0], t[2], t[3]}, {x[0], x[0], x[1]}, 3);
+                        times(y, {t[1], t[4], t[4]}, {x[1], x[2], x[2]}, 2);
                     } else {
-                        constexpr int rows[] = {0, 3, 3}, cols[] = {0, 0, 1}, rows2[] = {3, 3}, cols2[] = {2, 3};
-                        times(y, rows, cols);
-                        z[0] = y[1], z[1] = y[2];
-                        times(z, rows2, cols2);
-                        s_u[0][0][lane] = y[0];
-                        s_u[0][3][lane] = z[0] + z[1];
+                        times(y, {t[0], t[1], t[2]}, {x[0], x[0], x[1]}, 3);
+                        f32x4 z[3]{y[1], y[2], y[0]};
+                        times(z, {t[3], t[4], t[4]}, {x[2], x[3], x[3]}, 2);
+                        y[1] = z[0], y[2] = z[1];
                     }
+                    if (kOwnT) load_t(ahead);
+                    s_u[0][wave][lane] = y[0];
+                    s_u[0][3 - wave][lane] = y[1] + y[2];
                     __syncthreads();   // the helpers wait for U here
 #pragma unroll
                     for (int r = 0; r < 4; ++r) u[r] = s_u[0][r][lane];
@@ -891,7 +897,7 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
     auto load_p = [&](uint32_t chunk) {
         const ops_u32x4* from = operands_of(chunk) + kOperand + lane;
 #pragma unroll
-        for (uint32_t i = 0; i < 5; ++i) p[i] = ld_global<f32x4>(from + (i <= w ? w * (w + 1) / 2 + i : (3 - w) * (4 - w) / 2 + i - w - 1) * 64);
+        for (uint32_t i = 0; i < 5; ++i) p[i] = ld_global<f32x4>(from + row_and_other(w, i) * 64);
     };
     f32x4 qm[kN][2], sum[kN][2];
     float back[kN];
@@ -915,8 +921,8 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
 #pragma unroll
             for (uint32_t i = 0; i < 2; ++i) s_v[b][row_tile(i)][lane] = v[b][i];
 #pragma unroll
-        for (uint32_t i = 0; i < 5; ++i) s_t[w * 5 + i][lane] = t_in[i];
-        load_t(clamped(chunk + 1));
+        for (uint32_t i = 0; i < 5 && !kOwnT; ++i) s_t[w * 5 + i][lane] = t_in[i];
+        if (!kOwnT) load_t(clamped(chunk + 1));
     };
     auto second_half = [&](uint32_t chunk) {
         __syncthreads();
@@ -937,11 +943,12 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
 #pragma unroll
         for (int b = 0; b < kN; ++b) back[b] = s_back[b][col];
         load_queries(clamped(chunk + 1));
+        // the next chunk's V, while the state's waves form U
+        put_early(clamped(chunk + 1), chunk + 1 - c0);
+        load_early(clamped(chunk + 2));
         __syncthreads();
         products();
         load_p(clamped(chunk + 1));
-        put_early(clamped(chunk + 1), chunk + 1 - c0);
-        load_early(clamped(chunk + 2));
     };
     auto outputs = [&](uint32_t done) {
         const uint32_t last = last_row(done);
@@ -973,7 +980,7 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
         wave_sync();
     };
     load_early(c0);
-    load_t(c0);
+    if (!kOwnT) load_t(c0);
     put_early(c0, 0);
     load_queries(c0);
     load_early(clamped(c0 + 1));
