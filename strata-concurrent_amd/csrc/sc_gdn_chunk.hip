@@ -66,6 +66,16 @@ __device__ __forceinline__ f32x4 product(f32x4 x, f32x4 y, f32x4 acc) {
     for (int i = 0; i < 4; ++i) acc = mfma_f32(x[i], y[i], acc);
     return acc;
 }
+// n products of their own, side by side: one after the other, each instruction would wait for the one before.
+template <int n>
+__device__ __forceinline__ void products(f32x4 (&acc)[n], const f32x4 (&x)[n], const f32x4 (&y)[n]) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+#pragma unroll
+        for (int j = 0; j < n; ++j) acc[j] = mfma_f32(x[j][i], y[j][i], acc[j]);
+        __builtin_amdgcn_sched_barrier(0);
+    }
+}
 
 // Two values, each times `by`, as two f16 parts: the product rounded to nearest, and what that left out rounded likewise (a
 // fused multiply-add a value).  What is subtracted is what is multiplied later, not a product that the compiler would round
@@ -506,8 +516,8 @@ __device__ __forceinline__ void split_state(const f32x4 (&m)[2], float by, ops_u
     split_pair(f32x4{m[0].x, m[1].x, m[0].y, m[1].y}, f32x4{m[0].z, m[1].z, m[0].w, m[1].w}, four, four, hi, lo);
 }
 
-// kN tiles of 16 columns.  With one, both waves of the state form U from the whole of K M0; with two, each forms the one of
-// its tile and they exchange what the update needs.  One sequence is bound by the chain of a chunk's products, splits and
+// kN tiles of 16 columns.  With one, the state's two waves form half of U's rows each; with two, each forms U of its tile.  One
+// sequence is bound by the chain of a chunk's products, splits and
 // barriers, 1.8 us each (8192 tokens, 32 heads of 128, f16: 236 us), many by the operands that their workgroups read through
 // their caches (10 854 tokens of eight sequences, f32: 250-290 us, 10-12 TB/s of them).
 template <int S, int kN, bool kF16>
@@ -527,11 +537,9 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
     __shared__ f32x4 s_v[kN][4][64];                          // beta V: first half, second
     __shared__ f32x4 s_t[kOwnT ? 1 : 10][64];                 // T: first half, second
     __shared__ f32x4 s_km[kShares][4][64];                    // K M0 by a wave's keys: first half, second
-    __shared__ ops_u32x4 s_w[kN == 1 ? 1 : kN][2][2][64];     // U weighted for the state, with two tiles
     __shared__ __align__(16) uint8_t s_stage[kOutWaves][32 * kRowV];   // a wave's rows of V or O on their way
     __shared__ __align__(16) float s_f[2][(kFactors + 63) / 64 * 64];  // factors of rows: second half, all of the next and its next first
     __shared__ float s_back[kN][16];                          // what brings a column's products with the state back: first half, second
-    __shared__ int s_up[kN == 1 ? 1 : kN][16];                // the new units of a column's state, with two tiles
     __shared__ float s_top[kShares][kN][16];                  // the largest of a wave's state by column: second half, first
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t g = lane >> 4, col = lane & 15;
@@ -702,7 +710,7 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
                 if constexpr (kShares > 1) km[0][r] += s_km[wave ^ 1][r][lane];   // the same sum in both waves
             }
             // X; rows past the sequence's end are zero, as their V and factors are
-            f32x4 x[4], u[4];
+            f32x4 x[4];
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 if constexpr (kN > 1) fs[r] = factors_of(r);
@@ -711,7 +719,7 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
                 for (int j = 0; j < 4; ++j) x[r][j] = __builtin_fmaf(-fs[r][j], km[0][r][j], v[j]);
             }
             // U = T X; weighted, it is what the state takes, its column's largest at 2^kAim.  With one tile of columns the state's
-            // waves have two row tiles each, five of T's ten tiles, and exchange them; with two, each has its columns'.
+            // waves have two row tiles each, five of T's ten tiles; with two, each has its columns'.
             ops_u32x4 ws[kN][2][2];
             int to[kN];
             {
@@ -723,72 +731,56 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
                     f32x4 t[5];
 #pragma unroll
                     for (uint32_t i = 0; i < 5; ++i) t[i] = kOwnT ? t_own[i] : s_t[row_and_other(wave, i)][lane];
-                    // the sums of both rows side by side: row `wave`, and in two row 3 - wave
-                    auto times = [&](f32x4 (&y)[3], const f32x4 (&a)[3], const f32x4 (&b)[3], int n) {
-#pragma unroll
-                        for (int i = 0; i < 4; ++i)
-#pragma unroll
-                            for (int j = 0; j < n; ++j) y[j] = mfma_f32(a[j][i], b[j][i], y[j]);
-                    };
+                    // row `wave` in y[0], row 3 - wave in y[1] and y[2]
                     f32x4 y[3]{};
                     if (wave) {
-                        times(y, {t[0], t[2], t[3]}, {x[0], x[0], x[1]}, 3);
-                        times(y, {t[1], t[4], t[4]}, {x[1], x[2], x[2]}, 2);
+                        products(y, {t[0], t[2], t[3]}, {x[0], x[0], x[1]});
+                        f32x4 z[2]{y[0], y[1]};
+                        products(z, {t[1], t[4]}, {x[1], x[2]});
+                        y[0] = z[0], y[1] = z[1];
                     } else {
-                        times(y, {t[0], t[1], t[2]}, {x[0], x[0], x[1]}, 3);
-                        f32x4 z[3]{y[1], y[2], y[0]};
-                        times(z, {t[3], t[4], t[4]}, {x[2], x[3], x[3]}, 2);
+                        products(y, {t[0], t[1], t[2]}, {x[0], x[0], x[1]});
+                        f32x4 z[2]{y[1], y[2]};
+                        products(z, {t[3], t[4]}, {x[2], x[3]});
                         y[1] = z[0], y[2] = z[1];
                     }
                     if (kOwnT) load_t(ahead);
                     s_u[0][wave][lane] = y[0];
                     s_u[0][3 - wave][lane] = y[1] + y[2];
-                    __syncthreads();   // the helpers wait for U here
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) u[r] = s_u[0][r][lane];
                 } else {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        f32x4 sums[2]{};   // a chain half as long
-#pragma unroll
-                        for (int t = 0; t <= r; ++t) sums[t & 1] = product(s_t[tile_of(r, t)][lane], x[t], sums[t & 1]);
-                        u[r] = sums[0] + sums[1];
-                        s_u[tile][r][lane] = u[r];
-                    }
-                    if constexpr (kN == 1) __syncthreads();
+                    auto t = [&](int r, int c) { return s_t[tile_of(r, c)][lane]; };
+                    f32x4 y[4]{};
+                    products(y, {t(0, 0), t(1, 0), t(2, 0), t(3, 0)}, {x[0], x[0], x[0], x[0]});
+                    f32x4 z[3]{y[1], y[2], {}};   // row 3 in two sums
+                    products(z, {t(1, 1), t(2, 1), t(3, 1)}, {x[1], x[1], x[1]});
+                    f32x4 last[3]{z[1], y[3], z[2]};
+                    products(last, {t(2, 2), t(3, 2), t(3, 3)}, {x[2], x[2], x[3]});
+                    s_u[tile][0][lane] = y[0];
+                    s_u[tile][1][lane] = z[0];
+                    s_u[tile][2][lane] = last[0];
+                    s_u[tile][3][lane] = last[1] + last[2];
                 }
-                float top = 0;
-                f32x4 w[4];
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    if constexpr (kN > 1) fw[r] = *reinterpret_cast<const f32x4*>(&f[kFWrite + r * 16 + g * 4]);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        w[r][j] = u[r][j] * fw[r][j];
-                        top = fmaxf(top, fabsf(w[r][j]));
-                    }
-                }
-                top = over_rows(top, max_of);
-                const int most = kN == 1 ? reach[0] : pick(wave, reach[kN - 1], reach[0]), now = kN == 1 ? up[0] : pick(wave, up[kN - 1], up[0]);
-                to[0] = top > 0 ? max(max(exponent_of(top), most == INT_MIN ? INT_MIN : most - kFar), now - 126) : now;
-                const float by = __builtin_amdgcn_ldexpf(1.0f, -to[0]);
-                const f32x4 four{by, by, by, by};
-#pragma unroll
-                for (int step = 0; step < 2; ++step) {
-                    split_pair(w[step * 2], w[step * 2 + 1], four, four, ws[0][step][0], ws[0][step][1]);
-                    if (kN > 1) s_w[tile][step][0][lane] = ws[0][step][0], s_w[tile][step][1][lane] = ws[0][step][1];
-                }
-                if (kN > 1 && g == 0) s_up[tile][col] = to[0];
-            }
-            if constexpr (kN > 1) {
                 __syncthreads();
 #pragma unroll
                 for (int b = 0; b < kN; ++b) {
-                    to[b] = s_up[b][col];
+                    float top = 0;
+                    f32x4 w[4];
 #pragma unroll
-                    for (int step = 0; step < 2; ++step)
+                    for (int r = 0; r < 4; ++r) {
+                        const f32x4 u = s_u[b][r][lane];
+                        if constexpr (kN > 1) fw[r] = *reinterpret_cast<const f32x4*>(&f[kFWrite + r * 16 + g * 4]);
 #pragma unroll
-                        for (int part = 0; part < 2; ++part) ws[b][step][part] = s_w[b][step][part][lane];
+                        for (int j = 0; j < 4; ++j) {
+                            w[r][j] = u[j] * fw[r][j];
+                            top = fmaxf(top, fabsf(w[r][j]));
+                        }
+                    }
+                    top = over_rows(top, max_of);
+                    to[b] = top > 0 ? max(max(exponent_of(top), reach[b] == INT_MIN ? INT_MIN : reach[b] - kFar), up[b] - 126) : up[b];
+                    const float by = __builtin_amdgcn_ldexpf(1.0f, -to[b]);
+                    const f32x4 four{by, by, by, by};
+#pragma unroll
+                    for (int step = 0; step < 2; ++step) split_pair(w[step * 2], w[step * 2 + 1], four, four, ws[b][step][0], ws[b][step][1]);
                 }
             }
             // the state after the chunk, in the units of what is added
@@ -902,17 +894,16 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
     f32x4 qm[kN][2], sum[kN][2];
     float back[kN];
     // P U: a wave's second tile is of rows w or 3 - w
-    auto products = [&] {
+    auto outputs_of_u = [&] {
 #pragma unroll
         for (int b = 0; b < kN; ++b) {
-            sum[b][0] = product(p[0], s_u[b][0][lane], f32x4{});
-            const f32x4 x = product(p[1], s_u[b][w][lane], w ? sum[b][0] : f32x4{});
-            sum[b][1] = w ? f32x4{} : x;
-            if (w) sum[b][0] = x;
-            f32x4 odd = product(p[3], s_u[b][2 - w][lane], f32x4{});   // in two sums: a chain half as long
-            sum[b][1] = product(p[2], s_u[b][1 - w][lane], sum[b][1]);
-            odd = product(p[4], s_u[b][3 - w][lane], odd);
-            sum[b][1] += odd;
+            auto u = [&](uint32_t r) { return s_u[b][r][lane]; };
+            f32x4 near = product(p[0], u(0), f32x4{}), far{}, odd = product(p[3], u(2 - w), f32x4{});   // rows 3 - w in two sums
+            const f32x4 x = product(p[1], u(w), w ? near : far);
+            near = w ? x : near;
+            far = product(p[2], u(1 - w), w ? far : x);
+            odd = product(p[4], u(3 - w), odd);
+            sum[b][0] = near, sum[b][1] = far + odd;
         }
     };
     auto first_half = [&](uint32_t chunk) {
@@ -947,7 +938,7 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
         put_early(clamped(chunk + 1), chunk + 1 - c0);
         load_early(clamped(chunk + 2));
         __syncthreads();
-        products();
+        outputs_of_u();
         load_p(clamped(chunk + 1));
     };
     auto outputs = [&](uint32_t done) {
@@ -998,13 +989,12 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
     outputs(c1 - 1);
 }
 
-// Two tiles of columns a workgroup halve what a chunk's operands cost in reads (132 KB for f32, 72 for f16), one gives twice
+// Two tiles of columns a workgroup halve what a chunk's operands cost in reads (126 KB for f32, 68 for f16), one gives twice
 // as many workgroups, each with less to do between its barriers.  Measured in us for both kernels, sequences of 32 heads of
-// 128 and up to 1024 tokens, two tiles against one: f16 56 : 44 for one sequence, 60 : 62 for two, 93 : 123 for eight; f32
-// 67 : 51, 76 : 68, 78 : 78 for three, 149 : 172 for eight.  So two where that leaves three quarters of the chip's 256 units a
-// workgroup (f16), or two to each (f32).
-template <bool kF16>
-constexpr uint32_t kWideFrom = kF16 ? 192 : 512;
+// 128 and up to 1024 tokens, two tiles against one: f16 59 : 42 for one sequence, 64 : 58 for two, 74 : 68, 92 : 104 for four,
+// 112 : 136 for eight; f32 72 : 51, 86 : 78, 96 : 90, 120 : 136, 149 : 178.  So two where that leaves the chip's 256 units two
+// workgroups each, if all sequences of the call were in one piece.
+constexpr uint32_t kWideFrom = 512;
 
 template <int S, bool kF16>
 void launch_chunks(const GdnArgs& a, const ChunkArgs& c, hipStream_t stream) {
@@ -1013,7 +1003,7 @@ void launch_chunks(const GdnArgs& a, const ChunkArgs& c, hipStream_t stream) {
     const dim3 threads((kStateWaves<S> + kOutWaves) * 64);
     hipLaunchKernelGGL((gdn_prepare_kernel<S, kF16>), dim3(by_eight(c.count)), dim3(kThreadsC), 0, stream, a, c);
     if constexpr (S >= 64)
-        if (a.n_seqs * a.v_heads * (S / 32) >= kWideFrom<kF16>) {
+        if (a.n_seqs * a.v_heads * (S / 32) >= kWideFrom) {
             hipLaunchKernelGGL((gdn_chunk_kernel<S, 2, kF16>), dim3(heads * (S / 32)), threads, 0, stream, a, c);
             return;
         }
@@ -1033,9 +1023,10 @@ hipError_t launch_of(const GdnArgs& a, const ChunkArgs& plan, bool f16, hipStrea
 
 // Chunks of one pair of launches: a long prompt goes through the workspace in pieces, which bounds it (1.2 GB at most for 32
 // heads of 128 in f32).  A piece of one sequence stays in the memory's own cache, 256 MB, until it has been read: 32 768 tokens
-// of 32 heads of 128 take 1093, 1050, 1149 and 1126 us by pieces of 64, 128, 256 and 512 chunks in f16, 1421, 1643, 1587 and
-// 1550 in f32, whose pieces are twice as large.  Each further sequence adds as many, so that all have something to do: eight of
-// up to 8192 (f32) 2029, 1605 and 1455 by 64, 256 and 512.
+// of 32 heads of 128 take 1104, 1077, 1125 and 1115 us by pieces of 64, 128, 256 and 512 chunks in f16, 1426, 1666, 1611 and
+// 1576 in f32, whose pieces are twice as large.  The numbers are for such heads: fewer or smaller ones have pieces that are a
+// fraction of what fits.  Each further sequence adds as many chunks, up to 512; but a piece is a run of the chunks of all sequences
+// in order, so that it holds many short sequences, or one or two of several long ones.
 constexpr uint32_t kMostChunks = 512;
 
 }  // namespace
