@@ -56,17 +56,6 @@ __device__ __forceinline__ bool rarely(bool x) { return __builtin_expect(x, fals
 // 2^(a - b), at least the smallest normal number, which changes no sum but leaves infinities what they are; nothing weighs
 // nothing.
 __device__ __forceinline__ float weight(float a, float b) { return a == -kInf ? 0.0f : fmaxf(exp2_fast(a - b), kTiny); }
-
-// The maximum and the sum over the four lanes that share lane % 16 (the 16-lane rows of the wave), in every one of them.
-template <class F>
-__device__ __forceinline__ float over_rows(float x, F f) {
-    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
-
-__device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
 __device__ __forceinline__ float min_of(float a, float b) { return fminf(a, b); }
 
 // ---- which cells a workgroup takes ------------------------------------------------------------------------------------
@@ -119,7 +108,6 @@ __device__ __forceinline__ bool place_of(const AttnArgs& a, uint32_t lane, uint3
 
 // ---- a wave's turn ------------------------------------------------------------------------------------------------------
 
-using u16x2 = __attribute__((ext_vector_type(2))) uint16_t;
 __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
 __device__ __forceinline__ f16x2 two(uint32_t w) { return __builtin_bit_cast(f16x2, w); }
@@ -127,7 +115,6 @@ __device__ __forceinline__ uint32_t bits(f16x2 h) { return __builtin_bit_cast(ui
 __device__ __forceinline__ f16x8 eight(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     return __builtin_bit_cast(f16x8, ops_u32x4{a, b, c, d});
 }
-__device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 // Two f16 parts of eight values: the value rounded to nearest, and what that left out rounded likewise.
 __device__ __forceinline__ void split8(const float (&p)[8], f16x8& hi, f16x8& lo) {
     uint32_t h[4], r[4];

@@ -27,7 +27,6 @@
 namespace sc {
 namespace {
 
-using u16x2 = __attribute__((ext_vector_type(2))) uint16_t;
 constexpr int kC = 64;                       // tokens of a chunk
 constexpr int kWaves = 4, kThreadsC = kWaves * 64;
 constexpr float kLeastG = -200.0f;           // a decay of e^-200 is 0 in f32
@@ -58,7 +57,6 @@ constexpr uint32_t kRowWords = kParts * S * 8 * (kParts == 1 ? 1 : 3);
 __device__ __forceinline__ f32x4 mfma(ops_u32x4 a, ops_u32x4 b, f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-__device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 // The product of two tiles of 32-bit numbers: a lane has four values of its row of the left one and, as results lie, of its
 // column of the right one.
 __device__ __forceinline__ f32x4 product(f32x4 x, f32x4 y, f32x4 acc) {
@@ -94,16 +92,8 @@ __device__ __forceinline__ void power_of(float x, float& down, float& up) {
     down = __uint_as_float(uint32_t(127 - e) << 23);
     up = __uint_as_float(uint32_t(127 + e) << 23);
 }
-template <class F>
-__device__ __forceinline__ float over_rows(float x, F f) {   // over the four lanes that share lane % 16
-    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    x = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
-    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
-}
 // 2^x by the hardware's instruction, 1 unit in the last place
 __device__ __forceinline__ float exp2_of(double x) { return __builtin_amdgcn_exp2f(float(x)); }
-__device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
 
 // A sequence's rows and chunks: rows [t0, t1), its first chunk of all.
 struct Seq {

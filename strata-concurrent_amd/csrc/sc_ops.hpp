@@ -92,6 +92,7 @@ using f32x4 = __attribute__((ext_vector_type(4))) float;
 using f16x2 = __attribute__((ext_vector_type(2))) _Float16;
 using f16x4 = __attribute__((ext_vector_type(4))) _Float16;
 using f16x8 = __attribute__((ext_vector_type(8))) _Float16;
+using u16x2 = __attribute__((ext_vector_type(2))) uint16_t;
 
 __device__ __forceinline__ uint32_t ops_div(uint32_t n, const FastDiv& f) {
     return uint32_t((uint64_t(__umulhi(n, f.m)) + uint64_t(n)) >> f.s);
@@ -144,6 +145,20 @@ __device__ __forceinline__ void st_act4(uint8_t* row, uint32_t at, f32x4 v) {
         else st_global<ops_u32x4>(p, bits);
     }
 }
+
+// Products of matrix tiles of 32-bit numbers: a lane has one value of a row of the left and a column of the right one.
+__device__ __forceinline__ f32x4 mfma_f32(float a, float b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+// The maximum and the sum (or another function) over the four lanes that share lane % 16, the 16-lane rows of the wave, in
+// every one of them.
+template <class F>
+__device__ __forceinline__ float over_rows(float x, F f) {
+    auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float max_of(float a, float b) { return fmaxf(a, b); }
 
 // The physical page of a sequence's cell, or -1 where it is not resident.  `cell` is below c.cells.
 __device__ __forceinline__ int32_t cache_page(const CacheArgs& c, uint32_t seq, uint32_t page) {
