@@ -56,6 +56,13 @@ __device__ __forceinline__ bool rarely(bool x) { return __builtin_expect(x, fals
 // 2^(a - b), at least the smallest normal number, which changes no sum but leaves infinities what they are; nothing weighs
 // nothing.
 __device__ __forceinline__ float weight(float a, float b) { return a == -kInf ? 0.0f : fmaxf(exp2_fast(a - b), kTiny); }
+// Log of a sum of 2^(x - m), natural.  The sum's exponent goes to m, a whole number as well: added to the logarithm, which can
+// be 20 from m's other sign, it would take the bits of a result near 0.
+__device__ __forceinline__ float log_of_sum(float m, float sum) {
+    float e = float(__builtin_amdgcn_frexp_expf(sum)), f = __builtin_amdgcn_frexp_mantf(sum);
+    if (f < 0.70710678f) f *= 2, e -= 1;
+    return sum == 0 ? -kInf : ((m + e) + __builtin_log2f(f)) * kLn2;
+}
 __device__ __forceinline__ float min_of(float a, float b) { return fminf(a, b); }
 
 // ---- which cells a workgroup takes ------------------------------------------------------------------------------------
@@ -617,7 +624,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_part_kernel(AttnArgs a) 
         }
         if (p.parts == 1) {
             st_act4<kF16>(a.out + int64_t(p.s) * a.out_ld, (head0 + i) * D + d, sum == 0 ? f32x4{} : acc / sum);
-            if (d == 0 && a.lse) a.lse[uint64_t(p.s) * a.n_head + head0 + i] = sum == 0 ? -kInf : (top + __builtin_log2f(sum)) * kLn2;
+            if (d == 0 && a.lse) a.lse[uint64_t(p.s) * a.n_head + head0 + i] = log_of_sum(top, sum);
         } else {
             float* part = a.ws + uint64_t(p.ws0 + within) * (16 * kRowF) + i * kRowF;
             if (d == 0) *reinterpret_cast<f32x4*>(part) = f32x4{top, sum, 0, 0};
@@ -685,7 +692,7 @@ __global__ void __launch_bounds__(kAttnThreads) attn_join_kernel(AttnArgs a) {
     for (uint32_t k = 1; k < kSets; ++k) acc += s_acc[k][threadIdx.x];
     l = s_l[0] + s_l[1] + s_l[2] + s_l[3];
     st_act4<kF16>(a.out + int64_t(s) * a.out_ld, head * D + d, l == 0 ? f32x4{} : acc / l);
-    if (d == 0 && a.lse) a.lse[uint64_t(s) * a.n_head + head] = l == 0 ? -kInf : (m + __builtin_log2f(l)) * kLn2;
+    if (d == 0 && a.lse) a.lse[uint64_t(s) * a.n_head + head] = log_of_sum(m, l);
 }
 
 template <int D, bool kInt8, bool kF16>

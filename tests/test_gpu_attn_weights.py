@@ -251,3 +251,30 @@ def test_few_cells_as_32_bits_have_them(sc, ops, cuda, fmt):
         off.append((got[0, i] - w @ v[:, i // 512] / w.sum()) / (w @ np.abs(v[:, i // 512]) / w.sum()))
     rms = np.sqrt(np.mean(np.square(off)))
     assert rms <= 2.0 ** -23.5, np.log2(rms)
+
+
+@pytest.mark.parametrize("n,at", [(1, 0), (200, 0), (200, 150)])
+@pytest.mark.parametrize("fmt", ["f16", "int8"])
+def test_small_logs_of_sums(sc, ops, cuda, fmt, n, at):
+    """lse where one cell has nearly all the weight and a score near zero.  The score is one product and exact but for its scaling
+    (three roundings), which is of its own size, as the end's two roundings are: 2^-22 of it.  The exponential is within 2^-23
+    of itself, its mantissa's logarithm within 2^-24, the difference from the reference within 2^-24: 2^-22 together."""
+    rng = np.random.default_rng(12)
+    H, D, heads = 2, 256, 512
+    cache = Cache(sc, ops, rng, fmt, H, D, 4, 1, 50, table=None, n_pages=50)
+    k = np.zeros((n, H), np.float32)
+    k[:], k[at] = -100, 1
+    rows = cache.host["k"].reshape(50, H, 4, D)
+    rows[:] = 0
+    if fmt == "int8":
+        cache.host["ks"][:] = cache.host["vs"][:] = np.float16(1).view(np.uint16)
+    for c in range(n):
+        rows[c // 4, :, c % 4, 3] = k[c]
+    _put(cache)
+    q = np.zeros((1, heads, D), np.float32)
+    q[0, :, 3] = 8 + rng.random(heads) * 8
+    q[0, :, 3] *= np.where(rng.random(heads) < 0.5, 1, -1) if n == 1 else 1
+    _, lse = _run(sc, ops, cache, q, [n], n)
+    want = q[0, :, 3].astype(np.float64) * D ** -0.5   # the others' weights are below e^-50
+    off = np.abs(lse[0] - want)
+    assert (off <= 2.0 ** -22 * np.abs(want) + 2.0 ** -22).all(), (off / (2.0 ** -22 * np.abs(want) + 2.0 ** -22)).max()
