@@ -29,8 +29,8 @@ extern "C" {
  * (page * n_head_kv + h) * page_size + t % page_size of either pool, page = table[s * table_ld + t / page_size] for
  * sequence s.  Rows are head_dim f16 values (SC_KV_F16) or head_dim int8 codes with one f16 scale per 64 values in the
  * scale pools (SC_KV_INT8, the rule of sc_kv_append_async).  A page that is negative or not below n_pages is not
- * resident: a write to its cells is skipped, a read leaves them out.  q4_0 rows are kept rotated by their writer and are
- * not taken here. */
+ * resident: a write to its cells is skipped, a read leaves them out.  Slots in q4_0 or K8V4
+ * are not taken. */
 typedef struct sc_kv_cache {
     int32_t format;           /* SC_KV_F16 or SC_KV_INT8 */
     int64_t n_head_kv;        /* 1 .. 256 */
@@ -96,10 +96,11 @@ typedef struct sc_attn_decode {
 #define SC_ATTN_MAX_SEQS 1024
 
 /* out = softmax(scale * q . K) V over the resident cells of the window, and lse = log of the sum of the exponentials
- * (natural), which joins the result with one over other cells.  Sequences and softmax statistics in 32 bits; f16 queries
- * are exact, probabilities and f32 queries are carried as two f16 parts, so f32 results keep f32 accuracy.  A sequence
- * with no cell left (or whose every score is -inf) gets zeros and lse = -inf.  What lies in cells outside the sequence
- * does not matter.  The cache's length is split over the chip on the device from the lengths and the parts are joined by
+ * (natural), which joins the result with one over other cells.  Sums and softmax statistics in 32 bits; f16 queries are
+ * exact, weights and f32 queries are carried as two f16 parts in units of their own size, so f32 results keep f32 accuracy,
+ * also where one cell outweighs the rest by up to 2^80.  Infinite values that are attended make what the formula makes of
+ * them.  A sequence with no cell left (or whose every score is -inf) gets zeros and lse = -inf.  What lies in cells outside
+ * the sequence does not matter.  The cache's length is split over the chip on the device from the lengths and the parts are joined by
  * a second kernel; the result does not depend on timing. */
 uint64_t sc_attn_decode_workspace_bytes(const sc_kv_cache* cache, const sc_attn_decode* a);
 int sc_attn_decode_async(const sc_kv_cache* cache, const sc_attn_decode* a, void* workspace, uint64_t workspace_bytes,

@@ -14,11 +14,11 @@
 // The head is the lane's column in both results, so the running statistics are the lane's own: only the largest score of a
 // turn crosses lanes (two swaps), and bringing o to a new m is a product by the lane's own factor.
 //
-// Rows that are read once go past the caches' keeping: values always (267 us for 1.5 GB of eight sequences where they do
-// not, 241 where they do), keys in int8 (40.7 and 38.3 us for 135 MB), but not in f16, where a row's 512 bytes are read by
-// instructions of 64 of them (248 and 241 us).  Measured, 2 kv heads of 256 and 24 query heads: 1.5 GB of f16 rows in 238 us,
-// 6.3 TB/s where reading alone reaches 6.9; 135 MB of int8 rows in 37 us, where a call whose workgroups take one turn each
-// takes 12.
+// Rows that are read once go past the caches' keeping: values that are loaded by 16 bytes (262 us for 1.5 GB of eight
+// sequences where they do not, 236 where they do), keys in int8 (42.3 and 38.8 us for 135 MB), but not in f16, where a row's
+// 512 bytes are read by instructions of 64 of them (245 us where they do, 236).  Measured, 2 kv heads of 256 and 24 query
+// heads: 1.5 GB of f16 rows in 236 us, 6.4 TB/s where reading alone reaches 6.9; 135 MB of int8 rows in 39 us, where a call
+// whose workgroups take one turn each takes 12.5.
 //
 // Accuracy: weights and f32 queries enter the matrix instructions as two f16 parts, each rounded to nearest; keys, values and
 // f16 queries are exact, int8 codes are exact in f16 and their scales are applied in f32; sums are in 32 bits.  f16 is a fixed
@@ -699,8 +699,8 @@ template <int D, bool kInt8, bool kF16>
 hipError_t launch_of(const AttnArgs& a, hipStream_t stream) {
     hipLaunchKernelGGL((attn_part_kernel<D, kInt8, kF16>), dim3(a.grid), dim3(kAttnThreads), 0, stream, a);
     // A head's parts by one workgroup where the heads fill the chip or its threads have all the parts in flight at once, else by
-    // one for 64 values each: with 24 heads 11.0 us against 11.6 for 1 K cells, 11.6 against 12.2 for 4 K (both kernels), but
-    // 56.6 against 53.7 for 128 K; with 768 heads 38.3 against 41.5
+    // one for 64 values each: with 24 heads 12.5 us against 12.8 for 1 K cells (both kernels), but 53.3 against 51.8 for
+    // 128 K; with 768 heads 38.8 against 42.0
     const uint32_t rows = a.n_seqs * a.n_head;
     if (a.join && (rows >= 128 || a.parts <= 32)) hipLaunchKernelGGL((attn_join_kernel<D, D, kF16>), dim3(rows), dim3(kAttnThreads), 0, stream, a);
     else if (a.join) hipLaunchKernelGGL((attn_join_kernel<D, 64, kF16>), dim3(rows, D / 64), dim3(kAttnThreads), 0, stream, a);

@@ -11,8 +11,8 @@ constexpr int kTurn = 32;                       // cells of a wave's turn
 constexpr uint32_t kUnit = kTurn * kAttnWaves;  // cells of a workgroup's turn
 // Workgroups that the units are shared out among, one to each of the chip's 256 units, whose next turn's rows are in flight
 // while this one's are worked on.  Two to each have more in flight, but give twice the parts to write and to join; between
-// the two some run alone at the end.  Eight sequences of 1 K to 128 K cells: 236 us with 256, 273 with 384, 242 with 512; one
-// of 128 K 51, 61, 54; 32 of up to 8 K in int8 37, 41, 38.
+// the two some run alone at the end.  Eight sequences of 1 K to 128 K cells: 236 us with 256, 270 with 384, 239 with 512; one
+// of 128 K 52, 62, 54; 32 of up to 8 K in int8 39, 43, 40.
 constexpr uint32_t kAttnSlots = 256;
 
 // Cells [first, len) of a sequence, counted in units from `begin`, a multiple of a turn.
@@ -52,7 +52,7 @@ constexpr SplitPlan plan_split(uint32_t n_seqs, uint32_t tiles, uint32_t max_len
     const uint64_t most = ((window ? uint64_t(window) + kTurn : uint64_t(max_len)) + kUnit - 1) / kUnit;
     SplitPlan p{};
     p.join = most > 1;
-    // With a workgroup for every unit that there can be, none has to find its place: 12.4 us for 1 K cells, 13.3 without.
+    // With a workgroup for every unit that there can be, none has to find its place: 12.5 us for 1 K cells, 13.4 without.
     p.direct = p.join && !window && rows * most <= slots ? uint32_t(most) : 0;
     p.parts = uint32_t(most < slots ? most : slots + 1);
     // parts of all sequences: at most a slot's share each, and one more a sequence

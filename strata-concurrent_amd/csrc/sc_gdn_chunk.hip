@@ -8,15 +8,16 @@
 // one takes the chunks of a sequence in order with products only.  Columns of the state (values) do not meet: a workgroup
 // of the second kernel takes 16 or 32 of them with four waves.  Two carry the state, half the keys each, in their registers: a
 // result of a product (column = lane % 16, rows in registers) is the right operand of the next one as it stands, so nothing
-// crosses lanes but a column's largest value, and only parts of K M0 are exchanged.  The two others form the outputs from
-// the state and U that the first left in LDS; they also bring V, T and the factors of rows.
+// crosses lanes but a column's largest value, and the waves exchange parts of K M0 and U only.  The two others form the outputs
+// from the state and U that the first left in LDS; they also bring V, T and the factors of rows.
 //
 // Accuracy: T X and P U are products of 32-bit numbers, since a chunk's rows differ by whatever its gates leave of them.  The
 // other products run as f16 matrix instructions with sums in 32 bits, an f32 operand as two f16 parts: f16 keys and queries
 // enter as they are, f32 ones, and all keys that the state takes, scaled by row with a power of two, so that no row's weight
-// is larger for its key being short; unit length, decays and write strengths are factors of rows in f32.  The state before a chunk and the writes U that are added to it have a power of two a column each, from its largest,
-// so that neither takes bits from the other.  A column of the state is held in the units that its last writes came in.  Sums of
-// log decays are in 64 bits: what counts is their differences.
+// is larger for its key being short; unit length, decays and write strengths are factors of rows in f32.  The state before a
+// chunk and the writes U that are added to it have a power of two a column each, from its largest, so that neither takes bits
+// from the other.  A column of the state is held in the units that its last writes came in.  Sums of log decays are in 64 bits:
+// what counts is their differences.
 #include <hip/hip_runtime.h>
 
 #include <climits>
@@ -194,8 +195,9 @@ __device__ __forceinline__ void split_pair(f32x4 a, f32x4 b, f32x4 by_a, f32x4 b
 // rest of T by products of tiles, T_10 = - T_11 (A_10 T_00) for tiles of 16 and then of 32, with f32 matrix instructions.  A
 // product's left tile comes from LDS as rows, its right one is a result in registers as it is: the four terms a lane adds are
 // those whose rows it holds.  A chunk of one head is a chain of small steps whose latency bounds a small call (11 us for one
-// chunk of 32 heads of 128, f32; 20 by a single wave) and a large one (4096 of them in 60 us, f16, 3.7 TB/s; 50 by single waves,
-// which is not worth a kernel more; 5568 in 127 to 150 us, f32, where it also writes the parts of keys and queries, 4.4 TB/s).
+// chunk of 32 heads of 128, f32; 20 by a single wave) and a large one (4096 of them in 55 us, f16, 3.7 TB/s; 50 by single waves,
+// which is not worth a kernel more; 5568 in 123 to 147 us, f32, where it also writes the parts of keys and queries, 4 to
+// 4.8 TB/s).
 // So it keeps room for four workgroups a unit: A, T and P lie where the keys were, and the substitution asks for its rows a few
 // at a time (by three workgroups, with all of them at once: 68 and 132 to 165 us).
 template <int S, bool kF16>
@@ -507,9 +509,10 @@ __device__ __forceinline__ void split_state(const f32x4 (&m)[2], float by, ops_u
 }
 
 // kN tiles of 16 columns.  With one, the state's two waves form half of U's rows each; with two, each forms U of its tile.  One
-// sequence is bound by the chain of a chunk's products, splits and
-// barriers, 1.8 us each (8192 tokens, 32 heads of 128, f16: 236 us), many by the operands that their workgroups read through
-// their caches (10 854 tokens of eight sequences, f32: 250-290 us, 10-12 TB/s of them).
+// sequence is bound by the chain of a chunk's products, splits and barriers, 1.9 us each (8192 tokens, 32 heads of 128, f16:
+// 235 to 253 us, 4000 cycles a chunk).  Many are bound by that chain and by the operands that their workgroups read through
+// their caches, 2.8 GB for 10 854 tokens of eight sequences in f32: 280 to 350 us, 8 to 10 TB/s of them, with the matrix units
+// busy two fifths of the time.
 template <int S, int kN, bool kF16>
 __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chunk_kernel(GdnArgs a, ChunkArgs c) {
     constexpr int kParts = kF16 ? 1 : 2, kSteps = S / 32, kShares = kStateWaves<S>, kMine = kSteps / kShares;
@@ -520,17 +523,18 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
     constexpr uint32_t kEach = kC * kPieces / (kOutWaves * 64);          // pieces of a lane
     // where registers are few, the keys' second form is asked for within its chunk and the first one at its end
     constexpr bool kAhead = kF16, kOwnT = kF16 && kN == 1 && kShares == 2;
-    // Right operands are [tile][step][part][lane], results [tile of columns][tile of rows][lane].  A barrier opens a chunk,
-    // another is in its middle, a third where U is known; what lies here is written between two and read after the next.
-    __shared__ ops_u32x4 s_m[kN][kSteps][2][64];              // the state before the chunk: first half, second
-    __shared__ f32x4 s_u[kN][4][64];                          // U: second half, last part of it
-    __shared__ f32x4 s_v[kN][4][64];                          // beta V: first half, second
-    __shared__ f32x4 s_t[kOwnT ? 1 : 10][64];                 // T: first half, second
-    __shared__ f32x4 s_km[kShares][4][64];                    // K M0 by a wave's keys: first half, second
+    // Right operands are [tile][step][part][lane], results [tile of columns][tile of rows][lane].  A chunk has three parts: a
+    // barrier opens it, another comes where K M0 is known, the third where U is.  What lies here is written in one part and
+    // read in later ones, before the next chunk's part that writes it again.
+    __shared__ ops_u32x4 s_m[kN][kSteps][2][64];              // the state before the chunk: written in the first part, read in the second
+    __shared__ f32x4 s_u[kN][4][64];                          // U: second, third
+    __shared__ f32x4 s_v[kN][4][64];                          // beta V: first, second
+    __shared__ f32x4 s_t[kOwnT ? 1 : 10][64];                 // T: first, second
+    __shared__ f32x4 s_km[kShares][4][64];                    // K M0 by a wave's keys: first, second
     __shared__ __align__(16) uint8_t s_stage[kOutWaves][32 * kRowV];   // a wave's rows of V or O on their way
-    __shared__ __align__(16) float s_f[2][(kFactors + 63) / 64 * 64];  // factors of rows: second half, all of the next and its next first
-    __shared__ float s_back[kN][16];                          // what brings a column's products with the state back: first half, second
-    __shared__ float s_top[kShares][kN][16];                  // the largest of a wave's state by column: second half, first
+    __shared__ __align__(16) float s_f[2][(kFactors + 63) / 64 * 64];  // of rows: second; all of the next chunk, the first after it
+    __shared__ float s_back[kN][16];                          // what brings a column's products with the state back: first, second
+    __shared__ float s_top[kShares][kN][16];                  // the largest of a wave's state by column: third; the next first
     const uint32_t tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const uint32_t g = lane >> 4, col = lane & 15;
     // workgroups go to the eight XCDs in turn: the column blocks of the value heads of a key head are kept on one
@@ -896,7 +900,7 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
             sum[b][0] = near, sum[b][1] = far + odd;
         }
     };
-    auto first_half = [&](uint32_t chunk) {
+    auto first_part = [&](uint32_t chunk) {
 #pragma unroll
         for (int b = 0; b < kN; ++b)
 #pragma unroll
@@ -905,7 +909,7 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
         for (uint32_t i = 0; i < 5 && !kOwnT; ++i) s_t[w * 5 + i][lane] = t_in[i];
         if (!kOwnT) load_t(clamped(chunk + 1));
     };
-    auto second_half = [&](uint32_t chunk) {
+    auto rest = [&](uint32_t chunk) {
         __syncthreads();
 #pragma unroll
         for (int b = 0; b < kN; ++b)
@@ -966,14 +970,14 @@ __global__ void __launch_bounds__((kStateWaves<S> + kOutWaves) * 64, 2) gdn_chun
     load_queries(c0);
     load_early(clamped(c0 + 1));
     __syncthreads();
-    first_half(c0);
+    first_part(c0);
     load_p(c0);
-    second_half(c0);
+    rest(c0);
     for (uint32_t chunk = c0 + 1; chunk < c1; ++chunk) {
         __syncthreads();
-        first_half(chunk);
+        first_part(chunk);
         outputs(chunk - 1);
-        second_half(chunk);
+        rest(chunk);
     }
     __syncthreads();
     outputs(c1 - 1);
