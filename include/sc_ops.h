@@ -1,8 +1,9 @@
 /* sc_ops.h - the operators that run on a decode slot between two hand-offs, in libsc_handoff.so.
  *
  * A hand-off (sc_handoff.h) puts a sequence's paged K/V and its Gated-DeltaNet state into a decode slot.  These entry
- * points compute on such slots: new tokens' keys and values appended with the position rotation on the way, attention
- * of one new token a sequence over its paged cache, and the gated delta rule by single tokens and by whole prompts.
+ * points compute on such slots: new tokens' keys and values appended with the position rotation on the way (by one position a
+ * token, or by several axes'), attention of one new token a sequence over its paged cache, the cells that attention has use for
+ * kept and the others evicted, and the short convolution and the gated delta rule by single tokens and by whole prompts.
  *
  * Like every entry point of the library they take plain pointers, return a status of sc_handoff.h (the message in
  * sc_last_error()), let no exception out, check a request before anything is enqueued (SC_EINVAL / SC_ERANGE: nothing
@@ -77,6 +78,19 @@ typedef struct sc_rope_append {
  * launch. */
 int sc_rope_append_async(const sc_kv_cache* cache, const sc_rope_append* a, void* stream);
 
+/* Positions of several axes (time, height, width): a pair of a head turns by the position that its row has on the pair's axis. */
+typedef struct sc_rope_axes {
+    int32_t n_axes;           /* 1 .. 4 */
+    const uint8_t* host_axis; /* host [rot_dim / 2]: the axis of pair i, below n_axes; read before the call returns */
+    const int64_t* pos;       /* [n_axes][pos_ld]: the position of every row on every axis, 8-byte aligned */
+    int64_t pos_ld;           /* at least `tokens` */
+} sc_rope_axes;
+
+/* sc_rope_append_async with these positions: a->pos0 is only the cell of a sequence's first row, so a cell need not be its
+ * token's position (after a picture, whose tokens share positions, or after an eviction).  Angles are formed in 64 bits from
+ * positions of any sign.  One launch. */
+int sc_rope_axes_append_async(const sc_kv_cache* cache, const sc_rope_append* a, const sc_rope_axes* axes, void* stream);
+
 /* ---- paged attention of one new token ------------------------------------------------------------------------------- */
 
 typedef struct sc_attn_decode {
@@ -105,6 +119,39 @@ typedef struct sc_attn_decode {
 uint64_t sc_attn_decode_workspace_bytes(const sc_kv_cache* cache, const sc_attn_decode* a);
 int sc_attn_decode_async(const sc_kv_cache* cache, const sc_attn_decode* a, void* workspace, uint64_t workspace_bytes,
                          void* stream);
+
+/* ---- the short convolution before a recurrent layer --------------------------------------------------------------------- */
+
+enum { SC_CONV_NONE = 0, SC_CONV_SILU = 1 };             /* what is applied to the sums */
+enum { SC_CONV_SLOT = 0,       /* history [channels][taps - 1], a slot's GDN row from S * HV * S floats on */
+       SC_CONV_ROWS = 1 };     /* history [taps - 1][state_ld], the last rows of a prefill's convolution inputs */
+
+typedef struct sc_conv {
+    int64_t channels;         /* C: a multiple of 8, 8 .. 2^20 */
+    int32_t taps;             /* W: 2 .. 5 */
+    int32_t n_seqs;           /* 1 .. 4096 */
+    int64_t tokens;           /* rows of x and out, at most 2^23 */
+    const int64_t* cu;        /* [n_seqs + 1] as in sc_rope_append, a sequence's rows in order; NULL: row s is sequence s's one
+                                 new token (tokens == n_seqs) */
+    int32_t dtype;            /* SC_DTYPE_F16 or SC_DTYPE_F32: x and out */
+    const void* x;            /* [tokens][C], x_ld values from row to row, 16-byte aligned */
+    void* out;                /* [tokens][C]; shares no byte with x, but may be x itself without cu (then out_ld == x_ld) */
+    int64_t x_ld, out_ld;     /* multiples of 4 (f32) or 8 (f16) values, at most 2^22 */
+    const float* weight;      /* [C][W], 16-byte aligned: weight[c][W - 1] meets the row itself */
+    const float* bias;        /* [C], 16-byte aligned, or NULL */
+    int32_t activation;       /* SC_CONV_NONE or SC_CONV_SILU */
+    float* const* state;      /* device [n_seqs]: each sequence's base, 16-byte aligned, none of them twice; a NULL entry is a
+                                 sequence without a slot: its out rows are zeros.  A history shares no byte with x or out */
+    int64_t state_offset;     /* floats from the base to this layer's history, a multiple of 4 (e.g. layer * sc_gdn_row_floats +
+                                 S * HV * S), at most 2^40 */
+    int32_t state_layout;     /* SC_CONV_SLOT or SC_CONV_ROWS; the oldest row first in both */
+    int64_t state_ld;         /* SC_CONV_ROWS: floats from row to row, a multiple of 4, C .. 2^40 */
+} sc_conv;
+
+/* out[t][c] = f(bias[c] + sum over j of weight[c][j] * x[t - (W - 1) + j][c]), the rows before a sequence's first being its
+ * history, and the history becomes the last W - 1 rows of both together.  Sums in 32 bits; f is v / (1 + exp(-v)) for
+ * SC_CONV_SILU.  A sequence without rows keeps its history; rows past cu[n_seqs] are left out.  One launch. */
+int sc_conv_async(const sc_conv* a, void* stream);
 
 /* ---- the gated delta rule --------------------------------------------------------------------------------------------- */
 

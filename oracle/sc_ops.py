@@ -34,6 +34,17 @@ def rotate(x: np.ndarray, pos: int, inv_freq, rot: int, pairs: str) -> np.ndarra
     return y
 
 
+def rotate_axes(x: np.ndarray, pos, axis, inv_freq, rot: int, pairs: str) -> np.ndarray:
+    """The heads [.., D] of one token, each pair turned by the token's position on the pair's axis."""
+    y = np.array(x, np.float64)
+    for i in range(rot // 2):
+        angle = float(pos[axis[i]]) * float(inv_freq[i])
+        a, b = (i, i + rot // 2) if pairs == "halves" else (2 * i, 2 * i + 1)
+        xa, xb = np.array(y[..., a]), np.array(y[..., b])
+        y[..., a], y[..., b] = xa * np.cos(angle) - xb * np.sin(angle), xa * np.sin(angle) + xb * np.cos(angle)
+    return y
+
+
 def attention(q, keys, values, scale: float):
     """One head's query over its cells [n][D]: (out, lse); nothing left gives zeros and -inf."""
     q, keys, values = (np.asarray(x, np.float64) for x in (q, keys, values))
@@ -59,6 +70,19 @@ def delta_rule(state, q, k, v, g, beta, scale: float, l2norm: bool, eps: float):
         M += np.outer(k[t], beta[t] * (v[t] - M.T @ k[t]))
         out[t] = scale * (M.T @ q[t])
     return out, M
+
+
+def short_conv(history, x, weight, bias, silu: bool):
+    """One sequence: history [taps - 1][C] (the oldest row first), x [T][C], weight [C][taps], bias [C] or None;
+    (out [T][C], new history)."""
+    rows = np.concatenate([np.asarray(history, np.float64), np.asarray(x, np.float64)])
+    w, W, out = np.asarray(weight, np.float64), np.shape(weight)[1], np.zeros(np.shape(x))
+    for t in range(len(out)):
+        y = np.zeros(w.shape[0]) if bias is None else np.array(bias, np.float64)
+        for j in range(W):
+            y += w[:, j] * rows[t + j]
+        out[t] = y / (1 + np.exp(-y)) if silu else y
+    return out, rows[len(rows) - (W - 1):]
 
 
 def dequant(codes: np.ndarray, scales: np.ndarray) -> np.ndarray:

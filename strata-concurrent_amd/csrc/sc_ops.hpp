@@ -1,5 +1,5 @@
 // sc_ops.hpp - the arguments of the operators' kernels (include/sc_ops.h), shared by their host layer (sc_ops_capi.cpp)
-// and the kernels (sc_rope.hip, sc_attn.hip, sc_gdn.hip).  Everything travels in the kernel arguments.
+// and the kernels (sc_rope.hip, sc_attn.hip, sc_conv.hip, sc_gdn.hip).  Everything travels in the kernel arguments.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -33,6 +33,11 @@ struct RopeArgs {
     const int64_t *cu, *pos0;
     const float* inv_freq;
     uint32_t tokens, n_seqs, n_head, rot, neighbours;
+    // positions of several axes (axes > 0): `pos` of row t on an axis at axis * pos_ld + t, two bits of `axis` for each pair
+    uint32_t axes;
+    const int64_t* pos;
+    int64_t pos_ld;
+    uint32_t axis[8];
 };
 
 struct AttnArgs {
@@ -52,6 +57,17 @@ struct AttnArgs {
     uint32_t parts;                       // parts a sequence can have
     float* ws;                            // the parts' results
     ops_u32x2* where;                     // [n_seqs] parts of a sequence and its first one's place
+};
+
+struct ConvArgs {
+    const uint8_t* x;
+    uint8_t* out;
+    int64_t x_ld, out_ld;                 // bytes from row to row
+    const float *weight, *bias;
+    float* const* state;
+    int64_t state_offset, state_ld;
+    const int64_t* cu;
+    uint32_t n_seqs, tokens, channels, silu;
 };
 
 struct GdnArgs {
@@ -82,6 +98,7 @@ uint64_t plan_attn(AttnArgs& a, int head_dim);
 // Places its parts in a workspace of those bytes.
 void place_attn(AttnArgs& a, void* workspace, uint64_t bytes);
 hipError_t launch_attn(const AttnArgs& a, int head_dim, int format, bool f16, hipStream_t stream);
+hipError_t launch_conv(const ConvArgs& a, int taps, bool f16, bool slot, hipStream_t stream);
 hipError_t launch_gdn_step(const GdnArgs& a, int size, bool f16, hipStream_t stream);
 // Fills the pieces that a call goes in and returns the bytes of its workspace.
 uint64_t plan_gdn_chunks(const GdnArgs& a, int size, bool f16, ChunkArgs& c);

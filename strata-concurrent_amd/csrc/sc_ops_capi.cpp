@@ -37,6 +37,7 @@ bool off(const void* p, uintptr_t align) { return (reinterpret_cast<uintptr_t>(p
 bool row_stride(int64_t ld, int64_t row, int32_t dtype) {
     return ld >= row && ld <= (int64_t(1) << 22) && ld % (dtype == SC_DTYPE_F16 ? 8 : 4) == 0;
 }
+constexpr int64_t most_floats = int64_t(1) << 40;   // of a stride
 int64_t value_bytes(int32_t dtype) { return dtype == SC_DTYPE_F16 ? 2 : 4; }
 
 // Whether two tensors of `rows` rows have a byte in common, rows [p + t * ld, + row).  Rows side by side in one buffer, such
@@ -132,8 +133,7 @@ int gdn_args(const char* op, const sc_gdn* d, bool step, sc::GdnArgs& a) {
     if (d->state_offset < 0 || d->state_offset % 4 || d->state_head_ld < S || d->state_head_ld % 4 || d->state_key_ld < S ||
         d->state_key_ld % 4)
         return bad(op, "state strides must be multiples of 4 floats and hold a row");
-    constexpr int64_t most = int64_t(1) << 40;
-    if (d->state_offset > most || d->state_head_ld > most || d->state_key_ld > most) return bad(op, "state strides must be at most 2^40 floats");
+    if (d->state_offset > most_floats || d->state_head_ld > most_floats || d->state_key_ld > most_floats) return bad(op, "state strides must be at most 2^40 floats");
     // the heads' rows inside a key's, or the keys' inside a head's block: anything else puts two values in one place
     if (d->state_key_ld < (d->v_heads - 1) * d->state_head_ld + S && d->state_head_ld < (S - 1) * d->state_key_ld + S)
         return bad(op, "state strides overlap");
@@ -177,55 +177,74 @@ bool outputs_apart(const sc_gdn* d) {
 }
 constexpr const char* kOutputsMeet = "out must not overlap q or k, nor v unless it is v";
 
+// Checks an append, by one position a token or by several axes', and enqueues it.
+int rope_append(const char* op, const sc_kv_cache* cache, const sc_rope_append* d, const sc_rope_axes* x, bool axes, void* stream) {
+    if (!d || (axes && !x)) return bad(op, "missing request");
+    if (d->n_seqs < 1 || d->n_seqs > 4096) return bad(op, "n_seqs must be 1 .. 4096");
+    sc::RopeArgs a{};
+    if (const int e = cache_args(op, cache, d->n_seqs, a.c)) return e;
+    if (d->tokens < 0 || d->tokens > (int64_t(1) << 23)) return bad(op, "tokens must be 0 .. 2^23");
+    if (!d->cu && d->tokens != d->n_seqs) return bad(op, "without cu there is one row a sequence");
+    if (off(d->cu, 8) || !d->pos0 || off(d->pos0, 8)) return bad(op, "cu and pos0 must be 8-byte aligned, pos0 given");
+    if (d->dtype != SC_DTYPE_F16 && d->dtype != SC_DTYPE_F32) return bad(op, "dtype must be f16 or f32");
+    if (!d->k || !d->v || off(d->k, 16) || off(d->v, 16)) return bad(op, "k and v must be given, 16-byte aligned");
+    const int64_t row = cache->n_head_kv * cache->head_dim;
+    if (!row_stride(d->k_ld, row, d->dtype) || !row_stride(d->v_ld, row, d->dtype))
+        return bad(op, "k_ld and v_ld must be whole 16 bytes and hold n_head_kv * head_dim values");
+    if (!d->q ? d->n_head != 0 : d->n_head < 1 || d->n_head > 4096) return bad(op, "n_head must be 1 .. 4096 with q, 0 without");
+    if (d->q) {
+        if (!d->q_out || off(d->q, 16) || off(d->q_out, 16)) return bad(op, "q and q_out must be given, 16-byte aligned");
+        if (!row_stride(d->q_ld, d->n_head * cache->head_dim, d->dtype) ||
+            !row_stride(d->q_out_ld, d->n_head * cache->head_dim, d->dtype))
+            return bad(op, "q_ld and q_out_ld must be whole 16 bytes and hold n_head * head_dim values");
+        if (d->q == d->q_out && d->q_ld != d->q_out_ld) return bad(op, "queries rotated in place need one stride");
+    }
+    if (d->pairing != SC_ROPE_HALVES && d->pairing != SC_ROPE_NEIGHBOURS) return bad(op, "unknown pairing");
+    if (d->rot_dim < 0 || d->rot_dim > cache->head_dim || d->rot_dim % 8) return bad(op, "rot_dim must be a multiple of 8, 0 .. head_dim");
+    if (d->rot_dim && (!d->inv_freq || off(d->inv_freq, 4))) return bad(op, "inv_freq must be given, 4-byte aligned");
+    if (axes) {
+        if (x->n_axes < 1 || x->n_axes > 4) return bad(op, "n_axes must be 1 .. 4");
+        if (!x->pos || off(x->pos, 8) || x->pos_ld < d->tokens || x->pos_ld > most_floats)
+            return bad(op, "pos must be given, 8-byte aligned, pos_ld at least tokens");
+        if (d->rot_dim && !x->host_axis) return bad(op, "host_axis must be given");
+        for (int64_t i = 0; i < d->rot_dim / 2; ++i) {
+            if (x->host_axis[i] >= x->n_axes) return bad(op, "an entry of host_axis is not below n_axes");
+            a.axis[i / 16] |= uint32_t(x->host_axis[i]) << (i % 16 * 2);
+        }
+        a.axes = uint32_t(x->n_axes);
+        a.pos = x->pos;
+        a.pos_ld = x->pos_ld;
+    }
+    if (d->tokens == 0) return sc::record_ok();
+    const int64_t b = value_bytes(d->dtype);
+    a.k = static_cast<const uint8_t*>(d->k);
+    a.v = static_cast<const uint8_t*>(d->v);
+    a.q = static_cast<const uint8_t*>(d->q);
+    a.q_out = static_cast<uint8_t*>(d->q_out);
+    a.k_ld = d->k_ld * b;
+    a.v_ld = d->v_ld * b;
+    a.q_ld = d->q_ld * b;
+    a.q_out_ld = d->q_out_ld * b;
+    a.cu = d->cu;
+    a.pos0 = d->pos0;
+    a.inv_freq = d->inv_freq;
+    a.tokens = uint32_t(d->tokens);
+    a.n_seqs = uint32_t(d->n_seqs);
+    a.n_head = uint32_t(d->n_head);
+    a.rot = uint32_t(d->rot_dim);
+    a.neighbours = d->pairing == SC_ROPE_NEIGHBOURS;
+    return launched(sc::launch_rope(a, int(cache->head_dim), cache->format, d->dtype == SC_DTYPE_F16,
+                                    static_cast<hipStream_t>(stream)), op);
+}
+
 }  // namespace
 
 int sc_rope_append_async(const sc_kv_cache* cache, const sc_rope_append* d, void* stream) {
-    return guarded([&] {
-        const char* op = "rope_append";
-        if (!d) return bad(op, "missing request");
-        if (d->n_seqs < 1 || d->n_seqs > 4096) return bad(op, "n_seqs must be 1 .. 4096");
-        sc::RopeArgs a{};
-        if (const int e = cache_args(op, cache, d->n_seqs, a.c)) return e;
-        if (d->tokens < 0 || d->tokens > (int64_t(1) << 23)) return bad(op, "tokens must be 0 .. 2^23");
-        if (!d->cu && d->tokens != d->n_seqs) return bad(op, "without cu there is one row a sequence");
-        if (off(d->cu, 8) || !d->pos0 || off(d->pos0, 8)) return bad(op, "cu and pos0 must be 8-byte aligned, pos0 given");
-        if (d->dtype != SC_DTYPE_F16 && d->dtype != SC_DTYPE_F32) return bad(op, "dtype must be f16 or f32");
-        if (!d->k || !d->v || off(d->k, 16) || off(d->v, 16)) return bad(op, "k and v must be given, 16-byte aligned");
-        const int64_t row = cache->n_head_kv * cache->head_dim;
-        if (!row_stride(d->k_ld, row, d->dtype) || !row_stride(d->v_ld, row, d->dtype))
-            return bad(op, "k_ld and v_ld must be whole 16 bytes and hold n_head_kv * head_dim values");
-        if (!d->q ? d->n_head != 0 : d->n_head < 1 || d->n_head > 4096) return bad(op, "n_head must be 1 .. 4096 with q, 0 without");
-        if (d->q) {
-            if (!d->q_out || off(d->q, 16) || off(d->q_out, 16)) return bad(op, "q and q_out must be given, 16-byte aligned");
-            if (!row_stride(d->q_ld, d->n_head * cache->head_dim, d->dtype) ||
-                !row_stride(d->q_out_ld, d->n_head * cache->head_dim, d->dtype))
-                return bad(op, "q_ld and q_out_ld must be whole 16 bytes and hold n_head * head_dim values");
-            if (d->q == d->q_out && d->q_ld != d->q_out_ld) return bad(op, "queries rotated in place need one stride");
-        }
-        if (d->pairing != SC_ROPE_HALVES && d->pairing != SC_ROPE_NEIGHBOURS) return bad(op, "unknown pairing");
-        if (d->rot_dim < 0 || d->rot_dim > cache->head_dim || d->rot_dim % 8) return bad(op, "rot_dim must be a multiple of 8, 0 .. head_dim");
-        if (d->rot_dim && (!d->inv_freq || off(d->inv_freq, 4))) return bad(op, "inv_freq must be given, 4-byte aligned");
-        if (d->tokens == 0) return sc::record_ok();
-        const int64_t b = value_bytes(d->dtype);
-        a.k = static_cast<const uint8_t*>(d->k);
-        a.v = static_cast<const uint8_t*>(d->v);
-        a.q = static_cast<const uint8_t*>(d->q);
-        a.q_out = static_cast<uint8_t*>(d->q_out);
-        a.k_ld = d->k_ld * b;
-        a.v_ld = d->v_ld * b;
-        a.q_ld = d->q_ld * b;
-        a.q_out_ld = d->q_out_ld * b;
-        a.cu = d->cu;
-        a.pos0 = d->pos0;
-        a.inv_freq = d->inv_freq;
-        a.tokens = uint32_t(d->tokens);
-        a.n_seqs = uint32_t(d->n_seqs);
-        a.n_head = uint32_t(d->n_head);
-        a.rot = uint32_t(d->rot_dim);
-        a.neighbours = d->pairing == SC_ROPE_NEIGHBOURS;
-        return launched(sc::launch_rope(a, int(cache->head_dim), cache->format, d->dtype == SC_DTYPE_F16,
-                                        static_cast<hipStream_t>(stream)), op);
-    });
+    return guarded([&] { return rope_append("rope_append", cache, d, nullptr, false, stream); });
+}
+
+int sc_rope_axes_append_async(const sc_kv_cache* cache, const sc_rope_append* d, const sc_rope_axes* axes, void* stream) {
+    return guarded([&] { return rope_append("rope_axes_append", cache, d, axes, true, stream); });
 }
 
 uint64_t sc_attn_decode_workspace_bytes(const sc_kv_cache* cache, const sc_attn_decode* d) {
@@ -245,6 +264,53 @@ int sc_attn_decode_async(const sc_kv_cache* cache, const sc_attn_decode* d, void
             return bad(op, "workspace missing, not 16-byte aligned or below sc_attn_decode_workspace_bytes");
         sc::place_attn(a, workspace, need);
         return launched(sc::launch_attn(a, int(cache->head_dim), cache->format, d->dtype == SC_DTYPE_F16,
+                                        static_cast<hipStream_t>(stream)), op);
+    });
+}
+
+int sc_conv_async(const sc_conv* d, void* stream) {
+    return guarded([&] {
+        const char* op = "conv";
+        if (!d) return bad(op, "missing request");
+        if (d->channels < 8 || d->channels > (int64_t(1) << 20) || d->channels % 8) return bad(op, "channels must be a multiple of 8, 8 .. 2^20");
+        if (d->taps < 2 || d->taps > 5) return bad(op, "taps must be 2 .. 5");
+        if (d->n_seqs < 1 || d->n_seqs > 4096) return bad(op, "n_seqs must be 1 .. 4096");
+        if (d->tokens < 0 || d->tokens > (int64_t(1) << 23)) return bad(op, "tokens must be 0 .. 2^23");
+        if (!d->cu && d->tokens != d->n_seqs) return bad(op, "without cu there is one row a sequence");
+        if (off(d->cu, 8)) return bad(op, "cu must be 8-byte aligned");
+        if (d->dtype != SC_DTYPE_F16 && d->dtype != SC_DTYPE_F32) return bad(op, "dtype must be f16 or f32");
+        if (!d->x || !d->out || off(d->x, 16) || off(d->out, 16)) return bad(op, "x and out must be given, 16-byte aligned");
+        if (!row_stride(d->x_ld, d->channels, d->dtype) || !row_stride(d->out_ld, d->channels, d->dtype))
+            return bad(op, "x_ld and out_ld must be whole 16 bytes and hold a row");
+        if (!d->weight || off(d->weight, 16) || off(d->bias, 16)) return bad(op, "weight must be given, weight and bias 16-byte aligned");
+        if (d->activation != SC_CONV_NONE && d->activation != SC_CONV_SILU) return bad(op, "unknown activation");
+        if (!d->state || off(d->state, 8)) return bad(op, "state must be given, 8-byte aligned");
+        if (d->state_offset < 0 || d->state_offset % 4 || d->state_offset > most_floats) return bad(op, "state_offset must be a multiple of 4, 0 .. 2^40");
+        if (d->state_layout != SC_CONV_SLOT && d->state_layout != SC_CONV_ROWS) return bad(op, "unknown state_layout");
+        if (d->state_layout == SC_CONV_ROWS && (d->state_ld < d->channels || d->state_ld % 4 || d->state_ld > most_floats))
+            return bad(op, "state_ld must be a multiple of 4, channels .. 2^40");
+        // a prompt's rows are read by the workgroups of the rows after them; a single row by the lane that writes it
+        const int64_t b = value_bytes(d->dtype);
+        if ((d->cu || d->out != d->x || d->out_ld != d->x_ld) &&
+            share_bytes(d->out, d->out_ld * b, d->channels * b, d->x, d->x_ld * b, d->channels * b, d->tokens))
+            return bad(op, "out must not overlap x, unless it is x and there is no cu");
+        if (d->tokens == 0) return sc::record_ok();
+        sc::ConvArgs a{};
+        a.x = static_cast<const uint8_t*>(d->x);
+        a.out = static_cast<uint8_t*>(d->out);
+        a.x_ld = d->x_ld * b;
+        a.out_ld = d->out_ld * b;
+        a.weight = d->weight;
+        a.bias = d->bias;
+        a.state = d->state;
+        a.state_offset = d->state_offset;
+        a.state_ld = d->state_ld;
+        a.cu = d->cu;
+        a.n_seqs = uint32_t(d->n_seqs);
+        a.tokens = uint32_t(d->tokens);
+        a.channels = uint32_t(d->channels);
+        a.silu = d->activation == SC_CONV_SILU;
+        return launched(sc::launch_conv(a, d->taps, d->dtype == SC_DTYPE_F16, d->state_layout == SC_CONV_SLOT,
                                         static_cast<hipStream_t>(stream)), op);
     });
 }

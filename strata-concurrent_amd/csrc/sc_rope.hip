@@ -1,5 +1,5 @@
 // sc_rope.hip - new tokens' keys and values into a paged cache, the position rotation applied on the way, and the
-// queries rotated (sc_rope_append_async).
+// queries rotated (sc_rope_append_async, sc_rope_axes_append_async).
 //
 // A pair (a, b) of a head at position p turns by p * inv_freq[i]: a cos - b sin, a sin + b cos.  It is data movement: every
 // value is read and written once, and the few operations a value hide behind that.  A workgroup takes one token (and, when
@@ -59,7 +59,14 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(RopeArgs a) {
     }
     const int64_t pos = ld_global<int64_t>(a.pos0 + s) + local;
     for (uint32_t i = threadIdx.x; i < a.rot / 2; i += kRopeThreads) {
-        const double angle = double(pos) * double(ld_global<float>(a.inv_freq + i));
+        int64_t at = pos;
+        if (a.axes) {
+            uint32_t word = 0;
+#pragma unroll
+            for (uint32_t j = 0; j < D / 32; ++j) word = i / 16 == j ? a.axis[j] : word;
+            at = ld_global<int64_t>(a.pos + (word >> i % 16 * 2 & 3) * a.pos_ld + t);
+        }
+        const double angle = double(at) * double(ld_global<float>(a.inv_freq + i));
         const float r = float(angle - rint(angle / kTwoPi) * kTwoPi);
         sincosf(r, &s_sin[i], &s_cos[i]);
     }

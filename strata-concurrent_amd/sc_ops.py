@@ -11,6 +11,8 @@ import sc_handoff as sc
 from sc_handoff import lib
 
 SC_ROPE_HALVES, SC_ROPE_NEIGHBOURS = 0, 1
+SC_CONV_NONE, SC_CONV_SILU = 0, 1
+SC_CONV_SLOT, SC_CONV_ROWS = 0, 1
 ATTN_MAX_SEQS = 1024
 
 _P, _I64, _U64, _I32 = C.c_void_p, C.c_int64, C.c_uint64, C.c_int32
@@ -28,9 +30,19 @@ class RopeAppendDesc(C.Structure):
                 ("n_head", _I64), ("pairing", _I32), ("rot_dim", _I64), ("inv_freq", _P)]
 
 
+class RopeAxesDesc(C.Structure):
+    _fields_ = [("n_axes", _I32), ("host_axis", C.POINTER(C.c_uint8)), ("pos", _P), ("pos_ld", _I64)]
+
+
 class AttnDecodeDesc(C.Structure):
     _fields_ = [("n_seqs", _I32), ("lens", _P), ("max_len", _I64), ("window", _I64), ("dtype", _I32), ("n_head", _I64),
                 ("q", _P), ("out", _P), ("q_ld", _I64), ("out_ld", _I64), ("lse", _P), ("scale", C.c_float)]
+
+
+class ConvDesc(C.Structure):
+    _fields_ = [("channels", _I64), ("taps", _I32), ("n_seqs", _I32), ("tokens", _I64), ("cu", _P), ("dtype", _I32), ("x", _P),
+                ("out", _P), ("x_ld", _I64), ("out_ld", _I64), ("weight", _P), ("bias", _P), ("activation", _I32), ("state", _P),
+                ("state_offset", _I64), ("state_layout", _I32), ("state_ld", _I64)]
 
 
 class GdnDesc(C.Structure):
@@ -43,8 +55,10 @@ class GdnDesc(C.Structure):
 
 _SIGS = {
     "sc_rope_append_async": (C.c_int, [C.POINTER(KvCache), C.POINTER(RopeAppendDesc), _P]),
+    "sc_rope_axes_append_async": (C.c_int, [C.POINTER(KvCache), C.POINTER(RopeAppendDesc), C.POINTER(RopeAxesDesc), _P]),
     "sc_attn_decode_workspace_bytes": (_U64, [C.POINTER(KvCache), C.POINTER(AttnDecodeDesc)]),
     "sc_attn_decode_async": (C.c_int, [C.POINTER(KvCache), C.POINTER(AttnDecodeDesc), _P, _U64, _P]),
+    "sc_conv_async": (C.c_int, [C.POINTER(ConvDesc), _P]),
     "sc_gdn_step_async": (C.c_int, [C.POINTER(GdnDesc), _P]),
     "sc_gdn_chunk_workspace_bytes": (_U64, [C.POINTER(GdnDesc)]),
     "sc_gdn_chunk_async": (C.c_int, [C.POINTER(GdnDesc), _P, _U64, _P]),
@@ -57,6 +71,8 @@ for _name, (_res, _args) in _SIGS.items():
 EXPORTS = tuple(_SIGS)
 
 _DTYPES = {"f16": sc.SC_DTYPE_F16, "f32": sc.SC_DTYPE_F32, sc.SC_DTYPE_F16: sc.SC_DTYPE_F16, sc.SC_DTYPE_F32: sc.SC_DTYPE_F32}
+_ACTIVATIONS = {None: SC_CONV_NONE, "none": SC_CONV_NONE, "silu": SC_CONV_SILU}
+_HISTORIES = {"slot": SC_CONV_SLOT, "rows": SC_CONV_ROWS}
 _PAIRS = {"halves": SC_ROPE_HALVES, "neighbours": SC_ROPE_NEIGHBOURS}
 
 
@@ -117,6 +133,38 @@ class RopeAppend(_Op):
         self._args = (C.byref(cache), C.byref(self.desc))
 
 
+def axis_of_pairs(pairs_of_axis, by_turns: bool = False) -> list[int]:
+    """The axis of each pair of a head where axis a turns pairs_of_axis[a] of them: the axes one after another, or by turns for
+    as long as each has pairs left."""
+    runs = [a for a, n in enumerate(pairs_of_axis) for _ in range(n)]
+    if not by_turns:
+        return runs
+    seen, rank = [0] * len(pairs_of_axis), []
+    for a in runs:
+        rank.append((seen[a], a))
+        seen[a] += 1
+    return [a for _, a in sorted(rank)]
+
+
+class RopeAxesAppend(RopeAppend):
+    """RopeAppend with positions of several axes (sc_rope_axes_append_async): `axis` says for each pair which of the `n_axes`
+    rows of `pos` [n_axes][pos_ld] turns it; `pos0` is only the first cell."""
+    _name, _call = "sc_rope_axes_append_async", staticmethod(lib.sc_rope_axes_append_async)
+
+    def __init__(self, cache: KvCache, k, v, act, *, axis, pos, n_axes: int, pos_ld: int | None = None, **kw):
+        super().__init__(cache, k, v, act, **kw)
+        axis = list(axis)
+        if len(axis) != self.desc.rot_dim // 2:
+            raise ValueError(f"the axes of {len(axis)} pairs for rot_dim {self.desc.rot_dim}")
+        if any(not 0 <= a < n_axes for a in axis):
+            raise ValueError(f"an axis that is not below {n_axes}")
+        pairs = (C.c_uint8 * max(len(axis), 1))(*axis)
+        self.axes = RopeAxesDesc(n_axes=n_axes, host_axis=C.cast(pairs, C.POINTER(C.c_uint8)), pos=_ptr(pos),
+                                 pos_ld=self.desc.tokens if pos_ld is None else pos_ld)
+        self._axes_things = (pairs, pos)
+        self._args = (C.byref(cache), C.byref(self.desc), C.byref(self.axes))
+
+
 class AttnDecode(_Op):
     """One new token a sequence over its paged cache (sc_attn_decode_async).  `max_len` bounds every length; a workspace
     is allocated here unless one is given (`workspace`, `workspace_bytes`)."""
@@ -138,12 +186,62 @@ class AttnDecode(_Op):
         self._args = (C.byref(cache), C.byref(self.desc), _ptr(workspace), workspace_bytes)
 
 
+def _bases(bases) -> sc.DeviceBuffer:
+    """The device array of one pointer a sequence, 0 for None."""
+    buf = sc.DeviceBuffer(max(len(bases), 1), "uint64")
+    buf.upload([b or 0 for b in bases])
+    return buf
+
+
+class ConvStates:
+    """Where the histories of a batch lie: the bases, device array of one pointer a sequence, and the layout."""
+
+    def __init__(self, bases, channels: int, taps: int, offset: int, layout: str, ld: int, keep=()):
+        if layout not in _HISTORIES:
+            raise ValueError(f"a history's layout is 'slot' or 'rows', not {layout!r}")
+        self.bases, self.n_seqs = _bases(bases), len(bases)
+        self.channels, self.taps, self.offset, self.layout, self.ld, self.keep = channels, taps, offset, layout, ld, keep
+
+
+def conv_states(state, *, n_seqs: int, channels: int, taps: int, layout: str = "slot") -> ConvStates:
+    """Histories of one layer, one after the other in one f32 buffer: [channels][taps - 1] ("slot") or its transpose ("rows")."""
+    base, each = _ptr(state), 4 * channels * (taps - 1)
+    return ConvStates([base + i * each for i in range(n_seqs)], channels, taps, 0, layout, channels, keep=state)
+
+
+def slot_conv(geo: sc.Geometry, slots, layer: int) -> ConvStates:
+    """GDN layer `layer` of decode slots (sc_handoff.Slot, or None for a sequence without one): the history behind its state."""
+    bases = [None if s is None else s.gdn.data_ptr() for s in slots]
+    offset = layer * geo.gdn_row_floats + geo.ssm_state_size * geo.ssm_v_heads * geo.ssm_state_size
+    return ConvStates(bases, geo.ssm_conv_channels, geo.ssm_d_conv, offset, "slot", geo.ssm_conv_channels, keep=slots)
+
+
+class Conv(_Op):
+    """The short causal convolution before a recurrent layer (sc_conv_async): every sequence's rows, or without `cu` one new
+    token of each; `activation` is "silu" or None."""
+    _name, _call = "sc_conv_async", staticmethod(lib.sc_conv_async)
+
+    def __init__(self, states: ConvStates, x, weight, out, act, *, n_seqs: int, tokens: int, cu=None, bias=None, activation="silu",
+                 x_ld: int | None = None, out_ld: int | None = None):
+        if n_seqs != states.n_seqs:
+            raise ValueError(f"{n_seqs} sequences with the histories of {states.n_seqs}")
+        if activation not in _ACTIVATIONS:
+            raise ValueError(f"an activation is 'silu' or None, not {activation!r}")
+        C_ = states.channels
+        self.desc = ConvDesc(
+            channels=C_, taps=states.taps, n_seqs=n_seqs, tokens=tokens, cu=_ptr(cu), dtype=_dtype(act), x=_ptr(x), out=_ptr(out),
+            x_ld=C_ if x_ld is None else x_ld, out_ld=C_ if out_ld is None else out_ld, weight=_ptr(weight), bias=_ptr(bias),
+            activation=_ACTIVATIONS[activation], state=_ptr(states.bases), state_offset=states.offset,
+            state_layout=_HISTORIES[states.layout], state_ld=states.ld)
+        self._keep(states, x, weight, out, cu, bias)
+        self._args = (C.byref(self.desc),)
+
+
 class GdnStates:
     """Where the recurrent states of a batch lie: the bases, device array of one pointer a sequence, and the strides."""
 
     def __init__(self, bases, v_heads: int, state_size: int, offset: int, head_ld: int, key_ld: int, keep=()):
-        self.bases = sc.DeviceBuffer(max(len(bases), 1), "uint64")
-        self.bases.upload([b or 0 for b in bases])
+        self.bases = _bases(bases)
         self.n_seqs, self.v_heads, self.state_size = len(bases), v_heads, state_size
         self.offset, self.head_ld, self.key_ld, self.keep = offset, head_ld, key_ld, keep
 
