@@ -120,6 +120,36 @@ uint64_t sc_attn_decode_workspace_bytes(const sc_kv_cache* cache, const sc_attn_
 int sc_attn_decode_async(const sc_kv_cache* cache, const sc_attn_decode* a, void* workspace, uint64_t workspace_bytes,
                          void* stream);
 
+typedef struct sc_kv_evict {
+    int32_t n_seqs;           /* 1 .. SC_ATTN_MAX_SEQS */
+    const int64_t* lens;      /* [n_seqs] cells of each sequence; < 0 counts as 0, more than max_len as max_len */
+    int64_t max_len;          /* host bound on every length, at most table_ld * page_size */
+    int64_t keep;             /* cells that a sequence may keep, at least 1: one that has no more is left as it is */
+    int64_t sinks;            /* its first tokens and its latest ones are kept whatever their mass: sinks + recent <= keep */
+    int64_t recent;
+    const float* mass;        /* [n_seqs][n_head_kv][ld], 4-byte aligned */
+    float* mass_out;          /* likewise, or `mass` itself: the mass of the cells that are kept, at their new places, and 0 in the
+                                 rest of the old length */
+    const int32_t* born;      /* [n_seqs][n_head_kv][ld] the number of the token that each cell holds (0 the first), or NULL */
+    int32_t* born_out;        /* likewise, or `born` itself, or NULL: the numbers of the cells that are kept */
+    int64_t ld;               /* of all four: at least max_len, 1 .. 2^31 - 1 */
+    const int64_t* known;     /* [n_seqs] cells whose number `born` holds, the last eviction's lens_out: later cells are the latest
+                                 tokens in order.  Given with `born`; NULL: no cell's */
+    const int64_t* total;     /* [n_seqs] tokens so far, evicted ones too, below 2^31; NULL: the lengths, nothing was evicted */
+    int64_t* lens_out;        /* [n_seqs] the new lengths, min(length, keep); may be lens, known or total */
+} sc_kv_evict;
+
+/* Of each kv head of each sequence with more than `keep` cells, keeps `keep`: the first `sinks` tokens, the `recent` latest, then
+ * those with the largest mass (equal ones from the lowest cell on, NaN last).  A kept cell below `keep` stays; the others' rows (keys,
+ * values, scales) move to the places below `keep` that have become free, in ascending order both.  Cells from `keep` on keep
+ * what they hold and are no longer the sequence's: their pages can be given to others.  So a cache is in no order after this:
+ * attention over it needs none, but a window by cells means nothing there, and positions are given to the next append apart from its
+ * cells (sc_rope_axes_append_async).  Each kv head keeps cells of its own.  The pages below a length are to be resident and the
+ * sequence's own: a row is neither read from nor written to a page that is not resident.  Two launches; the result does not
+ * depend on timing. */
+uint64_t sc_kv_evict_workspace_bytes(const sc_kv_cache* cache, const sc_kv_evict* a);
+int sc_kv_evict_async(const sc_kv_cache* cache, const sc_kv_evict* a, void* workspace, uint64_t workspace_bytes, void* stream);
+
 /* ---- the short convolution before a recurrent layer --------------------------------------------------------------------- */
 
 enum { SC_CONV_NONE = 0, SC_CONV_SILU = 1 };             /* what is applied to the sums */

@@ -89,3 +89,20 @@ def dequant(codes: np.ndarray, scales: np.ndarray) -> np.ndarray:
     """int8 rows [..][D] with f16 scales (bits) [..][D / 64]."""
     s = scales.view(np.float16).astype(np.float64)
     return codes.astype(np.float64) * np.repeat(s, BLOCK, -1)
+
+
+def evict(mass, born, total: int, keep: int, sinks: int, recent: int):
+    """One kv head of one sequence: the mass and the token's number of each cell; the cell that each place holds afterwards
+    (places below min(len(mass), keep))."""
+    n = len(mass)
+    if n <= keep:
+        return np.arange(n)
+    weight = np.array([-np.inf if np.isnan(m) else m for m in np.asarray(mass, np.float64)])
+    nan = np.isnan(np.asarray(mass, np.float64))
+    always = np.array([b < sinks or b >= total - recent for b in born])
+    order = sorted(range(n), key=lambda c: (not always[c], nan[c], -weight[c], c) if not always[c] else (False, False, 0.0, c))
+    kept = set(order[:keep])
+    place = np.arange(keep)
+    free = [c for c in range(keep) if c not in kept]
+    place[free] = sorted(c for c in kept if c >= keep)
+    return place

@@ -1,5 +1,5 @@
 // sc_ops.hpp - the arguments of the operators' kernels (include/sc_ops.h), shared by their host layer (sc_ops_capi.cpp)
-// and the kernels (sc_rope.hip, sc_attn.hip, sc_conv.hip, sc_gdn.hip).  Everything travels in the kernel arguments.
+// and the kernels (sc_rope.hip, sc_attn.hip, sc_evict.hip, sc_conv.hip, sc_gdn.hip).  Everything travels in the kernel arguments.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -59,6 +59,26 @@ struct AttnArgs {
     ops_u32x2* where;                     // [n_seqs] parts of a sequence and its first one's place
 };
 
+// A sequence of an eviction: its cells, those with a number of their own, its tokens so far, and the cells that are left.
+struct EvictSeq {
+    uint32_t n, known, total, kept;
+};
+struct EvictArgs {
+    CacheArgs c;
+    const int64_t *lens, *known, *total;
+    int64_t* lens_out;
+    const float* mass;
+    float* mass_out;
+    const int32_t* born;
+    int32_t* born_out;
+    uint64_t ld;                          // cells from head to head of the four
+    uint32_t n_seqs, max_len, keep, sinks, recent;
+    // the workspace, by plan_evict: the cells that move and the places that they go to, `cap` of them a head at most
+    uint32_t cap;
+    EvictSeq* seqs;
+    uint32_t *moved, *dst, *src;
+};
+
 struct ConvArgs {
     const uint8_t* x;
     uint8_t* out;
@@ -98,6 +118,9 @@ uint64_t plan_attn(AttnArgs& a, int head_dim);
 // Places its parts in a workspace of those bytes.
 void place_attn(AttnArgs& a, void* workspace, uint64_t bytes);
 hipError_t launch_attn(const AttnArgs& a, int head_dim, int format, bool f16, hipStream_t stream);
+// Places what the kernels of an eviction leave each other in a workspace (or in none) and returns its bytes.
+uint64_t plan_evict(EvictArgs& a, void* workspace);
+hipError_t launch_evict(const EvictArgs& a, int head_dim, int format, hipStream_t stream);
 hipError_t launch_conv(const ConvArgs& a, int taps, bool f16, bool slot, hipStream_t stream);
 hipError_t launch_gdn_step(const GdnArgs& a, int size, bool f16, hipStream_t stream);
 // Fills the pieces that a call goes in and returns the bytes of its workspace.

@@ -111,6 +111,47 @@ int attn_args(const sc_kv_cache* cache, const sc_attn_decode* d, sc::AttnArgs& a
     return SC_OK;
 }
 
+// Whether two ranges of as many bytes meet without being the same one.
+bool half_over(const void* a, const void* b, uint64_t bytes) {
+    const uint64_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
+    return p != q && (p < q ? q - p : p - q) < bytes;
+}
+
+int evict_args(const sc_kv_cache* cache, const sc_kv_evict* d, sc::EvictArgs& a) {
+    const char* op = "kv_evict";
+    if (!d) return bad(op, "missing request");
+    if (d->n_seqs < 1 || d->n_seqs > SC_ATTN_MAX_SEQS) return bad(op, "n_seqs must be 1 .. SC_ATTN_MAX_SEQS");
+    if (const int e = cache_args(op, cache, d->n_seqs, a.c)) return e;
+    if (d->max_len < 0 || d->max_len > int64_t(a.c.cells)) return bad(op, "max_len must be 0 .. table_ld * page_size");
+    if (d->keep < 1 || d->keep > INT32_MAX) return bad(op, "keep must be 1 .. 2^31 - 1");
+    if (d->sinks < 0 || d->recent < 0 || d->sinks > d->keep || d->recent > d->keep - d->sinks)
+        return bad(op, "sinks and recent must not be negative, nor more than keep together");
+    if (!d->lens || off(d->lens, 8) || !d->lens_out || off(d->lens_out, 8)) return bad(op, "lens and lens_out must be given, 8-byte aligned");
+    if (off(d->known, 8) || off(d->total, 8)) return bad(op, "known and total must be 8-byte aligned");
+    if (!d->mass || off(d->mass, 4) || !d->mass_out || off(d->mass_out, 4)) return bad(op, "mass and mass_out must be given, 4-byte aligned");
+    if (off(d->born, 4) || off(d->born_out, 4)) return bad(op, "born and born_out must be 4-byte aligned");
+    if (!d->born != !d->known) return bad(op, "born and known are given together");
+    if (d->ld < d->max_len || d->ld < 1 || d->ld > INT32_MAX) return bad(op, "ld must be at least max_len, 1 .. 2^31 - 1");
+    const uint64_t bytes = uint64_t(d->n_seqs) * uint64_t(cache->n_head_kv) * uint64_t(d->ld) * 4;
+    if (half_over(d->mass, d->mass_out, bytes) || (d->born && d->born_out && half_over(d->born, d->born_out, bytes)))
+        return bad(op, "mass_out and born_out must be mass and born or share no byte with them");
+    a.lens = d->lens;
+    a.known = d->known;
+    a.total = d->total;
+    a.lens_out = d->lens_out;
+    a.mass = d->mass;
+    a.mass_out = d->mass_out;
+    a.born = d->born;
+    a.born_out = d->born_out;
+    a.ld = uint64_t(d->ld);
+    a.n_seqs = uint32_t(d->n_seqs);
+    a.max_len = uint32_t(d->max_len);
+    a.keep = uint32_t(d->keep);
+    a.sinks = uint32_t(d->sinks);
+    a.recent = uint32_t(d->recent);
+    return SC_OK;
+}
+
 int gdn_args(const char* op, const sc_gdn* d, bool step, sc::GdnArgs& a) {
     if (!d) return bad(op, "missing request");
     if (d->state_size != 32 && d->state_size != 64 && d->state_size != 128) return bad(op, "state_size must be 32, 64 or 128");
@@ -265,6 +306,22 @@ int sc_attn_decode_async(const sc_kv_cache* cache, const sc_attn_decode* d, void
         sc::place_attn(a, workspace, need);
         return launched(sc::launch_attn(a, int(cache->head_dim), cache->format, d->dtype == SC_DTYPE_F16,
                                         static_cast<hipStream_t>(stream)), op);
+    });
+}
+
+uint64_t sc_kv_evict_workspace_bytes(const sc_kv_cache* cache, const sc_kv_evict* d) {
+    sc::EvictArgs a{};
+    return guarded([&] { return evict_args(cache, d, a); }) == SC_OK ? sc::plan_evict(a, nullptr) : 0;
+}
+
+int sc_kv_evict_async(const sc_kv_cache* cache, const sc_kv_evict* d, void* workspace, uint64_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        const char* op = "kv_evict";
+        sc::EvictArgs a{};
+        if (const int e = evict_args(cache, d, a)) return e;
+        if (!workspace || off(workspace, 16) || workspace_bytes < sc::plan_evict(a, workspace))
+            return bad(op, "workspace missing, not 16-byte aligned or below sc_kv_evict_workspace_bytes");
+        return launched(sc::launch_evict(a, int(cache->head_dim), cache->format, static_cast<hipStream_t>(stream)), op);
     });
 }
 

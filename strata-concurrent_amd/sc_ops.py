@@ -39,6 +39,11 @@ class AttnDecodeDesc(C.Structure):
                 ("q", _P), ("out", _P), ("q_ld", _I64), ("out_ld", _I64), ("lse", _P), ("scale", C.c_float)]
 
 
+class KvEvictDesc(C.Structure):
+    _fields_ = [("n_seqs", _I32), ("lens", _P), ("max_len", _I64), ("keep", _I64), ("sinks", _I64), ("recent", _I64), ("mass", _P),
+                ("mass_out", _P), ("born", _P), ("born_out", _P), ("ld", _I64), ("known", _P), ("total", _P), ("lens_out", _P)]
+
+
 class ConvDesc(C.Structure):
     _fields_ = [("channels", _I64), ("taps", _I32), ("n_seqs", _I32), ("tokens", _I64), ("cu", _P), ("dtype", _I32), ("x", _P),
                 ("out", _P), ("x_ld", _I64), ("out_ld", _I64), ("weight", _P), ("bias", _P), ("activation", _I32), ("state", _P),
@@ -58,6 +63,8 @@ _SIGS = {
     "sc_rope_axes_append_async": (C.c_int, [C.POINTER(KvCache), C.POINTER(RopeAppendDesc), C.POINTER(RopeAxesDesc), _P]),
     "sc_attn_decode_workspace_bytes": (_U64, [C.POINTER(KvCache), C.POINTER(AttnDecodeDesc)]),
     "sc_attn_decode_async": (C.c_int, [C.POINTER(KvCache), C.POINTER(AttnDecodeDesc), _P, _U64, _P]),
+    "sc_kv_evict_workspace_bytes": (_U64, [C.POINTER(KvCache), C.POINTER(KvEvictDesc)]),
+    "sc_kv_evict_async": (C.c_int, [C.POINTER(KvCache), C.POINTER(KvEvictDesc), _P, _U64, _P]),
     "sc_conv_async": (C.c_int, [C.POINTER(ConvDesc), _P]),
     "sc_gdn_step_async": (C.c_int, [C.POINTER(GdnDesc), _P]),
     "sc_gdn_chunk_workspace_bytes": (_U64, [C.POINTER(GdnDesc)]),
@@ -183,6 +190,27 @@ class AttnDecode(_Op):
                 raise sc.ScError(sc.SC_EINVAL, "sc_attn_decode_workspace_bytes")
             workspace = sc.DeviceBuffer(workspace_bytes, "uint8")
         self._keep(cache, q, out, lens, lse, workspace)
+        self._args = (C.byref(cache), C.byref(self.desc), _ptr(workspace), workspace_bytes)
+
+
+class KvEvict(_Op):
+    """The cells with the most mass kept, moved to the front of a paged cache (sc_kv_evict_async).  `mass_out` is `mass`, and
+    `born_out` is `born`, unless they are given; a workspace is allocated here unless one is given."""
+    _name, _call = "sc_kv_evict_async", staticmethod(lib.sc_kv_evict_async)
+
+    def __init__(self, cache: KvCache, mass, *, n_seqs: int, lens, max_len: int, keep: int, lens_out, sinks: int = 0, recent: int = 0,
+                 mass_out=None, born=None, born_out=None, ld: int | None = None, known=None, total=None, workspace=None,
+                 workspace_bytes: int = 0):
+        mass_out, born_out = mass if mass_out is None else mass_out, born if born_out is None else born_out
+        self.desc = KvEvictDesc(n_seqs=n_seqs, lens=_ptr(lens), max_len=max_len, keep=keep, sinks=sinks, recent=recent, mass=_ptr(mass),
+                                mass_out=_ptr(mass_out), born=_ptr(born), born_out=_ptr(born_out), ld=max_len if ld is None else ld,
+                                known=_ptr(known), total=_ptr(total), lens_out=_ptr(lens_out))
+        if workspace is None:
+            workspace_bytes = int(lib.sc_kv_evict_workspace_bytes(C.byref(cache), C.byref(self.desc)))
+            if not workspace_bytes:
+                raise sc.ScError(sc.SC_EINVAL, "sc_kv_evict_workspace_bytes")
+            workspace = sc.DeviceBuffer(workspace_bytes, "uint8")
+        self._keep(cache, mass, mass_out, born, born_out, lens, known, total, lens_out, workspace)
         self._args = (C.byref(cache), C.byref(self.desc), _ptr(workspace), workspace_bytes)
 
 

@@ -145,3 +145,46 @@ def test_outputs_beside_inputs_taken(sc, ops, kw):
 def test_missing_and_empty_convolutions(sc, ops):
     _refused(sc, sc.lib.sc_conv_async(None, None), "missing request")
     assert sc.lib.sc_conv_async(C.byref(_conv(ops, tokens=0, cu=FAKE)), None) == sc.SC_OK
+
+
+# ---- eviction ------------------------------------------------------------------------------------------------------------
+
+
+def _evict(ops, **kw):
+    base = dict(n_seqs=5, lens=FAKE, max_len=256, keep=100, sinks=4, recent=16, mass=FAKE, mass_out=FAKE, born=FAKE, born_out=FAKE, ld=256,
+                known=FAKE, total=FAKE, lens_out=FAKE)
+    return ops.KvEvictDesc(**{**base, **kw})
+
+
+def test_evict_structure_matches_the_header(ops, tmp_path):
+    _same_as_the_header(ops, tmp_path, {"sc_kv_evict": ops.KvEvictDesc})
+
+
+BYTES = 5 * 2 * 256 * 4
+
+
+@pytest.mark.parametrize("kw,why", [
+    (dict(n_seqs=0), "n_seqs"), (dict(n_seqs=1025), "n_seqs"), (dict(max_len=-1), "max_len"), (dict(max_len=257, ld=300), "max_len"),
+    (dict(keep=0), "keep"), (dict(keep=1 << 31), "keep"), (dict(sinks=-1), "sinks"), (dict(recent=-1), "recent"), (dict(recent=97), "recent"),
+    (dict(sinks=1 << 62, recent=1 << 62), "sinks"), (dict(lens=None), "lens"), (dict(lens_out=None), "lens"), (dict(lens_out=FAKE + 4), "lens"),
+    (dict(known=FAKE + 4), "known"), (dict(total=FAKE + 2), "total"), (dict(mass=None), "mass"), (dict(mass_out=None), "mass"),
+    (dict(mass_out=FAKE + 2), "mass"), (dict(born=FAKE + 2), "born"), (dict(born=None), "together"), (dict(known=None), "together"),
+    (dict(ld=255), "ld"), (dict(ld=1 << 31), "ld"), (dict(max_len=0, ld=0), "ld"), (dict(mass_out=FAKE + BYTES - 4), "share no byte"),
+    (dict(mass_out=FAKE - BYTES + 4), "share no byte"), (dict(born_out=FAKE + 4), "share no byte")])
+def test_evictions_refused(sc, ops, kw, why):
+    c, e = _cache(ops), _evict(ops, **kw)
+    _refused(sc, sc.lib.sc_kv_evict_async(C.byref(c), C.byref(e), FAKE, 1 << 50, None), why)
+    assert sc.lib.sc_kv_evict_workspace_bytes(C.byref(c), C.byref(e)) == 0
+
+
+def test_evictions_without_what_they_need(sc, ops):
+    c, e = _cache(ops), _evict(ops)
+    _refused(sc, sc.lib.sc_kv_evict_async(C.byref(c), None, FAKE, 1 << 40, None), "missing request")
+    _refused(sc, sc.lib.sc_kv_evict_async(None, C.byref(e), FAKE, 1 << 40, None), "missing cache")
+    _refused(sc, sc.lib.sc_kv_evict_async(C.byref(_cache(ops, format=2)), C.byref(e), FAKE, 1 << 40, None), "format")
+    need = sc.lib.sc_kv_evict_workspace_bytes(C.byref(c), C.byref(e))
+    assert need > 0
+    for ws, n in ((None, need), (FAKE + 8, need), (FAKE, need - 1)):
+        _refused(sc, sc.lib.sc_kv_evict_async(C.byref(c), C.byref(e), ws, n, None), "workspace")
+    assert sc.lib.sc_kv_evict_workspace_bytes(C.byref(c), C.byref(_evict(ops, keep=256))) > 0   # nothing can be evicted
+    assert sc.lib.sc_kv_evict_workspace_bytes(C.byref(c), C.byref(_evict(ops, mass_out=FAKE + BYTES, born_out=FAKE - BYTES))) == need
