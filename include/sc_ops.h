@@ -120,6 +120,36 @@ uint64_t sc_attn_decode_workspace_bytes(const sc_kv_cache* cache, const sc_attn_
 int sc_attn_decode_async(const sc_kv_cache* cache, const sc_attn_decode* a, void* workspace, uint64_t workspace_bytes,
                          void* stream);
 
+/* ---- what attention has use for ------------------------------------------------------------------------------------------ */
+
+typedef struct sc_attn_mass {
+    int32_t n_seqs;           /* 1 .. SC_ATTN_MAX_SEQS */
+    const int64_t* lens;      /* [n_seqs] cells of each sequence, its latest rows' among them; < 0 counts as 0, more than
+                                 max_len as max_len */
+    int64_t max_len;          /* host bound on every length, at most table_ld * page_size */
+    int64_t window;           /* 0, or the attention's window: a row sees the last `window` of its cells */
+    int64_t rows;             /* R: the latest queries of each sequence, at least 1; rows * n_head / n_head_kv <= 1024 */
+    int32_t dtype;            /* SC_DTYPE_F16 or SC_DTYPE_F32: q */
+    int64_t n_head;           /* query heads, a multiple of n_head_kv, at most 4096 */
+    const void* q;            /* [n_seqs * R][n_head][head_dim], the rotated queries, q_ld values from row to row, 16-byte
+                                 aligned: row r of a sequence is the query of its cell len - R + r, and sees the cells up to it */
+    int64_t q_ld;             /* a multiple of 4 (f32) or 8 (f16) values, at most 2^22 */
+    const float* lse;         /* [n_seqs * R][n_head] the log of each query's sum of exponentials as the attention left it
+                                 (sc_attn_decode's lse), or NULL: formed here, from the same cells */
+    float scale;              /* scores are scale * q . k */
+    float decay;              /* what the mass that is there is multiplied by; 0: it is overwritten, whatever it is */
+    float* mass;              /* [n_seqs][n_head_kv][mass_ld], 4-byte aligned */
+    int64_t mass_ld;          /* at least max_len, at most 2^31 - 1 */
+} sc_attn_mass;
+
+/* mass[s][h][c] = decay * mass[s][h][c] + sum over the rows and the query heads of kv head h of exp(scale * q . k_c - lse), for
+ * the cells below each sequence's length; the rest of `mass` is left as it is.  A cell that a row does not see, or that is not
+ * resident, gets nothing from it; a row that sees no cell, or whose every score is -inf, gives none.  f16 queries are exact, f32
+ * ones two f16 parts, sums in 32 bits; the result does not depend on timing.  Reads the keys only: one launch with `lse`, three
+ * without.  A mass that begins at 0 and is never decayed sums to the number of queries so far times heads. */
+uint64_t sc_attn_mass_workspace_bytes(const sc_kv_cache* cache, const sc_attn_mass* a);
+int sc_attn_mass_async(const sc_kv_cache* cache, const sc_attn_mass* a, void* workspace, uint64_t workspace_bytes, void* stream);
+
 typedef struct sc_kv_evict {
     int32_t n_seqs;           /* 1 .. SC_ATTN_MAX_SEQS */
     const int64_t* lens;      /* [n_seqs] cells of each sequence; < 0 counts as 0, more than max_len as max_len */

@@ -106,3 +106,16 @@ def evict(mass, born, total: int, keep: int, sinks: int, recent: int):
     free = [c for c in range(keep) if c not in kept]
     place[free] = sorted(c for c in kept if c >= keep)
     return place
+
+
+def attention_mass(q, keys, scale: float, lse=None):
+    """The weights that one head's query gives its cells [n][D]; `lse` the log of its sum of exponentials, or formed here."""
+    if not len(keys):
+        return np.zeros(0)
+    s = scale * (np.asarray(keys, np.float64) @ np.asarray(q, np.float64))
+    if lse is not None:
+        return np.zeros(len(s)) if lse == -np.inf else np.exp(s - lse)
+    if s.max() == -np.inf:
+        return np.zeros(len(s))
+    p = np.exp(s - s.max())
+    return p / p.sum()

@@ -33,13 +33,12 @@
 #include <type_traits>
 
 #include "sc_attn_split.hpp"
+#include "sc_attn_tiles.hpp"
 #include "sc_ops.hpp"
 
 namespace sc {
 namespace {
 
-constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f;
-constexpr float kInf = __builtin_inff();
 constexpr int kAttnThreads = kAttnWaves * 64;
 // Log2 of a turn's weights, relative to m: at most kMost, at least kLeast.  Two f16 parts keep a weight to 2^-23 of itself from
 // 2^-2 on, and to 2^-17 from 2^kLeast on.  Where a turn's leave that range m moves, up or down by whole numbers, so that the
@@ -50,8 +49,6 @@ constexpr float kTop = 11.0f, kDeep = 14.0f, kMost = 15.0f, kLeast = -8.0f, kWai
 constexpr float kNear = 12.0f, kNearBy = 0x1p12f;
 constexpr float kTiny = 0x1p-126f;
 
-// 2^x by the hardware's instruction (1 unit in the last place; results below the normal range are 0).
-__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 __device__ __forceinline__ bool rarely(bool x) { return __builtin_expect(x, false); }
 // 2^(a - b), at least the smallest normal number, which changes no sum but leaves infinities what they are; nothing weighs
 // nothing.
@@ -115,13 +112,6 @@ __device__ __forceinline__ bool place_of(const AttnArgs& a, uint32_t lane, uint3
 
 // ---- a wave's turn ------------------------------------------------------------------------------------------------------
 
-__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
-
-__device__ __forceinline__ f16x2 two(uint32_t w) { return __builtin_bit_cast(f16x2, w); }
-__device__ __forceinline__ uint32_t bits(f16x2 h) { return __builtin_bit_cast(uint32_t, h); }
-__device__ __forceinline__ f16x8 eight(uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
-    return __builtin_bit_cast(f16x8, ops_u32x4{a, b, c, d});
-}
 // Two f16 parts of eight values: the value rounded to nearest, and what that left out rounded likewise.
 __device__ __forceinline__ void split8(const float (&p)[8], f16x8& hi, f16x8& lo) {
     uint32_t h[4], r[4];
@@ -164,13 +154,6 @@ __device__ __forceinline__ void add_values(f32x4& o, f16x8 v, const float (&p)[8
     }
 }
 
-// Four int8 codes with 128 added (one exclusive or) as f16: 0x64 above a byte is 1024 + the byte, exactly.
-__device__ __forceinline__ void codes4(uint32_t w, uint32_t& a, uint32_t& b) {
-    const f16x2 off = two(0xE480E480u);   // -1152
-    a = bits(two(__builtin_amdgcn_perm(0x64646464u, w, 0x04010400u)) + off);
-    b = bits(two(__builtin_amdgcn_perm(0x64646464u, w, 0x04030402u)) + off);
-}
-
 template <int D, bool kInt8>
 struct Rows {
     // f16: 16 bytes of 32 values a step; int8: 16 bytes of 64 values a step
@@ -188,36 +171,6 @@ __device__ __forceinline__ uint32_t value_of(uint32_t j, uint32_t r) {
     if constexpr (kInt8) return j / 4 * 64 + r * 4 + j % 4;
     constexpr uint32_t each = D >= 128 ? 8 : 4;
     return j / each * 128 + r * each + j % each;
-}
-
-template <int D>
-__device__ __forceinline__ void ld_scales(uint32_t (&s)[2], const uint16_t* scales, uint64_t row) {
-    if constexpr (D == 256) {
-        const ops_u32x2 w = ld_global<ops_u32x2>(scales + row * 4);
-        s[0] = w.x, s[1] = w.y;
-    } else if constexpr (D == 128) {
-        s[0] = ld_global<uint32_t>(scales + row * 2);
-    } else {
-        s[0] = ld_global<uint16_t>(scales + row);
-    }
-}
-__device__ __forceinline__ float scale_of(const uint32_t (&s)[2], int block) {
-    const f16x2 t = two(s[block / 2]);
-    return float(block & 1 ? t.y : t.x);
-}
-
-// The page table's entry for cell base + l % 32 of a sequence in lane l; a cell past the table reads the last entry.  The
-// load is only waited for where the entry becomes a row.
-__device__ __forceinline__ int32_t entry_of(const AttnArgs& a, uint32_t s, uint32_t base, uint32_t lane) {
-    const uint32_t cell = base + (lane & 31), page = ops_div(cell < a.c.cells ? cell : a.c.cells - 1, a.c.ps);
-    const int64_t at = int64_t(s) * a.c.table_ld + page;
-    return a.c.table ? ld_global<int32_t>(a.c.table + at) : int32_t(at);
-}
-// The pool row of that cell, or -1 where it is outside the span or not resident.
-__device__ __forceinline__ int32_t row_of(const AttnArgs& a, const Span& p, int32_t entry, uint32_t h, uint32_t base, uint32_t lane) {
-    const uint32_t cell = base + (lane & 31), page = ops_div(cell, a.c.ps);
-    const bool in = cell >= p.first && cell < p.len && uint32_t(entry) < a.c.n_pages;
-    return in ? int32_t((uint32_t(entry) * a.c.H + h) * a.c.ps.d + (cell - page * a.c.ps.d)) : -1;
 }
 
 template <int D, bool kInt8>
@@ -311,7 +264,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_part_kernel(AttnArgs a) 
     }
     uint32_t base0 = (a.direct ? 0u : p.span.begin) + wave * kTurn;
     // loads return in the order they are asked for: the first turn's table entries, the queries, then that turn's rows
-    int32_t entry = entry_of(a, p.s, base0 + u0 * kUnit, lane);
+    int32_t entry = entry_of(a.c, p.s, base0 + u0 * kUnit, lane);
     float xq[4][D / 64];   // heads wave, wave + 4, ...: values lane, lane + 64, ...
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i)
@@ -334,11 +287,11 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_part_kernel(AttnArgs a) 
 
     // the first turn's rows are on their way while the queries are laid out
     R r;
-    int32_t row = row_of(a, span, entry, h, base0 + u0 * kUnit, lane);
+    int32_t row = row_of(a.c, span, entry, h, base0 + u0 * kUnit, lane);
     uint32_t there = uint32_t(__ballot(row >= 0));
     row = row < 0 ? 0 : row;
     if (u0 < u1) {
-        entry = entry_of(a, p.s, base0 + (u0 + 1) * kUnit, lane);
+        entry = entry_of(a.c, p.s, base0 + (u0 + 1) * kUnit, lane);
         load_keys<D, kInt8>(r, a, row, lane);
         load_values<D, kInt8>(r, a, row, lane);
     }
@@ -383,10 +336,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_part_kernel(AttnArgs a) 
     float m, l;
     // the rows of turn u, by way of the table's entries
     auto load_row = [&](uint32_t u) {
-        row = row_of(a, span, entry_of(a, p.s, base0 + u * kUnit, lane), h, base0 + u * kUnit, lane);
+        row = row_of(a.c, span, entry_of(a.c, p.s, base0 + u * kUnit, lane), h, base0 + u * kUnit, lane);
         there = uint32_t(__ballot(row >= 0));
         row = row < 0 ? 0 : row;
-        entry = entry_of(a, p.s, base0 + (u + 1) * kUnit, lane);
+        entry = entry_of(a.c, p.s, base0 + (u + 1) * kUnit, lane);
     };
     // The part's turns: weights in two parts, or as they are.
     auto turns = [&](auto form) {
@@ -451,10 +404,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2) attn_part_kernel(AttnArgs a) 
             const uint32_t seen = there;
             const bool more = u + 1 < u1;
             if (more) {
-                row = row_of(a, span, entry, h, base0 + (u + 1) * kUnit, lane);
+                row = row_of(a.c, span, entry, h, base0 + (u + 1) * kUnit, lane);
                 there = uint32_t(__ballot(row >= 0));
                 row = row < 0 ? 0 : row;
-                entry = entry_of(a, p.s, base0 + (u + 2) * kUnit, lane);
+                entry = entry_of(a.c, p.s, base0 + (u + 2) * kUnit, lane);
                 load_keys<D, kInt8>(r, a, row, lane);
             }
             uint32_t gone[8];   // all ones where a cell is not there

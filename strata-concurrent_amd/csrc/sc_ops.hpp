@@ -1,5 +1,5 @@
 // sc_ops.hpp - the arguments of the operators' kernels (include/sc_ops.h), shared by their host layer (sc_ops_capi.cpp)
-// and the kernels (sc_rope.hip, sc_attn.hip, sc_evict.hip, sc_conv.hip, sc_gdn.hip).  Everything travels in the kernel arguments.
+// and the kernels (sc_rope.hip, sc_attn.hip, sc_mass.hip, sc_evict.hip, sc_conv.hip, sc_gdn.hip).  Everything travels in the kernel arguments.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -12,6 +12,7 @@ namespace sc {
 
 using ops_u32x2 = __attribute__((ext_vector_type(2))) uint32_t;
 using ops_u32x4 = __attribute__((ext_vector_type(4))) uint32_t;
+using f32x2 = __attribute__((ext_vector_type(2))) float;
 
 // A paged cache (sc_kv_cache) as the kernels see it.
 struct CacheArgs {
@@ -57,6 +58,23 @@ struct AttnArgs {
     uint32_t parts;                       // parts a sequence can have
     float* ws;                            // the parts' results
     ops_u32x2* where;                     // [n_seqs] parts of a sequence and its first one's place
+};
+
+struct MassArgs {
+    CacheArgs c;
+    const int64_t* lens;
+    const uint8_t* q;
+    const float* lse;
+    float* mass;
+    int64_t q_ld;                         // bytes from row to row
+    uint64_t mass_ld;                     // cells from head to head
+    uint32_t n_seqs, n_head, rows, cols, max_len, window;   // cols: columns of a kv head, rows times its query heads
+    FastDiv G;                            // query heads of a kv head
+    float scale, decay;
+    // without lse, by plan_mass: units of a part, parts of a sequence, their references and sums, the columns' references and
+    // inverse sums
+    uint32_t per, parts;
+    f32x2 *sums, *norm;
 };
 
 // A sequence of an eviction: its cells, those with a number of their own, its tokens so far, and the cells that are left.
@@ -118,6 +136,9 @@ uint64_t plan_attn(AttnArgs& a, int head_dim);
 // Places its parts in a workspace of those bytes.
 void place_attn(AttnArgs& a, void* workspace, uint64_t bytes);
 hipError_t launch_attn(const AttnArgs& a, int head_dim, int format, bool f16, hipStream_t stream);
+// Places what the kernels of a mass leave each other in a workspace (or in none) and returns its bytes.
+uint64_t plan_mass(MassArgs& a, void* workspace);
+hipError_t launch_mass(const MassArgs& a, int head_dim, int format, bool f16, hipStream_t stream);
 // Places what the kernels of an eviction leave each other in a workspace (or in none) and returns its bytes.
 uint64_t plan_evict(EvictArgs& a, void* workspace);
 hipError_t launch_evict(const EvictArgs& a, int head_dim, int format, hipStream_t stream);

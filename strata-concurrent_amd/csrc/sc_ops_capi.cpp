@@ -111,6 +111,44 @@ int attn_args(const sc_kv_cache* cache, const sc_attn_decode* d, sc::AttnArgs& a
     return SC_OK;
 }
 
+int mass_args(const sc_kv_cache* cache, const sc_attn_mass* d, sc::MassArgs& a) {
+    const char* op = "attn_mass";
+    if (!d) return bad(op, "missing request");
+    if (d->n_seqs < 1 || d->n_seqs > SC_ATTN_MAX_SEQS) return bad(op, "n_seqs must be 1 .. SC_ATTN_MAX_SEQS");
+    if (const int e = cache_args(op, cache, d->n_seqs, a.c)) return e;
+    if (d->max_len < 0 || d->max_len > int64_t(a.c.cells)) return bad(op, "max_len must be 0 .. table_ld * page_size");
+    if (d->window < 0) return bad(op, "window must not be negative");
+    if (d->dtype != SC_DTYPE_F16 && d->dtype != SC_DTYPE_F32) return bad(op, "dtype must be f16 or f32");
+    if (d->n_head < 1 || d->n_head > 4096 || d->n_head % cache->n_head_kv)
+        return bad(op, "n_head must be a multiple of n_head_kv, at most 4096");
+    const int64_t G = d->n_head / cache->n_head_kv;
+    if (d->rows < 1 || d->rows > 1024 / G) return bad(op, "rows must be at least 1, rows * n_head / n_head_kv at most 1024");
+    if (!d->lens || off(d->lens, 8)) return bad(op, "lens must be given, 8-byte aligned");
+    if (!d->q || off(d->q, 16)) return bad(op, "q must be given, 16-byte aligned");
+    if (!row_stride(d->q_ld, d->n_head * cache->head_dim, d->dtype))
+        return bad(op, "q_ld must be whole 16 bytes and hold n_head * head_dim values");
+    if (off(d->lse, 4)) return bad(op, "lse must be 4-byte aligned");
+    if (!(d->decay - d->decay == 0)) return bad(op, "decay must be a finite number");
+    if (!d->mass || off(d->mass, 4)) return bad(op, "mass must be given, 4-byte aligned");
+    if (d->mass_ld < d->max_len || d->mass_ld < 1 || d->mass_ld > INT32_MAX) return bad(op, "mass_ld must be at least max_len, 1 .. 2^31 - 1");
+    a.lens = d->lens;
+    a.q = static_cast<const uint8_t*>(d->q);
+    a.lse = d->lse;
+    a.mass = d->mass;
+    a.q_ld = d->q_ld * value_bytes(d->dtype);
+    a.mass_ld = uint64_t(d->mass_ld);
+    a.n_seqs = uint32_t(d->n_seqs);
+    a.n_head = uint32_t(d->n_head);
+    a.rows = uint32_t(d->rows);
+    a.cols = uint32_t(d->rows * G);
+    a.max_len = uint32_t(d->max_len);
+    a.window = d->window >= d->max_len ? 0 : uint32_t(d->window);
+    a.G = sc::make_fastdiv(uint32_t(G));
+    a.scale = d->scale;
+    a.decay = d->decay;
+    return SC_OK;
+}
+
 // Whether two ranges of as many bytes meet without being the same one.
 bool half_over(const void* a, const void* b, uint64_t bytes) {
     const uint64_t p = reinterpret_cast<uintptr_t>(a), q = reinterpret_cast<uintptr_t>(b);
@@ -305,6 +343,24 @@ int sc_attn_decode_async(const sc_kv_cache* cache, const sc_attn_decode* d, void
             return bad(op, "workspace missing, not 16-byte aligned or below sc_attn_decode_workspace_bytes");
         sc::place_attn(a, workspace, need);
         return launched(sc::launch_attn(a, int(cache->head_dim), cache->format, d->dtype == SC_DTYPE_F16,
+                                        static_cast<hipStream_t>(stream)), op);
+    });
+}
+
+uint64_t sc_attn_mass_workspace_bytes(const sc_kv_cache* cache, const sc_attn_mass* d) {
+    sc::MassArgs a{};
+    return guarded([&] { return mass_args(cache, d, a); }) == SC_OK ? sc::plan_mass(a, nullptr) : 0;
+}
+
+int sc_attn_mass_async(const sc_kv_cache* cache, const sc_attn_mass* d, void* workspace, uint64_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        const char* op = "attn_mass";
+        sc::MassArgs a{};
+        if (const int e = mass_args(cache, d, a)) return e;
+        if (!workspace || off(workspace, 16) || workspace_bytes < sc::plan_mass(a, workspace))
+            return bad(op, "workspace missing, not 16-byte aligned or below sc_attn_mass_workspace_bytes");
+        if (d->max_len == 0) return sc::record_ok();
+        return launched(sc::launch_mass(a, int(cache->head_dim), cache->format, d->dtype == SC_DTYPE_F16,
                                         static_cast<hipStream_t>(stream)), op);
     });
 }

@@ -39,6 +39,11 @@ class AttnDecodeDesc(C.Structure):
                 ("q", _P), ("out", _P), ("q_ld", _I64), ("out_ld", _I64), ("lse", _P), ("scale", C.c_float)]
 
 
+class AttnMassDesc(C.Structure):
+    _fields_ = [("n_seqs", _I32), ("lens", _P), ("max_len", _I64), ("window", _I64), ("rows", _I64), ("dtype", _I32), ("n_head", _I64),
+                ("q", _P), ("q_ld", _I64), ("lse", _P), ("scale", C.c_float), ("decay", C.c_float), ("mass", _P), ("mass_ld", _I64)]
+
+
 class KvEvictDesc(C.Structure):
     _fields_ = [("n_seqs", _I32), ("lens", _P), ("max_len", _I64), ("keep", _I64), ("sinks", _I64), ("recent", _I64), ("mass", _P),
                 ("mass_out", _P), ("born", _P), ("born_out", _P), ("ld", _I64), ("known", _P), ("total", _P), ("lens_out", _P)]
@@ -63,6 +68,8 @@ _SIGS = {
     "sc_rope_axes_append_async": (C.c_int, [C.POINTER(KvCache), C.POINTER(RopeAppendDesc), C.POINTER(RopeAxesDesc), _P]),
     "sc_attn_decode_workspace_bytes": (_U64, [C.POINTER(KvCache), C.POINTER(AttnDecodeDesc)]),
     "sc_attn_decode_async": (C.c_int, [C.POINTER(KvCache), C.POINTER(AttnDecodeDesc), _P, _U64, _P]),
+    "sc_attn_mass_workspace_bytes": (_U64, [C.POINTER(KvCache), C.POINTER(AttnMassDesc)]),
+    "sc_attn_mass_async": (C.c_int, [C.POINTER(KvCache), C.POINTER(AttnMassDesc), _P, _U64, _P]),
     "sc_kv_evict_workspace_bytes": (_U64, [C.POINTER(KvCache), C.POINTER(KvEvictDesc)]),
     "sc_kv_evict_async": (C.c_int, [C.POINTER(KvCache), C.POINTER(KvEvictDesc), _P, _U64, _P]),
     "sc_conv_async": (C.c_int, [C.POINTER(ConvDesc), _P]),
@@ -190,6 +197,26 @@ class AttnDecode(_Op):
                 raise sc.ScError(sc.SC_EINVAL, "sc_attn_decode_workspace_bytes")
             workspace = sc.DeviceBuffer(workspace_bytes, "uint8")
         self._keep(cache, q, out, lens, lse, workspace)
+        self._args = (C.byref(cache), C.byref(self.desc), _ptr(workspace), workspace_bytes)
+
+
+class AttnMass(_Op):
+    """The attention weights of the `rows` latest queries of each sequence added to each cell's mass (sc_attn_mass_async).  `lse` is
+    what AttnDecode left, or None; a workspace is allocated here unless one is given."""
+    _name, _call = "sc_attn_mass_async", staticmethod(lib.sc_attn_mass_async)
+
+    def __init__(self, cache: KvCache, q, mass, act, *, n_seqs: int, n_head: int, lens, max_len: int, scale: float, rows: int = 1,
+                 window: int = 0, lse=None, decay: float = 1.0, q_ld: int | None = None, mass_ld: int | None = None, workspace=None,
+                 workspace_bytes: int = 0):
+        self.desc = AttnMassDesc(n_seqs=n_seqs, lens=_ptr(lens), max_len=max_len, window=window, rows=rows, dtype=_dtype(act),
+                                 n_head=n_head, q=_ptr(q), q_ld=n_head * cache.head_dim if q_ld is None else q_ld, lse=_ptr(lse),
+                                 scale=scale, decay=decay, mass=_ptr(mass), mass_ld=max_len if mass_ld is None else mass_ld)
+        if workspace is None:
+            workspace_bytes = int(lib.sc_attn_mass_workspace_bytes(C.byref(cache), C.byref(self.desc)))
+            if not workspace_bytes:
+                raise sc.ScError(sc.SC_EINVAL, "sc_attn_mass_workspace_bytes")
+            workspace = sc.DeviceBuffer(workspace_bytes, "uint8")
+        self._keep(cache, q, mass, lens, lse, workspace)
         self._args = (C.byref(cache), C.byref(self.desc), _ptr(workspace), workspace_bytes)
 
 

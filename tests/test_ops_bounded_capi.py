@@ -188,3 +188,42 @@ def test_evictions_without_what_they_need(sc, ops):
         _refused(sc, sc.lib.sc_kv_evict_async(C.byref(c), C.byref(e), ws, n, None), "workspace")
     assert sc.lib.sc_kv_evict_workspace_bytes(C.byref(c), C.byref(_evict(ops, keep=256))) > 0   # nothing can be evicted
     assert sc.lib.sc_kv_evict_workspace_bytes(C.byref(c), C.byref(_evict(ops, mass_out=FAKE + BYTES, born_out=FAKE - BYTES))) == need
+
+
+# ---- mass ----------------------------------------------------------------------------------------------------------------
+
+
+def _mass(ops, **kw):
+    base = dict(n_seqs=5, lens=FAKE, max_len=256, window=0, rows=1, dtype=0, n_head=24, q=FAKE, q_ld=24 * 256, lse=FAKE, scale=0.0625,
+                decay=1.0, mass=FAKE, mass_ld=256)
+    return ops.AttnMassDesc(**{**base, **kw})
+
+
+def test_mass_structure_matches_the_header(ops, tmp_path):
+    _same_as_the_header(ops, tmp_path, {"sc_attn_mass": ops.AttnMassDesc})
+
+
+@pytest.mark.parametrize("kw,why", [
+    (dict(n_seqs=0), "n_seqs"), (dict(n_seqs=1025), "n_seqs"), (dict(max_len=-1), "max_len"), (dict(max_len=257, mass_ld=300), "max_len"),
+    (dict(window=-1), "window"), (dict(dtype=3), "dtype"), (dict(n_head=25), "n_head"), (dict(n_head=0), "n_head"), (dict(rows=0), "rows"),
+    (dict(rows=86), "rows"), (dict(rows=1 << 60), "rows"), (dict(n_head=4096, q_ld=4096 * 256), "rows"), (dict(lens=None), "lens"),
+    (dict(lens=FAKE + 4), "lens"), (dict(q=None), "q must"), (dict(q=FAKE + 8), "q must"), (dict(q_ld=24 * 256 - 8), "q_ld"),
+    (dict(q_ld=24 * 256 + 4), "q_ld"), (dict(lse=FAKE + 2), "lse"), (dict(decay=float("nan")), "decay"), (dict(decay=float("inf")), "decay"),
+    (dict(mass=None), "mass"), (dict(mass=FAKE + 2), "mass"), (dict(mass_ld=255), "mass_ld"), (dict(mass_ld=1 << 31), "mass_ld")])
+def test_masses_refused(sc, ops, kw, why):
+    c, m = _cache(ops), _mass(ops, **kw)
+    _refused(sc, sc.lib.sc_attn_mass_async(C.byref(c), C.byref(m), FAKE, 1 << 50, None), why)
+    assert sc.lib.sc_attn_mass_workspace_bytes(C.byref(c), C.byref(m)) == 0
+
+
+def test_masses_without_what_they_need(sc, ops):
+    c = _cache(ops)
+    _refused(sc, sc.lib.sc_attn_mass_async(C.byref(c), None, FAKE, 1 << 40, None), "missing request")
+    _refused(sc, sc.lib.sc_attn_mass_async(None, C.byref(_mass(ops)), FAKE, 1 << 40, None), "missing cache")
+    for lse in (FAKE, None):
+        m = _mass(ops, lse=lse, rows=85)
+        need = sc.lib.sc_attn_mass_workspace_bytes(C.byref(c), C.byref(m))
+        assert need > 0
+        for ws, n in ((None, need), (FAKE + 8, need), (FAKE, need - 1)):
+            _refused(sc, sc.lib.sc_attn_mass_async(C.byref(c), C.byref(m), ws, n, None), "workspace")
+    assert sc.lib.sc_attn_mass_async(C.byref(c), C.byref(_mass(ops, max_len=0)), FAKE, 16, None) == sc.SC_OK
