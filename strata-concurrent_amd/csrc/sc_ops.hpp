@@ -81,6 +81,9 @@ struct MassArgs {
 struct EvictSeq {
     uint32_t n, known, total, kept;
 };
+struct EvictFound {
+    uint32_t T, need;
+};
 struct EvictArgs {
     CacheArgs c;
     const int64_t *lens, *known, *total;
@@ -95,6 +98,10 @@ struct EvictArgs {
     uint32_t cap;
     EvictSeq* seqs;
     uint32_t *moved, *dst, *src;
+    // and where a head's cells are shared out among several workgroups what these have counted and found
+    uint32_t shares;
+    uint32_t *counts, *above;
+    EvictFound* found;
 };
 
 struct ConvArgs {

@@ -54,6 +54,14 @@ CASES = [
     ("f16", 2, 64, 4, [264, 264, 260, 250], 256, 4, 32, "spread", [256, 264, 0, 250], 1000),
     ("int8", 1, 256, 7, [1029], 1024, 0, 128, "few", [1024], 31337),
     ("f16", 2, 64, 4, [300, 100], 50, 20, 30, "bits", [100, 100], 7),
+    # heads of several workgroups
+    ("f16", 1, 64, 16, [40000, 3, 17000, 8192], 8192, 4, 100, "spread", None, 0),
+    ("int8", 2, 64, 16, [30001], 29000, 0, 0, "few", [20000], 50000),
+    ("f16", 1, 64, 64, [33000, 32999], 100, 50, 50, "bits", None, 9),
+    ("f16", 2, 64, 32, [25000], 12500, 0, 0, "late", None, 0),
+    ("int8", 1, 64, 8, [16385], 16384, 0, 0, "none", None, 0),
+    # more cells than a workgroup holds, too many heads to share them out
+    ("f16", 130, 64, 64, [8300], 5000, 3, 10, "few", None, 0),
 ]
 
 
