@@ -1,8 +1,13 @@
 // sc_conv.hip - the short causal convolution before a recurrent layer (sc_conv_async).
 //
 // out[t][c] = f(bias[c] + sum_j weight[c][j] x[t - (W - 1) + j][c]): a channel meets no other, and a row is needed by W - 1 rows
-// after it.  It is data movement: a lane has a few channels, their taps in registers, and goes down its rows with the last W - 1
-// of them in registers too, so a row is read once, but for the W - 1 before a tile's first.
+// after it.  It is data movement: a lane has four channels, their taps in registers, and goes down its rows with the last W - 1
+// of them in registers too, so a row is read once, but for the W - 1 before a tile's first.  Those the caches have: a tile's
+// workgroups across the channels are next to each other, so where they are 8 the tiles of the same channels are on one XCD.
+//
+// Measured, 10 854 rows of 8192 channels: f32 120 us, 5.9 TB/s where this library's plain copy reaches 5.7, f16 66 us, 5.4 TB/s.
+// Tiles of 16 rows 123 us in f32 and of 8 rows 69 us in f16; the tiles of the same channels next to each other 158 us; outputs
+// through the caches 125 us.  New tokens are a launch and a chain of loads: one of 8192 channels 3.1 us, 61 of them 4.6 us.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -13,9 +18,8 @@ namespace sc {
 namespace {
 
 constexpr uint32_t kConvThreads = 256;
-constexpr uint32_t kTileRows = 32;      // rows of a prompt's tile
-constexpr uint32_t kAhead = 8;          // rows that are asked for together
-static_assert(kTileRows % kAhead == 0);
+// Rows of a prompt's tile, which are all asked for at once: 128 bytes a lane.
+constexpr uint32_t tile_rows(bool f16) { return f16 ? 16 : 8; }
 
 // v / (1 + e^-v) by the hardware's exponential and reciprocal, 1 unit in the last place each; 0 where e^-v is beyond 2^128.
 __device__ __forceinline__ float silu(float v) { return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.44269504088896340736f)); }
@@ -104,6 +108,7 @@ __global__ void __launch_bounds__(kConvThreads) conv_step_kernel(ConvArgs a) {
 struct Tile {
     uint32_t s, first, rows, at;
 };
+template <uint32_t kRows>
 __device__ __forceinline__ bool tile_of(const ConvArgs& a, uint32_t tile, uint32_t lane, Tile& p) {
     uint32_t before = 0;
     for (uint32_t base = 0; base < a.n_seqs; base += 64) {
@@ -111,7 +116,7 @@ __device__ __forceinline__ bool tile_of(const ConvArgs& a, uint32_t tile, uint32
         int64_t b = in ? ld_global<int64_t>(a.cu + base + lane) : 0, e = in ? ld_global<int64_t>(a.cu + base + lane + 1) : 0;
         b = b < 0 ? 0 : b;
         e = e > int64_t(a.tokens) ? int64_t(a.tokens) : e;
-        const uint32_t rows = e > b ? uint32_t(e - b) : 0u, tiles = (rows + kTileRows - 1) / kTileRows;
+        const uint32_t rows = e > b ? uint32_t(e - b) : 0u, tiles = (rows + kRows - 1) / kRows;
         const uint32_t hi = before + scan_add(tiles), lo = hi - tiles;
         const uint64_t here = __ballot(tile >= lo && tile < hi);
         if (here) {
@@ -131,12 +136,13 @@ __device__ __forceinline__ bool tile_of(const ConvArgs& a, uint32_t tile, uint32
 // one touches it.
 template <int W, bool kF16, bool kSlot>
 __global__ void __launch_bounds__(kConvThreads) conv_prompt_kernel(ConvArgs a) {
-    static_assert(kTileRows >= W - 1);
-    const uint32_t c = (blockIdx.y * blockDim.x + threadIdx.x) * 4;
+    constexpr uint32_t kRows = tile_rows(kF16);
+    static_assert(kRows >= W - 1);
+    const uint32_t tile = ops_div(blockIdx.x, a.blocks), c = ((blockIdx.x - tile * a.blocks.d) * blockDim.x + threadIdx.x) * 4;
     Tile p;
-    if (!tile_of(a, blockIdx.x, threadIdx.x & 63, p)) return;
+    if (!tile_of<kRows>(a, tile, threadIdx.x & 63, p)) return;
     if (c >= a.channels) return;
-    const uint32_t r0 = p.at * kTileRows, n = p.rows - r0 < kTileRows ? p.rows - r0 : kTileRows;
+    const uint32_t r0 = p.at * kRows, n = p.rows - r0 < kRows ? p.rows - r0 : kRows;
     const uint8_t* x = a.x + int64_t(p.first) * a.x_ld;
     uint8_t* out = a.out + int64_t(p.first) * a.out_ld;
     float* base = a.state[p.s];
@@ -145,7 +151,7 @@ __global__ void __launch_bounds__(kConvThreads) conv_prompt_kernel(ConvArgs a) {
         return;
     }
     float* state = base + a.state_offset;
-    f32x4 h[W - 1], w[W];
+    f32x4 h[W - 1], w[W], rows[kRows];
     if (r0) {
 #pragma unroll
         for (int k = 0; k < W - 1; ++k) h[k] = ld_act4<kF16>(x + int64_t(r0 - (W - 1) + k) * a.x_ld, c);
@@ -166,34 +172,32 @@ __global__ void __launch_bounds__(kConvThreads) conv_prompt_kernel(ConvArgs a) {
         }
         st_history<W, kSlot>(next, state, a.state_ld, c);
     }
-    for (uint32_t r = 0; r < n; r += kAhead) {
-        f32x4 rows[kAhead];
 #pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) {
-            const uint32_t at = r0 + (r + i < n ? r + i : n - 1);   // past the tile's last row that row again
-            rows[i] = ld_act4<kF16>(x + int64_t(at) * a.x_ld, c);
-        }
+    for (uint32_t i = 0; i < kRows; ++i) {
+        const uint32_t at = r0 + (i < n ? i : n - 1);   // past the tile's last row that row again
+        rows[i] = ld_act4<kF16>(x + int64_t(at) * a.x_ld, c);
+    }
 #pragma unroll
-        for (uint32_t i = 0; i < kAhead; ++i) {
-            if (r + i < n) st_act4<kF16>(out + int64_t(r0 + r + i) * a.out_ld, c, sum_of<W>(h, rows[i], w, bias, a.silu));
+    for (uint32_t i = 0; i < kRows; ++i) {
+        if (i < n) st_act4<kF16, true>(out + int64_t(r0 + i) * a.out_ld, c, sum_of<W>(h, rows[i], w, bias, a.silu));
 #pragma unroll
-            for (int k = 0; k + 1 < W - 1; ++k) h[k] = h[k + 1];
-            h[W - 2] = rows[i];
-        }
+        for (int k = 0; k + 1 < W - 1; ++k) h[k] = h[k + 1];
+        h[W - 2] = rows[i];
     }
 }
 
 template <int W, bool kF16, bool kSlot>
-hipError_t launch_of(const ConvArgs& a, hipStream_t stream) {
+hipError_t launch_of(ConvArgs a, hipStream_t stream) {
     const uint32_t lanes = a.channels / 4;
     if (!a.cu) {
         hipLaunchKernelGGL((conv_step_kernel<W, kF16, kSlot>), dim3((lanes + kConvThreads - 1) / kConvThreads, a.n_seqs),
                            dim3(kConvThreads), 0, stream, a);
     } else {
         // a sequence has at most one tile that is not whole
-        const uint32_t tiles = a.tokens / kTileRows + (a.n_seqs < a.tokens ? a.n_seqs : a.tokens);
+        const uint32_t tiles = a.tokens / tile_rows(kF16) + (a.n_seqs < a.tokens ? a.n_seqs : a.tokens);
         const uint32_t threads = lanes >= kConvThreads ? kConvThreads : (lanes + 63) / 64 * 64;
-        hipLaunchKernelGGL((conv_prompt_kernel<W, kF16, kSlot>), dim3(tiles, (lanes + threads - 1) / threads), dim3(threads), 0, stream, a);
+        a.blocks = make_fastdiv((lanes + threads - 1) / threads);
+        hipLaunchKernelGGL((conv_prompt_kernel<W, kF16, kSlot>), dim3(tiles * a.blocks.d), dim3(threads), 0, stream, a);
     }
     return hipGetLastError();
 }

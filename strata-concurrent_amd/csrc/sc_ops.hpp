@@ -113,6 +113,7 @@ struct ConvArgs {
     int64_t state_offset, state_ld;
     const int64_t* cu;
     uint32_t n_seqs, tokens, channels, silu;
+    FastDiv blocks;                       // workgroups across the channels of a tile of rows
 };
 
 struct GdnArgs {
