@@ -5,10 +5,14 @@
 // value is read and written once, and the few operations a value hide behind that.  A workgroup takes one token (and, when
 // tokens are few, a share of its rows): the token's cosines and sines are formed once in 64 bits, where the angle at
 // position 10^5 still has its low digits, and its rows of queries, keys and values are then taken a wave each, four values
-// a lane.  A pair's other value is in the lane itself (neighbours) or rot / 8 lanes away (halves: one lane exchange).
-// 10 854 tokens of 24 + 2 x 2 heads of 256 (f32 into an f16 cache): 600 MB in 109 us, 5.5 TB/s where this library's plain copy
-// reaches 5.7.  Rows asked for several at a time, before they are turned, made it slower (119 us by twos, 127 by fours): many
-// waves with a row each keep memory busier than fewer with more.
+// a lane.  A pair's other value is in the lane itself (neighbours) or rot / 8 lanes away (halves: one lane exchange).  With positions
+// of several axes a pair's angle is formed of the position on its axis, which two bits of the arguments name.
+//
+// 10 854 tokens of 24 + 2 x 2 heads of 256: f32 into an f16 cache 600 MB in 107 us, 5.6 TB/s where this library's plain copy
+// reaches 5.7; f16, 311 MB, in 66 us, 4.7 TB/s, where half the bytes have as many rows to turn (half of the vector units' time).
+// Four rows of a wave are asked for together (by ones 106 and 67 us), where a row belongs is decided once a wave, and the
+// sines are read once, not a row: 111 and 68 us without both.  A token a wave instead of four waves a token: 120 and 83 us; its
+// first rows asked for before its sines are formed: 104 and 75.
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -25,6 +29,7 @@ constexpr int kRopeThreads = 256;
 // With fewer, a token's rows are shared by workgroups and the queries left in the caches for the attention that follows
 // (one token of 28 rows: 3.6 us in shares, 4.5 by one workgroup).
 constexpr uint32_t kManyTokens = 512;
+constexpr uint32_t kAhead = 4;    // rows of a wave that are asked for together
 constexpr double kTwoPi = 6.283185307179586476925286766559;
 
 // Writes four values of a pool row at `d` in the cache's format; `row` is the pool row.
@@ -48,7 +53,7 @@ template <int D, bool kInt8, bool kF16, bool kMany>
 __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(RopeArgs a) {
     constexpr uint32_t kLanes = D / 4, kRows = 64 / kLanes;   // lanes of a row, rows of a wave
     __shared__ float s_cos[D / 2], s_sin[D / 2];
-    const uint32_t t = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint32_t t = blockIdx.x, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint32_t s = t;
     int64_t local = 0;
     if (a.cu) {
@@ -78,35 +83,53 @@ __global__ void __launch_bounds__(kRopeThreads) rope_append_kernel(RopeArgs a) {
         if (phys >= 0) row0 = int64_t(phys) * a.c.H * a.c.ps.d + (cell - page * a.c.ps.d);
     }
     const uint32_t d = (lane % kLanes) * 4, total = a.n_head + 2 * a.c.H, half = a.rot / 2;
-    const uint32_t stride = gridDim.y * (kRopeThreads / 64) * kRows;
-    for (uint32_t base = (blockIdx.y * (kRopeThreads / 64) + wave) * kRows; base < total; base += stride) {
-        const uint32_t r = base + lane / kLanes;
-        const bool there = r < total, is_q = r < a.n_head, is_k = !is_q && r < a.n_head + a.c.H;
-        const uint32_t h = !there ? 0 : is_q ? r : is_k ? r - a.n_head : r - a.n_head - a.c.H;
-        const uint8_t* src = is_q ? a.q + t * a.q_ld : is_k ? a.k + t * a.k_ld : a.v + t * a.v_ld;
-        f32x4 x = ld_act4<kF16, true>(src, h * D + d);
-        if (a.rot) {
-            f32x4 o{};
-            uint32_t i[4];
-            float sign[4];
-            if (a.neighbours) {
-                o = f32x4{x.y, x.x, x.w, x.z};
-                for (int j = 0; j < 4; ++j) i[j] = (d + j) / 2, sign[j] = j & 1 ? 1.0f : -1.0f;
-            } else {
-                const uint32_t from = d < half ? lane + half / 4 : d < a.rot ? lane - half / 4 : lane;
-                for (int j = 0; j < 4; ++j) {
-                    o[j] = __shfl(x[j], int(from));
-                    i[j] = d + j < half ? d + j : d + j - half;
-                    sign[j] = d < half ? -1.0f : 1.0f;
-                }
-            }
-            if (d < a.rot && (is_q || is_k))
-                for (int j = 0; j < 4; ++j) x[j] = x[j] * s_cos[i[j]] + sign[j] * o[j] * s_sin[i[j]];
+    // the lane's turn is that of all its rows: of its value j, x cos[j] + (the pair's other value) sin[j], with the sine's sign
+    const bool turns = d < a.rot;
+    f32x4 cos{}, sin{};
+    if (turns)
+#pragma unroll
+        for (uint32_t j = 0; j < 4; ++j) {
+            const uint32_t i = a.neighbours ? (d + j) / 2 : d + j < half ? d + j : d + j - half;
+            cos[j] = s_cos[i];
+            sin[j] = (a.neighbours ? j % 2 == 0 : d < half) ? -s_sin[i] : s_sin[i];
         }
-        if (there && is_q) st_act4<kF16, kMany>(a.q_out + t * a.q_out_ld, h * D + d, x);
-        const bool keep = there && !is_q && row0 >= 0;
-        const uint64_t row = keep ? uint64_t(row0) + uint64_t(h) * a.c.ps.d : 0;
-        st_cache4<D, kInt8>(is_k ? a.c.k : a.c.v, is_k ? a.c.k_scale : a.c.v_scale, row, d, x, keep);
+    const uint32_t from = d < half ? lane + half / 4 : turns ? lane - half / 4 : lane;
+    auto turned = [&](f32x4 x) {
+        f32x4 o{};
+        if (a.neighbours) o = f32x4{x.y, x.x, x.w, x.z};
+        else
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = __shfl(x[j], int(from));
+        if (turns)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = x[j] * cos[j] + o[j] * sin[j];
+        return x;
+    };
+    // the rows of queries, then of keys and of values: for heads of 256 a wave has one row, and where it belongs is the same for its lanes
+    const uint32_t stride = gridDim.y * (kRopeThreads / 64) * kRows;
+    for (uint32_t base = (blockIdx.y * (kRopeThreads / 64) + wave) * kRows; base < total; base += stride * kAhead) {
+        f32x4 rows[kAhead];
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u) {
+            if (base + u * stride >= total) break;
+            const uint32_t r = base + u * stride + lane / kLanes, k = r - a.n_head, v = k - a.c.H;
+            if (r < a.n_head) rows[u] = ld_act4<kF16, true>(a.q + t * a.q_ld, r * D + d);
+            else if (k < a.c.H) rows[u] = ld_act4<kF16, true>(a.k + t * a.k_ld, k * D + d);
+            else if (r < total) rows[u] = ld_act4<kF16, true>(a.v + t * a.v_ld, v * D + d);
+        }
+#pragma unroll
+        for (uint32_t u = 0; u < kAhead; ++u) {
+            if (base + u * stride >= total) break;
+            const uint32_t r = base + u * stride + lane / kLanes, k = r - a.n_head, v = k - a.c.H;
+            f32x4 x = rows[u];
+            if (r < a.n_head) {
+                st_act4<kF16, kMany>(a.q_out + t * a.q_out_ld, r * D + d, a.rot ? turned(x) : x);
+            } else if (r < total && row0 >= 0) {
+                const bool is_k = k < a.c.H;
+                if (is_k && a.rot) x = turned(x);
+                st_cache4<D, kInt8>(is_k ? a.c.k : a.c.v, is_k ? a.c.k_scale : a.c.v_scale, uint64_t(row0) + uint64_t(is_k ? k : v) * a.c.ps.d, d, x, true);
+            }
+        }
     }
 }
 
