@@ -71,10 +71,12 @@ struct MassArgs {
     uint32_t n_seqs, n_head, rows, cols, max_len, window;   // cols: columns of a kv head, rows times its query heads
     FastDiv G;                            // query heads of a kv head
     float scale, decay;
-    // without lse, by plan_mass: units of a part, parts of a sequence, their references and sums, the columns' references and
-    // inverse sums
-    uint32_t per, parts;
+    // by plan_mass: parts of a sequence's cells; in the workspace, without lse, their references and sums and the columns'
+    // references and inverse sums, and many f32 queries' parts with what their products are scaled back by
+    uint32_t parts;
     f32x2 *sums, *norm;
+    ops_u32x4* split;
+    float* back;
 };
 
 // A sequence of an eviction: its cells, those with a number of their own, its tokens so far, and the cells that are left.
@@ -145,7 +147,7 @@ uint64_t plan_attn(AttnArgs& a, int head_dim);
 void place_attn(AttnArgs& a, void* workspace, uint64_t bytes);
 hipError_t launch_attn(const AttnArgs& a, int head_dim, int format, bool f16, hipStream_t stream);
 // Places what the kernels of a mass leave each other in a workspace (or in none) and returns its bytes.
-uint64_t plan_mass(MassArgs& a, void* workspace);
+uint64_t plan_mass(MassArgs& a, int head_dim, bool f16, void* workspace);
 hipError_t launch_mass(const MassArgs& a, int head_dim, int format, bool f16, hipStream_t stream);
 // Places what the kernels of an eviction leave each other in a workspace (or in none) and returns its bytes.
 uint64_t plan_evict(EvictArgs& a, void* workspace);

@@ -349,7 +349,8 @@ int sc_attn_decode_async(const sc_kv_cache* cache, const sc_attn_decode* d, void
 
 uint64_t sc_attn_mass_workspace_bytes(const sc_kv_cache* cache, const sc_attn_mass* d) {
     sc::MassArgs a{};
-    return guarded([&] { return mass_args(cache, d, a); }) == SC_OK ? sc::plan_mass(a, nullptr) : 0;
+    return guarded([&] { return mass_args(cache, d, a); }) == SC_OK
+               ? sc::plan_mass(a, int(cache->head_dim), d->dtype == SC_DTYPE_F16, nullptr) : 0;
 }
 
 int sc_attn_mass_async(const sc_kv_cache* cache, const sc_attn_mass* d, void* workspace, uint64_t workspace_bytes, void* stream) {
@@ -357,11 +358,11 @@ int sc_attn_mass_async(const sc_kv_cache* cache, const sc_attn_mass* d, void* wo
         const char* op = "attn_mass";
         sc::MassArgs a{};
         if (const int e = mass_args(cache, d, a)) return e;
-        if (!workspace || off(workspace, 16) || workspace_bytes < sc::plan_mass(a, workspace))
+        const bool f16 = d->dtype == SC_DTYPE_F16;
+        if (!workspace || off(workspace, 16) || workspace_bytes < sc::plan_mass(a, int(cache->head_dim), f16, workspace))
             return bad(op, "workspace missing, not 16-byte aligned or below sc_attn_mass_workspace_bytes");
         if (d->max_len == 0) return sc::record_ok();
-        return launched(sc::launch_mass(a, int(cache->head_dim), cache->format, d->dtype == SC_DTYPE_F16,
-                                        static_cast<hipStream_t>(stream)), op);
+        return launched(sc::launch_mass(a, int(cache->head_dim), cache->format, f16, static_cast<hipStream_t>(stream)), op);
     });
 }
 
