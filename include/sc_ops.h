@@ -145,8 +145,8 @@ typedef struct sc_attn_mass {
 /* mass[s][h][c] = decay * mass[s][h][c] + sum over the rows and the query heads of kv head h of exp(scale * q . k_c - lse), for
  * the cells below each sequence's length; the rest of `mass` is left as it is.  A cell that a row does not see, or that is not
  * resident, gets nothing from it; a row that sees no cell, or whose every score is -inf, gives none.  f16 queries are exact, f32
- * ones two f16 parts, sums in 32 bits; the result does not depend on timing.  Reads the keys only: one launch with `lse`, three
- * without.  A mass that begins at 0 and is never decayed sums to the number of queries so far times heads. */
+ * ones two f16 parts, sums in 32 bits; the result does not depend on timing.  Reads the keys only, once with `lse` and twice without; one to
+ * four launches.  A mass that begins at 0 and is never decayed sums to the number of queries so far times heads. */
 uint64_t sc_attn_mass_workspace_bytes(const sc_kv_cache* cache, const sc_attn_mass* a);
 int sc_attn_mass_async(const sc_kv_cache* cache, const sc_attn_mass* a, void* workspace, uint64_t workspace_bytes, void* stream);
 
@@ -175,8 +175,9 @@ typedef struct sc_kv_evict {
  * what they hold and are no longer the sequence's: their pages can be given to others.  So a cache is in no order after this:
  * attention over it needs none, but a window by cells means nothing there, and positions are given to the next append apart from its
  * cells (sc_rope_axes_append_async).  Each kv head keeps cells of its own.  The pages below a length are to be resident and the
- * sequence's own: a row is neither read from nor written to a page that is not resident.  Two launches; the result does not
- * depend on timing. */
+ * sequence's own: a row is neither read from nor written to a page that is not resident.  One launch where a head can
+ * move 128 cells at most and lens_out shares nothing with what it is made from, else two, or five for long heads that several
+ * workgroups share; the result does not depend on timing.  Layers that share an array of lengths need lens_out apart from it. */
 uint64_t sc_kv_evict_workspace_bytes(const sc_kv_cache* cache, const sc_kv_evict* a);
 int sc_kv_evict_async(const sc_kv_cache* cache, const sc_kv_evict* a, void* workspace, uint64_t workspace_bytes, void* stream);
 
