@@ -4,9 +4,17 @@
 // A cell's key is its mass in an order of whole numbers, the largest of all for tokens that are kept whatever their mass.  Of
 // the n cells of a kv head `keep` are kept: those above the keep-th largest key T, and as many of those equal to it, from the
 // lowest cell on, as there is room for.  T is found by parts of 11, 11 and 10 bits from the highest on: the counts of a part's
-// values among the keys that share the parts found so far.  In one more pass over the cells a prefix count gives each cell the number of kept
-// ones before it, and with that the place in the list of kept cells at or past `keep` or of free places below it: the i-th of
-// one goes to the i-th of the other.  No source is a destination, so rows move in any order.
+// values among the keys that share the parts found so far.  In one more pass over the cells a prefix count gives each cell the
+// number of kept ones before it, and with that the place in the list of kept cells at or past `keep` or of free places below it:
+// the i-th of one goes to the i-th of the other.  No source is a destination, so rows move in any order.
+//
+// A workgroup chooses for a head; its keys stay in registers where it has them all, and a thread asks for all of its cells at
+// once (asked for one by one 131 072 cells took it 210 us).  What bounds it is a chain of latencies and barriers: 9 us for 4 K
+// cells.  Where a head can move few rows the workgroup moves them itself (32 caches of 2064 cells to 2048: 10 us in all, 14
+// with a launch for the moves).  One workgroup is bound by its unit's instructions for many cells, so from three chunks on, if
+// heads are few, several share a head and a launch ends each part: 131 072 cells 35 us (134 by one), 16 K cells 33 us in all
+// where one workgroup takes 29.  The moves are bound by rows of 512 bytes at places all over the pool: 57 MB in 16 us, 3.6 TB/s;
+// two pairs of a wave on their way (four 18 us, and 15 us against 13.4 for 8 short caches), through the caches (past them 18).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -23,8 +31,9 @@ constexpr uint32_t kCopies = 4;         // counts of each value, for as many lan
 constexpr uint32_t kValues = 2048;      // of a part of a key
 constexpr uint32_t kCopy = kValues + 2; // from copy to copy: another bank
 constexpr uint32_t kFewMoves = 128;     // moves of a head at most that are made where they are chosen
-constexpr uint32_t kShares = 256;       // workgroups that heads of more than a chunk are shared out among
-constexpr uint32_t kMoveThreads = 256, kMoveWaves = kMoveThreads / 64, kMoveAhead = 4;
+constexpr uint32_t kShares = 256;       // workgroups that heads of more than a chunk are shared out among, a chunk each at least
+constexpr uint32_t kLeastShares = 3;    // that a head is shared out among
+constexpr uint32_t kMoveThreads = 256, kMoveWaves = kMoveThreads / 64, kMoveAhead = 2;
 constexpr int kParts = 3, kShift[kParts] = {21, 10, 0};   // the parts of a key, from the highest on
 
 // Masses as whole numbers in the same order: NaN below all, -0 with 0.
@@ -106,7 +115,7 @@ __device__ __forceinline__ void move_rows(const EvictArgs& a, const Cells& cells
             const int64_t r = row_of(a, s, h, from[u]), t = row_of(a, s, h, to[u]);
             r_to[u] = r < 0 || !there[u] ? -1 : t;
             const uint64_t row = r < 0 ? 0 : uint64_t(r);
-            x[u] = ld_once<ops_u32x4>(pool + row * R::kBytes + piece * 16);
+            x[u] = ld_global<ops_u32x4>(pool + row * R::kBytes + piece * 16);
             if constexpr (R::kInt8) {
                 const uint16_t* p = scales + row * R::kBlocks;
                 if constexpr (R::kBlocks == 4) scale[u] = ld_global<uint64_t>(p);
@@ -456,8 +465,9 @@ uint64_t plan_evict(EvictArgs& a, void* workspace) {
     a.src = reinterpret_cast<uint32_t*>(take(list));
     const uint64_t chunks = (uint64_t(a.max_len) + kChunk - 1) / kChunk, most = kShares / heads;
     a.shares = uint32_t(chunks < most ? chunks : most);
-    if (a.shares <= 1) a.shares = 1;
-    else {
+    if (a.shares < kLeastShares) {
+        a.shares = 1;
+    } else {
         a.counts = reinterpret_cast<uint32_t*>(take(heads * a.shares * kParts * kValues * 4));
         a.above = reinterpret_cast<uint32_t*>(take(heads * a.shares * (kParts - 1) * 4));
         a.found = reinterpret_cast<EvictFound*>(take(heads * kParts * sizeof(EvictFound)));
