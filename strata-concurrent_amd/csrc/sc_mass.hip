@@ -13,13 +13,13 @@
 // always in the same order.
 //   Up to 16 columns (a new token a sequence): the queries are laid out once, a wave takes 32 cells a turn and has its next turn's
 //   keys on the way while it forms weights.  Reading the keys bounds it, and for short calls the chain of latencies to the first
-//   weights.  2 kv heads of 256 and 24 query heads: 1021 cells 5.8 us; 24 sequences up to 8190 cells in int8, 57 MB, 24 us; 128 K
-//   cells in f16, 135 MB, 34 us.
+//   weights.  2 kv heads of 256 and 24 query heads: 1021 cells 5.8 us; 24 sequences up to 8190 cells in int8, 57 MB, 18 us (24
+//   where a lane loads the scales of its eight cells itself and keys go past the caches); 128 K cells in f16, 135 MB, 34 us.
 //   More columns: a workgroup's waves share 128 cells' keys and go over the tiles of columns, the next tiles' queries on their way to
 //   LDS meanwhile, and what the sets of waves have summed up is added at the end.  Half of a call is the products and the weights,
 //   half the way to the first of them.  32 queries of two prompts up to 16 381 cells without their sums, 23 GFLOP: 59 us (27 a
 //   pass, the join 5).  Tried: 64 cells a wave, which needs all registers of a SIMD for two waves (80 us), one tile of columns at
-//   a time for three waves a SIMD (65).
+//   a time for three waves a SIMD (65), the weights of cells that are all seen in a branch of their own (65).
 #include <hip/hip_runtime.h>
 
 #include <cstdint>
@@ -34,7 +34,7 @@ namespace {
 constexpr uint32_t kMassThreads = kAttnWaves * 64;
 constexpr uint32_t kMostColumns = 1024;         // rows times query heads of a kv head
 // Workgroups that the cells are shared out among where columns are few.  A long f16 sequence likes fewer (128 K cells: 30 us with 256,
-// 34 with 1024), a batch more (24 int8 sequences: 41 and 24; eight f16 ones with f32 queries: 22 and 16).
+// 34 with 1024), a batch more (24 int8 sequences: 41 and 24, before their scales came by LDS; eight f16 ones with f32 queries: 22 and 16).
 constexpr uint32_t kFewSlots = 1024;
 constexpr float kLog2eRest = 1.92596299e-8f;    // log2(e) - kLog2e
 
@@ -111,22 +111,34 @@ __device__ __forceinline__ void scaling(float top, float& by, float& back) {
 template <int D, bool kInt8>
 struct KeyRows {
     static constexpr int kLoads = kInt8 ? D / 64 : D / 32;
+    static constexpr uint32_t kScaleWords = D == 256 ? 2 : 1;   // f16 scales of a cell, a block of 64 each
     ops_u32x4 w[2][kLoads];
-    uint32_t scale[kInt8 ? 8 : 1][2];   // f16 scales of the lane's results' cells, a block of 64 each
+    uint32_t own[2];                    // scales of cell lane % 32
+    uint32_t scale[kInt8 ? 8 : 1][2];   // and of the cells of the lane's results
 
-    // `row`: the cells' pool rows, in lanes 0 .. 31
+    // `row`: the cells' pool rows, in lanes 0 .. 31 and again in the others
     __device__ __forceinline__ void load(const CacheArgs& c, uint32_t row, uint32_t lane) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             const uint32_t at = uint32_t(__shfl(int(row), int(t * 16 + (lane & 15))));
             const uint8_t* p = c.k + uint64_t(at) * (kInt8 ? D : D * 2) + (lane >> 4) * 16;
 #pragma unroll
-            for (int i = 0; i < kLoads; ++i) w[t][i] = kInt8 ? ld_once<ops_u32x4>(p + i * 64) : ld_global<ops_u32x4>(p + i * 64);
+            for (int i = 0; i < kLoads; ++i) w[t][i] = ld_global<ops_u32x4>(p + i * 64);
         }
-        if constexpr (kInt8)
+        if constexpr (kInt8) ld_scales<D>(own, c.k_scale, row);
+    }
+    // The scales to the lanes whose results they multiply, by way of the wave's own part of LDS: one load a cell, not one a lane.
+    __device__ __forceinline__ void spread(uint32_t* s, uint32_t lane) {
+        if constexpr (kInt8) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i)
-                ld_scales<D>(scale[i], c.k_scale, uint32_t(__shfl(int(row), int(i / 4 * 16 + (lane >> 4) * 4 + i % 4))));
+            for (uint32_t i = 0; i < kScaleWords; ++i) s[(lane & 31) * kScaleWords + i] = own[i];
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+#pragma unroll
+                for (uint32_t k = 0; k < kScaleWords; ++k) scale[i][k] = s[(i / 4 * 16 + (lane >> 4) * 4 + i % 4) * kScaleWords + k];
+            __builtin_amdgcn_wave_barrier();
+        }
     }
 };
 // The operand of step i.
@@ -140,10 +152,10 @@ __device__ __forceinline__ f16x8 operand(const KeyRows<D, true>& k, int t, int i
     return eight(x[0], x[1], x[2], x[3]);
 }
 
-// Scores of 16 columns: x[t * 4 + i] of the lane's column and cell 16 t + 4 (lane / 16) + i.  An infinite key makes the second
+// Products with 16 columns: x[t * 4 + i] of the lane's column and cell 16 t + 4 (lane / 16) + i.  An infinite key makes the second
 // part's product NaN: the first part has the score.
 template <int D, bool kInt8, int kParts>
-__device__ __forceinline__ void scores_of(float (&x)[8], const KeyRows<D, kInt8>& key, const ops_u32x4* q, uint32_t part, uint32_t lane, float c) {
+__device__ __forceinline__ void products_of(float (&x)[8], const KeyRows<D, kInt8>& key, const ops_u32x4* q, uint32_t part, uint32_t lane) {
     f32x4 hi[2]{}, lo[2]{};
 #pragma unroll
     for (int b = 0; b < D / 64; ++b) {
@@ -178,7 +190,7 @@ __device__ __forceinline__ void scores_of(float (&x)[8], const KeyRows<D, kInt8>
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float first = hi[i / 4][i % 4];
-        x[i] = c * (kParts == 1 || !(fabsf(first) < kInf) ? first : first + lo[i / 4][i % 4]);
+        x[i] = kParts == 1 || !(fabsf(first) < kInf) ? first : first + lo[i / 4][i % 4];
     }
 }
 
@@ -219,12 +231,13 @@ __device__ __forceinline__ f32x2 joined(f32x2 p, f32x2 q) {
     const float M = fmaxf(p.x, q.x), ref = M == -kInf ? 0.0f : M;
     return f32x2{M, p.y * exp2_fast(p.x - ref) + q.y * exp2_fast(q.x - ref)};
 }
-__device__ __forceinline__ void add_weights(float (&acc)[8], const float (&x)[8], f32x2 norm, uint32_t sees) {
+// Weights of scores c * x of the cells that the column sees.
+__device__ __forceinline__ void add_weights(float (&acc)[8], const float (&x)[8], float c, f32x2 norm, uint32_t sees) {
     sees = norm.y == 0 ? 0u : sees;   // nor past the columns, where an infinite key has made NaN with a query of zeros
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float w = exp2_fast(x[i] - norm.x) * norm.y;
-        acc[i] += sees >> i & 1 ? w : 0.0f;
+        const float w = exp2_fast(fmaf(x[i], c, -norm.x));
+        acc[i] += sees >> i & 1 ? w * norm.y : 0.0f;
     }
 }
 
@@ -236,6 +249,7 @@ __global__ void __launch_bounds__(kMassThreads, 2) mass_few_kernel(MassArgs a) {
     __shared__ ops_u32x4 s_q[kParts][kOps];
     __shared__ float s_back[16];
     __shared__ f32x2 s_ml[kAttnWaves][16];
+    __shared__ uint32_t s_scale[kInt8 ? kAttnWaves : 1][64];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t g = lane >> 4, col = lane & 15, h = blockIdx.y, s = blockIdx.z;
     const uint32_t n = length_of(a, s), units = (n + kUnit - 1) / kUnit;
@@ -303,7 +317,8 @@ __global__ void __launch_bounds__(kMassThreads, 2) mass_few_kernel(MassArgs a) {
             if (col < 8 && cell < n && a.decay != 0) old = a.decay * ld_global<float>(mass);
         }
         float x[8];
-        scores_of<D, kInt8, kParts>(x, key, s_q[0], kOps, lane, c);
+        key.spread(s_scale[kInt8 ? wave : 0], lane);
+        products_of<D, kInt8, kParts>(x, key, s_q[0], kOps, lane);
         const uint32_t now = there;
         if (u + a.parts < units) {   // the next turn's keys take the place of this one's
             const uint32_t next = u + a.parts;
@@ -315,11 +330,11 @@ __global__ void __launch_bounds__(kMassThreads, 2) mass_few_kernel(MassArgs a) {
         const uint32_t sees = now == 0xFFFFFFFFu && all_see(a, n, base) ? 0xFFu : seen_of(a, n, col, now, base, lane);
         if constexpr (kSums) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = sees >> i & 1 ? x[i] : -kInf;
+            for (int i = 0; i < 8; ++i) x[i] = sees >> i & 1 ? x[i] * c : -kInf;
             ml = summed(ml, x);
         } else {
             float w[8] = {}, mine = 0;
-            add_weights(w, x, norm, sees);
+            add_weights(w, x, c, norm, sees);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float sum = over_lanes(w[i], sum_of);
@@ -387,6 +402,7 @@ __global__ void __launch_bounds__((Many<kInt8, kF16>::kThreads), 2) mass_many_ke
     // sums: the references and sums of a wave's cells; weights: what they are formed with, at the end the sets' sums
     __shared__ f32x2 s_ml[kSums ? kAttnWaves : 1][kMostColumns];
     __shared__ float s_back[kF16 ? 1 : kMostColumns];
+    __shared__ uint32_t s_scale[kInt8 ? M::kSets * kAttnWaves : 1][64];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t g = lane >> 4, col = lane & 15, h = blockIdx.y, s = blockIdx.z;
     const uint32_t quarter = wave % kAttnWaves, set = wave / kAttnWaves;
@@ -423,6 +439,7 @@ __global__ void __launch_bounds__((Many<kInt8, kF16>::kThreads), 2) mass_many_ke
         key.load(a.c, row < 0 ? 0u : uint32_t(row), lane);
         const bool whole = there == 0xFFFFFFFFu && all_see(a, n, base);
         load(0);
+        key.spread(s_scale[kInt8 ? wave : 0], lane);
         for (uint32_t c = threadIdx.x; c < tiles * 16; c += M::kThreads) {
             if constexpr (!kSums) s_ml[0][c] = norm_of(a, s, h, c);
             if constexpr (!kF16) s_back[c] = ld_global<float>(a.back + sh * a.cols + (c < a.cols ? c : 0));
@@ -434,15 +451,16 @@ __global__ void __launch_bounds__((Many<kInt8, kF16>::kThreads), 2) mass_many_ke
             const uint32_t tile = stage * M::kSets + set, j = tile * 16 + col;
             if (tile < tiles) {
                 float x[8];
-                scores_of<D, kInt8, kParts>(x, key, s_q[stage & 1][set], kOps, lane, a.scale * kLog2e * (kF16 ? 1.0f : s_back[j]));
+                products_of<D, kInt8, kParts>(x, key, s_q[stage & 1][set], kOps, lane);
+                const float c = a.scale * kLog2e * (kF16 ? 1.0f : s_back[j]);
                 const uint32_t sees = whole ? 0xFFu : seen_of(a, n, j, there, base, lane);
                 if constexpr (kSums) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) x[i] = sees >> i & 1 ? x[i] : -kInf;
+                    for (int i = 0; i < 8; ++i) x[i] = sees >> i & 1 ? x[i] * c : -kInf;
                     const f32x2 v = summed(f32x2{-kInf, 0}, x);
                     if (g == 0) s_ml[quarter][j] = v;
                 } else {
-                    add_weights(acc, x, s_ml[0][j], sees);
+                    add_weights(acc, x, c, s_ml[0][j], sees);
                 }
             }
             if (stage + 1 < stages) lay_out((stage + 1) & 1);
