@@ -174,7 +174,8 @@ typedef struct sc_kv_evict {
  * values, scales) move to the places below `keep` that have become free, in ascending order both.  Cells from `keep` on keep
  * what they hold and are no longer the sequence's: their pages can be given to others.  So a cache is in no order after this:
  * attention over it needs none, but a window by cells means nothing there, and positions are given to the next append apart from its
- * cells (sc_rope_axes_append_async).  Each kv head keeps cells of its own.  The pages below a length are to be resident and the
+ * cells (sc_rope_axes_append_async).  Each kv head keeps cells of its own.  Nothing else that is kept by cell moves along (an
+ * indexer's pooled rows, sc_slot_layers).  The pages below a length are to be resident and the
  * sequence's own: a row is neither read from nor written to a page that is not resident.  One launch where a head can
  * move 128 cells at most and lens_out shares nothing with what it is made from, else two, or five for long heads that several
  * workgroups share; the result does not depend on timing.  Layers that share an array of lengths need lens_out apart from it. */

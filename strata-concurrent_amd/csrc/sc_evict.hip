@@ -465,7 +465,7 @@ uint64_t plan_evict(EvictArgs& a, void* workspace) {
     a.src = reinterpret_cast<uint32_t*>(take(list));
     const uint64_t chunks = (uint64_t(a.max_len) + kChunk - 1) / kChunk, most = kShares / heads;
     a.shares = uint32_t(chunks < most ? chunks : most);
-    if (a.shares < kLeastShares) {
+    if (a.cap == 0 || a.shares < kLeastShares) {
         a.shares = 1;
     } else {
         a.counts = reinterpret_cast<uint32_t*>(take(heads * a.shares * kParts * kValues * 4));

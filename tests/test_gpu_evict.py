@@ -244,3 +244,47 @@ def test_on_another_stream(sc, ops, cuda):
         stream.sync()
         got.append([dmass.numpy(), left.numpy(), *(b.numpy() for b in cache.dev.values())])
     assert all(np.array_equal(a.view(np.uint8), b.view(np.uint8)) for a, b in zip(*got))
+
+
+def test_two_calls_at_once(sc, ops, cuda):
+    """Masses and evictions of two caches on two streams at the same time, a workspace each, leave what they leave one by one."""
+    H, D, ps, t, heads = 2, 128, 4, 2000, 8
+    got = []
+    for together in (False, True):
+        streams, outs = [sc.Stream(), sc.Stream()], []
+        calls = []
+        for i in range(2):
+            rng = np.random.default_rng(20 + i)
+            cache = Cache(sc, ops, rng, "f16", H, D, ps, 1, t // ps)
+            mass, lens, left = upload(sc, np.zeros((1, H, t), np.float32)), upload(sc, np.array([t - i])), upload(sc, np.zeros(1, np.int64))
+            q = upload(sc, rng.standard_normal((5, heads, D)).astype(np.float32))
+            calls.append([ops.AttnMass(cache.c, q, mass, "f32", n_seqs=1, rows=5, n_head=heads, lens=lens, max_len=t, scale=D ** -0.5),
+                          ops.KvEvict(cache.c, mass, n_seqs=1, lens=lens, max_len=t, keep=300 + i, lens_out=left)])
+            outs.append((cache, mass, left))
+        sc.device_sync()
+        for a, b in zip(*calls) if together else ():
+            a.launch(streams[0])
+            b.launch(streams[1])
+        for i in range(2) if not together else ():
+            for call in calls[i]:
+                call.launch(streams[i])
+            streams[i].sync()
+        sc.device_sync()
+        got.append([x.numpy() for cache, mass, left in outs for x in (mass, left, *cache.dev.values())])
+    assert all(np.array_equal(a.view(np.uint8), b.view(np.uint8)) for a, b in zip(*got))
+
+
+def test_nothing_to_evict_in_a_long_cache(sc, ops, cuda):
+    """A bound that no sequence can pass leaves caches as they are and hands masses and numbers on."""
+    H, D, ps, ld = 1, 64, 64, 320
+    rng = np.random.default_rng(2)
+    cache = Cache(sc, ops, rng, "f16", H, D, ps, 2, ld)
+    mass, lens = rng.random((2, H, ld * ps)).astype(np.float32), np.array([ld * ps, 0], np.int64)
+    out, born, left = upload(sc, np.full_like(mass, 9)), upload(sc, np.full((2, H, ld * ps), -1, np.int32)), upload(sc, np.full(2, -1, np.int64))
+    ops.KvEvict(cache.c, upload(sc, mass), n_seqs=2, lens=upload(sc, lens), max_len=ld * ps, keep=ld * ps, mass_out=out, born_out=born,
+                lens_out=left).launch()
+    sc.device_sync()
+    assert np.array_equal(left.numpy(), lens) and np.array_equal(out.numpy().reshape(mass.shape)[0], mass[0])
+    assert (out.numpy().reshape(mass.shape)[1] == 9).all() and np.array_equal(born.numpy().reshape(mass.shape)[0, 0], np.arange(ld * ps))
+    for w, x in cache.host.items():
+        assert np.array_equal(cache.dev[w].numpy().reshape(x.shape), x)
