@@ -197,14 +197,15 @@ __device__ __forceinline__ void products_of(float (&x)[8], const KeyRows<D, kInt
 // Which of the lane's cells its column sees, where `there` has a bit for each of 32 cells from `base` on (the first of them cell 0).
 // Row r sees cells [ends - window, ends), ends = n - rows + 1 + r.
 __device__ __forceinline__ uint32_t seen_of(const MassArgs& a, uint32_t n, uint32_t col, uint32_t there, uint32_t base, uint32_t lane) {
-    const uint32_t r = ops_div(col < a.cols ? col : a.cols - 1, a.G);
-    const int64_t ends = int64_t(n) - a.rows + 1 + r, begins = a.window ? ends - a.window : 0;
+    const uint32_t r = ops_div(col < a.cols ? col : a.cols - 1, a.G), own = (lane >> 4) * 4;
+    // of the lane's first cell; lengths and windows are below 2^31
+    const int32_t ends = int32_t(n) - int32_t(a.rows) + 1 + int32_t(r) - int32_t(base) - int32_t(own);
+    const int32_t begins = a.window ? ends - int32_t(a.window) : INT32_MIN;
     uint32_t sees = 0;
 #pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-        const uint32_t in = i / 4 * 16 + (lane >> 4) * 4 + i % 4;
-        const int64_t cell = int64_t(base) + in;
-        sees |= uint32_t((there >> in & 1) && cell < ends && cell >= begins) << i;
+    for (int32_t i = 0; i < 8; ++i) {
+        const int32_t cell = i / 4 * 16 + i % 4;
+        sees |= uint32_t((there >> (uint32_t(cell) + own) & 1) && cell < ends && cell >= begins) << i;
     }
     return sees;
 }
@@ -231,14 +232,13 @@ __device__ __forceinline__ f32x2 joined(f32x2 p, f32x2 q) {
     const float M = fmaxf(p.x, q.x), ref = M == -kInf ? 0.0f : M;
     return f32x2{M, p.y * exp2_fast(p.x - ref) + q.y * exp2_fast(q.x - ref)};
 }
-// Weights of scores c * x of the cells that the column sees.
-__device__ __forceinline__ void add_weights(float (&acc)[8], const float (&x)[8], float c, f32x2 norm, uint32_t sees) {
-    sees = norm.y == 0 ? 0u : sees;   // nor past the columns, where an infinite key has made NaN with a query of zeros
+// The exponents of the weights of scores c * x of the cells that the column sees, -inf of the others.
+__device__ __forceinline__ void exponents_of(float (&x)[8], float c, float m, bool all, uint32_t sees) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float w = exp2_fast(fmaf(x[i], c, -norm.x));
-        acc[i] += sees >> i & 1 ? w * norm.y : 0.0f;
-    }
+    for (int i = 0; i < 8; ++i) x[i] = fmaf(x[i], c, -m);
+    if (!all)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = sees >> i & 1 ? x[i] : -kInf;
 }
 
 // ---- up to 16 columns ---------------------------------------------------------------------------------------------------------
@@ -333,11 +333,12 @@ __global__ void __launch_bounds__(kMassThreads, 2) mass_few_kernel(MassArgs a) {
             for (int i = 0; i < 8; ++i) x[i] = sees >> i & 1 ? x[i] * c : -kInf;
             ml = summed(ml, x);
         } else {
-            float w[8] = {}, mine = 0;
-            add_weights(w, x, c, norm, sees);
+            float mine = 0;
+            // nothing past the columns, where an infinite key has made NaN with a query of zeros
+            exponents_of(x, c, norm.x, false, norm.y == 0 ? 0u : sees);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float sum = over_lanes(w[i], sum_of);
+                const float sum = over_lanes(exp2_fast(x[i]) * norm.y, sum_of);
                 mine = int(col) == i ? sum : mine;
             }
             if (col < 8 && cell < n) st_global<float>(mass, old + mine);
@@ -413,6 +414,8 @@ __global__ void __launch_bounds__((Many<kInt8, kF16>::kThreads), 2) mass_many_ke
     const bool none = int64_t(first) + kUnit <= first_seen(a, n);
     const Span span{0, n, 0, 0};
 
+    const uint8_t* q0 = a.q + int64_t(s) * a.rows * a.q_ld;
+    const uint32_t q_ld16 = uint32_t(a.q_ld / 16);
     ops_u32x4 next[kEach];
     auto load = [&](uint32_t stage) {
 #pragma unroll
@@ -420,8 +423,12 @@ __global__ void __launch_bounds__((Many<kInt8, kF16>::kThreads), 2) mass_many_ke
             // operand `at` of a part of a tile; past the columns the last one's, whose results are left out
             const uint32_t e = threadIdx.x + i * M::kThreads, at = e % kOps, part = e / kOps % kParts, tile = stage * M::kSets + e / (kOps * kParts);
             const uint32_t j = tile * 16 + at % 16, c = j < a.cols ? j : a.cols - 1, d = value_at<kInt8>(at);
-            if constexpr (kF16) next[i] = ld_global<ops_u32x4>(values_of(a, s, h, c, D * 2) + d * 2);
-            else next[i] = ld_global<ops_u32x4>(a.split + (sh * a.cols + c) * (D / 4) + part * (D / 8) + d / 8);
+            if constexpr (kF16) {
+                // in pieces of 16 bytes, of which a sequence's rows have less than 2^32
+                const uint32_t r = ops_div(c, a.G), at16 = r * q_ld16 + (h * a.G.d + (c - r * a.G.d)) * (D / 8) + d / 8;
+                next[i] = ld_global<ops_u32x4>(q0 + uint64_t(at16) * 16);
+            }
+            if constexpr (!kF16) next[i] = ld_global<ops_u32x4>(a.split + (sh * a.cols + c) * (D / 4) + part * (D / 8) + d / 8);
         }
     };
     auto lay_out = [&](uint32_t half) {
@@ -460,7 +467,11 @@ __global__ void __launch_bounds__((Many<kInt8, kF16>::kThreads), 2) mass_many_ke
                     const f32x2 v = summed(f32x2{-kInf, 0}, x);
                     if (g == 0) s_ml[quarter][j] = v;
                 } else {
-                    add_weights(acc, x, c, s_ml[0][j], sees);
+                    // past the columns the last one's queries, of no weight
+                    const f32x2 norm = s_ml[0][j];
+                    exponents_of(x, c, norm.x, whole, sees);
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) acc[i] = fmaf(exp2_fast(x[i]), norm.y, acc[i]);
                 }
             }
             if (stage + 1 < stages) lay_out((stage + 1) & 1);
