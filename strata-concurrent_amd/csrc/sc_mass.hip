@@ -17,7 +17,7 @@
 //   where a lane loads the scales of its eight cells itself and keys go past the caches); 128 K cells in f16, 135 MB, 34 us.
 //   More columns: a workgroup's waves share 128 cells' keys and go over the tiles of columns, the next tiles' queries on their way to
 //   LDS meanwhile, and what the sets of waves have summed up is added at the end.  Half of a call is the products and the weights,
-//   half the way to the first of them.  32 queries of two prompts up to 16 381 cells without their sums, 23 GFLOP: 59 us (27 a
+//   half the way to the first of them.  32 queries of two prompts up to 16 381 cells without their sums, 23 GFLOP: 57 us (26 a
 //   pass, the join 5).  Tried: 64 cells a wave, which needs all registers of a SIMD for two waves (80 us), one tile of columns at
 //   a time for three waves a SIMD (65), the weights of cells that are all seen in a branch of their own (65).
 #include <hip/hip_runtime.h>
@@ -386,17 +386,19 @@ __global__ void __launch_bounds__(256) mass_parts_kernel(MassArgs a) {
     if (lane == 0) st_global<float>(a.back + at, back);
 }
 
-// The sets of four waves of a workgroup: each has all of its 128 cells, 32 a wave, and takes every kSets-th tile of columns.  Two where
-// neither keys nor queries need more registers: a wave's products then hide behind another's weights.
-template <bool kInt8, bool kF16>
+// The sets of four waves of a workgroup: each has all of its 128 cells, 32 a wave, and takes every kSets-th tile of columns.  Two for
+// f16 keys of 256 and f16 queries, whose workgroups are few enough to a unit for a wave's products to hide behind another's weights
+// (57 us and 62, 32 queries of 16 K cells); else one (16 queries of four sequences up to 8000 cells, 4 kv heads of 128: f16 12.4 us
+// and 16, f32 queries 19 and 25, int8 12.6 and 15.5).
+template <int D, bool kInt8, bool kF16>
 struct Many {
     static constexpr int kParts = kF16 ? 1 : 2;
-    static constexpr uint32_t kSets = kF16 && !kInt8 ? 2 : 1, kThreads = kSets * kMassThreads;
+    static constexpr uint32_t kSets = D == 256 && kF16 && !kInt8 ? 2 : 1, kThreads = kSets * kMassThreads;
 };
 
 template <int D, bool kInt8, bool kF16, bool kSums>
-__global__ void __launch_bounds__((Many<kInt8, kF16>::kThreads), 2) mass_many_kernel(MassArgs a) {
-    using M = Many<kInt8, kF16>;
+__global__ void __launch_bounds__((Many<D, kInt8, kF16>::kThreads), 2) mass_many_kernel(MassArgs a) {
+    using M = Many<D, kInt8, kF16>;
     constexpr int kParts = M::kParts, kOps = D / 32 * 64;
     constexpr uint32_t kEach = (M::kSets * kParts * kOps + M::kThreads - 1) / M::kThreads;   // operands that a thread brings of a tile a set
     __shared__ ops_u32x4 s_q[2][M::kSets][kParts * kOps];
@@ -527,7 +529,7 @@ __global__ void __launch_bounds__(64 * kJoinSets) mass_join_kernel(MassArgs a) {
 
 template <int D, bool kInt8, bool kF16>
 hipError_t launch_of(const MassArgs& a, hipStream_t stream) {
-    const dim3 block(kMassThreads), many(Many<kInt8, kF16>::kThreads), join((a.cols + 63) / 64, a.c.H, a.n_seqs), few(a.parts, a.c.H, a.n_seqs);
+    const dim3 block(kMassThreads), many(Many<D, kInt8, kF16>::kThreads), join((a.cols + 63) / 64, a.c.H, a.n_seqs), few(a.parts, a.c.H, a.n_seqs);
     if (a.cols <= 16) {
         if (!a.lse) {
             hipLaunchKernelGGL((mass_few_kernel<D, kInt8, kF16, true>), few, block, 0, stream, a);
