@@ -17,7 +17,7 @@
 //   where a lane loads the scales of its eight cells itself and keys go past the caches); 128 K cells in f16, 135 MB, 34 us.
 //   More columns: a workgroup's waves share 128 cells' keys and go over the tiles of columns, the next tiles' queries on their way to
 //   LDS meanwhile, and what the sets of waves have summed up is added at the end.  Half of a call is the products and the weights,
-//   half the way to the first of them.  32 queries of two prompts up to 16 381 cells without their sums, 23 GFLOP: 57 us (26 a
+//   half the way to the first of them.  32 queries of two prompts up to 16 381 cells without their sums, 23 GFLOP: 58 us (27 a
 //   pass, the join 5).  Tried: 64 cells a wave, which needs all registers of a SIMD for two waves (80 us), one tile of columns at
 //   a time for three waves a SIMD (65), the weights of cells that are all seen in a branch of their own (65).
 #include <hip/hip_runtime.h>
@@ -232,6 +232,8 @@ __device__ __forceinline__ f32x2 joined(f32x2 p, f32x2 q) {
     const float M = fmaxf(p.x, q.x), ref = M == -kInf ? 0.0f : M;
     return f32x2{M, p.y * exp2_fast(p.x - ref) + q.y * exp2_fast(q.x - ref)};
 }
+// A weight by its exponent; a cell that the column does not see has none (-inf), also where the column's sum is no number.
+__device__ __forceinline__ float weight_of(float x, float by) { return x == -kInf ? 0.0f : exp2_fast(x) * by; }
 // The exponents of the weights of scores c * x of the cells that the column sees, -inf of the others.
 __device__ __forceinline__ void exponents_of(float (&x)[8], float c, float m, bool all, uint32_t sees) {
 #pragma unroll
@@ -338,7 +340,7 @@ __global__ void __launch_bounds__(kMassThreads, 2) mass_few_kernel(MassArgs a) {
             exponents_of(x, c, norm.x, false, norm.y == 0 ? 0u : sees);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float sum = over_lanes(exp2_fast(x[i]) * norm.y, sum_of);
+                const float sum = over_lanes(weight_of(x[i], norm.y), sum_of);
                 mine = int(col) == i ? sum : mine;
             }
             if (col < 8 && cell < n) st_global<float>(mass, old + mine);
@@ -388,7 +390,7 @@ __global__ void __launch_bounds__(256) mass_parts_kernel(MassArgs a) {
 
 // The sets of four waves of a workgroup: each has all of its 128 cells, 32 a wave, and takes every kSets-th tile of columns.  Two for
 // f16 keys of 256 and f16 queries, whose workgroups are few enough to a unit for a wave's products to hide behind another's weights
-// (57 us and 62, 32 queries of 16 K cells); else one (16 queries of four sequences up to 8000 cells, 4 kv heads of 128: f16 12.4 us
+// (58 us and 62, 32 queries of 16 K cells); else one (16 queries of four sequences up to 8000 cells, 4 kv heads of 128: f16 12.4 us
 // and 16, f32 queries 19 and 25, int8 12.6 and 15.5).
 template <int D, bool kInt8, bool kF16>
 struct Many {
@@ -473,7 +475,7 @@ __global__ void __launch_bounds__((Many<D, kInt8, kF16>::kThreads), 2) mass_many
                     const f32x2 norm = s_ml[0][j];
                     exponents_of(x, c, norm.x, whole, sees);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) acc[i] = fmaf(exp2_fast(x[i]), norm.y, acc[i]);
+                    for (int i = 0; i < 8; ++i) acc[i] += weight_of(x[i], norm.y);
                 }
             }
             if (stage + 1 < stages) lay_out((stage + 1) & 1);
@@ -523,8 +525,8 @@ __global__ void __launch_bounds__(64 * kJoinSets) mass_join_kernel(MassArgs a) {
     __syncthreads();
     if (set) return;
     for (uint32_t k = 1; k < kJoinSets; ++k) v = joined(v, s_ml[k][lane]);
-    // nothing seen, or nothing but scores of -inf: no weight
-    if (c < a.cols) st_global<f32x2>(a.norm + sh * a.cols + c, v.y == 0 ? f32x2{kInf, 0} : f32x2{v.x, 1.0f / v.y});
+    // nothing seen, or nothing but scores of -inf: no weight; a sum that is no number makes every weight none
+    if (c < a.cols) st_global<f32x2>(a.norm + sh * a.cols + c, v.y == 0 ? f32x2{kInf, 0} : f32x2{v.y == v.y ? v.x : v.y, 1.0f / v.y});
 }
 
 template <int D, bool kInt8, bool kF16>

@@ -231,3 +231,41 @@ def test_the_same_bits_again_and_on_another_stream(sc, ops, cuda):
         stream.sync()
         got.append(mass.numpy())
     assert np.array_equal(got[0], got[1]) and np.array_equal(got[0], got[2])
+
+
+@pytest.mark.parametrize("rows,heads,dtype,fmt", [(1, 4, "f32", "f16"), (3, 4, "f16", "int8"), (32, 4, "f16", "f16"), (32, 2, "f32", "f16"), (20, 2, "f16", "int8")])
+def test_a_row_that_is_no_number_stays_in_what_it_sees(sc, ops, plain, cuda, rows, heads, dtype, fmt):
+    """A key that is NaN in the latest cell makes NaN of the cells that the latest row sees, and of no other: neither those before
+    its window, which earlier rows see, nor those that are not resident, nor those past the end."""
+    H, D, ps, t, window = 1, 64, 4, 200, 20
+    for given in (False, True):
+        got = []
+        for bad in (False, True):
+            rng = np.random.default_rng(31)
+            table = rng.permutation(60)[:50].astype(np.int32).reshape(1, 50)
+            table[0, (t - 10) // ps] = -1
+            cache = Cache(sc, ops, rng, fmt, H, D, ps, 1, 50, table=table, n_pages=60)
+            q, q64 = act(rng.standard_normal((rows, heads, D)), dtype)
+            lse = _sums(plain, cache, q64, [t], rows, window, D ** -0.5)
+            last = plain.pool_row(table, 0, t - 1, 0, H, ps, 60, 50)
+            if bad and fmt == "f16":
+                x = cache.host["k"]
+                x[last, 5] = np.nan
+                cache.dev["k"].upload(x)
+            elif bad:
+                x = cache.host["ks"]
+                x[last] = 0x7E00
+                cache.dev["ks"].upload(x)
+            if bad:
+                lse[rows - 1] = np.nan
+            mass = upload(sc, np.zeros((1, H, 210), np.float32))
+            ops.AttnMass(cache.c, upload(sc, q), mass, dtype, n_seqs=1, n_head=heads, rows=rows, lens=upload(sc, np.array([t])), max_len=t,
+                         scale=D ** -0.5, window=window, lse=upload(sc, lse) if given else None, mass_ld=210).launch()
+            sc.device_sync()
+            got.append(mass.numpy().reshape(210))
+        clean, odd = got
+        seen = np.zeros(210, bool)
+        seen[t - window:t] = True
+        seen[(t - 10) // ps * ps:(t - 10) // ps * ps + ps] = False
+        assert np.isfinite(clean).all() and np.isnan(odd[seen]).all()
+        assert np.array_equal(odd[~seen], clean[~seen]), (given, np.flatnonzero(odd[~seen] != clean[~seen]))
