@@ -232,8 +232,11 @@ __device__ __forceinline__ f32x2 joined(f32x2 p, f32x2 q) {
     const float M = fmaxf(p.x, q.x), ref = M == -kInf ? 0.0f : M;
     return f32x2{M, p.y * exp2_fast(p.x - ref) + q.y * exp2_fast(q.x - ref)};
 }
-// A weight by its exponent; a cell that the column does not see has none (-inf), also where the column's sum is no number.
-__device__ __forceinline__ float weight_of(float x, float by) { return x == -kInf ? 0.0f : exp2_fast(x) * by; }
+// A weight by its exponent.  Exponents of some classes have none: -inf, a cell that the column does not see, also where the column's
+// sum is no number; all of them where the column has no weight (its query saw nothing, or it is past the last one), also where an
+// infinite key or the query itself has made NaN.
+__device__ __forceinline__ int none_of(float by) { return by == 0 ? 0x3FF : 0x004; }
+__device__ __forceinline__ float weight_of(float x, float by, int none) { return __builtin_amdgcn_classf(x, none) ? 0.0f : exp2_fast(x) * by; }
 // The exponents of the weights of scores c * x of the cells that the column sees, -inf of the others.
 __device__ __forceinline__ void exponents_of(float (&x)[8], float c, float m, bool all, uint32_t sees) {
 #pragma unroll
@@ -336,11 +339,11 @@ __global__ void __launch_bounds__(kMassThreads, 2) mass_few_kernel(MassArgs a) {
             ml = summed(ml, x);
         } else {
             float mine = 0;
-            // nothing past the columns, where an infinite key has made NaN with a query of zeros
-            exponents_of(x, c, norm.x, false, norm.y == 0 ? 0u : sees);
+            exponents_of(x, c, norm.x, false, sees);
+            const int none = none_of(norm.y);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float sum = over_lanes(weight_of(x[i], norm.y), sum_of);
+                const float sum = over_lanes(weight_of(x[i], norm.y, none), sum_of);
                 mine = int(col) == i ? sum : mine;
             }
             if (col < 8 && cell < n) st_global<float>(mass, old + mine);
@@ -474,8 +477,9 @@ __global__ void __launch_bounds__((Many<D, kInt8, kF16>::kThreads), 2) mass_many
                     // past the columns the last one's queries, of no weight
                     const f32x2 norm = s_ml[0][j];
                     exponents_of(x, c, norm.x, whole, sees);
+                    const int none = none_of(norm.y);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) acc[i] += weight_of(x[i], norm.y);
+                    for (int i = 0; i < 8; ++i) acc[i] += weight_of(x[i], norm.y, none);
                 }
             }
             if (stage + 1 < stages) lay_out((stage + 1) & 1);
