@@ -401,6 +401,9 @@ struct Many {
     static constexpr uint32_t kSets = D == 256 && kF16 && !kInt8 ? 2 : 1, kThreads = kSets * kMassThreads;
 };
 
+// A launch has less than 2^32 threads across a sequence's cells: beyond 2^29 cells there are several, from cell a.first_part * kUnit on.
+constexpr uint32_t kMostParts = 1u << 22;
+
 template <int D, bool kInt8, bool kF16, bool kSums>
 __global__ void __launch_bounds__((Many<D, kInt8, kF16>::kThreads), 2) mass_many_kernel(MassArgs a) {
     using M = Many<D, kInt8, kF16>;
@@ -414,7 +417,7 @@ __global__ void __launch_bounds__((Many<D, kInt8, kF16>::kThreads), 2) mass_many
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t g = lane >> 4, col = lane & 15, h = blockIdx.y, s = blockIdx.z;
     const uint32_t quarter = wave % kAttnWaves, set = wave / kAttnWaves;
-    const uint32_t n = length_of(a, s), first = blockIdx.x * kUnit, base = first + quarter * kTurn;
+    const uint32_t n = length_of(a, s), unit = a.first_part + blockIdx.x, first = unit * kUnit, base = first + quarter * kTurn;
     if (first >= n) return;
     const uint64_t sh = uint64_t(s) * a.c.H + h;
     const uint32_t tiles = (a.cols + 15) / 16, stages = (tiles + M::kSets - 1) / M::kSets;
@@ -487,7 +490,7 @@ __global__ void __launch_bounds__((Many<D, kInt8, kF16>::kThreads), 2) mass_many
         }
     }
     if constexpr (kSums) {
-        f32x2* part = a.sums + (sh * a.parts + blockIdx.x) * a.cols;
+        f32x2* part = a.sums + (sh * a.parts + unit) * a.cols;
         for (uint32_t c = threadIdx.x; c < a.cols; c += M::kThreads) {
             f32x2 v{-kInf, 0};
             if (!none)
@@ -545,11 +548,18 @@ hipError_t launch_of(const MassArgs& a, hipStream_t stream) {
         return hipGetLastError();
     }
     if constexpr (!kF16) hipLaunchKernelGGL(mass_parts_kernel<D>, dim3((a.cols + 3) / 4, a.c.H, a.n_seqs), dim3(256), 0, stream, a);
+    auto pass = [&](auto kernel) {
+        MassArgs b = a;
+        for (b.first_part = 0; b.first_part < a.parts; b.first_part += kMostParts) {
+            const uint32_t left = a.parts - b.first_part;
+            hipLaunchKernelGGL(kernel, dim3(left < kMostParts ? left : kMostParts, a.c.H, a.n_seqs), many, 0, stream, b);
+        }
+    };
     if (!a.lse) {
-        hipLaunchKernelGGL((mass_many_kernel<D, kInt8, kF16, true>), few, many, 0, stream, a);
+        pass(mass_many_kernel<D, kInt8, kF16, true>);
         hipLaunchKernelGGL(mass_join_kernel, join, dim3(64 * kJoinSets), 0, stream, a);
     }
-    hipLaunchKernelGGL((mass_many_kernel<D, kInt8, kF16, false>), few, many, 0, stream, a);
+    pass(mass_many_kernel<D, kInt8, kF16, false>);
     return hipGetLastError();
 }
 template <int D>

@@ -73,7 +73,7 @@ struct MassArgs {
     float scale, decay;
     // by plan_mass: parts of a sequence's cells; in the workspace, without lse, their references and sums and the columns'
     // references and inverse sums, and many f32 queries' parts with what their products are scaled back by
-    uint32_t parts;
+    uint32_t parts, first_part;           // first_part: of a launch's parts, where many columns take more than one
     f32x2 *sums, *norm;
     ops_u32x4* split;
     float* back;
