@@ -62,4 +62,10 @@ constexpr SplitPlan plan_split(uint32_t n_seqs, uint32_t tiles, uint32_t max_len
     return p;
 }
 
+// Which cells the latest `rows` queries of a sequence of n cells see: row r those before cell n - rows + 1 + r, the last `window` of
+// them (0: all).  Counted from cell `from`, which is less than n + kUnit; lengths and windows are below 2^31, `from` may not be, and
+// the difference is.
+constexpr int32_t row_ends(uint32_t n, uint32_t rows, uint32_t r, uint32_t from) { return int32_t(n - rows + 1 + r - from); }
+constexpr bool row_sees(int32_t ends, uint32_t window, int32_t cell) { return uint32_t(ends - 1 - cell) < (window ? window : 0x80000000u); }
+
 }  // namespace sc

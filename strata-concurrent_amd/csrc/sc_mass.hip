@@ -195,17 +195,14 @@ __device__ __forceinline__ void products_of(float (&x)[8], const KeyRows<D, kInt
 }
 
 // Which of the lane's cells its column sees, where `there` has a bit for each of 32 cells from `base` on (the first of them cell 0).
-// Row r sees cells [ends - window, ends), ends = n - rows + 1 + r.
 __device__ __forceinline__ uint32_t seen_of(const MassArgs& a, uint32_t n, uint32_t col, uint32_t there, uint32_t base, uint32_t lane) {
     const uint32_t r = ops_div(col < a.cols ? col : a.cols - 1, a.G), own = (lane >> 4) * 4;
-    // of the lane's first cell; lengths and windows are below 2^31
-    const int32_t ends = int32_t(n) - int32_t(a.rows) + 1 + int32_t(r) - int32_t(base) - int32_t(own);
-    const int32_t begins = a.window ? ends - int32_t(a.window) : INT32_MIN;
+    const int32_t ends = row_ends(n, a.rows, r, base + own);
     uint32_t sees = 0;
 #pragma unroll
     for (int32_t i = 0; i < 8; ++i) {
         const int32_t cell = i / 4 * 16 + i % 4;
-        sees |= uint32_t((there >> (uint32_t(cell) + own) & 1) && cell < ends && cell >= begins) << i;
+        sees |= uint32_t((there >> (uint32_t(cell) + own) & 1) && row_sees(ends, a.window, cell)) << i;
     }
     return sees;
 }
