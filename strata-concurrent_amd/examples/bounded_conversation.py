@@ -62,15 +62,16 @@ class Bounded:
     """The slot, and beside it each attention layer's masses and the numbers of the tokens that its cells hold."""
 
     def __init__(self, geo: sc.Geometry, n_head: int, keep: int, prompt: int, between: int):
-        self.geo, self.n_head, self.keep = geo, n_head, keep
-        self.max_cells = geo.cells(max(prompt, keep + between))
+        self.geo, self.n_head, self.keep, self.between = geo, n_head, keep, between
+        # the slot's cells, which a hand-off makes fewer, and the width of the arrays beside it
+        self.max_cells = self.width = geo.cells(max(prompt, keep) + between)
         self.slot = sc.new_slot(geo, self.max_cells)
         self.inv_freq = _up((BASE ** (-np.arange(0, ROT, 2) / ROT)).astype(np.float32))
         self.axis = ops.axis_of_pairs(SECTIONS, by_turns=True)
         rng = np.random.default_rng(7)
         C, W = geo.ssm_conv_channels, geo.ssm_d_conv
         self.taps = [_up((rng.standard_normal((C, W)) / W).astype(np.float32)) for _ in range(geo.n_gdn)]
-        heads = (1, geo.n_head_kv, self.max_cells)
+        heads = (1, geo.n_head_kv, self.width)
         self.mass, self.born = ([sc.DeviceBuffer(heads, t) for _ in range(geo.n_qsa)] for t in ("float32", "int32"))
         for b in (*self.mass, *self.born):
             b.fill(0)
@@ -127,7 +128,7 @@ class Bounded:
         self.len.upload([T]), self.total.upload([T])
         for j in range(geo.n_qsa):
             ops.AttnMass(ops.slot_cache(geo, self.slot, j), q[j].ptr + 4 * (T - last) * n_head * D, self.mass[j], "f32", n_seqs=1, rows=last,
-                         n_head=n_head, lens=self.len, max_len=self.max_cells, scale=D ** -0.5, mass_ld=self.max_cells).launch()
+                         n_head=n_head, lens=self.len, max_len=self.max_cells, scale=D ** -0.5, mass_ld=self.width).launch()
         sc.device_sync()
         return [o.numpy() for o in outs]
 
@@ -135,7 +136,7 @@ class Bounded:
         """Every attention layer's eviction.  They read one array of lengths, so what they leave goes to another."""
         geo = self.geo
         return [ops.KvEvict(ops.slot_cache(geo, self.slot, j), self.mass[j], n_seqs=1, lens=self.len, max_len=self.max_cells, keep=self.keep,
-                            sinks=SINKS, recent=RECENT, born=self.born[j], ld=self.max_cells, known=self.known, total=self.total,
+                            sinks=SINKS, recent=RECENT, born=self.born[j], ld=self.width, known=self.known, total=self.total,
                             lens_out=self.left) for j in range(geo.n_qsa)]
 
     def evict(self, calls, stream=None) -> None:
@@ -145,11 +146,13 @@ class Bounded:
         self.cells = min(self.cells, self.keep)
 
     def hand_off(self) -> None:
-        """The slot parked at the length that it has and resumed into one with room for a bounded cache only."""
+        """The slot parked at the length that it has and resumed into one with room for a bounded cache only: what it has or may keep, and
+        the tokens up to the next eviction.  Calls made before are of the old slot."""
         geo = self.geo
         image = sc.PinnedBuffer(sc.image_layout(geo, self.cells)[1])
         sc.device_sync()
         sc.park_async(geo, self.slot, self.cells, image.ptr, image.nbytes)
+        self.max_cells = geo.cells(max(self.cells, self.keep) + self.between)
         target = sc.new_slot(geo, self.max_cells)
         sc.resume_async(geo, image.ptr, image.nbytes, self.cells, target)
         sc.device_sync()
@@ -180,7 +183,7 @@ class Decoder:
                 ops.AttnDecode(cache, q, self.attn_out[-1], "f32", n_seqs=1, n_head=n_head, lens=b.len, max_len=b.max_cells, scale=D ** -0.5,
                                lse=lse),
                 ops.AttnMass(cache, q, b.mass[j], "f32", n_seqs=1, n_head=n_head, lens=b.len, max_len=b.max_cells, scale=D ** -0.5, lse=lse,
-                             mass_ld=b.max_cells)]
+                             mass_ld=b.width)]
         for i, layer in enumerate(x.gdn):
             y = sc.DeviceBuffer((1, C), "float32")
             self.gdn_out.append(sc.DeviceBuffer((VH, S), "float32"))
