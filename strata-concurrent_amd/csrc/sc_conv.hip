@@ -21,8 +21,17 @@ constexpr uint32_t kConvThreads = 256;
 // Rows of a prompt's tile, which are all asked for at once: 128 bytes a lane.
 constexpr uint32_t tile_rows(bool f16) { return f16 ? 16 : 8; }
 
-// v / (1 + e^-v) by the hardware's exponential and reciprocal, 1 unit in the last place each; 0 where e^-v is beyond 2^128.
-__device__ __forceinline__ float silu(float v) { return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -1.44269504088896340736f)); }
+// v / (1 + e^-v) by the hardware's exponential and reciprocal, 1 unit in the last place each; 0 where e^-v is beyond 2^126.  The
+// exponent t = -v log2(e) is rounded to 2^-24 of itself, which is 2^-24 |v| of e^-v (4e-6 at v = -87): far below a unit of an f16 result.
+// For f32 ones what that left out, r = -v - t ln 2, is taken along, e^r being 1 + r: 2e-7 at any v, and 120.8 us as above (120.0 without).
+template <bool kF16>
+__device__ __forceinline__ float silu(float v) {
+    constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f, kLn2Rest = -1.90465421e-9f;   // kLn2Rest: ln 2 - kLn2
+    if constexpr (kF16) return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -kLog2e));
+    const float x = __builtin_amdgcn_fmed3f(v, -88.0f, 200.0f);   // finite, where the result is v or 0 or no number beyond
+    const float t = x * -kLog2e, e = __builtin_amdgcn_exp2f(t), r = fmaf(t, -kLn2Rest, fmaf(t, -kLn2, -x));
+    return v * __builtin_amdgcn_rcpf(1.0f + fmaf(e, r, e));
+}
 
 // Four channels of a history, a row a vector, from channel c on.
 template <int W, bool kSlot>
@@ -68,7 +77,7 @@ __device__ __forceinline__ void ld_taps(f32x4 (&w)[W], const float* weight, uint
         for (int j = 0; j < 4; ++j) w[k][j] = v[(j * W + k) / 4][(j * W + k) % 4];
 }
 
-template <int W>
+template <int W, bool kF16>
 __device__ __forceinline__ f32x4 sum_of(const f32x4 (&before)[W - 1], f32x4 x, const f32x4 (&w)[W], f32x4 bias, bool act) {
     f32x4 y = bias;
 #pragma unroll
@@ -76,7 +85,7 @@ __device__ __forceinline__ f32x4 sum_of(const f32x4 (&before)[W - 1], f32x4 x, c
     y += w[W - 1] * x;
     if (act)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = silu(y[j]);
+        for (int j = 0; j < 4; ++j) y[j] = silu<kF16>(y[j]);
     return y;
 }
 
@@ -96,7 +105,7 @@ __global__ void __launch_bounds__(kConvThreads) conv_step_kernel(ConvArgs a) {
     ld_history<W, kSlot>(h, state, a.state_ld, c);
     ld_taps<W>(w, a.weight, c);
     const f32x4 x = ld_act4<kF16>(a.x + int64_t(s) * a.x_ld, c), bias = a.bias ? ld_global<f32x4>(a.bias + c) : f32x4{};
-    st_act4<kF16>(out, c, sum_of<W>(h, x, w, bias, a.silu));
+    st_act4<kF16>(out, c, sum_of<W, kF16>(h, x, w, bias, a.silu));
 #pragma unroll
     for (int k = 0; k + 1 < W - 1; ++k) h[k] = h[k + 1];
     h[W - 2] = x;
@@ -179,7 +188,7 @@ __global__ void __launch_bounds__(kConvThreads) conv_prompt_kernel(ConvArgs a) {
     }
 #pragma unroll
     for (uint32_t i = 0; i < kRows; ++i) {
-        if (i < n) st_act4<kF16, true>(out + int64_t(r0 + i) * a.out_ld, c, sum_of<W>(h, rows[i], w, bias, a.silu));
+        if (i < n) st_act4<kF16, true>(out + int64_t(r0 + i) * a.out_ld, c, sum_of<W, kF16>(h, rows[i], w, bias, a.silu));
 #pragma unroll
         for (int k = 0; k + 1 < W - 1; ++k) h[k] = h[k + 1];
         h[W - 2] = rows[i];
