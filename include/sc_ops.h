@@ -144,10 +144,12 @@ typedef struct sc_attn_mass {
 
 /* mass[s][h][c] = decay * mass[s][h][c] + sum over the rows and the query heads of kv head h of exp(scale * q . k_c - lse), for
  * the cells below each sequence's length; the rest of `mass` is left as it is.  A cell that a row does not see, or that is not
- * resident, gets nothing from it; a row that sees no cell, or whose every score is -inf, gives none.  f16 queries are exact, f32
- * ones two f16 parts, sums in 32 bits; the result does not depend on timing.  Reads the keys only, once with `lse` and twice
- * without; one to four launches, or for more than 16 columns of max_len beyond 2^29 up to four for each time.  A mass that
- * begins at 0 and is never decayed sums to the number of queries so far times heads. */
+ * resident, gets nothing from it; a row that sees no cell, or whose every score is -inf, gives none, nor does a query whose
+ * `lse` is -inf, whatever it holds.  A score of +inf weighs inf under a finite `lse`, and NaN under one of +inf, under which the
+ * query's finite scores weigh nothing; where the sum is formed here, a query with a score of +inf or NaN makes NaN of every cell that
+ * it sees.  f16 queries are exact, f32 ones two f16 parts of 22 bits or more together, sums in 32 bits; the result does not depend on
+ * timing.  Reads the keys only, once with `lse` and twice without; one to four launches, or for more than 16 columns of max_len
+ * beyond 2^29 up to four for each time.  A mass that begins at 0 and is never decayed sums to the number of queries so far times heads. */
 uint64_t sc_attn_mass_workspace_bytes(const sc_kv_cache* cache, const sc_attn_mass* a);
 int sc_attn_mass_async(const sc_kv_cache* cache, const sc_attn_mass* a, void* workspace, uint64_t workspace_bytes, void* stream);
 

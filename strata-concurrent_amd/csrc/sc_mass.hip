@@ -13,11 +13,11 @@
 // always in the same order.
 //   Up to 16 columns (a new token a sequence): the queries are laid out once, a wave takes 32 cells a turn and has its next turn's
 //   keys on the way while it forms weights.  Reading the keys bounds it, and for short calls the chain of latencies to the first
-//   weights.  2 kv heads of 256 and 24 query heads: 1021 cells 5.8 us; 24 sequences up to 8190 cells in int8, 57 MB, 18 us (24
+//   weights.  2 kv heads of 256 and 24 query heads: 1021 cells 5.8 us; 24 sequences up to 8190 cells in int8, 57 MB, 17.7 us (24
 //   where a lane loads the scales of its eight cells itself and keys go past the caches); 128 K cells in f16, 135 MB, 34 us.
 //   More columns: a workgroup's waves share 128 cells' keys and go over the tiles of columns, the next tiles' queries on their way to
 //   LDS meanwhile, and what the sets of waves have summed up is added at the end.  Half of a call is the products and the weights,
-//   half the way to the first of them.  32 queries of two prompts up to 16 381 cells without their sums, 23 GFLOP: 58 us (27 a
+//   half the way to the first of them.  32 queries of two prompts up to 16 381 cells without their sums, 11.5 GFLOP a pass: 57 us (26 a
 //   pass, the join 5).  Tried: 64 cells a wave, which needs all registers of a SIMD for two waves (80 us), one tile of columns at
 //   a time for three waves a SIMD (65), the weights of cells that are all seen in a branch of their own (65).
 #include <hip/hip_runtime.h>
@@ -33,8 +33,9 @@ namespace {
 
 constexpr uint32_t kMassThreads = kAttnWaves * 64;
 constexpr uint32_t kMostColumns = 1024;         // rows times query heads of a kv head
-// Workgroups that the cells are shared out among where columns are few.  A long f16 sequence likes fewer (128 K cells: 30 us with 256,
-// 34 with 1024), a batch more (24 int8 sequences: 41 and 24, before their scales came by LDS; eight f16 ones with f32 queries: 22 and 16).
+// Workgroups that the cells are shared out among where columns are few.  One long f16 sequence likes fewer (128 K cells: 30.5 us with
+// 256, 33.4 with 512, 34.3 with 1024; int8 18.9, 16.0, 16.0), a batch more (24 int8 sequences up to 8190 cells 28, 22.7 and 17.7, f16
+// 47, 40 and 28; eight f16 ones up to 16 000 cells 20.5, 18.7 and 13.3, with f32 queries 21.8, 14.9 and 15.7).
 constexpr uint32_t kFewSlots = 1024;
 constexpr float kLog2eRest = 1.92596299e-8f;    // log2(e) - kLog2e
 
@@ -97,7 +98,10 @@ __device__ __forceinline__ void parts_of(const float (&x)[8], ops_u32x4& hi, ops
     hi = __builtin_bit_cast(ops_u32x4, h), lo = __builtin_bit_cast(ops_u32x4, l);
 }
 // An f32 query is scaled by a power of two to a largest value of 2^14 .. 2^15, so that the two parts of values down to 2^-16 of
-// that keep all bits: a key can be as much larger there.
+// that keep 22 bits or more: a key can be as much larger there.  They do not keep all 24: the first part leaves up to 12 bits, and
+// the second has 11, so one value in four is a unit in its last place off.  A third part would be half as many products again, for an
+// error that is small beside the others: of 1021 weights by queries of 256 values 1.4e-8 is the parts', 4.6e-8 the rounding of
+// x - m, 3.2e-8 the products' sums.
 __device__ __forceinline__ void scaling(float top, float& by, float& back) {
     by = back = 1.0f;
     if (top > 0) {

@@ -89,3 +89,32 @@ def test_a_query_that_saw_nothing_gives_nothing(sc, ops, plain, cuda, rows, head
     q[0, 1], q[rows - 1, heads - 1], q[rows // 2, 0, 5] = np.nan, np.nan, np.inf
     got = _run(sc, ops, cache, q, dtype, t, rows, heads, scale, lse)
     assert (np.abs(got - want) <= near).all(), np.abs(got - want).max()
+
+
+@pytest.mark.parametrize("rows,heads,D,dtype,fmt", [s for s in SHAPES if s[4] == "f16"], ids=[i for i, s in zip(IDS, SHAPES) if s[4] == "f16"])
+def test_an_infinite_score_under_its_own_sum(sc, ops, plain, cuda, rows, heads, D, dtype, fmt):
+    """The log of a sum with inf in it is inf: finite scores weigh exp(-inf) under it, the infinite one is NaN.  Where the sum is formed
+    here every cell that the query sees is NaN, and none that it does not see."""
+    t, bad, rng = 140, 139, np.random.default_rng(rows)
+    cache = Cache(sc, ops, rng, fmt, 1, D, 4, 1, 35, missing=0.1)
+    at = [plain.pool_row(cache.table, 0, c, 0, 1, 4, cache.n_pages, 35) for c in range(t)]
+    if at[bad] < 0:   # the latest cell is there
+        cache.table[0, 34] = next(p for p in range(cache.n_pages) if p not in cache.table[0])
+        cache.t_dev.upload(cache.table)
+        at = [plain.pool_row(cache.table, 0, c, 0, 1, 4, cache.n_pages, 35) for c in range(t)]
+    q, q64 = act(np.abs(rng.standard_normal((rows, heads, D))) + 0.1, dtype)
+    k = cache.host["k"]
+    k[at[bad]] = np.abs(k[at[bad]]) + 1
+    k[at[bad], 3] = np.inf
+    cache.dev["k"].upload(k)
+    lse = np.full((rows, heads), -np.inf)   # only the last row, the only one that sees the latest cell, has a weight
+    lse[rows - 1] = np.inf
+    scale = float(np.float32(0.25 * D ** -0.5))
+    got = _run(sc, ops, cache, q, dtype, t, rows, heads, scale, lse)
+    assert np.isnan(got[bad]) and not got[:bad].any()
+    mass = upload(sc, np.zeros((1, 1, t + 3), np.float32))
+    ops.AttnMass(cache.c, upload(sc, q), mass, dtype, n_seqs=1, n_head=heads, rows=rows, lens=upload(sc, np.array([t])), max_len=t, scale=scale,
+                 mass_ld=t + 3).launch()
+    sc.device_sync()
+    got, there = mass.numpy().reshape(t + 3), np.array([r >= 0 for r in at])
+    assert np.isnan(got[:t][there]).all() and not got[:t][~there].any() and not got[t:].any()
