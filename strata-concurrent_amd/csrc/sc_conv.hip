@@ -22,15 +22,17 @@ constexpr uint32_t kConvThreads = 256;
 constexpr uint32_t tile_rows(bool f16) { return f16 ? 16 : 8; }
 
 // v / (1 + e^-v) by the hardware's exponential and reciprocal, 1 unit in the last place each; 0 where e^-v is beyond 2^126.  The
-// exponent t = -v log2(e) is rounded to 2^-24 of itself, which is 2^-24 |v| of e^-v (4e-6 at v = -87): far below a unit of an f16 result.
-// For f32 ones what that left out, r = -v - t ln 2, is taken along, e^r being 1 + r: 2e-7 at any v, and 120.8 us as above (120.0 without).
-template <bool kF16>
-__device__ __forceinline__ float silu(float v) {
-    constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f, kLn2Rest = -1.90465421e-9f;   // kLn2Rest: ln 2 - kLn2
-    if constexpr (kF16) return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -kLog2e));
+// exponent t = -v log2(e) is rounded to 2^-24 of itself, which is 2^-24 |v| of e^-v: little beside a unit of an f16 result, and of an f32
+// one down to kNear (3e-7), not below (4e-6 at v = -87).
+constexpr float kLog2e = 1.44269504088896340736f, kLn2 = 0.69314718055994530942f, kLn2Rest = -1.90465421e-9f;   // kLn2Rest: ln 2 - kLn2
+constexpr float kNear = -5.5f;
+__device__ __forceinline__ float silu(float v) { return v * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(v * -kLog2e)); }
+// Below kNear what the rounding left out, r = -v - t ln 2, is taken along, e^r being 1 + r: 2e-7 at any v.  The others get the bits
+// that they get without: a wave comes here only if one of its values is far.
+__device__ __forceinline__ float silu_far(float v) {
     const float x = __builtin_amdgcn_fmed3f(v, -88.0f, 200.0f);   // finite, where the result is v or 0 or no number beyond
     const float t = x * -kLog2e, e = __builtin_amdgcn_exp2f(t), r = fmaf(t, -kLn2Rest, fmaf(t, -kLn2, -x));
-    return v * __builtin_amdgcn_rcpf(1.0f + fmaf(e, r, e));
+    return v * __builtin_amdgcn_rcpf(1.0f + fmaf(e, v < kNear ? r : 0.0f, e));
 }
 
 // Four channels of a history, a row a vector, from channel c on.
@@ -83,9 +85,14 @@ __device__ __forceinline__ f32x4 sum_of(const f32x4 (&before)[W - 1], f32x4 x, c
 #pragma unroll
     for (int k = 0; k < W - 1; ++k) y += w[k] * before[k];
     y += w[W - 1] * x;
-    if (act)
+    if (!act) return y;
+    if (!kF16 && __any(fminf(fminf(y[0], y[1]), fminf(y[2], y[3])) < kNear)) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) y[j] = silu<kF16>(y[j]);
+        for (int j = 0; j < 4; ++j) y[j] = silu_far(y[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) y[j] = silu(y[j]);
+    }
     return y;
 }
 

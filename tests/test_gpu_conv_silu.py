@@ -50,3 +50,20 @@ def test_silu_of_no_numbers(sc, ops, cuda, dtype):
     sc.device_sync()
     got = out.numpy()[0]
     assert got[0] == np.inf and np.isnan(got[1:3]).all() and not got[3:].any()
+
+
+@pytest.mark.parametrize("tokens", [1, 9], ids=["step", "prompt"])
+def test_silu_where_no_sum_is_far(sc, ops, cuda, tokens):
+    """Sums above -5.5 alone: the exponent, 8 at most, is rounded to 2^-22 and its factor to 2^-26 of it, which is 2^-22 of e^-v beside
+    what the exponential, 1 + e, the reciprocal and the product leave, 2^-21.5."""
+    rng = np.random.default_rng(6)
+    x = rng.uniform(-5.499, 30, (tokens, C)).astype(np.float32)
+    x[:, ::3] = -x[:, ::3].clip(0, 5.499)
+    weight = np.zeros((C, 2), np.float32)
+    weight[:, 1] = 1
+    state, out = upload(sc, np.zeros((C, 1), np.float32)), sc.DeviceBuffer((tokens, C), "float32")
+    ops.Conv(ops.conv_states(state, n_seqs=1, channels=C, taps=2), upload(sc, x), upload(sc, weight), out, "f32", n_seqs=1, tokens=tokens,
+             cu=None if tokens == 1 else upload(sc, np.array([0, tokens]))).launch()
+    sc.device_sync()
+    want = x.astype(np.float64) / (1 + np.exp(-x.astype(np.float64)))
+    assert (np.abs(out.numpy().astype(np.float64) - want) <= np.abs(want) * (2.0 ** -22 + 2.0 ** -21.5)).all()
